@@ -32,6 +32,10 @@ ACL_SPARSE_INDEX_32I, ACL_SPARSE_INDEX_64I = 0, 1
 ACL_SPARSE_INDEX_BASE_ZERO, ACL_SPARSE_INDEX_BASE_ONE = 0, 1
 ACL_SPARSE_FORMAT_COO, ACL_SPARSE_FORMAT_CSR, ACL_SPARSE_FORMAT_CSC = 0, 1, 2
 ACL_SPARSE_POINTER_MODE_HOST, ACL_SPARSE_POINTER_MODE_DEVICE = 0, 1
+# include/b200sp_tokens.h
+B200SP_ROUTE_SOFTMAX, B200SP_ROUTE_SIGMOID = 0, 1
+B200SP_GROUP_MAX, B200SP_GROUP_TOP2 = 0, 1
+B200SP_ROWS_OF_TOKENS, B200SP_ROWS_OF_ENTRIES = 0, 1
 
 STATUS_NAMES = [
     "SUCCESS", "NOT_INITIALIZED", "ALLOC_FAILED", "INVALID_VALUE", "ARCH_MISMATCH", "EXECUTION_FAILED",
@@ -147,6 +151,17 @@ _SIGNATURES = {
     "aclsparseGetMatFillMode": [P],
     "aclsparseXcsrsort_bufferSizeExt": [P, c_int, c_int, c_int, P, P, POINTER(c_size_t)],
     "aclsparseXcsrsort": [P, c_int, c_int, c_int, P, P, P, P, P],
+    # token operators (include/b200sp_tokens.h)
+    "b200spEmbedding": [P, P, P, P, P, P],
+    "b200spEmbeddingGradBufferSize": [P, P, P, P, POINTER(c_size_t)],
+    "b200spEmbeddingGrad": [P, P, P, P, P, P, P],
+    "b200spRoute": [P, P, P, P, P],
+    "b200spRouteGrad": [P, P, P, P, P, P],
+    "b200spExpertsPreprocess": [P, P, P],
+    "b200spExpertsMMBufferSize": [P, c_int, c_int, P, P, P, P, POINTER(c_size_t)],
+    "b200spExpertsMM": [P, c_int, c_int, P, P, P, P, P, P, P],
+    "b200spExpertsGradBufferSize": [P, c_int, P, P, P, P, POINTER(c_size_t)],
+    "b200spExpertsGrad": [P, c_int, P, P, P, P, P, P, P],
     # multi-GPU helpers (include/b200sp_mg.h)
     "b200spMgPartitionRows": [P, c_int64, c_int32, POINTER(c_int64)],
 }
@@ -181,9 +196,11 @@ def __getattr__(name: str):
 
 
 from .api import (  # noqa: E402  (needs the names above)
-    CsrMatrix, DnMat, DnVec, Handle, acl_type_of, spmm, spmv,
+    CsrMatrix, DnMat, DnVec, Handle, RouteRule, acl_type_of, embedding, embedding_grad, experts_grad, experts_mm,
+    experts_preprocess, route, route_grad, spmm, spmv,
 )
 
 __all__ = [
     "lib", "check", "AclSparseError", "Handle", "CsrMatrix", "DnVec", "DnMat", "spmv", "spmm", "acl_type_of",
+    "RouteRule", "embedding", "embedding_grad", "route", "route_grad", "experts_preprocess", "experts_mm", "experts_grad",
 ]

@@ -13,15 +13,16 @@ from ctypes import Structure, addressof, byref, c_float, c_int, c_int32, c_size_
 import torch
 
 from . import (
-    ACL_BF16, ACL_FLOAT, ACL_FLOAT16, ACL_INT8, ACL_INT32, ACL_SPARSE_INDEX_32I, ACL_SPARSE_INDEX_64I,
+    ACL_BF16, ACL_FLOAT, ACL_FLOAT16, ACL_INT8, ACL_INT32, ACL_INT64, ACL_SPARSE_INDEX_32I, ACL_SPARSE_INDEX_64I,
     ACL_SPARSE_INDEX_BASE_ZERO, ACL_SPARSE_SPMVOP_ALG_DEFAULT, ACL_SPARSE_SPMVOP_ALG2,
     ACL_SPARSE_OP_NON_TRANSPOSE, ACL_SPARSE_ORDER_COL, ACL_SPARSE_ORDER_ROW, ACL_SPARSE_POINTER_MODE_DEVICE,
-    ACL_SPARSE_SPMM_ALG_DEFAULT, ACL_SPARSE_SPMV_ALG_DEFAULT, check, lib,
+    ACL_SPARSE_OP_TRANSPOSE, ACL_SPARSE_SPMM_ALG_DEFAULT, ACL_SPARSE_SPMV_ALG_DEFAULT, B200SP_GROUP_MAX, B200SP_GROUP_TOP2,
+    B200SP_ROUTE_SIGMOID, B200SP_ROUTE_SOFTMAX, B200SP_ROWS_OF_ENTRIES, B200SP_ROWS_OF_TOKENS, check, lib,
 )
 
 _ACL_OF = {
     torch.float32: ACL_FLOAT, torch.float16: ACL_FLOAT16, torch.bfloat16: ACL_BF16,
-    torch.int32: ACL_INT32, torch.int8: ACL_INT8,
+    torch.int32: ACL_INT32, torch.int8: ACL_INT8, torch.int64: ACL_INT64,
 }
 
 
@@ -338,3 +339,114 @@ class SpMVOpPlan:
             self.close()
         except Exception:
             pass
+
+
+# ---- token operators (include/b200sp_tokens.h) ----
+
+class RouteRule(Structure):
+    """b200spRouteRule: how experts are scored and chosen.  score 'softmax' or 'sigmoid'; experts in `groups` of which the
+    `kept` best take part, by their best value ('max') or the sum of their two best ('top2')."""
+
+    _fields_ = [("score", c_int32), ("groups", c_int32), ("groups_kept", c_int32), ("group_score", c_int32),
+                ("renormalise", c_int32), ("scale", c_float)]
+
+    def __init__(self, score: str = "softmax", groups: int = 1, kept: int = 1, group_score: str = "max",
+                 renormalise: bool = True, scale: float = 1.0):
+        super().__init__({"softmax": B200SP_ROUTE_SOFTMAX, "sigmoid": B200SP_ROUTE_SIGMOID}[score], groups, kept,
+                         {"max": B200SP_GROUP_MAX, "top2": B200SP_GROUP_TOP2}[group_score], int(renormalise), scale)
+        self.address = addressof(self)
+
+
+def _float_scalars(handle: Handle, alpha, beta):
+    """alpha and beta of a token operator; their defaults need no memory (NULL is 1 and 0)."""
+    if handle.device_scalars:
+        return (alpha if alpha is None else _ptr(alpha)), (beta if beta is None else _ptr(beta))
+    return None if alpha == 1.0 else byref(c_float(alpha)), None if beta == 0.0 else byref(c_float(beta))
+
+
+def embedding(handle: Handle, table: DnMat, tokens: DnVec, out: DnMat, alpha=1.0, beta=0.0) -> None:
+    """out[i] = alpha * table[tokens[i]] + beta * out[i]; tokens int32 or int64, those outside the table are padding.
+    (With device scalars, here and below: tensors, or None for the defaults.)"""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spEmbedding(handle._h, a, table._d, tokens._d, b, out._d)
+    if status:
+        check(status, "b200spEmbedding")
+
+
+def embedding_grad_buffer_size(handle: Handle, grad: DnMat, tokens: DnVec, d_table: DnMat) -> int:
+    size = c_size_t()
+    check(lib().b200spEmbeddingGradBufferSize(handle.raw, grad.raw, tokens.raw, d_table.raw, byref(size)),
+          "b200spEmbeddingGradBufferSize")
+    return size.value
+
+
+def embedding_grad(handle: Handle, grad: DnMat, tokens: DnVec, d_table: DnMat, alpha=1.0, beta=0.0,
+                   buffer: torch.Tensor | None = None) -> None:
+    """d_table[v] = alpha * sum of grad[i] over tokens[i] == v + beta * d_table[v].  Without a buffer one is allocated."""
+    if buffer is None:
+        with torch.cuda.stream(handle.stream):  # memory that is this stream's, also when it is freed below
+            buffer = torch.empty(embedding_grad_buffer_size(handle, grad, tokens, d_table), dtype=torch.uint8,
+                                 device=d_table.values.device)
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spEmbeddingGrad(handle._h, a, grad._d, tokens._d, b, d_table._d, buffer.data_ptr())
+    if status:
+        check(status, "b200spEmbeddingGrad")
+
+
+def route(handle: Handle, rule: RouteRule, logits: DnMat, bias: DnVec | None, R: CsrMatrix) -> None:
+    """Writes R (tokens x experts, the same number of entries in every row): offsets, ascending columns and values."""
+    status = lib().b200spRoute(handle._h, rule.address, logits._d, None if bias is None else bias._d, R._d)
+    if status:
+        check(status, "b200spRoute")
+
+
+def route_grad(handle: Handle, rule: RouteRule, logits: DnMat, R: CsrMatrix, d_values: DnVec, d_logits: DnMat) -> None:
+    """Gradient of the logits (whole) from that of R's values."""
+    status = lib().b200spRouteGrad(handle._h, rule.address, logits._d, R._d, d_values._d, d_logits._d)
+    if status:
+        check(status, "b200spRouteGrad")
+
+
+_ROWS = {"tokens": B200SP_ROWS_OF_TOKENS, "entries": B200SP_ROWS_OF_ENTRIES}
+
+
+def experts_buffer_size(handle: Handle, R: CsrMatrix, X: DnMat, W: DnMat, Y: DnMat, transpose: bool = True,
+                        rows: str = "tokens") -> int:
+    size = c_size_t()
+    check(lib().b200spExpertsMMBufferSize(handle.raw, ACL_SPARSE_OP_TRANSPOSE if transpose else ACL_SPARSE_OP_NON_TRANSPOSE,
+                                          _ROWS[rows], R.raw, X.raw, W.raw, Y.raw, byref(size)), "b200spExpertsMMBufferSize")
+    return size.value
+
+
+def experts_grad_buffer_size(handle: Handle, R: CsrMatrix, dY: DnMat, X: DnMat, dW: DnMat, rows: str = "tokens") -> int:
+    size = c_size_t()
+    check(lib().b200spExpertsGradBufferSize(handle.raw, _ROWS[rows], R.raw, dY.raw, X.raw, dW.raw, byref(size)),
+          "b200spExpertsGradBufferSize")
+    return size.value
+
+
+def experts_preprocess(handle: Handle, R: CsrMatrix, buffer: torch.Tensor) -> None:
+    """Orders R's entries by expert in the buffer, for the products that follow with it."""
+    status = lib().b200spExpertsPreprocess(handle._h, R._d, buffer.data_ptr())
+    if status:
+        check(status, "b200spExpertsPreprocess")
+
+
+def experts_mm(handle: Handle, R: CsrMatrix, X: DnMat, W: DnMat, Y: DnMat, alpha=1.0, beta=0.0, transpose: bool = True,
+               rows: str = "tokens", buffer: torch.Tensor | None = None) -> None:
+    """Y[i] = alpha * X[row of entry i] * op(W of its expert) + beta * Y[i]; W: the experts' matrices stacked."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsMM(handle._h, ACL_SPARSE_OP_TRANSPOSE if transpose else ACL_SPARSE_OP_NON_TRANSPOSE,
+                                   _ROWS[rows], a, R._d, X._d, W._d, b, Y._d, None if buffer is None else buffer.data_ptr())
+    if status:
+        check(status, "b200spExpertsMM")
+
+
+def experts_grad(handle: Handle, R: CsrMatrix, dY: DnMat, X: DnMat, dW: DnMat, alpha=1.0, beta=0.0, rows: str = "tokens",
+                 buffer: torch.Tensor | None = None) -> None:
+    """dW of every expert = alpha * sum over its entries of dY[i]^T X[row of entry i] + beta * dW."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsGrad(handle._h, _ROWS[rows], a, R._d, dY._d, X._d, b, dW._d,
+                                     None if buffer is None else buffer.data_ptr())
+    if status:
+        check(status, "b200spExpertsGrad")

@@ -37,6 +37,9 @@ SOURCES = [
     "sddmm/sddmm.cu",
     "spmm/spmm_host.cpp",
     "spmm/spmm_kernels.cu",
+    "tokens/embedding.cu",
+    "tokens/route.cu",
+    "tokens/experts.cu",
     "mg/partition.cpp",
     "mg/exchange.cu",
 ]

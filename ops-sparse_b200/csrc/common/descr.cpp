@@ -174,6 +174,8 @@ aclsparseStatus_t aclsparseCsrSetPointers(aclsparseSpMatDescr_t descr, void *row
     descr->values = values;
     // A new sparsity pattern invalidates any analysis recorded for the old arrays.
     descr->active = b200sp::ActivePlan{};
+    std::lock_guard<std::mutex> lock(descr->expertsMutex);
+    descr->experts = b200sp::ExpertsPlan{};
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 

@@ -83,6 +83,14 @@ struct TileOrderPlan {
     uint64_t generation = 0;
 };
 
+// The experts' products: the order of this matrix's entries by expert that a buffer holds.
+struct ExpertsPlan {
+    const void *buffer = nullptr;  // nullptr: none
+    const void *offsets = nullptr, *indices = nullptr;
+    int64_t rows = 0, cols = 0, nnz = 0;
+    uint64_t generation = 0;
+};
+
 // Every library call that writes an analysis or scratch data into a caller buffer stamps that buffer with a new
 // generation; a recorded plan is valid only while its generation is still the buffer's current one.  Without it
 // a stale plan would be trusted after its bytes were overwritten: Preprocess(A, buf), then a call that re-analyses
@@ -131,6 +139,8 @@ struct aclsparseSpMatDescr {
     mutable int64_t spmmSizedN = -1;
     b200sp::TileOrderPlan sddmm;  // of the SDDMM products that write this matrix
     mutable std::mutex sddmmMutex;  // held while it is read or written
+    mutable b200sp::ExpertsPlan experts;
+    mutable std::mutex expertsMutex;  // held while it is read or written
     mutable std::mutex copyMutex;  // held while a product that copies into the analysed buffer is enqueued
 };
 

@@ -1,0 +1,492 @@
+// b200spEmbedding, b200spEmbeddingGrad: rows of a table by token, and the gradient of the table.
+//
+// Both are products with a matrix of one entry a row, S: out = alpha S table + beta out, dTable = alpha S^T grad + beta
+// dTable.  Neither reuses anything, so both are bound by the bytes of their rows.
+#include <algorithm>
+#include <climits>
+
+#include "b200sp_tokens.h"
+#include "tokens/common.cuh"
+#include "tokens/sort.cuh"
+
+namespace {
+
+using namespace b200sp_tokens;
+
+// ---------------------------------------------------------------- rows of the table
+
+struct EmbedArgs {
+    const void *table, *tokens;
+    void *out;
+    int vocab, width;
+    long long ldTable, ldOut;
+    int lanes;             // lanes side by side on a row: a power of two, 32 at most
+    unsigned perRow;       // pieces of `lanes` vectors that a row has
+    unsigned long long pieces;
+    Scalars sc;
+};
+
+constexpr int kEmbedDepth = 4;  // vectors in flight per thread
+
+template <typename In, typename Out, typename Key, int kN>
+__global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
+{
+    b200sp::WaitForPrevious();
+    constexpr bool kVector = kN > 1;
+    const int lane = threadIdx.x & 31;
+    const int rowsPerWarp = 32 / a.lanes, sub = lane / a.lanes, at = lane % a.lanes;
+    const unsigned long long first = ((unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kEmbedDepth * rowsPerWarp + sub;
+    const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
+    float v[kEmbedDepth][kN];
+    long long row[kEmbedDepth];
+    int col[kEmbedDepth];
+#pragma unroll
+    for (int u = 0; u < kEmbedDepth; ++u) {
+        const unsigned long long piece = first + (unsigned long long)u * rowsPerWarp;
+        row[u] = -1;
+        if (piece >= a.pieces) continue;
+        if (a.pieces <= UINT_MAX) {
+            row[u] = (unsigned)piece / a.perRow;
+            col[u] = (int)(((unsigned)piece % a.perRow) * a.lanes + at) * kN;
+        } else {
+            row[u] = (long long)(piece / a.perRow);
+            col[u] = (int)(piece % a.perRow * a.lanes + at) * kN;
+        }
+        if (col[u] >= a.width) row[u] = -1;
+        if (row[u] < 0) continue;
+        const Key token = static_cast<const Key *>(a.tokens)[row[u]];
+        const bool in = token >= 0 && token < (Key)a.vocab;
+        const In *const from = static_cast<const In *>(a.table) + (long long)(in ? token : 0) * a.ldTable + col[u];
+        if (in && col[u] + kN <= a.width) {
+            LoadFloats<In, kN, kVector>(from, v[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[u][i] = in && col[u] + i < a.width ? ToFloat(from[i]) : 0.0f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < kEmbedDepth; ++u) {
+        if (row[u] < 0) continue;
+        Out *const to = static_cast<Out *>(a.out) + row[u] * a.ldOut + col[u];
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            v[u][i] *= alpha;
+            if (beta != 0.0f && col[u] + i < a.width) v[u][i] = fmaf(beta, ToFloat(to[i]), v[u][i]);
+        }
+        if (col[u] + kN <= a.width) {
+            StoreFloats<Out, kN, kVector>(to, v[u]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < kN; ++i)
+                if (col[u] + i < a.width) to[i] = FromFloat<Out>(v[u][i]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the gradient of the table
+
+// The positions are sorted by token (sort.cuh), in the same launch as the zeros of dTable: the sort is one cluster's work
+// and the zeros everyone else's.  Then a group of lanes takes `chunk` sorted positions and sums their rows of grad, in
+// that order, one token after the other.  A token whose positions lie in one chunk is finished there; of one that
+// crosses chunks every chunk leaves a partial row, which EmbeddingJoinKernel adds up in their order.
+struct GradArgs {
+    const void *grad;
+    void *table;
+    int count, vocab, width;
+    long long ldGrad, ldTable;
+    const int *keys, *positions;  // sorted
+    int chunk, chunks;
+    float *heads, *tails;         // [chunk][pitch]: of the run that comes from the chunk before, that goes on in the next
+    int pitch;
+    int lanes;                    // threads side by side on a row
+    Scalars sc;
+};
+
+template <typename Out> __device__ __forceinline__ void FillTable(const GradArgs &a, int block, int blocks)
+{
+    Out *const table = static_cast<Out *>(a.table);
+    const bool whole = a.ldTable == a.width;
+    if (whole && (reinterpret_cast<uintptr_t>(table) & 15) == 0) {
+        const long long bytes = (long long)a.vocab * a.width * (long long)sizeof(Out);
+        uint4 *const to = reinterpret_cast<uint4 *>(table);
+        for (long long i = (long long)block * blockDim.x + threadIdx.x; i < bytes / 16; i += (long long)blocks * blockDim.x)
+            __stcs(to + i, make_uint4(0, 0, 0, 0));
+        if (block == 0 && threadIdx.x < bytes % 16 / (long long)sizeof(Out)) table[bytes / 16 * (16 / sizeof(Out)) + threadIdx.x] = FromFloat<Out>(0.0f);
+        return;
+    }
+    for (int r = block; r < a.vocab; r += blocks)
+        for (int c = threadIdx.x; c < a.width; c += blockDim.x) table[r * a.ldTable + c] = FromFloat<Out>(0.0f);
+}
+
+template <typename Out, typename Key>
+__global__ void __launch_bounds__(kSortThreads, 1) EmbeddingSortKernel(const SortArgs s, const GradArgs a, int clusters)
+{
+    extern __shared__ unsigned char sSort[];
+    b200sp::WaitForPrevious();
+    const int size = gridDim.x / clusters;
+    if ((int)blockIdx.x < size) {
+        ClusterSort<Key>(s, sSort, [](int, int, int) {});
+    } else if (a.sc.Beta() == 0.0f) {
+        FillTable<Out>(a, blockIdx.x - size, gridDim.x - size);
+    }
+}
+
+// First place of the ascending keys that is >= key.
+__device__ __forceinline__ int LowerBound(const int *keys, int count, int key)
+{
+    int lo = 0, hi = count;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (__ldg(keys + mid) < key) lo = mid + 1;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// beta other than 0 and 1: rows of tokens that do not occur.  (The rows of those that do are scaled where they are rounded.)
+template <typename Out> __global__ void __launch_bounds__(256) EmbeddingScaleKernel(const GradArgs a)
+{
+    b200sp::WaitForPrevious();
+    const float beta = a.sc.Beta();
+    if (beta == 0.0f || beta == 1.0f) return;
+    for (int r = blockIdx.x; r < a.vocab; r += gridDim.x) {
+        const int at = LowerBound(a.keys, a.count, r);
+        if (at < a.count && __ldg(a.keys + at) == r) continue;
+        Out *const row = static_cast<Out *>(a.table) + r * a.ldTable;
+        for (int c = threadIdx.x; c < a.width; c += 256) row[c] = FromFloat<Out>(beta * ToFloat(row[c]));
+    }
+}
+
+template <typename Out, int kN> __device__ __forceinline__ void FinishRow(const GradArgs &a, int key, int col, float (&sum)[kN])
+{
+    const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
+    Out *const to = static_cast<Out *>(a.table) + key * a.ldTable + col;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        sum[i] *= alpha;
+        if (beta != 0.0f && col + i < a.width) sum[i] = fmaf(beta, ToFloat(to[i]), sum[i]);
+    }
+    if (col + kN <= a.width) {
+        StoreFloats<Out, kN, (kN > 1)>(to, sum);
+    } else {
+#pragma unroll
+        for (int i = 0; i < kN; ++i)
+            if (col + i < a.width) to[i] = FromFloat<Out>(sum[i]);
+    }
+}
+
+constexpr int kGradDepth = 8;  // rows in flight
+
+template <typename In, typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingSumKernel(const GradArgs a)
+{
+    b200sp::WaitForPrevious();
+    const int chunk = blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(blockIdx.y * a.lanes + threadIdx.x % a.lanes) * kN;
+    if (chunk >= a.chunks || col >= a.width) return;
+    const int lo = chunk * a.chunk, hi = min(a.count, lo + a.chunk);
+    const int before = lo > 0 ? __ldg(a.keys + lo - 1) : -1, after = hi < a.count ? __ldg(a.keys + hi) : -1;
+    float sum[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) sum[i] = 0.0f;
+    int now = __ldg(a.keys + lo);
+    bool continued = now == before;
+    auto flush = [&](bool end) {
+        if (now < a.vocab) {
+            if (continued || (end && now == after)) {
+                float *const to = (continued ? a.heads : a.tails) + (long long)chunk * a.pitch + col;
+#pragma unroll
+                for (int i = 0; i < kN; ++i) to[i] = sum[i];  // the pitch has room for whole vectors
+            } else {
+                FinishRow<Out, kN>(a, now, col, sum);
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < kN; ++i) sum[i] = 0.0f;
+        continued = false;
+    };
+    for (int e = lo; e < hi; e += kGradDepth) {
+        float v[kGradDepth][kN];
+        int key[kGradDepth];
+#pragma unroll
+        for (int u = 0; u < kGradDepth; ++u) {
+            key[u] = -1;
+            if (e + u >= hi) continue;
+            key[u] = __ldg(a.keys + e + u);
+            const In *const from = static_cast<const In *>(a.grad) + (long long)__ldg(a.positions + e + u) * a.ldGrad + col;
+            if (col + kN <= a.width) {
+                LoadFloats<In, kN, (kN > 1)>(from, v[u]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < kN; ++i) v[u][i] = col + i < a.width ? ToFloat(from[i]) : 0.0f;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < kGradDepth; ++u) {
+            if (key[u] < 0) continue;
+            if (key[u] != now) {
+                flush(false);
+                now = key[u];
+            }
+#pragma unroll
+            for (int i = 0; i < kN; ++i) sum[i] += v[u][i];
+        }
+    }
+    flush(true);
+}
+
+// Tokens whose positions cross chunks: the chunk where one begins adds up what the others left.
+template <typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingJoinKernel(const GradArgs a)
+{
+    b200sp::WaitForPrevious();
+    const int chunk = blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(blockIdx.y * a.lanes + threadIdx.x % a.lanes) * kN;
+    if (chunk >= a.chunks - 1 || col >= a.width) return;
+    const int hi = (chunk + 1) * a.chunk, lo = hi - a.chunk;
+    const int key = __ldg(a.keys + hi - 1);
+    if (key >= a.vocab || __ldg(a.keys + hi) != key) return;
+    if (lo > 0 && __ldg(a.keys + lo - 1) == key) return;  // began before
+    const int end = LowerBound(a.keys + hi, a.count - hi, key + 1) + hi;
+    const int lastChunk = (end - 1) / a.chunk;
+    float sum[kN];
+    const float *at = a.tails + (long long)chunk * a.pitch + col;
+#pragma unroll
+    for (int i = 0; i < kN; ++i) sum[i] = at[i];
+    for (int c = chunk + 1; c <= lastChunk; c += kGradDepth) {
+        float v[kGradDepth][kN];
+#pragma unroll
+        for (int u = 0; u < kGradDepth; ++u) {
+            const float *from = a.heads + (long long)min(c + u, lastChunk) * a.pitch + col;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[u][i] = from[i];
+        }
+#pragma unroll
+        for (int u = 0; u < kGradDepth; ++u) {
+            if (c + u > lastChunk) continue;
+#pragma unroll
+            for (int i = 0; i < kN; ++i) sum[i] += v[u][i];
+        }
+    }
+    FinishRow<Out, kN>(a, key, col, sum);
+}
+
+// ---------------------------------------------------------------- host
+
+aclsparseStatus_t CheckTokens(const aclsparseDnVecDescr *tokens)
+{
+    if (tokens == nullptr || tokens->magic != b200sp::kDnVecMagic) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (tokens->valueType != ACL_INT32 && tokens->valueType != ACL_INT64) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (tokens->size > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (reinterpret_cast<uintptr_t>(tokens->values) % (tokens->valueType == ACL_INT64 ? 8 : 4) != 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+// The rows that a call reads or writes, and the tokens that name them.
+aclsparseStatus_t CheckEmbedding(const aclsparseDnMatDescr *table, const aclsparseDnVecDescr *tokens, const aclsparseDnMatDescr *rows)
+{
+    for (const aclsparseDnMatDescr *m : {table, rows}) {
+        const aclsparseStatus_t st = CheckDense(m);
+        if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    }
+    const aclsparseStatus_t st = CheckTokens(tokens);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (rows->rows != tokens->size || rows->cols != table->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (table->rows >= INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;  // the number after the last row is a key, too
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+int LanesFor(long long vectors, int most)
+{
+    int lanes = 1;
+    while (lanes < most && lanes < vectors) lanes *= 2;
+    return lanes;
+}
+
+// Chunks of the gradient.  Long ones leave fewer partial rows, short ones fill the SMs.
+int ChunkFor(long long count)
+{
+    int chunk = count <= 8192 ? 8 : 32;
+    while (count > 4096ll * chunk) chunk *= 2;
+    return chunk;
+}
+
+struct GradLayout {
+    size_t keyA, posA, keyB, posB, heads, tails, total;
+    int chunk, chunks, pitch;
+};
+GradLayout GradLayoutFor(long long count, long long width)
+{
+    GradLayout L;
+    const size_t words = AlignUp(sizeof(int) * (size_t)count, 256);
+    L.keyA = 0;
+    L.posA = words;
+    L.keyB = 2 * words;
+    L.posB = 3 * words;
+    L.heads = 4 * words;
+    L.chunk = ChunkFor(count);
+    L.chunks = (int)((count + L.chunk - 1) / L.chunk);
+    L.pitch = (int)AlignUp((size_t)width, 64);
+    const size_t partial = sizeof(float) * (size_t)L.chunks * (size_t)L.pitch;
+    L.tails = L.heads + partial;
+    L.total = L.tails + partial + 256;  // any address is accepted
+    return L;
+}
+
+template <typename In, typename Out, typename Key, int kN> cudaError_t LaunchEmbedding(EmbedArgs a, long long rows, cudaStream_t stream)
+{
+    const long long vectors = (a.width + kN - 1) / kN;
+    a.lanes = LanesFor(vectors, 32);
+    a.perRow = (unsigned)((vectors + a.lanes - 1) / a.lanes);
+    a.pieces = (unsigned long long)rows * a.perRow;
+    const unsigned long long perBlock = 8ull * kEmbedDepth * (32 / a.lanes), blocks = (a.pieces + perBlock - 1) / perBlock;
+    if (blocks > INT32_MAX) return cudaErrorInvalidConfiguration;
+    b200sp_note_launches(1);
+    return b200sp::LaunchChained(EmbeddingKernel<In, Out, Key, kN>, (unsigned)blocks, 256, 0, stream, a);
+}
+
+template <typename In, typename Out, int kN> cudaError_t LaunchSums(GradArgs a, bool scales, cudaStream_t stream)
+{
+    if (scales) {
+        b200sp_note_launches(1);
+        const cudaError_t e = b200sp::LaunchChained(EmbeddingScaleKernel<Out>, (unsigned)std::min(a.vocab, b200sp_sm_count() * 8), 256, 0, stream, a);
+        if (e != cudaSuccess) return e;
+    }
+    const long long vectors = (a.width + kN - 1) / kN;
+    a.lanes = LanesFor(vectors, 256);
+    const int perBlock = 256 / a.lanes;
+    const dim3 grid((unsigned)((a.chunks + perBlock - 1) / perBlock), (unsigned)((vectors + a.lanes - 1) / a.lanes));
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(256);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+    b200sp_note_launches(2);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, EmbeddingSumKernel<In, Out, kN>, a);
+    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, EmbeddingJoinKernel<Out, kN>, a);
+}
+
+template <typename Out, typename Key> cudaError_t LaunchSort(const SortArgs &s, const GradArgs &a, cudaStream_t stream)
+{
+    const int size = SortCtas(a.count), shared = SortShared(s.digitBits);
+    const cudaError_t set = cudaFuncSetAttribute(EmbeddingSortKernel<Out, Key>, cudaFuncAttributeMaxDynamicSharedMemorySize, SortShared(kSortMaxBits));
+    if (set != cudaSuccess) return set;
+    // one cluster sorts; the others fill the table, if it has to be (one CTA per SM: what the sort needs of shared memory)
+    const bool fills = a.sc.betaAt != nullptr || a.sc.beta == 0.0f;
+    const int clusters = fills ? std::max(2, b200sp_sm_count() / size) : 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(size * clusters));
+    cfg.blockDim = dim3(kSortThreads);
+    cfg.dynamicSmemBytes = (size_t)shared;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)size;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    b200sp_note_launches(1);
+    return cudaLaunchKernelEx(&cfg, EmbeddingSortKernel<Out, Key>, s, a, clusters);
+}
+
+}  // namespace
+
+extern "C" {
+
+aclsparseStatus_t b200spEmbedding(aclsparseHandle_t handle, const void *alpha, aclsparseConstDnMatDescr_t table,
+                                  aclsparseConstDnVecDescr_t tokens, const void *beta, aclsparseDnMatDescr_t out)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    const aclsparseStatus_t st = CheckEmbedding(table, tokens, out);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    const OnDevice device(handle);
+    EmbedArgs a{table->values, tokens->values, out->values, (int)table->rows, (int)table->cols, table->ld, out->ld, 0, 0, 0,
+                ScalarsOf(handle, alpha, beta)};
+    const bool vectors = RowsAligned(table) && RowsAligned(out);
+    const cudaError_t e = WithType(table->valueType, [&](auto in) {
+        return WithType(out->valueType, [&](auto to) {
+            using In = decltype(in);
+            using Out = decltype(to);
+            // 16 bytes of the narrower type
+            constexpr int kN = sizeof(In) == 2 || sizeof(Out) == 2 ? 8 : 4;
+            if (tokens->valueType == ACL_INT64)
+                return vectors ? LaunchEmbedding<In, Out, long long, kN>(a, out->rows, handle->stream)
+                               : LaunchEmbedding<In, Out, long long, 1>(a, out->rows, handle->stream);
+            return vectors ? LaunchEmbedding<In, Out, int, kN>(a, out->rows, handle->stream)
+                           : LaunchEmbedding<In, Out, int, 1>(a, out->rows, handle->stream);
+        });
+    });
+    return Finished(e, "b200spEmbedding");
+}
+
+aclsparseStatus_t b200spEmbeddingGradBufferSize(aclsparseHandle_t handle, aclsparseConstDnMatDescr_t grad,
+                                                aclsparseConstDnVecDescr_t tokens, aclsparseConstDnMatDescr_t dTable,
+                                                size_t *bufferSize)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const aclsparseStatus_t st = CheckEmbedding(dTable, tokens, grad);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    *bufferSize = GradLayoutFor(tokens->size, dTable->cols).total;
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+aclsparseStatus_t b200spEmbeddingGrad(aclsparseHandle_t handle, const void *alpha, aclsparseConstDnMatDescr_t grad,
+                                      aclsparseConstDnVecDescr_t tokens, const void *beta, aclsparseDnMatDescr_t dTable,
+                                      void *buffer)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    const aclsparseStatus_t st = CheckEmbedding(dTable, tokens, grad);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
+    const OnDevice device(handle);
+    (void)NoteWrite(buffer);
+    const GradLayout L = GradLayoutFor(tokens->size, dTable->cols);
+    char *const p = reinterpret_cast<char *>(AlignUp(reinterpret_cast<uintptr_t>(buffer), 256));
+    SortArgs s{};
+    s.keys = tokens->values;
+    s.count = (int)tokens->size;
+    s.limit = (int)dTable->rows;
+    SortPasses(s.limit, &s);
+    s.keyA = reinterpret_cast<int *>(p + L.keyA);
+    s.posA = reinterpret_cast<int *>(p + L.posA);
+    s.keyB = reinterpret_cast<int *>(p + L.keyB);
+    s.posB = reinterpret_cast<int *>(p + L.posB);
+    GradArgs a{};
+    a.grad = grad->values;
+    a.table = dTable->values;
+    a.count = s.count;
+    a.vocab = s.limit;
+    a.width = (int)dTable->cols;
+    a.ldGrad = grad->ld;
+    a.ldTable = dTable->ld;
+    a.keys = s.keyA;
+    a.positions = s.posA;
+    a.chunk = L.chunk;
+    a.chunks = L.chunks;
+    a.heads = reinterpret_cast<float *>(p + L.heads);
+    a.tails = reinterpret_cast<float *>(p + L.tails);
+    a.pitch = L.pitch;
+    a.sc = ScalarsOf(handle, alpha, beta);
+    const bool scales = a.sc.betaAt != nullptr || (a.sc.beta != 0.0f && a.sc.beta != 1.0f);
+    const bool vectors = RowsAligned(grad) && RowsAligned(dTable);
+    const cudaError_t e = WithType(dTable->valueType, [&](auto to) {
+        using Out = decltype(to);
+        const cudaError_t sorted = tokens->valueType == ACL_INT64 ? LaunchSort<Out, long long>(s, a, handle->stream)
+                                                                  : LaunchSort<Out, int>(s, a, handle->stream);
+        if (sorted != cudaSuccess) return sorted;
+        return WithType(grad->valueType, [&](auto from) {
+            using In = decltype(from);
+            constexpr int kN = sizeof(In) == 2 || sizeof(Out) == 2 ? 8 : 4;
+            return vectors ? LaunchSums<In, Out, kN>(a, scales, handle->stream) : LaunchSums<In, Out, 1>(a, scales, handle->stream);
+        });
+    });
+    return Finished(e, "b200spEmbeddingGrad");
+}
+
+}  // extern "C"

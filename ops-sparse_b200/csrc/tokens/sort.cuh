@@ -1,0 +1,192 @@
+// Positions in the order of their keys, stable: a radix sort by one thread-block cluster, in one launch.
+//
+// The token operators sort few and small things -- thousands of positions by token, or by expert -- in the middle of a chain of
+// kernels, where launches cost more than the sort.  So every pass over a digit (up to ten bits: one pass for experts, two for
+// the tokens of a large table) is one phase of a kernel of up to eight CTAs, each with a contiguous share of the positions:
+// count the digits of the share in shared memory; read the other CTAs' counts through the cluster, which gives every digit's
+// first place; then rank tile by tile (by warp, step and lane, which is the order in memory) and store.  Passes meet at
+// cluster barriers.  Nothing is atomic across CTAs, so the result is unique and the same in every run.
+// 16,384 tokens of a table of 65,536 rows (two passes): see the embedding's gradient, which hides them behind its zeros.
+#pragma once
+
+#include <cooperative_groups.h>
+#include <cuda_runtime.h>
+
+#include "tokens/common.cuh"
+
+namespace b200sp_tokens {
+
+constexpr int kSortThreads = 1024;
+constexpr int kSortWarps = kSortThreads / 32;
+constexpr int kSortSteps = 4;                            // positions per thread and tile
+constexpr int kSortTile = kSortThreads * kSortSteps;
+constexpr int kSortMaxBits = 10;
+constexpr int kSortMaxCtas = 8;                          // the portable cluster size
+
+struct SortArgs {
+    const void *keys;     // int32 or int64, the caller's
+    int count, limit;     // keys outside [0, limit) count as limit
+    int passes, digitBits;
+    int *keyA, *posA;     // sorted, after the last pass
+    int *keyB, *posB;     // between passes (unused with one pass)
+    int *offsets;         // with one pass, or nullptr: first place of every key 0 ... limit, and the end, limit + 2 numbers
+};
+
+inline int SortBits(long long limit)  // of the numbers 0 ... limit
+{
+    int bits = 1;
+    while ((1ll << bits) <= limit) ++bits;
+    return bits;
+}
+inline void SortPasses(long long limit, SortArgs *a)
+{
+    const int bits = SortBits(limit);
+    a->passes = (bits + kSortMaxBits - 1) / kSortMaxBits;
+    a->digitBits = (bits + a->passes - 1) / a->passes;
+}
+inline int SortCtas(long long count)
+{
+    int ctas = 1;
+    while (ctas < kSortMaxCtas && count > (long long)ctas * kSortTile / 2) ctas *= 2;
+    return ctas;
+}
+// Shared memory: a word and a count per warp and digit, three numbers per digit.
+inline int SortShared(int digitBits) { return (1 << digitBits) * (kSortWarps * 6 + 3 * 4); }
+
+template <typename Key> __device__ __forceinline__ int SortKey(const SortArgs &a, int i)
+{
+    const Key k = static_cast<const Key *>(a.keys)[i];
+    return k < 0 || k >= (Key)a.limit ? a.limit : (int)k;
+}
+
+// All CTAs of the cluster, 1024 threads each; place(key, position, where) is told of every position in the last pass.
+template <typename Key, typename Place> __device__ __forceinline__ void ClusterSort(const SortArgs &a, unsigned char *shared, Place &&place)
+{
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int ctas = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+    const int bins = 1 << a.digitBits;
+    uint32_t *const sMask = reinterpret_cast<uint32_t *>(shared);          // [warp][digit]
+    int *const sCount = reinterpret_cast<int *>(sMask + kSortWarps * bins);  // [digit]: this CTA's
+    int *const sBase = sCount + bins;                                      // [digit]: next place
+    int *const sTile = sBase + bins;                                       // [digit]: of the tile (the others may still read sCount)
+    uint16_t *const sWarp = reinterpret_cast<uint16_t *>(sTile + bins);    // [warp][digit]
+    __shared__ int sScan[kSortWarps];
+    // shares of whole warps' segments
+    const int share = ((a.count + ctas - 1) / ctas + 31) / 32 * 32;
+    const int lo = min((long long)a.count, (long long)rank * share), hi = min((long long)a.count, (long long)lo + share);
+    for (int i = tid; i < kSortWarps * bins; i += kSortThreads) sMask[i] = 0;
+    for (int p = 0; p < a.passes; ++p) {
+        const bool last = p == a.passes - 1;
+        const int shift = p * a.digitBits;
+        // the last pass ends in A
+        const bool fromA = (a.passes - p) % 2 == 0;
+        const int *const keyIn = fromA ? a.keyA : a.keyB, *const posIn = fromA ? a.posA : a.posB;
+        int *const keyOut = fromA ? a.keyB : a.keyA, *const posOut = fromA ? a.posB : a.posA;
+        for (int i = tid; i < bins; i += kSortThreads) sCount[i] = 0;
+        __syncthreads();
+        for (int i = lo + tid; i < hi; i += kSortThreads) {
+            const int k = p == 0 ? SortKey<Key>(a, i) : __ldcg(keyIn + i);
+            atomicAdd(sCount + ((k >> shift) & (bins - 1)), 1);
+        }
+        cluster.sync();
+        int all = 0, before = 0;  // of digit tid
+        if (tid < bins) {
+            for (int c = 0; c < ctas; ++c) {
+                const int n = cluster.map_shared_rank(sCount, c)[tid];
+                before += c < rank ? n : 0;
+                all += n;
+            }
+        }
+        int incl = all;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += t;
+        }
+        if (lane == 31) sScan[warp] = incl;
+        __syncthreads();
+        if (warp == 0) {
+            int w = sScan[lane];
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, w, d);
+                if (lane >= d) w += t;
+            }
+            sScan[lane] = w;
+        }
+        __syncthreads();
+        if (tid < bins) {
+            const int start = incl - all + (warp > 0 ? sScan[warp - 1] : 0);
+            sBase[tid] = start + before;
+            if (a.offsets != nullptr && rank == 0 && tid <= a.limit + 1) a.offsets[tid] = start;
+            // 2^bits > limit: the end of the last key has a digit of its own unless the digits are used up
+            if (a.offsets != nullptr && rank == 0 && tid == a.limit && a.limit + 1 == bins) a.offsets[bins] = a.count;
+        }
+        for (int tile = lo; tile < hi; tile += kSortTile) {
+            for (int i = tid; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(sWarp)[i] = 0;
+            __syncthreads();
+            int key[kSortSteps], pos[kSortSteps], at[kSortSteps];
+            const int first = tile + warp * (32 * kSortSteps) + lane;
+#pragma unroll
+            for (int u = 0; u < kSortSteps; ++u) {
+                const int i = first + 32 * u;
+                key[u] = -1;
+                if (i < hi) {
+                    key[u] = p == 0 ? SortKey<Key>(a, i) : __ldcg(keyIn + i);
+                    pos[u] = p == 0 ? i : __ldcg(posIn + i);
+                }
+            }
+            // rank among the warp's positions of the same digit: the lanes of a digit find each other through its word
+            uint32_t *const mask = sMask + warp * bins;
+            uint16_t *const count = sWarp + warp * bins;
+#pragma unroll
+            for (int u = 0; u < kSortSteps; ++u) {
+                const int d = (key[u] >> shift) & (bins - 1);
+                const bool in = key[u] >= 0;
+                if (in) atomicOr(mask + d, 1u << lane);
+                __syncwarp();
+                uint32_t peers = 0;
+                int had = 0;
+                if (in) {
+                    peers = *static_cast<volatile uint32_t *>(mask + d);
+                    had = *static_cast<volatile uint16_t *>(count + d);
+                }
+                const int among = __popc(peers & ((1u << lane) - 1u));
+                __syncwarp();
+                if (in && among == 0) {
+                    mask[d] = 0;
+                    count[d] = (uint16_t)(had + __popc(peers));
+                }
+                __syncwarp();
+                at[u] = had + among;
+            }
+            __syncthreads();
+            if (tid < bins) {  // counts become the places of every warp's first
+                int run = 0;
+                for (int w = 0; w < kSortWarps; ++w) {
+                    const int n = sWarp[w * bins + tid];
+                    sWarp[w * bins + tid] = (uint16_t)run;
+                    run += n;
+                }
+                sTile[tid] = run;
+            }
+            __syncthreads();
+#pragma unroll
+            for (int u = 0; u < kSortSteps; ++u) {
+                if (key[u] < 0) continue;
+                const int d = (key[u] >> shift) & (bins - 1);
+                const int to = sBase[d] + sWarp[warp * bins + d] + at[u];
+                keyOut[to] = key[u];
+                posOut[to] = pos[u];
+                if (last) place(key[u], pos[u], to);
+            }
+            __syncthreads();
+            if (tid < bins) sBase[tid] += sTile[tid];
+        }
+        cluster.sync();  // what was stored is read by the others from here on
+    }
+}
+
+}  // namespace b200sp_tokens
