@@ -121,6 +121,14 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
                                     aclsparseConstDnMatDescr_t matX, const void *beta, aclsparseDnMatDescr_t dW,
                                     void *buffer);
 
+/* 1 if a bounded wait of the experts' kernels ran out since the flag was cleared (never observed outside the test that
+ * provokes it): rows of an output are unwritten then.  Both synchronise the device. */
+int b200sp_experts_error(void);
+int b200sp_experts_error_clear(void);
+/* For tests of that path: later products wait at most wait_cycles SM clocks (0 = the default, about two seconds) and expect
+ * extra_tx bytes more than they copy on every barrier, so that with extra_tx > 0 every wait runs out. */
+void b200sp_experts_wait_test(long long wait_cycles, unsigned extra_tx);
+
 #ifdef __cplusplus
 }
 #endif

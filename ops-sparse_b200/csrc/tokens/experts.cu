@@ -4,6 +4,7 @@
 // expert after the other.  Its rows are gathered from X as they lie and its results stored in the rows of their
 // entries: nothing is laid out in between.
 #include <algorithm>
+#include <type_traits>
 
 #include "b200sp_tokens.h"
 #include "tokens/common.cuh"
@@ -199,6 +200,8 @@ template <typename T, typename Out> __global__ void __launch_bounds__(256) Exper
     }
 }
 
+#include "tokens/experts_tensor.cuh"
+
 // ---------------------------------------------------------------- host
 
 aclsparseStatus_t CheckRouted(const aclsparseSpMatDescr *R)
@@ -282,9 +285,43 @@ ProductArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, voi
     return a;
 }
 
+MmaArgs TensorArgsOf(const ProductArgs &a, const aclsparseSpMatDescr *R)
+{
+    MmaArgs t{};
+    t.offsets = a.offsets;
+    t.entries = a.entries;
+    t.rows = a.rows;
+    t.out = a.out;
+    t.ldo = a.ldo;
+    t.experts = (int)R->cols;
+    t.n = a.n;
+    t.d = a.d;
+    t.byEntry = a.byEntry;
+    t.sc = a.sc;
+    return t;
+}
+
 }  // namespace
 
 extern "C" {
+
+int b200sp_experts_error(void)
+{
+    int flag = 0;
+    return cudaMemcpyFromSymbol(&flag, gExpertsError, sizeof(flag)) == cudaSuccess ? flag : -1;
+}
+
+int b200sp_experts_error_clear(void)
+{
+    const int zero = 0;
+    return (int)cudaMemcpyToSymbol(gExpertsError, &zero, sizeof(zero));
+}
+
+void b200sp_experts_wait_test(long long wait_cycles, unsigned extra_tx)
+{
+    gExpertsWaitCycles = wait_cycles > 0 ? wait_cycles : kMmaWaitCycles;
+    gExpertsExtraTx = extra_tx;
+}
 
 aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, void *buffer)
 {
@@ -365,6 +402,27 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     a.n = (int)(matW->rows / matR->cols);
     a.d = (int)matW->cols;
     a.transposed = opW == ACL_SPARSE_OP_TRANSPOSE;
+    if (RowsAligned(matX) && RowsAligned(matW)) {
+        MmaArgs t = TensorArgsOf(a, matR);
+        t.colsMost = TileColumns(matR->nnz, matR->cols);
+        t.rowsB = (int)matX->rows;
+        CUtensorMap mapW, mapX;
+        if (!MapOf(&mapW, matW->valueType, matW->values, a.d, a.n, matW->ld, (int)matR->cols, a.transposed ? kMmaRows : kMmaDepth) ||
+            !MapOf(&mapX, matX->valueType, matX->values, matX->cols, matX->rows, matX->ld, 0, 1))
+            return ACL_SPARSE_STATUS_INTERNAL_ERROR;
+        const cudaError_t e = WithType(matX->valueType, [&](auto in) {
+            return WithType(matY->valueType, [&](auto out) {
+                using T = decltype(in);
+                using Out = decltype(out);
+                if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
+                    return a.transposed ? LaunchTensor<T, Out, Mode::kProductT>(t, mapW, mapX, handle->stream)
+                                        : LaunchTensor<T, Out, Mode::kProductN>(t, mapW, mapX, handle->stream);
+                else
+                    return cudaErrorInvalidValue;  // refused above
+            });
+        });
+        return Finished(e, "b200spExpertsMM");
+    }
     const dim3 grid((unsigned)((matY->cols + kTile - 1) / kTile), (unsigned)((a.nnz + kTile - 1) / kTile + a.experts + 1));
     b200sp_note_launches(1);
     WithType(matX->valueType, [&](auto in) {
@@ -406,6 +464,27 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     a.ldo = dW->ld;
     a.n = (int)(dW->rows / matR->cols);
     a.d = (int)dW->cols;
+    if (RowsAligned(matX) && RowsAligned(dY)) {
+        MmaArgs t = TensorArgsOf(a, matR);
+        t.colsMost = kMmaColsMost;
+        t.rowsA = (int)dY->rows;
+        t.rowsB = (int)matX->rows;
+        CUtensorMap mapY, mapX;
+        if (!MapOf(&mapY, dY->valueType, dY->values, a.n, dY->rows, dY->ld, 0, 1) ||
+            !MapOf(&mapX, matX->valueType, matX->values, a.d, matX->rows, matX->ld, 0, 1))
+            return ACL_SPARSE_STATUS_INTERNAL_ERROR;
+        const cudaError_t e = WithType(matX->valueType, [&](auto in) {
+            return WithType(dW->valueType, [&](auto out) {
+                using T = decltype(in);
+                using Out = decltype(out);
+                if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
+                    return LaunchTensor<T, Out, Mode::kGrad>(t, mapY, mapX, handle->stream);
+                else
+                    return cudaErrorInvalidValue;  // refused above
+            });
+        });
+        return Finished(e, "b200spExpertsGrad");
+    }
     const dim3 grid((unsigned)((a.d + kTile - 1) / kTile), (unsigned)((a.n + kTile - 1) / kTile), (unsigned)a.experts);
     b200sp_note_launches(1);
     WithType(matX->valueType, [&](auto in) {

@@ -674,3 +674,36 @@ def test_scalars_on_the_device(pkg, handle):
     api.embedding(handle, mat(api, table), api.DnVec(tokens), mat(api, out), None, None)
     assert torch.equal(out, table[tokens])
     handle.set_pointer_mode_device(False)
+
+
+def test_experts_wait_that_runs_out(pkg, handle):
+    """Every barrier expects 16 bytes that nobody sends, and the limit is short: the product ends, says so, and the next works."""
+    import ctypes
+    from ops_sparse_b200 import api
+    L = pkg.lib()
+    L.b200sp_experts_wait_test.argtypes, L.b200sp_experts_wait_test.restype = [ctypes.c_longlong, ctypes.c_uint], None
+    g = gen(4)
+    offsets, columns = ragged(g, 50, 4, 2, wild=0)
+    nnz = len(columns)
+    x, w = matrix(g, 50, 64, "bf16")[0], matrix(g, 4 * 128, 64, "bf16")[0]
+    y, dw = torch.full((nnz, 128), 5.0, dtype=torch.bfloat16, device="cuda"), torch.full((512, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+    R = api.CsrMatrix(offsets, columns, torch.empty(nnz, device="cuda"), 50, 4)
+    X, W, Y, DW = mat(api, x), mat(api, w), mat(api, y), mat(api, dw)
+    buffer = torch.empty(max(api.experts_buffer_size(handle, R, X, W, Y), api.experts_grad_buffer_size(handle, R, Y, X, DW)), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    torch.cuda.synchronize()
+    assert L.b200sp_experts_error() == 0
+    for call, out in ((lambda: api.experts_mm(handle, R, X, W, Y, buffer=buffer), y), (lambda: api.experts_grad(handle, R, Y, X, DW, buffer=buffer), dw)):
+        try:
+            L.b200sp_experts_wait_test(2_000_000, 16)
+            call()
+            torch.cuda.synchronize()
+        finally:
+            L.b200sp_experts_wait_test(0, 0)
+        assert L.b200sp_experts_error() == 1 and L.b200sp_experts_error_clear() == 0
+        assert (out == 5).all()
+    api.experts_mm(handle, R, X, W, Y, buffer=buffer)
+    torch.cuda.synchronize()
+    assert L.b200sp_experts_error() == 0
+    want, size = ref.experts_mm(offsets, columns, x, w.view(4, 128, 64), 4, True, False, 1.0, 0.0, y)
+    ref.close(y, want, ref.rounding(y.dtype, want) + size * 68 * 2 * F32)
