@@ -292,6 +292,10 @@ MmaArgs TensorArgsOf(const ProductArgs &a, const aclsparseSpMatDescr *R)
     t.entries = a.entries;
     t.rows = a.rows;
     t.out = a.out;
+    t.dy = a.dy;
+    t.x = a.x;
+    t.ldy = a.ldy;
+    t.ldx = a.ldx;
     t.ldo = a.ldo;
     t.experts = (int)R->cols;
     t.n = a.n;
@@ -405,18 +409,17 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     if (RowsAligned(matX) && RowsAligned(matW)) {
         MmaArgs t = TensorArgsOf(a, matR);
         t.colsMost = TileColumns(matR->nnz, matR->cols);
-        t.rowsB = (int)matX->rows;
-        CUtensorMap mapW, mapX;
-        if (!MapOf(&mapW, matW->valueType, matW->values, a.d, a.n, matW->ld, (int)matR->cols, a.transposed ? kMmaRows : kMmaDepth) ||
-            !MapOf(&mapX, matX->valueType, matX->values, matX->cols, matX->rows, matX->ld, 0, 1))
+        t.pairs = matY->ld % 2 == 0 && reinterpret_cast<uintptr_t>(matY->values) % 4 == 0;
+        CUtensorMap mapW;
+        if (!MapOf(&mapW, matW->valueType, matW->values, a.d, a.n, matW->ld, (int)matR->cols, a.transposed ? kMmaRows : kMmaDepth))
             return ACL_SPARSE_STATUS_INTERNAL_ERROR;
         const cudaError_t e = WithType(matX->valueType, [&](auto in) {
             return WithType(matY->valueType, [&](auto out) {
                 using T = decltype(in);
                 using Out = decltype(out);
                 if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
-                    return a.transposed ? LaunchTensor<T, Out, Mode::kProductT>(t, mapW, mapX, handle->stream)
-                                        : LaunchTensor<T, Out, Mode::kProductN>(t, mapW, mapX, handle->stream);
+                    return a.transposed ? LaunchTensor<T, Out, Mode::kProductT>(t, mapW, handle->stream)
+                                        : LaunchTensor<T, Out, Mode::kProductN>(t, mapW, handle->stream);
                 else
                     return cudaErrorInvalidValue;  // refused above
             });
@@ -467,18 +470,14 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     if (RowsAligned(matX) && RowsAligned(dY)) {
         MmaArgs t = TensorArgsOf(a, matR);
         t.colsMost = kMmaColsMost;
-        t.rowsA = (int)dY->rows;
-        t.rowsB = (int)matX->rows;
-        CUtensorMap mapY, mapX;
-        if (!MapOf(&mapY, dY->valueType, dY->values, a.n, dY->rows, dY->ld, 0, 1) ||
-            !MapOf(&mapX, matX->valueType, matX->values, a.d, matX->rows, matX->ld, 0, 1))
-            return ACL_SPARSE_STATUS_INTERNAL_ERROR;
+        t.pairs = RowsAligned(dW);
+        const CUtensorMap none{};
         const cudaError_t e = WithType(matX->valueType, [&](auto in) {
             return WithType(dW->valueType, [&](auto out) {
                 using T = decltype(in);
                 using Out = decltype(out);
                 if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
-                    return LaunchTensor<T, Out, Mode::kGrad>(t, mapY, mapX, handle->stream);
+                    return LaunchTensor<T, Out, Mode::kGrad>(t, none, handle->stream);
                 else
                     return cudaErrorInvalidValue;  // refused above
             });

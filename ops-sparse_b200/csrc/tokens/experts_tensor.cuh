@@ -5,10 +5,10 @@
 // at full width; the accumulator's lanes are then columns of Y, and a store is 32 of them for one entry.
 // The gradient's tile is 128 rows of dW by up to 256 of its columns, summed over the expert's entries.
 //
-// One CTA per SM walks over the tiles of all experts.  One warp requests: W by tiles, rows of X (and dY) by
-// tile::gather4, four rows of 128 bytes that may lie anywhere, so that nothing is laid out in between; a row
-// past the tile's last is asked for past the matrix's end and arrives as zeros.  One thread starts the products, four warps
-// empty the accumulators, of which there are two: the next tile is summed meanwhile.
+// One CTA per SM walks over the tiles of all experts.  One thread requests W by TMA; eight warps gather the rows of X (and
+// dY), which may lie anywhere, by cp.async, so that nothing is laid out in between; one thread starts the products, four warps
+// empty the accumulators, of which there are two: the next tile is summed meanwhile.  (Rows by TMA, tile::gather4, come at one
+// row of 128 bytes in 18 clocks and SM: 8192 tokens, four of 32 experts, 2048 x 2048: 1250 us.)
 // Operands arrive in rows of 128 bytes, swizzled: K-major where those run along the sum (X; W with opW = T), MN-major
 // where they run along the tile (W with opW = N; both of the gradient's).
 //
@@ -26,7 +26,9 @@ constexpr int kMmaABytes = kMmaRows * kMmaDepth * 2;
 constexpr int kMmaBlockBytes = kMmaDepth * 128;    // MN-major: 64 rows along the sum, 64 elements along the tile
 constexpr int kMmaShared = 208 << 10;              // for stages
 constexpr int kMmaStagesMost = 12;
-constexpr int kMmaThreads = 192;                   // warp 0 requests, 1 multiplies, 2 ... 5 store
+constexpr int kMmaGatherWarps = 8, kMmaGatherThreads = 32 * kMmaGatherWarps;
+constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
+constexpr int kMmaThreads = 32 * kMmaFirstGather + kMmaGatherThreads;
 constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
 
 enum class Mode { kProductT, kProductN, kGrad };
@@ -37,12 +39,14 @@ struct MmaArgs {
     long long ldo;
     int experts, n, d;
     int byEntry;
-    int rowsA, rowsB;      // rows of what is gathered: dY, X.  One more is past the end
+    const void *dy, *x;
+    long long ldy, ldx;
+    int pairs;             // rows of a 16-bit output start on 4 bytes, or (kGrad) rows of any on 16
     int colsMost;          // of a tile
     int stages, stageBytes;
     Scalars sc;
     long long waitCycles;
-    unsigned extraTx;      // bytes expected on every barrier beyond those copied (0 outside the wait test)
+    unsigned extraTx;      // 0 outside the wait test: bytes that W's barrier expects beyond those copied; gathering threads do not arrive
 };
 
 __device__ int gExpertsError = 0;
@@ -77,6 +81,11 @@ __device__ __forceinline__ bool BarWait(uint64_t *bar, uint32_t parity, long lon
         if (clock64() - t0 > limit) return false;
     return true;
 }
+// Arrives when all plain copies of this thread so far have landed.
+__device__ __forceinline__ void BarArriveCopies(uint64_t *bar)
+{
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(Shared(bar)) : "memory");
+}
 // By a whole warp: all of its lanes go on, or none.
 __device__ __forceinline__ bool BarWaitWarp(uint64_t *bar, uint32_t parity, long long limit)
 {
@@ -88,12 +97,10 @@ __device__ __forceinline__ void CopyTile3(uint32_t dst, const CUtensorMap *map, 
                  "l"(map), "r"(x), "r"(y), "r"(z), "r"(Shared(bar))
                  : "memory");
 }
-__device__ __forceinline__ void CopyRows4(uint32_t dst, const CUtensorMap *map, int x, const int (&row)[4], uint64_t *bar)
+// 16 bytes of a row, of which the first `bytes` exist and the others arrive as zeros.
+__device__ __forceinline__ void CopyPiece(uint32_t dst, const void *src, int bytes)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, %6}], [%7];" ::"r"(
-                     dst),
-                 "l"(map), "r"(x), "r"(row[0]), "r"(row[1]), "r"(row[2]), "r"(row[3]), "r"(Shared(bar))
-                 : "memory");
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // Shared-memory operands.  K-major: rows of 128 bytes along the sum, eight of them 1024 bytes.  MN-major: rows of 64 elements along the
 // tile, eight along the sum 1024 bytes, the next 64 elements a block further.
@@ -112,17 +119,35 @@ __device__ __forceinline__ void MmaCommit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(Shared(bar)) : "memory");
 }
-__device__ __forceinline__ void LoadColumns16(uint32_t at, float (&v)[16])
+__device__ __forceinline__ void LoadColumns32(uint32_t at, float (&v)[32])
 {
-    uint32_t r[16];
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-                   "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(at));
+    uint32_t r[32];
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
+        "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]),
+          "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]),
+          "=r"(r[31])
+        : "r"(at));
     asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 #pragma unroll
-    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
+
+// The stages in turn, and the parity that a wait for one is for.
+struct Ring {
+    int stage = 0, round = 0;
+    __device__ __forceinline__ void Next(int stages)
+    {
+        if (++stage == stages) {
+            stage = 0;
+            ++round;
+        }
+    }
+    __device__ __forceinline__ uint32_t Filled() const { return (uint32_t)round & 1u; }
+    __device__ __forceinline__ uint32_t Emptied() const { return (uint32_t)(round - 1) & 1u; }  // not in the first round
+};
 
 // What a tile is: columns [f0, f0 + 128) of Y for entries [first, first + many) of the expert, or rows [f0, ...) and columns
 // [first, first + many) of its gradient.
@@ -170,8 +195,7 @@ template <Mode kMode> struct Tiles {
 };
 
 template <typename T, typename Out, Mode kMode>
-__global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaArgs a, const __grid_constant__ CUtensorMap mapA,
-                                                                      const __grid_constant__ CUtensorMap mapB)
+__global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaArgs a, const __grid_constant__ CUtensorMap mapW)
 {
     extern __shared__ unsigned char sRaw[];
     __shared__ uint64_t sFull[kMmaStagesMost], sEmpty[kMmaStagesMost], sDone[2], sFree[2], sLast;
@@ -185,7 +209,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            BarInit(sFull + s, 1);
+            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaGatherThreads);
             BarInit(sEmpty + s, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -221,82 +245,121 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     const int all = sStart[groups];
     bool failed = false;
 
-    if (warp == 0) {
-        int asked = 0;  // stages
-        // a stage that is free, or false
-        auto stage = [&](uint32_t bytes) {
-            const int s = asked % a.stages, use = asked / a.stages;
-            if (use > 0 && !BarWaitWarp(sEmpty + s, (uint32_t)(use - 1) & 1u, a.waitCycles)) return false;
-            if (lane == 0) BarExpect(sFull + s, bytes + a.extraTx);
-            __syncwarp();
-            ++asked;
-            return true;
+    if (kMode != Mode::kGrad && tid == 0) {
+        Ring ring;
+        for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
+            const MmaTile m = tiles.At(t);
+            for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
+                uint64_t *const full = sFull + ring.stage;
+                if (ring.round > 0 && !BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles)) {
+                    failed = true;
+                    break;
+                }
+                BarExpect(full, kMmaABytes + a.extraTx);
+                const uint32_t at = base + ring.stage * a.stageBytes;
+                if (kMode == Mode::kProductT) {
+                    CopyTile3(at, &mapW, k * kMmaDepth, m.f0, m.expert, full);
+                } else {
+                    CopyTile3(at, &mapW, m.f0, k * kMmaDepth, m.expert, full);
+                    CopyTile3(at + kMmaBlockBytes, &mapW, m.f0 + 64, k * kMmaDepth, m.expert, full);
+                }
+            }
+        }
+        if (failed)  // copies on their way: a bounded chance to land
+            for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
+                if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
+    } else if (warp >= kMmaFirstGather) {
+        // Eight threads side by side on 128 bytes of a row: thread t has piece t % 8 of rows t / 8, t / 8 + 32, ...
+        const int thread = tid - 32 * kMmaFirstGather, piece = thread & 7, first = thread >> 3;
+        const uint32_t place = base + first * 128 + ((piece ^ (first & 7)) << 4);  // 32 rows further the swizzle is the same
+        Ring ring;
+        auto free = [&]() { return ring.round == 0 || BarWaitWarp(sEmpty + ring.stage, ring.Emptied(), a.waitCycles); };
+        auto asked = [&]() {
+            if (a.extraTx == 0) BarArriveCopies(sFull + ring.stage);
+            ring.Next(a.stages);
         };
         for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
             const MmaTile m = tiles.At(t);
             if constexpr (kMode != Mode::kGrad) {
-                const int gathers = (m.many + 15) / 16 * 4;
-                int row[2][4];
+                constexpr int kRows = kMmaColsMost / 32;
+                const int depth = kMode == Mode::kProductT ? a.d : a.n, high = (m.many + 15) / 16 * 16;
+                const T *from[kRows];
+                int live = 0;  // bit i: row i exists
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = 4 * (lane + 32 * h) + i;
-                        row[h][i] = at < m.many ? __ldg((a.byEntry ? a.entries : a.rows) + m.first + at) : a.rowsB;
+                for (int i = 0; i < kRows; ++i) {
+                    const int r = first + 32 * i;
+                    from[i] = static_cast<const T *>(a.x);
+                    if (m.steps > 0 && r < m.many) {
+                        live |= 1 << i;
+                        from[i] += (long long)__ldg((a.byEntry ? a.entries : a.rows) + m.first + r) * a.ldx + 8 * piece;
                     }
+                }
                 for (int k = 0; k < m.steps; ++k) {
-                    const int s = asked % a.stages;
-                    if (!stage(kMmaABytes + gathers * 512)) {
+                    const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes;
+                    if (!free()) {
                         failed = true;
                         break;
                     }
-                    const uint32_t at = base + s * a.stageBytes;
-                    if (kMode == Mode::kProductT) {
-                        if (lane == 0) CopyTile3(at, &mapA, k * kMmaDepth, m.f0, m.expert, sFull + s);
-                    } else if (lane < 2) {
-                        CopyTile3(at + lane * kMmaBlockBytes, &mapA, m.f0 + 64 * lane, k * kMmaDepth, m.expert, sFull + s);
-                    }
+                    const int left = min(16, 2 * (depth - k * kMmaDepth - 8 * piece));  // bytes of the piece, if there are any
 #pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        if (lane + 32 * h < gathers)
-                            CopyRows4(at + kMmaABytes + (lane + 32 * h) * 512, &mapB, k * kMmaDepth, row[h], sFull + s);
+                    for (int i = 0; i < kRows; ++i) {
+                        if (first + 32 * i >= high) break;
+                        const bool some = (live >> i & 1) && left > 0;
+                        CopyPiece(at + i * 4096, some ? from[i] + k * kMmaDepth : a.x, some ? left : 0);
+                    }
+                    asked();
                 }
             } else {
-                const int from = __ldg(a.offsets + m.expert), to = __ldg(a.offsets + m.expert + 1);
-                const int blocks = (m.many + 63) / 64, mine = lane % 16, half = lane / 16;
-                int rowA[4], rowB[4];
-                auto rows = [&](int k) {  // of the lane's four entries of a step
+                const int lo = __ldg(a.offsets + m.expert), hi = __ldg(a.offsets + m.expert + 1);
+                const int blocks = (m.many + 63) / 64;
+                long long rowY[2], rowX[2];
+                auto rows = [&](int k) {  // of the thread's two entries of a step; -1: none
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int at = from + k * kMmaDepth + 4 * mine + i;
-                        rowA[i] = at < to ? __ldg(a.entries + at) : a.rowsA;
-                        rowB[i] = at < to ? (a.byEntry ? rowA[i] : __ldg(a.rows + at)) : a.rowsB;
+                    for (int i = 0; i < 2; ++i) {
+                        const int at = lo + k * kMmaDepth + first + 32 * i;
+                        rowY[i] = at < hi ? __ldg(a.entries + at) : -1;
+                        rowX[i] = at < hi ? (a.byEntry ? rowY[i] : __ldg(a.rows + at)) : -1;
                     }
                 };
                 if (m.steps > 0) rows(0);
                 for (int k = 0; k < m.steps; ++k) {
-                    const int s = asked % a.stages;
-                    if (!stage(kMmaABytes + blocks * kMmaBlockBytes)) {
+                    const uint32_t at = place + ring.stage * a.stageBytes;
+                    if (!free()) {
                         failed = true;
                         break;
                     }
-                    const uint32_t at = base + s * a.stageBytes + mine * 512;
-                    CopyRows4(at + half * kMmaBlockBytes, &mapA, m.f0 + 64 * half, rowA, sFull + s);
-                    for (int b = half; b < blocks; b += 2)
-                        CopyRows4(at + kMmaABytes + b * kMmaBlockBytes, &mapB, m.first + 64 * b, rowB, sFull + s);
+#pragma unroll
+                    for (int b = 0; b < kMmaRows / 64; ++b) {
+                        const int col = m.f0 + 64 * b + 8 * piece, left = min(16, 2 * (a.n - col));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const bool some = rowY[i] >= 0 && left > 0;
+                            CopyPiece(at + b * kMmaBlockBytes + i * 4096, some ? static_cast<const T *>(a.dy) + rowY[i] * a.ldy + col : a.dy, some ? left : 0);
+                        }
+                    }
+#pragma unroll
+                    for (int b = 0; b < kMmaColsMost / 64; ++b) {
+                        if (b >= blocks) break;
+                        const int col = m.first + 64 * b + 8 * piece, left = min(16, 2 * (a.d - col));
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const bool some = rowX[i] >= 0 && left > 0;
+                            CopyPiece(at + kMmaABytes + b * kMmaBlockBytes + i * 4096, some ? static_cast<const T *>(a.x) + rowX[i] * a.ldx + col : a.x,
+                                      some ? left : 0);
+                        }
+                    }
                     if (k + 1 < m.steps) rows(k + 1);
+                    asked();
                 }
             }
         }
-        // copies on their way after a failure: a bounded chance to land
-        if (failed && lane == 0)
-            for (int i = asked > a.stages ? asked - a.stages : 0; i < asked; ++i)
-                (void)BarWait(sFull + i % a.stages, (uint32_t)(i / a.stages) & 1u, a.waitCycles);
+        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (tid == 32) {
         constexpr bool kAcrossA = kMode != Mode::kProductT, kAcrossB = kMode == Mode::kGrad;
         const uint32_t type = sizeof(T) == 2 && std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
         const uint32_t instr = 1u << 4 | type << 7 | type << 10 | (uint32_t)kAcrossA << 15 | (uint32_t)kAcrossB << 16 | (uint32_t)(kMmaRows >> 4) << 24;
-        int used = 0, tile = 0;
+        Ring ring;
+        int tile = 0;
         for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
             const MmaTile m = tiles.At(t);
             if (m.steps == 0) continue;
@@ -307,12 +370,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t shape = instr | (uint32_t)((m.many + 15) / 16 * 16 >> 3) << 17, to = tmem + acc * kMmaColsMost;
-            for (int k = 0; k < m.steps; ++k, ++used) {
-                const int s = used % a.stages;
-                if (!BarWait(sFull + s, (uint32_t)(used / a.stages) & 1u, a.waitCycles)) {
+            for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
+                const int s = ring.stage;
+                if (!BarWait(sFull + s, ring.Filled(), a.waitCycles)) {
                     failed = true;
                     break;
                 }
+                // What plain copies have written is read by the tensor cores from here on.
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 const uint32_t at = base + s * a.stageBytes;
 #pragma unroll
                 for (int i = 0; i < kMmaDepth / 16; ++i)
@@ -343,34 +408,67 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             }
             const int f = m.f0 + quarter * 32 + lane;
             const uint32_t from = tmem + ((uint32_t)quarter << 21) + acc * kMmaColsMost;
-            for (int c0 = 0; c0 < m.many; c0 += 16) {
-                float v[16] = {};
-                if (m.steps > 0) LoadColumns16(from + c0, v);
-                if (m.steps > 0 && c0 + 16 >= m.many) {  // all that this warp reads of the accumulator
+            for (int c0 = 0; c0 < m.many; c0 += 32) {
+                int entry = 0;
+                if (kMode != Mode::kGrad && c0 + lane < m.many) entry = __ldg(a.entries + m.first + c0 + lane);
+                float v[32] = {};
+                if (m.steps > 0) LoadColumns32(from + c0, v);
+                if (m.steps > 0 && c0 + 32 >= m.many) {  // all that this warp reads of the accumulator
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
                     if (lane == 0) BarArrive(sFree + acc);
                 }
+                const float by = m.steps > 0 ? alpha : 0.0f;
                 if constexpr (kMode != Mode::kGrad) {
-                    const int entry = c0 + (lane & 15) < m.many ? __ldg(a.entries + m.first + c0 + (lane & 15)) : 0;
+                    Out *const out = static_cast<Out *>(a.out) + f;
+                    if (sizeof(Out) == 2 && a.pairs && beta == 0.0f) {
+                        // Neighbouring lanes exchange, so that each stores two columns for every other entry.
+                        const bool odd = lane & 1;
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        const long long row = __shfl_sync(0xffffffffu, entry, i);
-                        if (c0 + i >= m.many || f >= features) continue;
-                        Out *const to = static_cast<Out *>(a.out) + row * a.ldo + f;
-                        float u = alpha * v[i];
-                        if (m.steps == 0) u = 0.0f;
-                        if (beta != 0.0f) u = fmaf(beta, ToFloat(*to), u);
-                        *to = FromFloat<Out>(u);
+                        for (int i = 0; i < 32; i += 2) {
+                            const float mine = by * v[i], next = by * v[i + 1];
+                            const float got = __shfl_xor_sync(0xffffffffu, odd ? mine : next, 1);
+                            const long long row0 = __shfl_sync(0xffffffffu, entry, i), row1 = __shfl_sync(0xffffffffu, entry, i + 1);
+                            const int c = c0 + i + odd;
+                            if ((f | 1) < features) {
+                                if (c < m.many) {
+                                    Out two[2] = {FromFloat<Out>(odd ? got : mine), FromFloat<Out>(odd ? next : got)};
+                                    *reinterpret_cast<uint32_t *>(out + (odd ? row1 : row0) * a.ldo - odd) = *reinterpret_cast<const uint32_t *>(two);
+                                }
+                            } else if (f < features) {  // the last column, alone
+                                if (c0 + i < m.many) out[row0 * a.ldo] = FromFloat<Out>(mine);
+                                if (c0 + i + 1 < m.many) out[row1 * a.ldo] = FromFloat<Out>(next);
+                            }
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            const long long row = __shfl_sync(0xffffffffu, entry, i);
+                            if (c0 + i >= m.many || f >= features) continue;
+                            Out *const to = out + row * a.ldo;
+                            float u = by * v[i];
+                            if (beta != 0.0f) u = fmaf(beta, ToFloat(*to), u);
+                            *to = FromFloat<Out>(u);
+                        }
                     }
                 } else if (f < features) {
                     Out *const to = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f) * a.ldo + m.first + c0;
+                    constexpr int kN = 16 / (int)sizeof(Out);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) {
-                        if (c0 + i >= m.many) continue;
-                        float u = m.steps == 0 ? 0.0f : alpha * v[i];
-                        if (beta != 0.0f) u = fmaf(beta, ToFloat(to[i]), u);
-                        to[i] = FromFloat<Out>(u);
+                    for (int i = 0; i < 32; i += kN) {
+                        float u[kN];
+#pragma unroll
+                        for (int j = 0; j < kN; ++j) {
+                            u[j] = by * v[i + j];
+                            if (beta != 0.0f && c0 + i + j < m.many) u[j] = fmaf(beta, ToFloat(to[i + j]), u[j]);
+                        }
+                        if (a.pairs && c0 + i + kN <= m.many) {
+                            StoreFloats<Out, kN, true>(to + i, u);
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < kN; ++j)
+                                if (c0 + i + j < m.many) to[i + j] = FromFloat<Out>(u[j]);
+                        }
                     }
                 }
             }
@@ -399,7 +497,7 @@ inline EncodeTiled Encoder()
     return encode;
 }
 
-// Rows of 64 elements of a matrix, swizzled: four anywhere (gather), or `high` neighbours of one of `deep` stacked matrices.
+// Of stacked matrices, `high` rows of 64 elements of one, swizzled.
 inline bool MapOf(CUtensorMap *map, aclDataType type, const void *at, long long cols, long long rows, long long ld, int deep, int high)
 {
     const EncodeTiled encode = Encoder();
@@ -407,7 +505,7 @@ inline bool MapOf(CUtensorMap *map, aclDataType type, const void *at, long long 
     const cuuint64_t size[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)deep};
     const cuuint64_t strides[2] = {(cuuint64_t)(ld * 2), (cuuint64_t)(ld * 2 * rows)};
     const cuuint32_t box[3] = {64, (cuuint32_t)high, 1}, step[3] = {1, 1, 1};
-    return encode(map, type == ACL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, deep > 0 ? 3 : 2,
+    return encode(map, type == ACL_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3,
                   const_cast<void *>(at), size, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
@@ -426,7 +524,7 @@ long long gExpertsWaitCycles = kMmaWaitCycles;
 unsigned gExpertsExtraTx = 0;
 
 template <typename T, typename Out, Mode kMode>
-cudaError_t LaunchTensor(MmaArgs a, const CUtensorMap &mapA, const CUtensorMap &mapB, cudaStream_t stream)
+cudaError_t LaunchTensor(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
 {
     a.stageBytes = kMmaABytes + a.colsMost * 128;
     a.stages = std::min(kMmaShared / a.stageBytes, kMmaStagesMost);
@@ -436,5 +534,5 @@ cudaError_t LaunchTensor(MmaArgs a, const CUtensorMap &mapA, const CUtensorMap &
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmaShared + 1024);
     if (e != cudaSuccess) return e;
     b200sp_note_launches(1);
-    return b200sp::LaunchChained(kernel, (unsigned)b200sp_sm_count(), kMmaThreads, (size_t)(a.stages * a.stageBytes + 1024), stream, a, mapA, mapB);
+    return b200sp::LaunchChained(kernel, (unsigned)b200sp_sm_count(), kMmaThreads, (size_t)(a.stages * a.stageBytes + 1024), stream, a, mapW);
 }
