@@ -409,7 +409,7 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     if (RowsAligned(matX) && RowsAligned(matW)) {
         MmaArgs t = TensorArgsOf(a, matR);
         t.colsMost = TileColumns(matR->nnz, matR->cols);
-        t.pairs = matY->ld % 2 == 0 && reinterpret_cast<uintptr_t>(matY->values) % 4 == 0;
+        t.vectors = RowsAligned(matY);
         CUtensorMap mapW;
         if (!MapOf(&mapW, matW->valueType, matW->values, a.d, a.n, matW->ld, (int)matR->cols, a.transposed ? kMmaRows : kMmaDepth))
             return ACL_SPARSE_STATUS_INTERNAL_ERROR;
@@ -470,7 +470,7 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     if (RowsAligned(matX) && RowsAligned(dY)) {
         MmaArgs t = TensorArgsOf(a, matR);
         t.colsMost = kMmaColsMost;
-        t.pairs = RowsAligned(dW);
+        t.vectors = RowsAligned(dW);
         const CUtensorMap none{};
         const cudaError_t e = WithType(matX->valueType, [&](auto in) {
             return WithType(dW->valueType, [&](auto out) {

@@ -24,8 +24,9 @@ constexpr int kMmaDepth = 64;                      // of a stage: 128 bytes
 constexpr int kMmaColsMost = 256;                  // of a tile: an accumulator's columns
 constexpr int kMmaABytes = kMmaRows * kMmaDepth * 2;
 constexpr int kMmaBlockBytes = kMmaDepth * 128;    // MN-major: 64 rows along the sum, 64 elements along the tile
-constexpr int kMmaShared = 208 << 10;              // for stages
+constexpr int kMmaShared = 192 << 10;              // for stages
 constexpr int kMmaStagesMost = 12;
+template <typename Out> constexpr int kMmaStoreBytes = 4 * 32 * 32 * (int)sizeof(Out);  // 32 x 32 results of each storing warp
 constexpr int kMmaGatherWarps = 8, kMmaGatherThreads = 32 * kMmaGatherWarps;
 constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
 constexpr int kMmaThreads = 32 * kMmaFirstGather + kMmaGatherThreads;
@@ -41,7 +42,7 @@ struct MmaArgs {
     int byEntry;
     const void *dy, *x;
     long long ldy, ldx;
-    int pairs;             // rows of a 16-bit output start on 4 bytes, or (kGrad) rows of any on 16
+    int vectors;           // rows of the output start on 16 bytes
     int colsMost;          // of a tile
     int stages, stageBytes;
     Scalars sc;
@@ -60,14 +61,21 @@ __device__ __forceinline__ void BarExpect(uint64_t *bar, uint32_t bytes)
 {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(Shared(bar)), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void BarArrive(uint64_t *bar)
+// The barrier in the shared memory of the cluster's first CTA.
+__device__ __forceinline__ uint32_t LeadersBar(uint64_t *bar)
 {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(Shared(bar)) : "memory");
+    uint32_t at;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(Shared(bar)));
+    return at;
+}
+__device__ __forceinline__ void BarArriveAt(uint32_t bar)
+{
+    asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ bool BarTry(uint64_t *bar, uint32_t parity)
 {
     uint32_t ok;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(ok)
                  : "r"(Shared(bar)), "r"(parity)
                  : "memory");
@@ -86,16 +94,25 @@ __device__ __forceinline__ void BarArriveCopies(uint64_t *bar)
 {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(Shared(bar)) : "memory");
 }
-// By a whole warp: all of its lanes go on, or none.
+// By a whole warp, of which one lane asks: all of its lanes go on, or none.
 __device__ __forceinline__ bool BarWaitWarp(uint64_t *bar, uint32_t parity, long long limit)
 {
-    return __all_sync(0xffffffffu, BarWait(bar, parity, limit));
+    bool ok = true;
+    if ((threadIdx.x & 31) == 0) ok = BarWait(bar, parity, limit);
+    return __all_sync(0xffffffffu, ok);
 }
-__device__ __forceinline__ void CopyTile3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint64_t *bar)
+// bar: of this CTA, or with a pair of the first.
+template <bool kPair> __device__ __forceinline__ void CopyTile3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
-                 "l"(map), "r"(x), "r"(y), "r"(z), "r"(Shared(bar))
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+                         dst),
+                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.3d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+                     : "memory");
 }
 // 16 bytes of a row, of which the first `bytes` exist and the others arrive as zeros.
 __device__ __forceinline__ void CopyPiece(uint32_t dst, const void *src, int bytes)
@@ -109,15 +126,26 @@ __device__ __forceinline__ uint64_t OperandAt(uint32_t at, bool alongTile)
     const uint64_t leading = alongTile ? kMmaBlockBytes >> 4 : 1, stride = 1024 >> 4;
     return (uint64_t)((at & 0x3ffff) >> 4) | leading << 16 | stride << 32 | 1ull << 46 | 2ull << 61;
 }
-__device__ __forceinline__ void Mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add)
+template <bool kPair> __device__ __forceinline__ void Mma(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                     : "memory");
 }
-__device__ __forceinline__ void MmaCommit(uint64_t *bar)
+// Arrives, in both CTAs of a pair, when the products so far are complete.
+template <bool kPair> __device__ __forceinline__ void MmaCommit(uint64_t *bar)
 {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(Shared(bar)) : "memory");
+    if constexpr (kPair)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(Shared(bar)),
+                     "h"((uint16_t)3)
+                     : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(Shared(bar)) : "memory");
 }
 __device__ __forceinline__ void LoadColumns32(uint32_t at, float (&v)[32])
 {
@@ -152,13 +180,17 @@ struct Ring {
 // What a tile is: columns [f0, f0 + 128) of Y for entries [first, first + many) of the expert, or rows [f0, ...) and columns
 // [first, first + many) of its gradient.
 struct MmaTile {
-    int expert, f0, first, many, steps;
+    int expert, f0, first, many, wide, steps;  // wide: many, in whole units
 };
 
-template <Mode kMode> struct Tiles {
+template <Mode kMode, bool kPair> struct Tiles {
     const MmaArgs &a;
-    const int *sStart;  // [experts + 2]: the first tile of every expert, and of the group of no expert
+    const int *sStart;   // [experts + 2]: the first tile of every expert, and of the group of no expert
+    const int *sOffset;  // [experts + 2]: their first entries
     int fTiles;
+    static constexpr int kHigh = kPair ? 2 * kMmaRows : kMmaRows;
+    // Products take entries by sixteens, gradients whole blocks of 64 columns, for each CTA of a pair.
+    static constexpr int kUnit = kMode != Mode::kGrad ? 16 : kPair ? 128 : 64;
 
     __device__ __forceinline__ int Groups() const { return kMode == Mode::kGrad ? a.experts : a.experts + 1; }
     __device__ __forceinline__ int Features() const { return kMode == Mode::kProductN ? a.d : a.n; }
@@ -178,56 +210,64 @@ template <Mode kMode> struct Tiles {
         }
         MmaTile m;
         m.expert = lo;
-        const int within = t - sStart[lo], from = __ldg(a.offsets + lo), count = __ldg(a.offsets + lo + 1) - from;
+        const int within = t - sStart[lo], from = sOffset[lo], count = sOffset[lo + 1] - from;
         const int length = kMode == Mode::kGrad ? a.d : count;
         const int across = (length + a.colsMost - 1) / a.colsMost;
-        // kGrad: whole blocks of 64 columns; products: sixteens of entries
-        const int unit = kMode == Mode::kGrad ? 64 : 16;
-        const int per = ((length + across - 1) / across + unit - 1) / unit * unit;
+        const int per = ((length + across - 1) / across + kUnit - 1) / kUnit * kUnit;
         const int c = within % across * per;
-        m.f0 = within / across * kMmaRows;
+        m.f0 = within / across * kHigh;
         m.first = kMode == Mode::kGrad ? c : from + c;
         m.many = min(per, length - c);
+        m.wide = (m.many + kUnit - 1) / kUnit * kUnit;
         if (kMode == Mode::kGrad) m.steps = (count + kMmaDepth - 1) / kMmaDepth;
         else m.steps = lo < a.experts && m.many > 0 ? ((kMode == Mode::kProductT ? a.d : a.n) + kMmaDepth - 1) / kMmaDepth : 0;
         return m;
     }
 };
 
-template <typename T, typename Out, Mode kMode>
+template <typename T, typename Out, Mode kMode, bool kPair>
 __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaArgs a, const __grid_constant__ CUtensorMap mapW)
 {
     extern __shared__ unsigned char sRaw[];
-    __shared__ uint64_t sFull[kMmaStagesMost], sEmpty[kMmaStagesMost], sDone[2], sFree[2], sLast;
+    __shared__ uint64_t sFull[kMmaStagesMost], sEmpty[kMmaStagesMost], sGathered[kMmaStagesMost], sDone[2], sFree[2], sLast;
     __shared__ uint32_t sTmem;
-    __shared__ int sStart[kMaxExperts + 2];
+    __shared__ int sStart[kMaxExperts + 2], sOffset[kMaxExperts + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = kPair ? (int)(blockIdx.x & 1) : 0, first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
     const uint32_t base = (Shared(sRaw) + 1023u) & ~1023u;
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaGatherThreads);
+            // W's request, the gathering threads; of a pair the second CTA's as one
+            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaGatherThreads + kPair);
             BarInit(sEmpty + s, 1);
+            BarInit(sGathered + s, kMmaGatherThreads);
         }
         for (int i = 0; i < 2; ++i) {
             BarInit(sDone + i, 1);
-            BarInit(sFree + i, 4);
+            BarInit(sFree + i, kPair ? 8 : 4);
         }
         BarInit(&sLast, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b200sp::WaitForPrevious();
-    const Tiles<kMode> tiles{a, sStart, ((kMode == Mode::kProductN ? a.d : a.n) + kMmaRows - 1) / kMmaRows};
+    const Tiles<kMode, kPair> tiles{a, sStart, sOffset,
+                                    ((kMode == Mode::kProductN ? a.d : a.n) + Tiles<kMode, kPair>::kHigh - 1) / Tiles<kMode, kPair>::kHigh};
     const int groups = tiles.Groups();
-    for (int e = tid; e < groups; e += kMmaThreads) sStart[e] = tiles.Count(__ldg(a.offsets + e), __ldg(a.offsets + e + 1));
+    for (int e = tid; e <= groups; e += kMmaThreads) sOffset[e] = __ldg(a.offsets + e);
     __syncthreads();
     if (warp == 0) {
         int run = 0;
         for (int e0 = 0; e0 <= groups; e0 += 32) {
-            const int own = e0 + lane < groups ? sStart[e0 + lane] : 0;
+            const int own = e0 + lane < groups ? tiles.Count(sOffset[e0 + lane], sOffset[e0 + lane + 1]) : 0;
             int incl = own;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -240,6 +280,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sTmem;
     const int all = sStart[groups];
@@ -247,53 +288,65 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
 
     if (kMode != Mode::kGrad && tid == 0) {
         Ring ring;
-        for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
+        for (int t = first; t < all && !failed; t += step) {
             const MmaTile m = tiles.At(t);
+            const int f0 = m.f0 + rank * kMmaRows;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
-                uint64_t *const full = sFull + ring.stage;
                 if (ring.round > 0 && !BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles)) {
                     failed = true;
                     break;
                 }
-                BarExpect(full, kMmaABytes + a.extraTx);
-                const uint32_t at = base + ring.stage * a.stageBytes;
+                const uint32_t at = base + ring.stage * a.stageBytes, full = kPair ? LeadersBar(sFull + ring.stage) : Shared(sFull + ring.stage);
+                if (rank == 0) BarExpect(sFull + ring.stage, (kPair ? 2 : 1) * kMmaABytes + a.extraTx);
                 if (kMode == Mode::kProductT) {
-                    CopyTile3(at, &mapW, k * kMmaDepth, m.f0, m.expert, full);
+                    CopyTile3<kPair>(at, &mapW, k * kMmaDepth, f0, m.expert, full);
                 } else {
-                    CopyTile3(at, &mapW, m.f0, k * kMmaDepth, m.expert, full);
-                    CopyTile3(at + kMmaBlockBytes, &mapW, m.f0 + 64, k * kMmaDepth, m.expert, full);
+                    CopyTile3<kPair>(at, &mapW, f0, k * kMmaDepth, m.expert, full);
+                    CopyTile3<kPair>(at + kMmaBlockBytes, &mapW, f0 + 64, k * kMmaDepth, m.expert, full);
                 }
             }
         }
-        if (failed)  // copies on their way: a bounded chance to land
+        if (failed && rank == 0)  // copies on their way: a bounded chance to land
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
     } else if (warp >= kMmaFirstGather) {
         // Eight threads side by side on 128 bytes of a row: thread t has piece t % 8 of rows t / 8, t / 8 + 32, ...
-        const int thread = tid - 32 * kMmaFirstGather, piece = thread & 7, first = thread >> 3;
-        const uint32_t place = base + first * 128 + ((piece ^ (first & 7)) << 4);  // 32 rows further the swizzle is the same
+        const int thread = tid - 32 * kMmaFirstGather, piece = thread & 7, high = thread >> 3;
+        const uint32_t place = base + high * 128 + ((piece ^ (high & 7)) << 4);  // 32 rows further the swizzle is the same
+        uint64_t *const bars = rank == 0 ? sFull : sGathered;
         Ring ring;
         auto free = [&]() { return ring.round == 0 || BarWaitWarp(sEmpty + ring.stage, ring.Emptied(), a.waitCycles); };
         auto asked = [&]() {
-            if (a.extraTx == 0) BarArriveCopies(sFull + ring.stage);
+            if (a.extraTx == 0) BarArriveCopies(bars + ring.stage);
             ring.Next(a.stages);
         };
-        for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
-            const MmaTile m = tiles.At(t);
-            if constexpr (kMode != Mode::kGrad) {
-                constexpr int kRows = kMmaColsMost / 32;
-                const int depth = kMode == Mode::kProductT ? a.d : a.n, high = (m.many + 15) / 16 * 16;
+        if constexpr (kMode != Mode::kGrad) {
+            constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32;
+            const int depth = kMode == Mode::kProductT ? a.d : a.n;
+            const int *const rowOf = a.byEntry ? a.entries : a.rows;
+            int row[kRows];  // of the tile to come; -1: none
+            MmaTile next;
+            auto look = [&](int t) {
+                if (t >= all) return;
+                next = tiles.At(t);
+#pragma unroll
+                for (int i = 0; i < kRows; ++i) {
+                    const int r = rank * (next.wide / 2) + high + 32 * i;
+                    row[i] = next.steps > 0 && r < next.many && high + 32 * i < (kPair ? next.wide / 2 : next.wide) ? __ldg(rowOf + next.first + r) : -1;
+                }
+            };
+            look(first);
+            for (int t = first; t < all && !failed; t += step) {
+                const MmaTile m = next;
+                const int share = kPair ? m.wide / 2 : m.wide;
                 const T *from[kRows];
                 int live = 0;  // bit i: row i exists
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    const int r = first + 32 * i;
-                    from[i] = static_cast<const T *>(a.x);
-                    if (m.steps > 0 && r < m.many) {
-                        live |= 1 << i;
-                        from[i] += (long long)__ldg((a.byEntry ? a.entries : a.rows) + m.first + r) * a.ldx + 8 * piece;
-                    }
+                    live |= (row[i] >= 0) << i;
+                    from[i] = static_cast<const T *>(a.x) + (long long)max(row[i], 0) * a.ldx + 8 * piece;
                 }
+                look(t + step);
                 for (int k = 0; k < m.steps; ++k) {
                     const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes;
                     if (!free()) {
@@ -303,20 +356,23 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     const int left = min(16, 2 * (depth - k * kMmaDepth - 8 * piece));  // bytes of the piece, if there are any
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
-                        if (first + 32 * i >= high) break;
+                        if (high + 32 * i >= share) break;
                         const bool some = (live >> i & 1) && left > 0;
                         CopyPiece(at + i * 4096, some ? from[i] + k * kMmaDepth : a.x, some ? left : 0);
                     }
                     asked();
                 }
-            } else {
-                const int lo = __ldg(a.offsets + m.expert), hi = __ldg(a.offsets + m.expert + 1);
-                const int blocks = (m.many + 63) / 64;
+            }
+        } else {
+            for (int t = first; t < all && !failed; t += step) {
+                const MmaTile m = tiles.At(t);
+                const int lo = sOffset[m.expert], hi = sOffset[m.expert + 1], f0 = m.f0 + rank * kMmaRows;
+                const int share = kPair ? m.wide / 2 : m.wide, c0 = m.first + rank * share, blocks = (share + 63) / 64;
                 long long rowY[2], rowX[2];
                 auto rows = [&](int k) {  // of the thread's two entries of a step; -1: none
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int at = lo + k * kMmaDepth + first + 32 * i;
+                        const int at = lo + k * kMmaDepth + high + 32 * i;
                         rowY[i] = at < hi ? __ldg(a.entries + at) : -1;
                         rowX[i] = at < hi ? (a.byEntry ? rowY[i] : __ldg(a.rows + at)) : -1;
                     }
@@ -330,7 +386,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     }
 #pragma unroll
                     for (int b = 0; b < kMmaRows / 64; ++b) {
-                        const int col = m.f0 + 64 * b + 8 * piece, left = min(16, 2 * (a.n - col));
+                        const int col = f0 + 64 * b + 8 * piece, left = min(16, 2 * (a.n - col));
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const bool some = rowY[i] >= 0 && left > 0;
@@ -338,9 +394,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         }
                     }
 #pragma unroll
-                    for (int b = 0; b < kMmaColsMost / 64; ++b) {
+                    for (int b = 0; b < kMmaColsMost / (kPair ? 2 : 1) / 64; ++b) {
                         if (b >= blocks) break;
-                        const int col = m.first + 64 * b + 8 * piece, left = min(16, 2 * (a.d - col));
+                        const int col = c0 + 64 * b + 8 * piece, left = min(16, 2 * (a.d - col));
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
                             const bool some = rowX[i] >= 0 && left > 0;
@@ -354,13 +410,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             }
         }
         asm volatile("cp.async.wait_all;" ::: "memory");
-    } else if (tid == 32) {
+    } else if (tid == 32 && rank == 0) {
         constexpr bool kAcrossA = kMode != Mode::kProductT, kAcrossB = kMode == Mode::kGrad;
-        const uint32_t type = sizeof(T) == 2 && std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
-        const uint32_t instr = 1u << 4 | type << 7 | type << 10 | (uint32_t)kAcrossA << 15 | (uint32_t)kAcrossB << 16 | (uint32_t)(kMmaRows >> 4) << 24;
+        constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
+        constexpr uint32_t kInstr = 1u << 4 | kType << 7 | kType << 10 | (uint32_t)kAcrossA << 15 | (uint32_t)kAcrossB << 16 |
+                                    (uint32_t)(Tiles<kMode, kPair>::kHigh >> 4) << 24;
         Ring ring;
         int tile = 0;
-        for (int t = blockIdx.x; t < all && !failed; t += gridDim.x) {
+        for (int t = first; t < all && !failed; t += step) {
             const MmaTile m = tiles.At(t);
             if (m.steps == 0) continue;
             const int acc = tile & 1, turn = tile >> 1;
@@ -369,33 +426,47 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            const uint32_t shape = instr | (uint32_t)((m.many + 15) / 16 * 16 >> 3) << 17, to = tmem + acc * kMmaColsMost;
+            const uint32_t shape = kInstr | (uint32_t)(m.wide >> 3) << 17, to = tmem + acc * kMmaColsMost;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
-                const int s = ring.stage;
-                if (!BarWait(sFull + s, ring.Filled(), a.waitCycles)) {
+                if (!BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles)) {
                     failed = true;
                     break;
                 }
                 // What plain copies have written is read by the tensor cores from here on.
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                const uint32_t at = base + s * a.stageBytes;
+                const uint32_t at = base + ring.stage * a.stageBytes;
 #pragma unroll
                 for (int i = 0; i < kMmaDepth / 16; ++i)
-                    Mma(to, OperandAt(at + i * (kAcrossA ? 2048 : 32), kAcrossA), OperandAt(at + kMmaABytes + i * (kAcrossB ? 2048 : 32), kAcrossB),
-                        shape, k > 0 || i > 0);
-                MmaCommit(sEmpty + s);
+                    Mma<kPair>(to, OperandAt(at + i * (kAcrossA ? 2048 : 32), kAcrossA),
+                               OperandAt(at + kMmaABytes + i * (kAcrossB ? 2048 : 32), kAcrossB), shape, k > 0 || i > 0);
+                MmaCommit<kPair>(sEmpty + ring.stage);
             }
-            if (!failed) MmaCommit(sDone + acc);
+            if (!failed) MmaCommit<kPair>(sDone + acc);
             ++tile;
         }
-        MmaCommit(&sLast);  // when every product started here is complete, also after a failure
+        MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
         (void)BarWait(&sLast, 0, a.waitCycles);
-    } else if (warp >= 2) {
+    } else if (kPair && tid == 32) {
+        // The second CTA: what its threads have gathered is told to the first, which starts the products.
+        Ring ring;
+        for (int t = first; t < all && !failed; t += step) {
+            const MmaTile m = tiles.At(t);
+            for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
+                if (!BarWait(sGathered + ring.stage, ring.Filled(), a.waitCycles)) {
+                    failed = true;
+                    break;
+                }
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                BarArriveAt(LeadersBar(sFull + ring.stage));
+            }
+        }
+    } else if (warp >= 2 && warp < kMmaFirstGather) {
         const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
         const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
         const int features = kMode == Mode::kProductN ? a.d : a.n;
+        Out *const sOut = reinterpret_cast<Out *>(sRaw + (base - Shared(sRaw)) + a.stages * a.stageBytes) + quarter * 1024;
         int tile = 0;
-        for (int t = blockIdx.x; t < all; t += gridDim.x) {
+        for (int t = first; t < all; t += step) {
             const MmaTile m = tiles.At(t);
             const int acc = tile & 1, turn = tile >> 1;
             if (m.steps > 0) {
@@ -406,53 +477,51 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 ++tile;
             }
-            const int f = m.f0 + quarter * 32 + lane;
+            const int f0 = m.f0 + rank * kMmaRows + quarter * 32;  // the warp's 32 rows of the tile
+            int entry = 0;
             const uint32_t from = tmem + ((uint32_t)quarter << 21) + acc * kMmaColsMost;
+            if (kMode != Mode::kGrad) entry = lane < m.many ? __ldg(a.entries + m.first + lane) : 0;
             for (int c0 = 0; c0 < m.many; c0 += 32) {
-                int entry = 0;
-                if (kMode != Mode::kGrad && c0 + lane < m.many) entry = __ldg(a.entries + m.first + c0 + lane);
                 float v[32] = {};
                 if (m.steps > 0) LoadColumns32(from + c0, v);
                 if (m.steps > 0 && c0 + 32 >= m.many) {  // all that this warp reads of the accumulator
                     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) BarArrive(sFree + acc);
+                    if (lane == 0) BarArriveAt(LeadersBar(sFree + acc));
                 }
                 const float by = m.steps > 0 ? alpha : 0.0f;
+                const int live = min(32, m.many - c0);
                 if constexpr (kMode != Mode::kGrad) {
-                    Out *const out = static_cast<Out *>(a.out) + f;
-                    if (sizeof(Out) == 2 && a.pairs && beta == 0.0f) {
-                        // Neighbouring lanes exchange, so that each stores two columns for every other entry.
-                        const bool odd = lane & 1;
+                    const int now = entry;
+                    if (c0 + 32 + lane < m.many) entry = __ldg(a.entries + m.first + c0 + 32 + lane);
+                    Out *const out = static_cast<Out *>(a.out);
+                    if (a.vectors && beta == 0.0f && f0 + 32 <= features) {
+                        // Through shared memory, so that 16 bytes of a row are stored at once and a row's 32 columns side by side.
+                        constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
 #pragma unroll
-                        for (int i = 0; i < 32; i += 2) {
-                            const float mine = by * v[i], next = by * v[i + 1];
-                            const float got = __shfl_xor_sync(0xffffffffu, odd ? mine : next, 1);
-                            const long long row0 = __shfl_sync(0xffffffffu, entry, i), row1 = __shfl_sync(0xffffffffu, entry, i + 1);
-                            const int c = c0 + i + odd;
-                            if ((f | 1) < features) {
-                                if (c < m.many) {
-                                    Out two[2] = {FromFloat<Out>(odd ? got : mine), FromFloat<Out>(odd ? next : got)};
-                                    *reinterpret_cast<uint32_t *>(out + (odd ? row1 : row0) * a.ldo - odd) = *reinterpret_cast<const uint32_t *>(two);
-                                }
-                            } else if (f < features) {  // the last column, alone
-                                if (c0 + i < m.many) out[row0 * a.ldo] = FromFloat<Out>(mine);
-                                if (c0 + i + 1 < m.many) out[row1 * a.ldo] = FromFloat<Out>(next);
-                            }
+                        for (int i = 0; i < 32; ++i) sOut[32 * i + lane] = FromFloat<Out>(by * v[i]);
+                        __syncwarp();
+#pragma unroll
+                        for (int i = 0; i < kPieces; ++i) {
+                            const int c = (32 * i + lane) / kPieces, at = lane % kPieces * kN;
+                            const long long row = __shfl_sync(0xffffffffu, now, c);
+                            const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + 32 * c + at);
+                            if (c < live) *reinterpret_cast<uint4 *>(out + row * a.ldo + f0 + at) = piece;
                         }
+                        __syncwarp();
                     } else {
 #pragma unroll
                         for (int i = 0; i < 32; ++i) {
-                            const long long row = __shfl_sync(0xffffffffu, entry, i);
-                            if (c0 + i >= m.many || f >= features) continue;
-                            Out *const to = out + row * a.ldo;
+                            const long long row = __shfl_sync(0xffffffffu, now, i);
+                            if (i >= live || f0 + lane >= features) continue;
+                            Out *const to = out + row * a.ldo + f0 + lane;
                             float u = by * v[i];
                             if (beta != 0.0f) u = fmaf(beta, ToFloat(*to), u);
                             *to = FromFloat<Out>(u);
                         }
                     }
-                } else if (f < features) {
-                    Out *const to = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f) * a.ldo + m.first + c0;
+                } else if (f0 + lane < features) {
+                    Out *const to = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f0 + lane) * a.ldo + m.first + c0;
                     constexpr int kN = 16 / (int)sizeof(Out);
 #pragma unroll
                     for (int i = 0; i < 32; i += kN) {
@@ -460,14 +529,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
 #pragma unroll
                         for (int j = 0; j < kN; ++j) {
                             u[j] = by * v[i + j];
-                            if (beta != 0.0f && c0 + i + j < m.many) u[j] = fmaf(beta, ToFloat(to[i + j]), u[j]);
+                            if (beta != 0.0f && i + j < live) u[j] = fmaf(beta, ToFloat(to[i + j]), u[j]);
                         }
-                        if (a.pairs && c0 + i + kN <= m.many) {
+                        if (a.vectors && i + kN <= live) {
                             StoreFloats<Out, kN, true>(to + i, u);
                         } else {
 #pragma unroll
                             for (int j = 0; j < kN; ++j)
-                                if (c0 + i + j < m.many) to[i + j] = FromFloat<Out>(u[j]);
+                                if (i + j < live) to[i + j] = FromFloat<Out>(u[j]);
                         }
                     }
                 }
@@ -478,7 +547,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     if (failed) atomicExch(&gExpertsError, 1);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.
+    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 0) {
+        if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -523,16 +597,39 @@ inline int TileColumns(long long nnz, long long experts)
 long long gExpertsWaitCycles = kMmaWaitCycles;
 unsigned gExpertsExtraTx = 0;
 
-template <typename T, typename Out, Mode kMode>
-cudaError_t LaunchTensor(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
+template <typename T, typename Out, Mode kMode, bool kPair>
+cudaError_t LaunchTiles(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
 {
-    a.stageBytes = kMmaABytes + a.colsMost * 128;
+    a.stageBytes = kMmaABytes + a.colsMost * 128 / (kPair ? 2 : 1);
     a.stages = std::min(kMmaShared / a.stageBytes, kMmaStagesMost);
     a.waitCycles = gExpertsWaitCycles;
     a.extraTx = gExpertsExtraTx;
-    const auto kernel = ExpertsTensorKernel<T, Out, kMode>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmaShared + 1024);
+    const auto kernel = ExpertsTensorKernel<T, Out, kMode, kPair>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmaShared + kMmaStoreBytes<Out> + 1024);
     if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(b200sp_sm_count() / 2 * 2));
+    cfg.blockDim = dim3(kMmaThreads);
+    cfg.dynamicSmemBytes = (size_t)(a.stages * a.stageBytes + kMmaStoreBytes<Out> + 1024);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = kPair ? 2 : 1;
     b200sp_note_launches(1);
-    return b200sp::LaunchChained(kernel, (unsigned)b200sp_sm_count(), kMmaThreads, (size_t)(a.stages * a.stageBytes + 1024), stream, a, mapW);
+    return cudaLaunchKernelEx(&cfg, kernel, a, mapW);
+}
+
+// A pair of CTAs on a tile of 256 columns reads half as much of X (or of both operands of a gradient) per product.  That counts where there are
+// products enough to be bound by them.
+template <typename T, typename Out, Mode kMode>
+cudaError_t LaunchTensor(const MmaArgs &a, const CUtensorMap &mapW, cudaStream_t stream)
+{
+    const int features = kMode == Mode::kProductN ? a.d : a.n;
+    return a.colsMost >= 128 && features > kMmaRows ? LaunchTiles<T, Out, kMode, true>(a, mapW, stream)
+                                                    : LaunchTiles<T, Out, kMode, false>(a, mapW, stream);
 }
