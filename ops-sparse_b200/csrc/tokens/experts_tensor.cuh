@@ -6,7 +6,7 @@
 // The gradient's tile is 128 rows of dW by up to 256 of its columns, summed over the expert's entries.
 //
 // One CTA per SM walks over the tiles of all experts.  One thread requests W by TMA; eight warps gather the rows of X (and
-// dY), which may lie anywhere, by cp.async, so that nothing is laid out in between; one thread starts the products, four warps
+// dY), which may lie anywhere, by cp.async, a stage each in turn, so that nothing is laid out in between; one thread starts the products, four warps
 // empty the accumulators, of which there are two: the next tile is summed meanwhile.  (Rows by TMA, tile::gather4, come at one
 // row of 128 bytes in 18 clocks and SM: 8192 tokens, four of 32 experts, 2048 x 2048: 1250 us.)
 // Operands arrive in rows of 128 bytes, swizzled: K-major where those run along the sum (X; W with opW = T), MN-major
@@ -27,9 +27,9 @@ constexpr int kMmaBlockBytes = kMmaDepth * 128;    // MN-major: 64 rows along th
 constexpr int kMmaShared = 192 << 10;              // for stages
 constexpr int kMmaStagesMost = 12;
 template <typename Out> constexpr int kMmaStoreBytes = 4 * 32 * 32 * (int)sizeof(Out);  // 32 x 32 results of each storing warp
-constexpr int kMmaGatherWarps = 8, kMmaGatherThreads = 32 * kMmaGatherWarps;
+constexpr int kMmaGatherWarps = 8;
 constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
-constexpr int kMmaThreads = 32 * kMmaFirstGather + kMmaGatherThreads;
+constexpr int kMmaThreads = 32 * (kMmaFirstGather + kMmaGatherWarps);
 constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
 
 enum class Mode { kProductT, kProductN, kGrad };
@@ -88,11 +88,6 @@ __device__ __forceinline__ bool BarWait(uint64_t *bar, uint32_t parity, long lon
     while (!BarTry(bar, parity))
         if (clock64() - t0 > limit) return false;
     return true;
-}
-// Arrives when all plain copies of this thread so far have landed.
-__device__ __forceinline__ void BarArriveCopies(uint64_t *bar)
-{
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(Shared(bar)) : "memory");
 }
 // By a whole warp, of which one lane asks: all of its lanes go on, or none.
 __device__ __forceinline__ bool BarWaitWarp(uint64_t *bar, uint32_t parity, long long limit)
@@ -166,12 +161,10 @@ __device__ __forceinline__ void LoadColumns32(uint32_t at, float (&v)[32])
 // The stages in turn, and the parity that a wait for one is for.
 struct Ring {
     int stage = 0, round = 0;
-    __device__ __forceinline__ void Next(int stages)
+    __device__ __forceinline__ void Next(int stages) { On(1, stages); }
+    __device__ __forceinline__ void On(int by, int stages)
     {
-        if (++stage == stages) {
-            stage = 0;
-            ++round;
-        }
+        for (stage += by; stage >= stages; stage -= stages) ++round;
     }
     __device__ __forceinline__ uint32_t Filled() const { return (uint32_t)round & 1u; }
     __device__ __forceinline__ uint32_t Emptied() const { return (uint32_t)(round - 1) & 1u; }  // not in the first round
@@ -229,7 +222,7 @@ template <typename T, typename Out, Mode kMode, bool kPair>
 __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaArgs a, const __grid_constant__ CUtensorMap mapW)
 {
     extern __shared__ unsigned char sRaw[];
-    __shared__ uint64_t sFull[kMmaStagesMost], sEmpty[kMmaStagesMost], sGathered[kMmaStagesMost], sDone[2], sFree[2], sLast;
+    __shared__ uint64_t sFull[kMmaStagesMost], sEmpty[kMmaStagesMost], sDone[2], sFree[2], sLast;
     __shared__ uint32_t sTmem;
     __shared__ int sStart[kMaxExperts + 2], sOffset[kMaxExperts + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -246,10 +239,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            // W's request, the gathering threads; of a pair the second CTA's as one
-            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaGatherThreads + kPair);
+            BarInit(sFull + s, (kMode != Mode::kGrad) + 1 + kPair);  // W's request, a gathering warp of every CTA
             BarInit(sEmpty + s, 1);
-            BarInit(sGathered + s, kMmaGatherThreads);
         }
         for (int i = 0; i < 2; ++i) {
             BarInit(sDone + i, 1);
@@ -309,107 +300,116 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         if (failed && rank == 0)  // copies on their way: a bounded chance to land
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
-    } else if (warp >= kMmaFirstGather) {
-        // Eight threads side by side on 128 bytes of a row: thread t has piece t % 8 of rows t / 8, t / 8 + 32, ...
-        const int thread = tid - 32 * kMmaFirstGather, piece = thread & 7, high = thread >> 3;
-        const uint32_t place = base + high * 128 + ((piece ^ (high & 7)) << 4);  // 32 rows further the swizzle is the same
-        uint64_t *const bars = rank == 0 ? sFull : sGathered;
+    } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + a.stages) {
+        // Stages are the warps' in turn: one asks for all of its rows, waits for them and says so, while the others are at the stages
+        // beside it.  No more warps than stages: whoever is at stage q knows that q - stages has been used up, so that the wait for
+        // q + warps - stages can not be answered by the round before it.  (All warps at every stage, a share each, take turns with it: with the arrivals of 256 threads, and a
+        // thread that passes them on to the other CTA, a stage's round took 2900 clocks without any copy.)
+        // Eight lanes side by side on 128 bytes of a row: lane l has piece l % 8 of rows l / 8, l / 8 + 4, ...
+        const int mine = warp - kMmaFirstGather, warps = min(kMmaGatherWarps, a.stages), piece = lane & 7, high = lane >> 3;
+        const uint32_t place = base + high * 128;
+        const uint32_t even = (uint32_t)(piece ^ high) << 4, odd = (uint32_t)(piece ^ (high + 4)) << 4;  // swizzled: rows high, high + 4 of eight
         Ring ring;
+        ring.On(mine, a.stages);
         auto free = [&]() { return ring.round == 0 || BarWaitWarp(sEmpty + ring.stage, ring.Emptied(), a.waitCycles); };
         auto asked = [&]() {
-            if (a.extraTx == 0) BarArriveCopies(bars + ring.stage);
-            ring.Next(a.stages);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the tensor cores read it from here on
+            __syncwarp();
+            if (lane == 0 && a.extraTx == 0) BarArriveAt(LeadersBar(sFull + ring.stage));
+            ring.On(warps, a.stages);
         };
+        int turn = mine;  // steps until the next of this warp's stages
         if constexpr (kMode != Mode::kGrad) {
             constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32;
             const int depth = kMode == Mode::kProductT ? a.d : a.n;
             const int *const rowOf = a.byEntry ? a.entries : a.rows;
-            int row[kRows];  // of the tile to come; -1: none
+            const T *const x = static_cast<const T *>(a.x);
+            int row[kRows];  // rows lane, lane + 32, ... of the tile to come; -1: none
             MmaTile next;
             auto look = [&](int t) {
                 if (t >= all) return;
                 next = tiles.At(t);
+                const int share = kPair ? next.wide / 2 : next.wide;
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    const int r = rank * (next.wide / 2) + high + 32 * i;
-                    row[i] = next.steps > 0 && r < next.many && high + 32 * i < (kPair ? next.wide / 2 : next.wide) ? __ldg(rowOf + next.first + r) : -1;
+                    const int r = rank * share + lane + 32 * i;
+                    row[i] = next.steps > 0 && lane + 32 * i < share && r < next.many ? __ldg(rowOf + next.first + r) : -1;
                 }
             };
             look(first);
             for (int t = first; t < all && !failed; t += step) {
                 const MmaTile m = next;
                 const int share = kPair ? m.wide / 2 : m.wide;
-                const T *from[kRows];
-                int live = 0;  // bit i: row i exists
+                int now[kRows];
 #pragma unroll
-                for (int i = 0; i < kRows; ++i) {
-                    live |= (row[i] >= 0) << i;
-                    from[i] = static_cast<const T *>(a.x) + (long long)max(row[i], 0) * a.ldx + 8 * piece;
-                }
+                for (int i = 0; i < kRows; ++i) now[i] = row[i];
                 look(t + step);
-                for (int k = 0; k < m.steps; ++k) {
-                    const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes;
+                for (; turn < m.steps; turn += warps) {
                     if (!free()) {
                         failed = true;
                         break;
                     }
-                    const int left = min(16, 2 * (depth - k * kMmaDepth - 8 * piece));  // bytes of the piece, if there are any
+                    const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes;
+                    const int col = turn * kMmaDepth + 8 * piece, left = max(0, min(16, 2 * (depth - col)));  // bytes of the piece
+                    const T *const from = x + (left > 0 ? col : 0);
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
-                        if (high + 32 * i >= share) break;
-                        const bool some = (live >> i & 1) && left > 0;
-                        CopyPiece(at + i * 4096, some ? from[i] + k * kMmaDepth : a.x, some ? left : 0);
+                        if (32 * i >= share) break;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = __shfl_sync(0xffffffffu, now[i], 4 * j + high);
+                            if (32 * i + 4 * j + high < share)
+                                CopyPiece(at + i * 4096 + j * 512 + (j & 1 ? odd : even), from + (long long)max(r, 0) * a.ldx, r < 0 ? 0 : left);
+                        }
                     }
                     asked();
                 }
+                turn -= m.steps;
             }
         } else {
             for (int t = first; t < all && !failed; t += step) {
                 const MmaTile m = tiles.At(t);
                 const int lo = sOffset[m.expert], hi = sOffset[m.expert + 1], f0 = m.f0 + rank * kMmaRows;
                 const int share = kPair ? m.wide / 2 : m.wide, c0 = m.first + rank * share, blocks = (share + 63) / 64;
-                long long rowY[2], rowX[2];
-                auto rows = [&](int k) {  // of the thread's two entries of a step; -1: none
+                int rowY[2], rowX[2];
+                auto rows = [&](int k) {  // entries lane and lane + 32 of a step; -1: none
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const int at = lo + k * kMmaDepth + high + 32 * i;
+                        const int at = lo + k * kMmaDepth + lane + 32 * i;
                         rowY[i] = at < hi ? __ldg(a.entries + at) : -1;
                         rowX[i] = at < hi ? (a.byEntry ? rowY[i] : __ldg(a.rows + at)) : -1;
                     }
                 };
-                if (m.steps > 0) rows(0);
-                for (int k = 0; k < m.steps; ++k) {
-                    const uint32_t at = place + ring.stage * a.stageBytes;
+                // a block: 64 columns of 64 rows
+                auto block = [&](uint32_t at, const void *matrix, long long ld, int col, int cols, const int (&row)[2]) {
+                    const int left = max(0, min(16, 2 * (cols - col)));
+                    const T *const from = static_cast<const T *>(matrix) + (left > 0 ? col : 0);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) {
+                            const int r = __shfl_sync(0xffffffffu, row[i], 4 * j + high);
+                            CopyPiece(at + i * 4096 + j * 512 + (j & 1 ? odd : even), from + (long long)max(r, 0) * ld, r < 0 ? 0 : left);
+                        }
+                };
+                if (turn < m.steps) rows(turn);
+                for (; turn < m.steps; turn += warps) {
                     if (!free()) {
                         failed = true;
                         break;
                     }
+                    const uint32_t at = place + ring.stage * a.stageBytes;
 #pragma unroll
-                    for (int b = 0; b < kMmaRows / 64; ++b) {
-                        const int col = f0 + 64 * b + 8 * piece, left = min(16, 2 * (a.n - col));
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const bool some = rowY[i] >= 0 && left > 0;
-                            CopyPiece(at + b * kMmaBlockBytes + i * 4096, some ? static_cast<const T *>(a.dy) + rowY[i] * a.ldy + col : a.dy, some ? left : 0);
-                        }
-                    }
-#pragma unroll
-                    for (int b = 0; b < kMmaColsMost / (kPair ? 2 : 1) / 64; ++b) {
-                        if (b >= blocks) break;
-                        const int col = c0 + 64 * b + 8 * piece, left = min(16, 2 * (a.d - col));
-#pragma unroll
-                        for (int i = 0; i < 2; ++i) {
-                            const bool some = rowX[i] >= 0 && left > 0;
-                            CopyPiece(at + kMmaABytes + b * kMmaBlockBytes + i * 4096, some ? static_cast<const T *>(a.x) + rowX[i] * a.ldx + col : a.x,
-                                      some ? left : 0);
-                        }
-                    }
-                    if (k + 1 < m.steps) rows(k + 1);
+                    for (int b = 0; b < kMmaRows / 64; ++b) block(at + b * kMmaBlockBytes, a.dy, a.ldy, f0 + 64 * b + 8 * piece, a.n, rowY);
+                    for (int b = 0; b < blocks; ++b)
+                        block(at + kMmaABytes + b * kMmaBlockBytes, a.x, a.ldx, c0 + 64 * b + 8 * piece, a.d, rowX);
+                    if (turn + warps < m.steps) rows(turn + warps);
                     asked();
                 }
+                turn -= m.steps;
             }
         }
-        asm volatile("cp.async.wait_all;" ::: "memory");
     } else if (tid == 32 && rank == 0) {
         constexpr bool kAcrossA = kMode != Mode::kProductT, kAcrossB = kMode == Mode::kGrad;
         constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
@@ -432,8 +432,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     failed = true;
                     break;
                 }
-                // What plain copies have written is read by the tensor cores from here on.
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 const uint32_t at = base + ring.stage * a.stageBytes;
 #pragma unroll
                 for (int i = 0; i < kMmaDepth / 16; ++i)
@@ -446,20 +444,6 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         }
         MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
         (void)BarWait(&sLast, 0, a.waitCycles);
-    } else if (kPair && tid == 32) {
-        // The second CTA: what its threads have gathered is told to the first, which starts the products.
-        Ring ring;
-        for (int t = first; t < all && !failed; t += step) {
-            const MmaTile m = tiles.At(t);
-            for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
-                if (!BarWait(sGathered + ring.stage, ring.Filled(), a.waitCycles)) {
-                    failed = true;
-                    break;
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                BarArriveAt(LeadersBar(sFull + ring.stage));
-            }
-        }
     } else if (warp >= 2 && warp < kMmaFirstGather) {
         const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
         const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
