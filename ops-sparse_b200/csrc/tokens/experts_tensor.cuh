@@ -89,6 +89,14 @@ __device__ __forceinline__ bool BarWait(uint64_t *bar, uint32_t parity, long lon
         if (clock64() - t0 > limit) return false;
     return true;
 }
+// One lane of the warp, always the same.  Requests and products are left to it inside code that the whole warp runs, so that their
+// operands stay in uniform registers.
+__device__ __forceinline__ bool Elected()
+{
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
+}
 // By a whole warp, of which one lane asks: all of its lanes go on, or none.
 __device__ __forceinline__ bool BarWaitWarp(uint64_t *bar, uint32_t parity, long long limit)
 {
@@ -277,24 +285,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     const int all = sStart[groups];
     bool failed = false;
 
-    if (kMode != Mode::kGrad && tid == 0) {
+    if (kMode != Mode::kGrad && warp == 0) {
         Ring ring;
         for (int t = first; t < all && !failed; t += step) {
             const MmaTile m = tiles.At(t);
             const int f0 = m.f0 + rank * kMmaRows;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
-                if (ring.round > 0 && !BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles)) {
+                if (ring.round > 0 && !__all_sync(0xffffffffu, BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles))) {
                     failed = true;
                     break;
                 }
                 const uint32_t at = base + ring.stage * a.stageBytes, full = kPair ? LeadersBar(sFull + ring.stage) : Shared(sFull + ring.stage);
-                if (rank == 0) BarExpect(sFull + ring.stage, (kPair ? 2 : 1) * kMmaABytes + a.extraTx);
-                if (kMode == Mode::kProductT) {
-                    CopyTile3<kPair>(at, &mapW, k * kMmaDepth, f0, m.expert, full);
-                } else {
-                    CopyTile3<kPair>(at, &mapW, f0, k * kMmaDepth, m.expert, full);
-                    CopyTile3<kPair>(at + kMmaBlockBytes, &mapW, f0 + 64, k * kMmaDepth, m.expert, full);
+                if (Elected()) {
+                    if (rank == 0) BarExpect(sFull + ring.stage, (kPair ? 2 : 1) * kMmaABytes + a.extraTx);
+                    if (kMode == Mode::kProductT) {
+                        CopyTile3<kPair>(at, &mapW, k * kMmaDepth, f0, m.expert, full);
+                    } else {
+                        CopyTile3<kPair>(at, &mapW, f0, k * kMmaDepth, m.expert, full);
+                        CopyTile3<kPair>(at + kMmaBlockBytes, &mapW, f0 + 64, k * kMmaDepth, m.expert, full);
+                    }
                 }
+                __syncwarp();
             }
         }
         if (failed && rank == 0)  // copies on their way: a bounded chance to land
@@ -410,7 +421,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 turn -= m.steps;
             }
         }
-    } else if (tid == 32 && rank == 0) {
+    } else if (warp == 1 && rank == 0) {
         constexpr bool kAcrossA = kMode != Mode::kProductT, kAcrossB = kMode == Mode::kGrad;
         constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
         constexpr uint32_t kInstr = 1u << 4 | kType << 7 | kType << 10 | (uint32_t)kAcrossA << 15 | (uint32_t)kAcrossB << 16 |
@@ -421,28 +432,32 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             const MmaTile m = tiles.At(t);
             if (m.steps == 0) continue;
             const int acc = tile & 1, turn = tile >> 1;
-            if (turn > 0 && !BarWait(sFree + acc, (uint32_t)(turn - 1) & 1u, a.waitCycles)) {
+            if (turn > 0 && !__all_sync(0xffffffffu, BarWait(sFree + acc, (uint32_t)(turn - 1) & 1u, a.waitCycles))) {
                 failed = true;
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const uint32_t shape = kInstr | (uint32_t)(m.wide >> 3) << 17, to = tmem + acc * kMmaColsMost;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
-                if (!BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles)) {
+                if (!__all_sync(0xffffffffu, BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles))) {
                     failed = true;
                     break;
                 }
                 const uint32_t at = base + ring.stage * a.stageBytes;
+                if (Elected()) {
 #pragma unroll
-                for (int i = 0; i < kMmaDepth / 16; ++i)
-                    Mma<kPair>(to, OperandAt(at + i * (kAcrossA ? 2048 : 32), kAcrossA),
-                               OperandAt(at + kMmaABytes + i * (kAcrossB ? 2048 : 32), kAcrossB), shape, k > 0 || i > 0);
-                MmaCommit<kPair>(sEmpty + ring.stage);
+                    for (int i = 0; i < kMmaDepth / 16; ++i)
+                        Mma<kPair>(to, OperandAt(at + i * (kAcrossA ? 2048 : 32), kAcrossA),
+                                   OperandAt(at + kMmaABytes + i * (kAcrossB ? 2048 : 32), kAcrossB), shape, k > 0 || i > 0);
+                    MmaCommit<kPair>(sEmpty + ring.stage);
+                    if (k == m.steps - 1) MmaCommit<kPair>(sDone + acc);
+                }
+                __syncwarp();
             }
-            if (!failed) MmaCommit<kPair>(sDone + acc);
             ++tile;
         }
-        MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
+        if (Elected()) MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
+        __syncwarp();
         (void)BarWait(&sLast, 0, a.waitCycles);
     } else if (warp >= 2 && warp < kMmaFirstGather) {
         const int quarter = warp & 3;  // the lanes of tensor memory that the warp may read
