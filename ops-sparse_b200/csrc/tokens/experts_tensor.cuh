@@ -27,7 +27,7 @@ constexpr int kMmaBlockBytes = kMmaDepth * 128;    // MN-major: 64 rows along th
 constexpr int kMmaShared = 192 << 10;              // for stages
 constexpr int kMmaStagesMost = 12;
 template <typename Out> constexpr int kMmaStoreBytes = 4 * 32 * 32 * (int)sizeof(Out);  // 32 x 32 results of each storing warp
-constexpr int kMmaGatherWarps = 8;
+constexpr int kMmaParts = 2, kMmaGatherStages = 6, kMmaGatherWarps = kMmaParts * kMmaGatherStages;  // warps at a stage, stages at a time
 constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
 constexpr int kMmaThreads = 32 * (kMmaFirstGather + kMmaGatherWarps);
 constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            BarInit(sFull + s, (kMode != Mode::kGrad) + 1 + kPair);  // W's request, a gathering warp of every CTA
+            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaParts * (kPair ? 2 : 1));  // W's request, the gathering warps of every CTA
             BarInit(sEmpty + s, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -311,13 +311,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         if (failed && rank == 0)  // copies on their way: a bounded chance to land
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
-    } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + a.stages) {
+    } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + kMmaParts * a.stages) {
         // Stages are the warps' in turn: one asks for all of its rows, waits for them and says so, while the others are at the stages
         // beside it.  No more warps than stages: whoever is at stage q knows that q - stages has been used up, so that the wait for
         // q + warps - stages can not be answered by the round before it.  (All warps at every stage, a share each, take turns with it: with the arrivals of 256 threads, and a
         // thread that passes them on to the other CTA, a stage's round took 2900 clocks without any copy.)
         // Eight lanes side by side on 128 bytes of a row: lane l has piece l % 8 of rows l / 8, l / 8 + 4, ...
-        const int mine = warp - kMmaFirstGather, warps = min(kMmaGatherWarps, a.stages), piece = lane & 7, high = lane >> 3;
+        const int mine = (warp - kMmaFirstGather) / kMmaParts, part = (warp - kMmaFirstGather) % kMmaParts;
+        const int warps = min(kMmaGatherStages, a.stages), piece = lane & 7, high = lane >> 3;
         const uint32_t place = base + high * 128;
         const uint32_t even = (uint32_t)(piece ^ high) << 4, odd = (uint32_t)(piece ^ (high + 4)) << 4;  // swizzled: rows high, high + 4 of eight
         Ring ring;
@@ -332,11 +333,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         };
         int turn = mine;  // steps until the next of this warp's stages
         if constexpr (kMode != Mode::kGrad) {
-            constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32;
+            constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32 / kMmaParts;  // times 32: rows part + kMmaParts * (0, 1, ...) of eight each
             const int depth = kMode == Mode::kProductT ? a.d : a.n;
             const int *const rowOf = a.byEntry ? a.entries : a.rows;
             const T *const x = static_cast<const T *>(a.x);
-            int row[kRows];  // rows lane, lane + 32, ... of the tile to come; -1: none
+            // Eights of rows belong to the parts in turn: the lane's own, of which it knows the places, are row 8 * (part + kMmaParts * e)
+            // + lane % 8 with e = lane / 8, lane / 8 + 4, ...; -1: none.  (Its copy is left out: nobody looks at its sums.)
+            int row[kRows];
             MmaTile next;
             auto look = [&](int t) {
                 if (t >= all) return;
@@ -344,8 +347,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 const int share = kPair ? next.wide / 2 : next.wide;
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    const int r = rank * share + lane + 32 * i;
-                    row[i] = next.steps > 0 && lane + 32 * i < share && r < next.many ? __ldg(rowOf + next.first + r) : -1;
+                    const int within = 8 * (part + kMmaParts * (4 * i + lane / 8)) + lane % 8, r = rank * share + within;
+                    row[i] = next.steps > 0 && within < share && r < next.many ? __ldg(rowOf + next.first + r) : -1;
                 }
             };
             look(first);
@@ -361,17 +364,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         failed = true;
                         break;
                     }
-                    const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes;
+                    const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes + part * 1024;
                     const int col = turn * kMmaDepth + 8 * piece, left = max(0, min(16, 2 * (depth - col)));  // bytes of the piece
                     const T *const from = x + (left > 0 ? col : 0);
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
-                        if (32 * i >= share) break;
+                        if (8 * (part + kMmaParts * 4 * i) >= share) break;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
                             const int r = __shfl_sync(0xffffffffu, now[i], 4 * j + high);
-                            if (32 * i + 4 * j + high < share)
-                                CopyPiece(at + i * 4096 + j * 512 + (j & 1 ? odd : even), from + (long long)max(r, 0) * a.ldx, r < 0 ? 0 : left);
+                            if (r >= 0)
+                                CopyPiece(at + (4 * i + j / 2) * (1024 * kMmaParts) + (j & 1) * 512 + (j & 1 ? odd : even), from + r * a.ldx, left);
                         }
                     }
                     asked();
@@ -383,26 +386,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 const MmaTile m = tiles.At(t);
                 const int lo = sOffset[m.expert], hi = sOffset[m.expert + 1], f0 = m.f0 + rank * kMmaRows;
                 const int share = kPair ? m.wide / 2 : m.wide, c0 = m.first + rank * share, blocks = (share + 63) / 64;
-                int rowY[2], rowX[2];
-                auto rows = [&](int k) {  // entries lane and lane + 32 of a step; -1: none
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int at = lo + k * kMmaDepth + lane + 32 * i;
-                        rowY[i] = at < hi ? __ldg(a.entries + at) : -1;
-                        rowX[i] = at < hi ? (a.byEntry ? rowY[i] : __ldg(a.rows + at)) : -1;
-                    }
-                };
-                // a block: 64 columns of 64 rows
-                auto block = [&](uint32_t at, const void *matrix, long long ld, int col, int cols, const int (&row)[2]) {
-                    const int left = max(0, min(16, 2 * (cols - col)));
-                    const T *const from = static_cast<const T *>(matrix) + (left > 0 ? col : 0);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i)
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const int r = __shfl_sync(0xffffffffu, row[i], 4 * j + high);
-                            CopyPiece(at + i * 4096 + j * 512 + (j & 1 ? odd : even), from + (long long)max(r, 0) * ld, r < 0 ? 0 : left);
-                        }
+                int rowY, rowX;
+                auto rows = [&](int k) {  // the part's entry `lane` of a step; -1: none
+                    const int at = lo + k * kMmaDepth + 32 * part + lane;
+                    rowY = at < hi ? __ldg(a.entries + at) : -1;
+                    rowX = at < hi ? (a.byEntry ? rowY : __ldg(a.rows + at)) : -1;
                 };
                 if (turn < m.steps) rows(turn);
                 for (; turn < m.steps; turn += warps) {
@@ -410,11 +398,26 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         failed = true;
                         break;
                     }
-                    const uint32_t at = place + ring.stage * a.stageBytes;
+                    const uint32_t at = place + ring.stage * a.stageBytes + part * 4096;
+                    const int colY = f0 + 8 * piece, colX = c0 + 8 * piece;
 #pragma unroll
-                    for (int b = 0; b < kMmaRows / 64; ++b) block(at + b * kMmaBlockBytes, a.dy, a.ldy, f0 + 64 * b + 8 * piece, a.n, rowY);
-                    for (int b = 0; b < blocks; ++b)
-                        block(at + kMmaABytes + b * kMmaBlockBytes, a.x, a.ldx, c0 + 64 * b + 8 * piece, a.d, rowX);
+                    for (int j = 0; j < 8; ++j) {
+                        const uint32_t to = at + j * 512 + (j & 1 ? odd : even);
+                        const int y = __shfl_sync(0xffffffffu, rowY, 4 * j + high), xr = __shfl_sync(0xffffffffu, rowX, 4 * j + high);
+                        const T *const fromY = static_cast<const T *>(a.dy) + max(y, 0) * a.ldy;
+                        const T *const fromX = static_cast<const T *>(a.x) + max(xr, 0) * a.ldx;
+#pragma unroll
+                        for (int b = 0; b < kMmaRows / 64; ++b) {
+                            const int left = y < 0 ? 0 : max(0, min(16, 2 * (a.n - colY - 64 * b)));
+                            CopyPiece(to + b * kMmaBlockBytes, fromY + (left > 0 ? colY + 64 * b : 0), left);
+                        }
+#pragma unroll
+                        for (int b = 0; b < kMmaColsMost / (kPair ? 2 : 1) / 64; ++b) {
+                            if (b >= blocks) break;
+                            const int left = xr < 0 ? 0 : max(0, min(16, 2 * (a.d - colX - 64 * b)));
+                            CopyPiece(to + kMmaABytes + b * kMmaBlockBytes, fromX + (left > 0 ? colX + 64 * b : 0), left);
+                        }
+                    }
                     if (turn + warps < m.steps) rows(turn + warps);
                     asked();
                 }
