@@ -90,7 +90,7 @@ inline aclsparseStatus_t CheckDense(const aclsparseDnMatDescr *m)
 {
     if (m == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (m->order != ACL_SPARSE_ORDER_ROW || !IsFloatType(m->valueType)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (m->rows > INT32_MAX || m->cols > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (m->rows > INT32_MAX || m->cols > INT32_MAX || m->ld > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (m->values == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (reinterpret_cast<uintptr_t>(m->values) % BytesOf(m->valueType) != 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;

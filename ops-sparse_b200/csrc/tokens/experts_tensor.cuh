@@ -336,10 +336,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32 / kMmaParts;  // times 32: rows part + kMmaParts * (0, 1, ...) of eight each
             const int depth = kMode == Mode::kProductT ? a.d : a.n;
             const int *const rowOf = a.byEntry ? a.entries : a.rows;
-            const T *const x = static_cast<const T *>(a.x);
+            const char *const x = static_cast<const char *>(a.x);
+            const uint32_t pitch = (uint32_t)a.ldx * 2;
             // Eights of rows belong to the parts in turn: the lane's own, of which it knows the places, are row 8 * (part + kMmaParts * e)
-            // + lane % 8 with e = lane / 8, lane / 8 + 4, ...; -1: none.  (Its copy is left out: nobody looks at its sums.)
-            int row[kRows];
+            // + lane % 8 with e = lane / 8, lane / 8 + 4, ...  (What is past the last entry is a copy of row 0, of whose sums nobody asks.)
+            uint32_t row[kRows];
             MmaTile next;
             auto look = [&](int t) {
                 if (t >= all) return;
@@ -348,16 +349,17 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
                     const int within = 8 * (part + kMmaParts * (4 * i + lane / 8)) + lane % 8, r = rank * share + within;
-                    row[i] = next.steps > 0 && within < share && r < next.many ? __ldg(rowOf + next.first + r) : -1;
+                    row[i] = next.steps > 0 && within < share && r < next.many ? (uint32_t)__ldg(rowOf + next.first + r) : 0;
                 }
             };
             look(first);
             for (int t = first; t < all && !failed; t += step) {
                 const MmaTile m = next;
                 const int share = kPair ? m.wide / 2 : m.wide;
-                int now[kRows];
+                uint32_t now[kRows];
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) now[i] = row[i];
+                const int eights = (share / 8 - part + kMmaParts - 1) / kMmaParts;  // of this part
                 look(t + step);
                 for (; turn < m.steps; turn += warps) {
                     if (!free()) {
@@ -366,15 +368,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     }
                     const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes + part * 1024;
                     const int col = turn * kMmaDepth + 8 * piece, left = max(0, min(16, 2 * (depth - col)));  // bytes of the piece
-                    const T *const from = x + (left > 0 ? col : 0);
+                    const char *const from = x + (left > 0 ? 2 * col : 0);
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
-                        if (8 * (part + kMmaParts * 4 * i) >= share) break;
 #pragma unroll
                         for (int j = 0; j < 8; ++j) {
-                            const int r = __shfl_sync(0xffffffffu, now[i], 4 * j + high);
-                            if (r >= 0)
-                                CopyPiece(at + (4 * i + j / 2) * (1024 * kMmaParts) + (j & 1) * 512 + (j & 1 ? odd : even), from + r * a.ldx, left);
+                            if (4 * i + j / 2 >= eights) break;
+                            const uint32_t r = __shfl_sync(0xffffffffu, now[i], 4 * j + high);
+                            CopyPiece(at + (4 * i + j / 2) * (1024 * kMmaParts) + (j & 1) * 512 + (j & 1 ? odd : even), from + (uint64_t)r * pitch, left);
                         }
                     }
                     asked();
@@ -386,6 +387,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 const MmaTile m = tiles.At(t);
                 const int lo = sOffset[m.expert], hi = sOffset[m.expert + 1], f0 = m.f0 + rank * kMmaRows;
                 const int share = kPair ? m.wide / 2 : m.wide, c0 = m.first + rank * share, blocks = (share + 63) / 64;
+                // the lane's columns of every block: where they are, and how many bytes of its piece exist
+                constexpr int kBlocksY = kMmaRows / 64, kBlocksX = kMmaColsMost / (kPair ? 2 : 1) / 64;
+                int leftY[kBlocksY], leftX[kBlocksX];
+#pragma unroll
+                for (int b = 0; b < kBlocksY; ++b) leftY[b] = max(0, min(16, 2 * (a.n - f0 - 8 * piece - 64 * b)));
+#pragma unroll
+                for (int b = 0; b < kBlocksX; ++b) leftX[b] = max(0, min(16, 2 * (a.d - c0 - 8 * piece - 64 * b)));
+                const char *const y = static_cast<const char *>(a.dy) + 2ll * (f0 + 8 * piece), *const x = static_cast<const char *>(a.x) + 2ll * (c0 + 8 * piece);
+                const uint32_t pitchY = (uint32_t)a.ldy * 2, pitchX = (uint32_t)a.ldx * 2;
                 int rowY, rowX;
                 auto rows = [&](int k) {  // the part's entry `lane` of a step; -1: none
                     const int at = lo + k * kMmaDepth + 32 * part + lane;
@@ -399,23 +409,19 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         break;
                     }
                     const uint32_t at = place + ring.stage * a.stageBytes + part * 4096;
-                    const int colY = f0 + 8 * piece, colX = c0 + 8 * piece;
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const uint32_t to = at + j * 512 + (j & 1 ? odd : even);
-                        const int y = __shfl_sync(0xffffffffu, rowY, 4 * j + high), xr = __shfl_sync(0xffffffffu, rowX, 4 * j + high);
-                        const T *const fromY = static_cast<const T *>(a.dy) + max(y, 0) * a.ldy;
-                        const T *const fromX = static_cast<const T *>(a.x) + max(xr, 0) * a.ldx;
+                        const int ry = __shfl_sync(0xffffffffu, rowY, 4 * j + high), rx = __shfl_sync(0xffffffffu, rowX, 4 * j + high);
+                        // no row: zeros, from wherever
+                        const char *const fromY = y + (uint64_t)(uint32_t)max(ry, 0) * pitchY, *const fromX = x + (uint64_t)(uint32_t)max(rx, 0) * pitchX;
 #pragma unroll
-                        for (int b = 0; b < kMmaRows / 64; ++b) {
-                            const int left = y < 0 ? 0 : max(0, min(16, 2 * (a.n - colY - 64 * b)));
-                            CopyPiece(to + b * kMmaBlockBytes, fromY + (left > 0 ? colY + 64 * b : 0), left);
-                        }
+                        for (int b = 0; b < kBlocksY; ++b)
+                            CopyPiece(to + b * kMmaBlockBytes, leftY[b] > 0 ? fromY + 128 * b : static_cast<const char *>(a.dy), ry < 0 ? 0 : leftY[b]);
 #pragma unroll
-                        for (int b = 0; b < kMmaColsMost / (kPair ? 2 : 1) / 64; ++b) {
+                        for (int b = 0; b < kBlocksX; ++b) {
                             if (b >= blocks) break;
-                            const int left = xr < 0 ? 0 : max(0, min(16, 2 * (a.d - colX - 64 * b)));
-                            CopyPiece(to + kMmaABytes + b * kMmaBlockBytes, fromX + (left > 0 ? colX + 64 * b : 0), left);
+                            CopyPiece(to + kMmaABytes + b * kMmaBlockBytes, leftX[b] > 0 ? fromX + 128 * b : static_cast<const char *>(a.x), rx < 0 ? 0 : leftX[b]);
                         }
                     }
                     if (turn + warps < m.steps) rows(turn + warps);
@@ -429,6 +435,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         constexpr uint32_t kType = std::is_same_v<T, __nv_bfloat16> ? 1u : 0u;
         constexpr uint32_t kInstr = 1u << 4 | kType << 7 | kType << 10 | (uint32_t)kAcrossA << 15 | (uint32_t)kAcrossB << 16 |
                                     (uint32_t)(Tiles<kMode, kPair>::kHigh >> 4) << 24;
+        const bool elected = Elected();
+        // Of the descriptors only the address changes, and that within 14 bits.
+        const uint64_t first64A = OperandAt(base, kAcrossA), first64B = OperandAt(base + kMmaABytes, kAcrossB);
+        constexpr int kAlongA = (kAcrossA ? 2048 : 32) >> 4, kAlongB = (kAcrossB ? 2048 : 32) >> 4;
         Ring ring;
         int tile = 0;
         for (int t = first; t < all && !failed; t += step) {
@@ -446,12 +456,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     failed = true;
                     break;
                 }
-                const uint32_t at = base + ring.stage * a.stageBytes;
-                if (Elected()) {
+                const uint32_t at = (uint32_t)(ring.stage * a.stageBytes) >> 4;
+                if (elected) {
 #pragma unroll
                     for (int i = 0; i < kMmaDepth / 16; ++i)
-                        Mma<kPair>(to, OperandAt(at + i * (kAcrossA ? 2048 : 32), kAcrossA),
-                                   OperandAt(at + kMmaABytes + i * (kAcrossB ? 2048 : 32), kAcrossB), shape, k > 0 || i > 0);
+                        Mma<kPair>(to, first64A + (at + i * kAlongA), first64B + (at + i * kAlongB), shape, k > 0 || i > 0);
                     MmaCommit<kPair>(sEmpty + ring.stage);
                     if (k == m.steps - 1) MmaCommit<kPair>(sDone + acc);
                 }
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             }
             ++tile;
         }
-        if (Elected()) MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
+        if (elected) MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
         __syncwarp();
         (void)BarWait(&sLast, 0, a.waitCycles);
     } else if (warp >= 2 && warp < kMmaFirstGather) {
