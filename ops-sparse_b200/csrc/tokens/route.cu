@@ -1,8 +1,8 @@
 // b200spRoute, b200spRouteGrad: the k best experts of every token as a CSR matrix, and the gradient of its values.
 //
-// A warp has a token; its lanes hold the token's logits, 1 to 32 each (expert 32 j + lane).  The k experts are taken one after the
-// other: the largest key of the warp, then the lowest expert that has it.  Keys are the selection values as unsigned
-// integers of the same order.
+// A warp has a token; its lanes hold the token's logits, 1 to 32 each (expert 32 j + lane).  Every lane sorts its own; then the k experts are
+// taken one after the other: the largest key among the lanes' first, the lowest expert that has it, and that lane goes on to its
+// next.  Keys are the selection values as unsigned integers of the same order.
 // The choice is that of exact arithmetic.  Without a bias it is made on the logits themselves, which both scores ascend
 // with.  With one, p + bias is computed in f32 together with a bound of its error; where another expert lies as near the last
 // one taken as the two bounds together, or a group that is kept as near one that is not, the row is done again in
@@ -27,6 +27,7 @@ struct RouteArgs {
     int tokens, experts, k;
     int sigmoid, groups, kept, top2, renormalise;
     float scale;
+    int groupSize, groupLanes;  // lanes side by side on a group: a power of two
     int *offsets, *columns;
     void *values;
 };
@@ -69,7 +70,7 @@ __device__ __forceinline__ unsigned long long KeyOf(double v)
     const unsigned long long b = (unsigned long long)__double_as_longlong(v + 0.0);
     return b >> 63 ? ~b : b | 1ull << 63;
 }
-__device__ __forceinline__ uint32_t MaxKey(uint32_t v) { return __reduce_max_sync(kAll, v); }
+__device__ __forceinline__ float ValueOf(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 __device__ __forceinline__ unsigned long long MaxKey(unsigned long long v)
 {
     const uint32_t high = __reduce_max_sync(kAll, (uint32_t)(v >> 32));
@@ -77,13 +78,24 @@ __device__ __forceinline__ unsigned long long MaxKey(unsigned long long v)
     return (unsigned long long)high << 32 | low;
 }
 
-// Scores of the lanes' logits (masked: -infinity), 0 for the masked.
-template <typename Real, int kPer> __device__ __forceinline__ void Scores(const RouteArgs &a, const float (&x)[kPer], Real (&p)[kPer], float *most)
+// Scores of the lanes' logits (masked: -infinity), 0 for the masked.  In f32 a sigmoid is taken from the fast exponential and division: it
+// serves the choice alone.  *error: how far they may be from exact ones.
+//   sigmoid: __expf is off by 2 + 1.16 |x| units of 2^-23 relative to e^-x, of which p (1 - p) <= p / (1 + |x|) reaches p: less
+//   than 4 of p with the division's 2 and the addition; 8 are allowed.
+//   softmax: expf is off by 2, the difference of the logits by |x - most| / 2 (of which p |x - most| <= 0.4 reaches p), a sum of kPer +
+//   5 additions by half of that, at most 24 units of p <= the largest score; 32 are allowed.
+template <typename Real, int kPer>
+__device__ __forceinline__ void Scores(const RouteArgs &a, const float (&x)[kPer], Real (&p)[kPer], float *most, Real *inverse, float *error)
 {
+    constexpr float kUnit = 1.2e-7f;
+    constexpr bool kFast = sizeof(Real) == 4;
     if (a.sigmoid) {
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) p[j] = (Real)1 / ((Real)1 + Exp(-(Real)x[j]));
-        *most = 0.0f;
+        for (int j = 0; j < kPer; ++j) {
+            if constexpr (kFast) p[j] = __fdividef(1.0f, 1.0f + __expf(-x[j]));
+            else p[j] = 1.0 / (1.0 + exp(-(double)x[j]));
+        }
+        *error = 8 * kUnit;
         return;
     }
     float m = -INFINITY;
@@ -102,206 +114,218 @@ template <typename Real, int kPer> __device__ __forceinline__ void Scores(const 
 #pragma unroll
     for (int j = 0; j < kPer; ++j) p[j] *= inv;
     *most = m;
+    *inverse = inv;
+    *error = 32 * kUnit * (float)inv;
 }
 
-// How far p, in f32, may be from the score: expf 2 units of its last place and the division 1, a softmax's sum of kPer + 5 additions and the
-// difference of its logits, each 2^-24 of p (a few more are allowed).
-__device__ __forceinline__ float ErrorOf(const RouteArgs &a, float x, float p, float most)
-{
-    constexpr float kUnit = 6.0e-8f;
-    return p * (a.sigmoid ? 8 * kUnit : kUnit * (64.0f + 2.0f * fminf(most - x, 200.0f)));
-}
-
-struct Chosen {
-    uint32_t mine;       // bit j: the lane's expert 32 j + lane is taken
-    uint32_t weightless; // and has no selection value
-    bool unsure;         // f32 does not tell
-};
-
+// The selection values: of masked experts, and of those in groups that are not kept, -infinity.  Returns whether f32 can not tell
+// which groups are kept.
 template <typename Real, int kPer>
-__device__ __forceinline__ Chosen Choose(const RouteArgs &a, const float (&x)[kPer], const Real (&p)[kPer], float most, float *sRow, int lane)
+__device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer], const Real (&p)[kPer], float error, void *sRow, int lane,
+                                       Real (&s)[kPer])
 {
-    constexpr bool kBounds = sizeof(Real) == 4;
-    Chosen c{0, 0, false};
-    Real s[kPer];
+    const Real nothing = Limits<Real>::Lowest();
+    bool unsure = false;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) s[j] = (Real)x[j];
+    if (a.bias != nullptr) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+            const int e = 32 * j + lane;
+            const float b = e < a.experts ? __ldg(a.bias + e) : -INFINITY;
+            s[j] = x[j] == -INFINITY || !(b > -INFINITY) ? nothing : p[j] + (Real)b;
+        }
+    }
+    if (a.groups == 1) return false;
+    // Lanes side by side on a group: the two best of their experts, then of the group.
+    Real *const sValues = static_cast<Real *>(sRow);
+    const bool sums = a.top2 != 0;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         const int e = 32 * j + lane;
-        s[j] = (Real)x[j];
-        if (a.bias != nullptr && e < a.experts) {
-            const float b = __ldg(a.bias + e);
-            s[j] = x[j] == -INFINITY || !(b > -INFINITY) ? Limits<Real>::Lowest() : p[j] + (Real)b;
+        const Real v = sums && a.bias == nullptr ? (x[j] == -INFINITY ? nothing : p[j]) : s[j];
+        if (e < a.experts) sValues[e + (e >> 5)] = v;
+    }
+    __syncwarp();
+    const int wide = a.groupLanes, group = lane / wide, size = a.groupSize;
+    Real first = nothing, second = nothing;
+    if (group < a.groups) {
+        for (int i = lane % wide; i < size; i += wide) {
+            const int e = group * size + i;
+            const Real v = sValues[e + (e >> 5)];
+            const Real low = v > first ? first : v;
+            first = v > first ? v : first;
+            second = low > second ? low : second;
         }
     }
-    if (a.groups > 1) {
-        // Lanes side by side on a group: the two best of their experts, then of the group.
-        Real *const sValues = reinterpret_cast<Real *>(sRow);
-        const bool sums = a.top2 != 0;
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int e = 32 * j + lane;
-            const Real v = sums && a.bias == nullptr ? (x[j] == -INFINITY ? Limits<Real>::Lowest() : p[j]) : s[j];
-            if (e < a.experts) sValues[e + (e >> 5)] = v;
-        }
-        __syncwarp();
-        int wide = 32;  // lanes of a group
-        while (wide * a.groups > 32) wide >>= 1;
-        const int group = lane / wide, size = a.experts / a.groups;
-        Real first = Limits<Real>::Lowest(), second = Limits<Real>::Lowest();
-        if (group < a.groups) {
-            for (int i = lane % wide; i < size; i += wide) {
-                const int e = group * size + i;
-                const Real v = sValues[e + (e >> 5)];
-                if (v > first) {
-                    second = first;
-                    first = v;
-                } else if (v > second) {
-                    second = v;
-                }
-            }
-        }
-        for (int d = 1; d < wide; d <<= 1) {
-            const Real f = __shfl_xor_sync(kAll, first, d), t = __shfl_xor_sync(kAll, second, d);
-            const Real low = f > first ? first : f;
-            if (f > first) first = f;
-            Real high = t > second ? t : second;
-            second = low > high ? low : high;
-        }
-        __syncwarp();
-        const Real value = sums && second > Limits<Real>::Lowest() ? first + second : first;
-        // lane g < groups: group g
-        const Real mine = __shfl_sync(kAll, value, (lane * wide) & 31);
-        int place = 0;
-        for (int g = 0; g < a.groups; ++g) {
-            const Real o = __shfl_sync(kAll, mine, g);
-            place += o > mine || (o == mine && g < lane);
-        }
-        const unsigned open = __ballot_sync(kAll, lane < a.groups && place < a.kept);
-        if (kBounds && (a.bias != nullptr || sums)) {
-            // both values of a sum have an error of at most ErrorOf(p = 1), each addition half a unit of its result
-            const float unit = a.sigmoid ? 2.0e-6f : 1.5e-5f;
-            for (int g = 0; g < a.groups; ++g) {
-                const float o = (float)__shfl_sync(kAll, mine, g), own = (float)mine;
-                const bool apart = lane < a.groups && (((open >> g) ^ (open >> lane)) & 1) != 0;
-                c.unsure |= apart && fabsf(o - own) <= unit + 2.4e-7f * (fabsf(o) + fabsf(own));
-            }
-        }
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            const int e = 32 * j + lane;
-            if (e < a.experts && !(open >> (e / size) & 1)) s[j] = Limits<Real>::Lowest();
-        }
+    for (int d = 1; d < wide; d <<= 1) {
+        const Real f = __shfl_xor_sync(kAll, first, d), t = __shfl_xor_sync(kAll, second, d);
+        const Real low = f > first ? first : f, high = t > second ? t : second;
+        first = f > first ? f : first;
+        second = low > high ? low : high;
     }
-    using Key = decltype(KeyOf(Real{}));
-    Key key[kPer];
+    __syncwarp();  // the values may be written again
+    const Real value = sums && second > nothing ? first + second : first;
+    // lane g < groups: group g
+    const Real own = __shfl_sync(kAll, value, (lane * wide) & 31), mine = lane < a.groups ? own : nothing;
+    int place = 0;
+    for (int g = 0; g < a.groups; ++g) {
+        const Real o = __shfl_sync(kAll, mine, g);
+        place += o > mine || (o == mine && g < lane);
+    }
+    const bool kept = lane < a.groups && place < a.kept;
+    const unsigned open = __ballot_sync(kAll, kept);
+    if (sizeof(Real) == 4 && (a.bias != nullptr || sums)) {
+        // the last group kept, and the first that is not
+        const uint32_t key = KeyOf((float)mine);
+        const float least = ValueOf(__reduce_min_sync(kAll, kept ? key : ~0u));
+        const float other = ValueOf(__reduce_max_sync(kAll, lane < a.groups && !kept ? key : KeyOf(-INFINITY)));
+        // two scores each, and three additions that round
+        unsure = least - other <= 4 * error + 4.8e-7f * (fabsf(least) + fabsf(other));
+    }
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) key[j] = 32 * j + lane < a.experts ? KeyOf(s[j]) : 0;
-    const Key nothing = KeyOf(Limits<Real>::Lowest());
-    Real lastValue = 0;
-    float lastX = 0, lastBias = 0, lastError = 0;
+    for (int j = 0; j < kPer; ++j) {
+        const int e = 32 * j + lane;
+        if (e < a.experts && !(open >> (e / size) & 1)) s[j] = nothing;
+    }
+    return unsure;
+}
+
+// Lane i < k has the i-th expert taken.
+struct Chosen {
+    int expert;
+    bool weightless;  // it has no selection value
+};
+
+// By the f64 values, one expert after the other.
+template <int kPer> __device__ __noinline__ Chosen ChooseExactly(const RouteArgs &a, const float *sLogits, void *sRow, int lane)
+{
+    float x[kPer], most, error;
+#pragma unroll
+    for (int j = 0; j < kPer; ++j) x[j] = sLogits[32 * j + lane];
+    double p[kPer], s[kPer], inverse;
+    Scores<double, kPer>(a, x, p, &most, &inverse, &error);
+    Values<double, kPer>(a, x, p, error, sRow, lane, s);
+    Chosen c{-1, false};
     for (int i = 0; i < a.k; ++i) {
-        Key best = 0;
+        unsigned long long best = 0;
         int at = 0;
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
-            if (key[j] > best) {
-                best = key[j];
+            const unsigned long long key = 32 * j + lane < a.experts && s[j] == s[j] ? KeyOf(s[j]) : 0;
+            if (key > best) {
+                best = key;
                 at = j;
             }
         }
-        const Key top = MaxKey(best);
+        const unsigned long long top = MaxKey(best);
         const unsigned e = __reduce_min_sync(kAll, best == top && top != 0 ? 32u * at + lane : ~0u);
-        const bool won = (e & 31) == (unsigned)lane && e != ~0u;
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) {
-            if (!won || (int)(e >> 5) != j) continue;
-            key[j] = 0;
-            c.mine |= 1u << j;
-            if (top == nothing) c.weightless |= 1u << j;
-            if (kBounds && i == a.k - 1) {
-                lastValue = s[j];
-                lastX = x[j];
-                lastError = ErrorOf(a, x[j], (float)p[j], most);
-                lastBias = a.bias != nullptr ? __ldg(a.bias + e) : 0.0f;
-            }
-        }
-        if (kBounds && i == a.k - 1 && a.bias != nullptr) {
-            const int from = (int)(e & 31);
-            lastValue = __shfl_sync(kAll, lastValue, from);
-            lastX = __shfl_sync(kAll, lastX, from);
-            lastError = __shfl_sync(kAll, lastError, from);
-            lastBias = __shfl_sync(kAll, lastBias, from);
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                // Neighbours of the last one taken, but for those that are its equals in exact arithmetic too.
-                if (32 * j + lane >= a.experts || 32u * j + lane == e || key[j] == nothing) continue;
-                const float gap = fabsf((float)(s[j] - lastValue));
-                const float room = ErrorOf(a, x[j], (float)p[j], most) + lastError + 1.2e-7f * (fabsf((float)s[j]) + fabsf((float)lastValue));
-                if (gap <= room) c.unsure |= !(x[j] == lastX && __ldg(a.bias + 32 * j + lane) == lastBias);
-            }
-        }
+        for (int j = 0; j < kPer; ++j)
+            if (e == 32u * j + lane) s[j] = NAN;  // taken
+        if (lane == i) c = {(int)e, top == KeyOf(Limits<double>::Lowest())};
     }
-    c.unsure = kBounds && __any_sync(kAll, c.unsure);
     return c;
 }
 
-template <int kPer> __device__ __noinline__ Chosen ChooseExactly(const RouteArgs &a, const float *sLogits, float *sRow, int lane)
+// Sorts the lane's keys, the largest first, with their places; of equal ones the lower place first.  (Batcher's odd-even merge sort.)
+template <int kPer> __device__ __forceinline__ void SortDown(uint32_t (&key)[kPer], int (&place)[kPer])
 {
-    float x[kPer], most;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) x[j] = sLogits[32 * j + lane];
-    double p[kPer];
-    Scores<double, kPer>(a, x, p, &most);
-    return Choose<double, kPer>(a, x, p, most, sRow, lane);
+    for (int p = 1; p < kPer; p *= 2)
+#pragma unroll
+        for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+            for (int j = k % p; j + k < kPer; j += 2 * k)
+#pragma unroll
+                for (int i = 0; i < k; ++i) {
+                    if (i + j + k >= kPer || (i + j) / (2 * p) != (i + j + k) / (2 * p)) continue;
+                    const int u = i + j, v = i + j + k;
+                    const bool swap = key[v] > key[u] || (key[v] == key[u] && place[v] < place[u]);
+                    const uint32_t ku = swap ? key[v] : key[u], kv = swap ? key[u] : key[v];
+                    const int pu = swap ? place[v] : place[u], pv = swap ? place[u] : place[v];
+                    key[u] = ku, key[v] = kv, place[u] = pu, place[v] = pv;
+                }
 }
 
 template <typename In, typename Out, int kPer> __global__ void __launch_bounds__(32 * kRouteWarps<kPer>) RouteKernel(const RouteArgs a)
 {
-    // of a warp: its selection values by expert, a word apart every 32 (f64 too), and its logits for a second pass
+    // of a warp: its selection values by expert, a word apart every 32 (f64 too), and its logits
     __shared__ double sRows[kRouteWarps<kPer>][33 * kPer];
-    __shared__ float sLogits[kRouteWarps<kPer>][32 * kPer];
+    __shared__ float sAllLogits[kRouteWarps<kPer>][32 * kPer];
     b200sp::WaitForPrevious();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long token = (long long)blockIdx.x * kRouteWarps<kPer> + warp;
     if (token >= a.tokens) return;
     const In *const row = static_cast<const In *>(a.logits) + token * a.ld;
+    float *const sLogits = sAllLogits[warp];
     float x[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         x[j] = 32 * j + lane < a.experts ? ToFloat(row[32 * j + lane]) : -INFINITY;
         if (!(x[j] > -INFINITY)) x[j] = -INFINITY;  // NaN, too
+        sLogits[32 * j + lane] = x[j];
     }
-    float p[kPer], most;
-    Scores<float, kPer>(a, x, p, &most);
-    float *const sRow = reinterpret_cast<float *>(sRows[warp]);
-    Chosen c = Choose<float, kPer>(a, x, p, most, sRow, lane);
-    if (c.unsure) {
-#pragma unroll
-        for (int j = 0; j < kPer; ++j) sLogits[warp][32 * j + lane] = x[j];
-        __syncwarp();
-        c = ChooseExactly<kPer>(a, sLogits[warp], sRow, lane);
-    }
-    float sum = 0;
+    __syncwarp();
+    float p[kPer], s[kPer], most = 0.0f, inverse = 0.0f, error = 0.0f;
+    const bool scored = !a.sigmoid || a.bias != nullptr || (a.groups > 1 && a.top2);  // without, the choice goes by the logits alone
+    if (scored) Scores<float, kPer>(a, x, p, &most, &inverse, &error);
+    bool unsure = Values<float, kPer>(a, x, p, error, sRows[warp], lane, s);
+    uint32_t key[kPer];
+    int place[kPer];
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        if (c.weightless >> j & 1) p[j] = 0.0f;
-        if (c.mine >> j & 1) sum += p[j];
+        key[j] = 32 * j + lane < a.experts ? KeyOf(s[j]) : 0;
+        place[j] = j;
+    }
+    SortDown<kPer>(key, place);
+    const uint32_t nothing = KeyOf(-INFINITY);
+    Chosen c{-1, false};
+    uint32_t top = 0;
+    unsigned e = 0;
+    for (int i = 0; i < a.k; ++i) {
+        top = __reduce_max_sync(kAll, key[0]);
+        e = __reduce_min_sync(kAll, key[0] == top ? 32u * place[0] + lane : ~0u);
+        if (lane == i) c = {(int)e, top == nothing};
+        if (lane == (int)(e & 31)) {
+#pragma unroll
+            for (int j = 0; j + 1 < kPer; ++j) {
+                key[j] = key[j + 1];
+                place[j] = place[j + 1];
+            }
+            key[kPer - 1] = 0;
+        }
+    }
+    if (a.bias != nullptr) {
+        // Neighbours of the last one taken, but for its equals in exact arithmetic too.
+        const float last = ValueOf(top), room = 2 * error + 4.8e-7f * fabsf(last);
+        const uint32_t near = top == nothing ? ~0u : KeyOf(last - room);
+        if (__any_sync(kAll, key[0] > nothing && key[0] >= near)) {
+            const float lastX = sLogits[e], lastBias = __ldg(a.bias + e);
+#pragma unroll
+            for (int j = 0; j < kPer; ++j) {
+                const int other = 32 * place[j] + lane;
+                if (key[j] > nothing && key[j] >= near) unsure |= !(sLogits[other] == lastX && __ldg(a.bias + other) == lastBias);
+            }
+        }
+    }
+    if (__any_sync(kAll, unsure)) c = ChooseExactly<kPer>(a, sLogits, sRows[warp], lane);
+    // the weights, of the experts taken alone; their places by column
+    float w = 0.0f;
+    if (c.expert >= 0 && !c.weightless) {
+        const float own = sLogits[c.expert];
+        w = a.sigmoid ? 1.0f / (1.0f + expf(-own)) : (own == most ? 1.0f : expf(own - most)) * inverse;
     }
     float by = a.scale;
     if (a.renormalise) {
-        sum = WarpSum(sum);
+        const float sum = WarpSum(w);
         by = sum > 0 ? a.scale / sum : 0.0f;
     }
-    long long at = token * a.k;
-#pragma unroll
-    for (int j = 0; j < kPer; ++j) {
-        const unsigned taken = __ballot_sync(kAll, c.mine >> j & 1);
-        if (c.mine >> j & 1) {
-            const long long to = at + __popc(taken & ((1u << lane) - 1u));
-            a.columns[to] = 32 * j + lane;
-            static_cast<Out *>(a.values)[to] = FromFloat<Out>(p[j] * by);
-        }
-        at += __popc(taken);
+    int to = 0;
+    for (int i = 0; i < a.k; ++i) to += __shfl_sync(kAll, c.expert, i) < c.expert;
+    if (lane < a.k) {
+        a.columns[token * a.k + to] = c.expert;
+        static_cast<Out *>(a.values)[token * a.k + to] = FromFloat<Out>(w * by);
     }
     if (lane == 0) a.offsets[token] = (int)(token * a.k);
     if (lane == 0 && token == a.tokens - 1) a.offsets[a.tokens] = (int)((token + 1) * a.k);
@@ -462,9 +486,11 @@ aclsparseStatus_t b200spRoute(aclsparseHandle_t handle, const b200spRouteRule *r
     const OnDevice device(handle);
     RouteArgs a{logits->values, bias != nullptr ? static_cast<const float *>(bias->values) : nullptr, logits->ld, (int)matR->rows,
                 (int)matR->cols, (int)(matR->nnz / matR->rows), rule->score == B200SP_ROUTE_SIGMOID, rule->groups, rule->groupsKept,
-                rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, static_cast<int *>(matR->offsets),
+                rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, 0, 0, static_cast<int *>(matR->offsets),
                 static_cast<int *>(matR->indices), matR->values};
     if (a.kept == a.groups) a.groups = a.kept = 1;  // all are kept
+    a.groupSize = a.experts / a.groups;
+    for (a.groupLanes = 32; a.groupLanes * a.groups > 32;) a.groupLanes /= 2;
     const cudaError_t e = WithPer(a.experts, [&](auto per) {
         return WithType(logits->valueType, [&](auto in) {
             return WithType(matR->valueType, [&](auto out) {
