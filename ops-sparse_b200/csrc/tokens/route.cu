@@ -28,6 +28,7 @@ struct RouteArgs {
     int sigmoid, groups, kept, top2, renormalise;
     float scale;
     int groupSize, groupLanes;  // lanes side by side on a group: a power of two
+    unsigned perGroup;          // e / groupSize = e * perGroup >> 20 for e, groupSize <= 1024
     int *offsets, *columns;
     void *values;
 };
@@ -42,6 +43,11 @@ template <> struct Limits<double> {
 
 __device__ __forceinline__ float Exp(float v) { return expf(v); }
 __device__ __forceinline__ double Exp(double v) { return exp(v); }
+
+__device__ __forceinline__ float Larger(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ double Larger(double a, double b) { return fmax(a, b); }
+__device__ __forceinline__ float Smaller(float a, float b) { return fminf(a, b); }
+__device__ __forceinline__ double Smaller(double a, double b) { return fmin(a, b); }
 
 template <typename Real> __device__ __forceinline__ Real WarpMax(Real v)
 {
@@ -153,16 +159,14 @@ __device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer
         for (int i = lane % wide; i < size; i += wide) {
             const int e = group * size + i;
             const Real v = sValues[e + (e >> 5)];
-            const Real low = v > first ? first : v;
-            first = v > first ? v : first;
-            second = low > second ? low : second;
+            second = Larger(second, Smaller(first, v));
+            first = Larger(first, v);
         }
     }
     for (int d = 1; d < wide; d <<= 1) {
         const Real f = __shfl_xor_sync(kAll, first, d), t = __shfl_xor_sync(kAll, second, d);
-        const Real low = f > first ? first : f, high = t > second ? t : second;
-        first = f > first ? f : first;
-        second = low > high ? low : high;
+        second = Larger(Larger(second, t), Smaller(first, f));
+        first = Larger(first, f);
     }
     __syncwarp();  // the values may be written again
     const Real value = sums && second > nothing ? first + second : first;
@@ -186,7 +190,7 @@ __device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         const int e = 32 * j + lane;
-        if (e < a.experts && !(open >> (e / size) & 1)) s[j] = nothing;
+        if (!(open >> (e * a.perGroup >> 20 & 31) & 1)) s[j] = nothing;
     }
     return unsure;
 }
@@ -228,35 +232,45 @@ template <int kPer> __device__ __noinline__ Chosen ChooseExactly(const RouteArgs
     return c;
 }
 
-// Sorts the lane's keys, the largest first, with their places; of equal ones the lower place first.  (Batcher's odd-even merge sort.)
+// Sorts the lane's keys, the largest first, with their places; of equal ones the lower place first: neighbours are exchanged, up to eight
+// keys; more by Batcher's odd-even merge sort, which compares the places of equal keys.
 template <int kPer> __device__ __forceinline__ void SortDown(uint32_t (&key)[kPer], int (&place)[kPer])
 {
+    auto exchange = [&](int u, int v, bool swap) {
+        const uint32_t high = max(key[u], key[v]), low = min(key[u], key[v]);
+        const int pu = swap ? place[v] : place[u], pv = swap ? place[u] : place[v];
+        key[u] = high, key[v] = low, place[u] = pu, place[v] = pv;
+    };
+    if constexpr (kPer <= 8) {
 #pragma unroll
-    for (int p = 1; p < kPer; p *= 2)
+        for (int round = 0; round < kPer; ++round)
 #pragma unroll
-        for (int k = p; k >= 1; k /= 2)
+            for (int i = round & 1; i + 1 < kPer; i += 2) exchange(i, i + 1, key[i + 1] > key[i]);
+    } else {
 #pragma unroll
-            for (int j = k % p; j + k < kPer; j += 2 * k)
+        for (int p = 1; p < kPer; p *= 2)
 #pragma unroll
-                for (int i = 0; i < k; ++i) {
-                    if (i + j + k >= kPer || (i + j) / (2 * p) != (i + j + k) / (2 * p)) continue;
-                    const int u = i + j, v = i + j + k;
-                    const bool swap = key[v] > key[u] || (key[v] == key[u] && place[v] < place[u]);
-                    const uint32_t ku = swap ? key[v] : key[u], kv = swap ? key[u] : key[v];
-                    const int pu = swap ? place[v] : place[u], pv = swap ? place[u] : place[v];
-                    key[u] = ku, key[v] = kv, place[u] = pu, place[v] = pv;
-                }
+            for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+                for (int j = k % p; j + k < kPer; j += 2 * k)
+#pragma unroll
+                    for (int i = 0; i < k; ++i) {
+                        const int u = i + j, v = i + j + k;
+                        if (v < kPer && u / (2 * p) == v / (2 * p)) exchange(u, v, key[v] > key[u] || (key[v] == key[u] && place[v] < place[u]));
+                    }
+    }
 }
 
 template <typename In, typename Out, int kPer> __global__ void __launch_bounds__(32 * kRouteWarps<kPer>) RouteKernel(const RouteArgs a)
 {
     // of a warp: its selection values by expert, a word apart every 32 (f64 too), and its logits
-    __shared__ double sRows[kRouteWarps<kPer>][33 * kPer];
+    __shared__ __align__(8) double sRows[kRouteWarps<kPer>][33 * kPer];
     __shared__ float sAllLogits[kRouteWarps<kPer>][32 * kPer];
     b200sp::WaitForPrevious();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const long long token = (long long)blockIdx.x * kRouteWarps<kPer> + warp;
     if (token >= a.tokens) return;
+    uint2 *const sList = reinterpret_cast<uint2 *>(sRows[warp]) + lane;  // the lane's sorted keys and experts, 32 apart
     const In *const row = static_cast<const In *>(a.logits) + token * a.ld;
     float *const sLogits = sAllLogits[warp];
     float x[kPer];
@@ -279,33 +293,30 @@ template <typename In, typename Out, int kPer> __global__ void __launch_bounds__
         place[j] = j;
     }
     SortDown<kPer>(key, place);
+    // The lists lie in shared memory; a lane has its first in hand.
+#pragma unroll
+    for (int j = 1; j < kPer; ++j) sList[32 * (j - 1)] = make_uint2(key[j], 32u * place[j] + lane);
+    sList[32 * (kPer - 1)] = make_uint2(0u, 0u);
+    uint2 head = make_uint2(key[0], 32u * place[0] + lane);
+    int at = 0;
     const uint32_t nothing = KeyOf(-INFINITY);
     Chosen c{-1, false};
     uint32_t top = 0;
     unsigned e = 0;
     for (int i = 0; i < a.k; ++i) {
-        top = __reduce_max_sync(kAll, key[0]);
-        e = __reduce_min_sync(kAll, key[0] == top ? 32u * place[0] + lane : ~0u);
+        top = __reduce_max_sync(kAll, head.x);
+        e = __reduce_min_sync(kAll, head.x == top ? head.y : ~0u);
         if (lane == i) c = {(int)e, top == nothing};
-        if (lane == (int)(e & 31)) {
-#pragma unroll
-            for (int j = 0; j + 1 < kPer; ++j) {
-                key[j] = key[j + 1];
-                place[j] = place[j + 1];
-            }
-            key[kPer - 1] = 0;
-        }
+        if (head.y == e && head.x != 0) head = sList[at], at += 32;
     }
     if (a.bias != nullptr) {
         // Neighbours of the last one taken, but for its equals in exact arithmetic too.
         const float last = ValueOf(top), room = 2 * error + 4.8e-7f * fabsf(last);
         const uint32_t near = top == nothing ? ~0u : KeyOf(last - room);
-        if (__any_sync(kAll, key[0] > nothing && key[0] >= near)) {
-            const float lastX = sLogits[e], lastBias = __ldg(a.bias + e);
-#pragma unroll
-            for (int j = 0; j < kPer; ++j) {
-                const int other = 32 * place[j] + lane;
-                if (key[j] > nothing && key[j] >= near) unsure |= !(sLogits[other] == lastX && __ldg(a.bias + other) == lastBias);
+        while (__any_sync(kAll, head.x > nothing && head.x >= near)) {
+            if (head.x > nothing && head.x >= near) {
+                unsure |= !(sLogits[head.y] == sLogits[e] && __ldg(a.bias + head.y) == __ldg(a.bias + e));
+                head = sList[at], at += 32;
             }
         }
     }
@@ -486,10 +497,11 @@ aclsparseStatus_t b200spRoute(aclsparseHandle_t handle, const b200spRouteRule *r
     const OnDevice device(handle);
     RouteArgs a{logits->values, bias != nullptr ? static_cast<const float *>(bias->values) : nullptr, logits->ld, (int)matR->rows,
                 (int)matR->cols, (int)(matR->nnz / matR->rows), rule->score == B200SP_ROUTE_SIGMOID, rule->groups, rule->groupsKept,
-                rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, 0, 0, static_cast<int *>(matR->offsets),
+                rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, 0, 0, 0, static_cast<int *>(matR->offsets),
                 static_cast<int *>(matR->indices), matR->values};
     if (a.kept == a.groups) a.groups = a.kept = 1;  // all are kept
     a.groupSize = a.experts / a.groups;
+    a.perGroup = ((1u << 20) + a.groupSize - 1) / a.groupSize;
     for (a.groupLanes = 32; a.groupLanes * a.groups > 32;) a.groupLanes /= 2;
     const cudaError_t e = WithPer(a.experts, [&](auto per) {
         return WithType(logits->valueType, [&](auto in) {
