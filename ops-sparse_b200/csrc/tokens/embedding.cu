@@ -6,6 +6,7 @@
 #include <climits>
 
 #include "b200sp_tokens.h"
+#include "common/rows.cuh"
 #include "tokens/common.cuh"
 #include "tokens/sort.cuh"
 
@@ -85,8 +86,8 @@ __global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
 
 // ---------------------------------------------------------------- the gradient of the table
 
-// The positions are sorted by token (sort.cuh), in the same launch as the zeros of dTable: the sort is one cluster's work
-// and the zeros everyone else's.  Then a group of lanes takes `chunk` sorted positions and sums their rows of grad, in
+// The positions are sorted by token (sort.cuh), in the same launch as some zeros of dTable: the sort is one cluster's work
+// and the zeros everyone else's; the other zeros are written beside the sums.  Then a group of lanes takes `chunk` sorted positions and sums their rows of grad, in
 // that order, one token after the other.  A token whose positions lie in one chunk is finished there; of one that
 // crosses chunks every chunk leaves a partial row, which EmbeddingJoinKernel adds up in their order.
 struct GradArgs {
@@ -99,23 +100,52 @@ struct GradArgs {
     float *heads, *tails;         // [chunk][pitch]: of the run that comes from the chunk before, that goes on in the next
     int pitch;
     int lanes;                    // threads side by side on a row
+    int fillFirst;                // with beta = 0: rows that get zeros while the tokens are sorted
+    unsigned sumBlocks, fillBlocks, sumAcross;  // CTAs of EmbeddingSumKernel: of either kind, and side by side on a row
     Scalars sc;
 };
 
+// Zeros for the first `fillFirst` rows.
 template <typename Out> __device__ __forceinline__ void FillTable(const GradArgs &a, int block, int blocks)
 {
     Out *const table = static_cast<Out *>(a.table);
-    const bool whole = a.ldTable == a.width;
-    if (whole && (reinterpret_cast<uintptr_t>(table) & 15) == 0) {
-        const long long bytes = (long long)a.vocab * a.width * (long long)sizeof(Out);
+    if (a.ldTable == a.width && (reinterpret_cast<uintptr_t>(table) & 15) == 0) {
+        const long long elements = (long long)a.fillFirst * a.width, pieces = elements * (long long)sizeof(Out) / 16;
         uint4 *const to = reinterpret_cast<uint4 *>(table);
-        for (long long i = (long long)block * blockDim.x + threadIdx.x; i < bytes / 16; i += (long long)blocks * blockDim.x)
-            __stcs(to + i, make_uint4(0, 0, 0, 0));
-        if (block == 0 && threadIdx.x < bytes % 16 / (long long)sizeof(Out)) table[bytes / 16 * (16 / sizeof(Out)) + threadIdx.x] = FromFloat<Out>(0.0f);
+        const long long step = (long long)blocks * blockDim.x;
+        long long i = (long long)block * blockDim.x + threadIdx.x;
+        for (; i + 3 * step < pieces; i += 4 * step) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) __stcs(to + i + u * step, make_uint4(0, 0, 0, 0));
+        }
+        for (; i < pieces; i += step) __stcs(to + i, make_uint4(0, 0, 0, 0));
+        const long long rest = pieces * (16 / (long long)sizeof(Out)) + threadIdx.x;
+        if (block == 0 && rest < elements) table[rest] = FromFloat<Out>(0.0f);
         return;
     }
-    for (int r = block; r < a.vocab; r += blocks)
+    for (int r = block; r < a.fillFirst; r += blocks)
         for (int c = threadIdx.x; c < a.width; c += blockDim.x) table[r * a.ldTable + c] = FromFloat<Out>(0.0f);
+}
+
+// Zeros for the rows after them whose tokens do not occur: a warp per row, some rows each.
+constexpr int kFillRows = 4;
+template <typename Out> __device__ __forceinline__ void FillOthers(const GradArgs &a, int block)
+{
+    const int lane = threadIdx.x & 31;
+    for (int i = 0; i < kFillRows; ++i) {
+        const long long r = (long long)a.fillFirst + ((long long)block * 8 + (threadIdx.x >> 5)) * kFillRows + i;
+        if (r >= a.vocab) return;
+        const int at = b200sp::WarpLowerBound(a.keys, a.count, r, lane);
+        if (at < a.count && __ldg(a.keys + at) == r) continue;
+        Out *const row = static_cast<Out *>(a.table) + r * a.ldTable;
+        int c = 0;
+        if ((reinterpret_cast<uintptr_t>(row) & 15) == 0) {
+            const int pieces = a.width * (int)sizeof(Out) / 16;
+            for (int k = lane; k < pieces; k += 32) __stcs(reinterpret_cast<uint4 *>(row) + k, make_uint4(0, 0, 0, 0));
+            c = pieces * (16 / (int)sizeof(Out));
+        }
+        for (c += lane; c < a.width; c += 32) row[c] = FromFloat<Out>(0.0f);
+    }
 }
 
 template <typename Out, typename Key>
@@ -180,8 +210,16 @@ constexpr int kGradDepth = 8;  // rows in flight
 template <typename In, typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingSumKernel(const GradArgs a)
 {
     b200sp::WaitForPrevious();
-    const int chunk = blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = (int)(blockIdx.y * a.lanes + threadIdx.x % a.lanes) * kN;
+    // CTAs that sum wait for rows of grad, CTAs that fill for nothing: they are mixed evenly.
+    const unsigned long long all = a.sumBlocks + a.fillBlocks;
+    const unsigned fills = (unsigned)(blockIdx.x * (unsigned long long)a.fillBlocks / all);  // before this one
+    if ((blockIdx.x + 1ull) * a.fillBlocks / all != fills) {
+        if (a.sc.Beta() == 0.0f) FillOthers<Out>(a, (int)fills);
+        return;
+    }
+    const unsigned block = blockIdx.x - fills;
+    const int chunk = (int)(block / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(block % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
     if (chunk >= a.chunks || col >= a.width) return;
     const int lo = chunk * a.chunk, hi = min(a.count, lo + a.chunk);
     const int before = lo > 0 ? __ldg(a.keys + lo - 1) : -1, after = hi < a.count ? __ldg(a.keys + hi) : -1;
@@ -234,36 +272,37 @@ template <typename In, typename Out, int kN> __global__ void __launch_bounds__(2
     flush(true);
 }
 
-// Tokens whose positions cross chunks: the chunk where one begins adds up what the others left.
+// Tokens whose positions cross chunks: the chunk where one begins adds up what the others left, eight at a time.
 template <typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingJoinKernel(const GradArgs a)
 {
     b200sp::WaitForPrevious();
-    const int chunk = blockIdx.x * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = (int)(blockIdx.y * a.lanes + threadIdx.x % a.lanes) * kN;
+    const int chunk = (int)(blockIdx.x / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(blockIdx.x % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
     if (chunk >= a.chunks - 1 || col >= a.width) return;
     const int hi = (chunk + 1) * a.chunk, lo = hi - a.chunk;
-    const int key = __ldg(a.keys + hi - 1);
-    if (key >= a.vocab || __ldg(a.keys + hi) != key) return;
-    if (lo > 0 && __ldg(a.keys + lo - 1) == key) return;  // began before
-    const int end = LowerBound(a.keys + hi, a.count - hi, key + 1) + hi;
-    const int lastChunk = (end - 1) / a.chunk;
+    const int key = __ldg(a.keys + hi - 1), next = __ldg(a.keys + hi), before = lo > 0 ? __ldg(a.keys + lo - 1) : -1;
+    if (key >= a.vocab || next != key || before == key) return;  // none crosses, or it began before
     float sum[kN];
     const float *at = a.tails + (long long)chunk * a.pitch + col;
 #pragma unroll
     for (int i = 0; i < kN; ++i) sum[i] = at[i];
-    for (int c = chunk + 1; c <= lastChunk; c += kGradDepth) {
+    bool more = true;
+    for (int c = chunk + 1; more && c < a.chunks; c += kGradDepth) {
         float v[kGradDepth][kN];
+        int starts[kGradDepth];
 #pragma unroll
         for (int u = 0; u < kGradDepth; ++u) {
-            const float *from = a.heads + (long long)min(c + u, lastChunk) * a.pitch + col;
+            const int from = min(c + u, a.chunks - 1);
+            starts[u] = c + u < a.chunks ? __ldg(a.keys + from * a.chunk) : -1;
+            const float *heads = a.heads + (long long)from * a.pitch + col;
 #pragma unroll
-            for (int i = 0; i < kN; ++i) v[u][i] = from[i];
+            for (int i = 0; i < kN; ++i) v[u][i] = heads[i];
         }
 #pragma unroll
         for (int u = 0; u < kGradDepth; ++u) {
-            if (c + u > lastChunk) continue;
+            more = more && starts[u] == key;  // the chunk begins with this token: its head is a piece of it
 #pragma unroll
-            for (int i = 0; i < kN; ++i) sum[i] += v[u][i];
+            for (int i = 0; i < kN; ++i) sum[i] = more ? sum[i] + v[u][i] : sum[i];
         }
     }
     FinishRow<Out, kN>(a, key, col, sum);
@@ -353,26 +392,30 @@ template <typename In, typename Out, int kN> cudaError_t LaunchSums(GradArgs a, 
     const long long vectors = (a.width + kN - 1) / kN;
     a.lanes = LanesFor(vectors, 256);
     const int perBlock = 256 / a.lanes;
-    const dim3 grid((unsigned)((a.chunks + perBlock - 1) / perBlock), (unsigned)((vectors + a.lanes - 1) / a.lanes));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(256);
-    cfg.stream = stream;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (grid.y > 65535) return cudaErrorInvalidConfiguration;
+    const long long across = (vectors + a.lanes - 1) / a.lanes, sums = (a.chunks + perBlock - 1) / perBlock * across;
+    const bool fills = a.sc.betaAt != nullptr || a.sc.beta == 0.0f;
+    const long long others = fills ? ((long long)a.vocab - a.fillFirst + 8 * kFillRows - 1) / (8 * kFillRows) : 0;
+    if (sums + others > INT32_MAX) return cudaErrorInvalidConfiguration;
+    a.sumAcross = (unsigned)across;
+    a.sumBlocks = (unsigned)sums;
+    a.fillBlocks = (unsigned)others;
     b200sp_note_launches(2);
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, EmbeddingSumKernel<In, Out, kN>, a);
-    return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, EmbeddingJoinKernel<Out, kN>, a);
+    const cudaError_t e = b200sp::LaunchChained(EmbeddingSumKernel<In, Out, kN>, (unsigned)(sums + others), 256, 0, stream, a);
+    return e != cudaSuccess ? e : b200sp::LaunchChained(EmbeddingJoinKernel<Out, kN>, (unsigned)sums, 256, 0, stream, a);
+}
+
+// Rows that are filled while the tokens are sorted: what is written in that time.  Rows of less than 1024 bytes all are: to look up whether a
+// token occurs costs more than to write them.
+constexpr long long kFillAhead = 64 << 20;
+int FillFirst(long long vocab, long long rowBytes)
+{
+    return (int)(rowBytes < 1024 ? vocab : std::min(vocab, std::max(1ll, kFillAhead / rowBytes)));
 }
 
 template <typename Out, typename Key> cudaError_t LaunchSort(const SortArgs &s, const GradArgs &a, cudaStream_t stream)
 {
-    const int size = SortCtas(a.count), shared = SortShared(s.digitBits);
-    const cudaError_t set = cudaFuncSetAttribute(EmbeddingSortKernel<Out, Key>, cudaFuncAttributeMaxDynamicSharedMemorySize, SortShared(kSortMaxBits));
+    const int size = SortCtas(a.count), shared = SortShared(s.digitBits, a.count <= kSortTile && s.passes > 1);
+    const cudaError_t set = cudaFuncSetAttribute(EmbeddingSortKernel<Out, Key>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSharedMost);
     if (set != cudaSuccess) return set;
     // one cluster sorts; the others fill the table, if it has to be (one CTA per SM: what the sort needs of shared memory)
     const bool fills = a.sc.betaAt != nullptr || a.sc.beta == 0.0f;
@@ -452,7 +495,7 @@ aclsparseStatus_t b200spEmbeddingGrad(aclsparseHandle_t handle, const void *alph
     s.keys = tokens->values;
     s.count = (int)tokens->size;
     s.limit = (int)dTable->rows;
-    SortPasses(s.limit, &s);
+    SortPasses(s.limit, s.count, &s);
     s.keyA = reinterpret_cast<int *>(p + L.keyA);
     s.posA = reinterpret_cast<int *>(p + L.posA);
     s.keyB = reinterpret_cast<int *>(p + L.keyB);
@@ -472,6 +515,7 @@ aclsparseStatus_t b200spEmbeddingGrad(aclsparseHandle_t handle, const void *alph
     a.heads = reinterpret_cast<float *>(p + L.heads);
     a.tails = reinterpret_cast<float *>(p + L.tails);
     a.pitch = L.pitch;
+    a.fillFirst = FillFirst(dTable->rows, dTable->cols * BytesOf(dTable->valueType));
     a.sc = ScalarsOf(handle, alpha, beta);
     const bool scales = a.sc.betaAt != nullptr || (a.sc.beta != 0.0f && a.sc.beta != 1.0f);
     const bool vectors = RowsAligned(grad) && RowsAligned(dTable);

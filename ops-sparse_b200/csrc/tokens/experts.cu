@@ -343,18 +343,18 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
     s.keys = matR->indices;
     s.count = (int)matR->nnz;
     s.limit = (int)matR->cols;
-    SortPasses(s.limit, &s);
+    SortPasses(s.limit, s.count, &s);
     s.keyA = reinterpret_cast<int *>(p + L.keyA);
     s.posA = reinterpret_cast<int *>(p + L.entries);
     s.keyB = reinterpret_cast<int *>(p + L.keyB);
     s.posB = reinterpret_cast<int *>(p + L.posB);
     s.offsets = s.passes == 1 ? offsets : nullptr;
-    cudaError_t e = cudaFuncSetAttribute(ExpertsOrderKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SortShared(kSortMaxBits));
+    cudaError_t e = cudaFuncSetAttribute(ExpertsOrderKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSharedMost);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)SortCtas(s.count));
         cfg.blockDim = dim3(kSortThreads);
-        cfg.dynamicSmemBytes = (size_t)SortShared(s.digitBits);
+        cfg.dynamicSmemBytes = (size_t)SortShared(s.digitBits, s.count <= kSortTile && s.passes > 1);
         cfg.stream = handle->stream;
         cudaLaunchAttribute attr[2] = {};
         attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

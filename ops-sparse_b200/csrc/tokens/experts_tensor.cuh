@@ -531,23 +531,34 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                             *to = FromFloat<Out>(u);
                         }
                     }
-                } else if (f0 + lane < features) {
-                    Out *const to = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f0 + lane) * a.ldo + m.first + c0;
-                    constexpr int kN = 16 / (int)sizeof(Out);
+                } else {
+                    constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
+                    Out *const out = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f0) * a.ldo + m.first + c0;
+                    if (a.vectors && beta == 0.0f && live == 32) {
+                        // The lane's row, its pieces exchanged so that neither side meets in a bank; then pieces of a row side by side.
 #pragma unroll
-                    for (int i = 0; i < 32; i += kN) {
-                        float u[kN];
+                        for (int i = 0; i < kPieces; ++i) {
+                            float u[kN];
 #pragma unroll
-                        for (int j = 0; j < kN; ++j) {
-                            u[j] = by * v[i + j];
-                            if (beta != 0.0f && i + j < live) u[j] = fmaf(beta, ToFloat(to[i + j]), u[j]);
+                            for (int j = 0; j < kN; ++j) u[j] = by * v[kN * i + j];
+                            StoreFloats<Out, kN, true>(sOut + 32 * lane + kN * (i ^ (lane * kPieces / 8 & (kPieces - 1))), u);
                         }
-                        if (a.vectors && i + kN <= live) {
-                            StoreFloats<Out, kN, true>(to + i, u);
-                        } else {
+                        __syncwarp();
 #pragma unroll
-                            for (int j = 0; j < kN; ++j)
-                                if (i + j < live) to[i + j] = FromFloat<Out>(u[j]);
+                        for (int i = 0; i < kPieces; ++i) {
+                            const int r = (32 * i + lane) / kPieces, at = lane % kPieces;
+                            const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + 32 * r + kN * (at ^ (r * kPieces / 8 & (kPieces - 1))));
+                            if (f0 + r < features) *reinterpret_cast<uint4 *>(out + r * a.ldo + kN * at) = piece;
+                        }
+                        __syncwarp();
+                    } else if (f0 + lane < features) {
+                        Out *const to = out + lane * a.ldo;
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) {
+                            if (i >= live) continue;
+                            float u = by * v[i];
+                            if (beta != 0.0f) u = fmaf(beta, ToFloat(to[i]), u);
+                            to[i] = FromFloat<Out>(u);
                         }
                     }
                 }

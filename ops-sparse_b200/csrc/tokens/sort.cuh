@@ -38,20 +38,24 @@ inline int SortBits(long long limit)  // of the numbers 0 ... limit
     while ((1ll << bits) <= limit) ++bits;
     return bits;
 }
-inline void SortPasses(long long limit, SortArgs *a)
+inline void SortPasses(long long limit, long long count, SortArgs *a)
 {
-    const int bits = SortBits(limit);
-    a->passes = (bits + kSortMaxBits - 1) / kSortMaxBits;
+    // in several passes a tile of its own lies beside the counts of a digit
+    const int bits = SortBits(limit), most = bits > kSortMaxBits && count <= kSortTile ? kSortMaxBits - 1 : kSortMaxBits;
+    a->passes = (bits + most - 1) / most;
     a->digitBits = (bits + a->passes - 1) / a->passes;
 }
+// Up to a tile one CTA, which keeps the positions in shared memory between the passes.
 inline int SortCtas(long long count)
 {
     int ctas = 1;
-    while (ctas < kSortMaxCtas && count > (long long)ctas * kSortTile / 2) ctas *= 2;
+    while (ctas < kSortMaxCtas && count > kSortTile && count > (long long)ctas * kSortTile / 2) ctas *= 2;
     return ctas;
 }
-// Shared memory: a word and a count per warp and digit, three numbers per digit.
-inline int SortShared(int digitBits) { return (1 << digitBits) * (kSortWarps * 6 + 3 * 4); }
+// Shared memory: a word and a count per warp and digit, three numbers per digit; a tile's keys and positions.
+inline int SortShared(int digitBits, bool tile) { return (1 << digitBits) * (kSortWarps * 6 + 3 * 4) + (tile ? kSortTile * 8 : 0); }
+constexpr int kSortSharedMost = (1 << kSortMaxBits) * (kSortWarps * 6 + 3 * 4);
+static_assert((1 << (kSortMaxBits - 1)) * (kSortWarps * 6 + 3 * 4) + kSortTile * 8 <= kSortSharedMost);
 
 template <typename Key> __device__ __forceinline__ int SortKey(const SortArgs &a, int i)
 {
@@ -59,9 +63,139 @@ template <typename Key> __device__ __forceinline__ int SortKey(const SortArgs &a
     return k < 0 || k >= (Key)a.limit ? a.limit : (int)k;
 }
 
+// Rank of the lane's position among its warp's of the same digit so far: the lanes of a digit find each other through its word
+// (mask: zero before and after).
+__device__ __forceinline__ int RankInWarp(uint32_t *mask, uint16_t *count, int d, bool in, int lane)
+{
+    if (in) atomicOr(mask + d, 1u << lane);
+    __syncwarp();
+    uint32_t peers = 0;
+    int had = 0;
+    if (in) {
+        peers = *static_cast<volatile uint32_t *>(mask + d);
+        had = *static_cast<volatile uint16_t *>(count + d);
+    }
+    const int among = __popc(peers & ((1u << lane) - 1u));
+    __syncwarp();
+    if (in && among == 0) {
+        mask[d] = 0;
+        count[d] = (uint16_t)(had + __popc(peers));
+    }
+    __syncwarp();
+    return had + among;
+}
+// A digit's counts by warp become the places of every warp's first; returns their sum.
+__device__ __forceinline__ int PlacesByWarp(uint16_t *counts, int bins, int warps)
+{
+    int run = 0;
+    for (int w = 0; w < warps; w += 8) {
+        int n[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) n[u] = w + u < warps ? counts[(w + u) * bins] : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+            if (w + u < warps) counts[(w + u) * bins] = (uint16_t)run;
+            run += n[u];
+        }
+    }
+    return run;
+}
+// Inclusive sums over the CTA's threads.
+__device__ __forceinline__ int SumsBefore(int own, int *sScan)
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = own;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += t;
+    }
+    if (lane == 31) sScan[warp] = incl;
+    __syncthreads();
+    if (warp == 0) {
+        int w = sScan[lane];
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int t = __shfl_up_sync(0xffffffffu, w, d);
+            if (lane >= d) w += t;
+        }
+        sScan[lane] = w;
+    }
+    __syncthreads();
+    return incl + (warp > 0 ? sScan[warp - 1] : 0);
+}
+
+// At most a tile, by one CTA: a thread holds four positions, which change places through shared memory.
+template <typename Key, typename Place> __device__ __forceinline__ void TileSort(const SortArgs &a, unsigned char *shared, Place &&place)
+{
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, bins = 1 << a.digitBits;
+    uint32_t *const sMask = reinterpret_cast<uint32_t *>(shared);            // [warp][digit]
+    int *const sBase = reinterpret_cast<int *>(sMask + kSortWarps * bins);   // [digit]
+    uint16_t *const sWarp = reinterpret_cast<uint16_t *>(sBase + 3 * bins);  // [warp][digit]
+    int2 *const sTile = reinterpret_cast<int2 *>(sWarp + kSortWarps * bins);
+    __shared__ int sScan[kSortWarps];
+    // As few warps as have positions, 128 each; the others only help to count.
+    const int warps = (a.count + 32 * kSortSteps - 1) / (32 * kSortSteps), first = warp * (32 * kSortSteps) + lane;
+    int key[kSortSteps], pos[kSortSteps];
+#pragma unroll
+    for (int u = 0; u < kSortSteps; ++u) {
+        pos[u] = first + 32 * u;
+        key[u] = pos[u] < a.count ? SortKey<Key>(a, pos[u]) : -1;
+    }
+    for (int i = tid; i < warps * bins; i += kSortThreads) sMask[i] = 0;
+    for (int p = 0; p < a.passes; ++p) {
+        const bool last = p == a.passes - 1;
+        const int shift = p * a.digitBits;
+        for (int i = tid; i < warps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(sWarp)[i] = 0;
+        __syncthreads();
+        int at[kSortSteps];
+        if (warp < warps) {
+#pragma unroll
+            for (int u = 0; u < kSortSteps; ++u)
+                at[u] = RankInWarp(sMask + warp * bins, sWarp + warp * bins, (key[u] >> shift) & (bins - 1), key[u] >= 0, lane);
+        }
+        __syncthreads();
+        const int own = tid < bins ? PlacesByWarp(sWarp + tid, bins, warps) : 0;
+        const int start = SumsBefore(own, sScan) - own;
+        if (tid < bins) {
+            sBase[tid] = start;
+            if (a.offsets != nullptr && tid <= a.limit + 1) a.offsets[tid] = start;
+            // 2^bits > limit: the end of the last key has a digit of its own unless the digits are used up
+            if (a.offsets != nullptr && tid == a.limit && a.limit + 1 == bins) a.offsets[bins] = a.count;
+        }
+        __syncthreads();
+        if (warp < warps) {
+#pragma unroll
+            for (int u = 0; u < kSortSteps; ++u) {
+                if (key[u] < 0) continue;
+                const int d = (key[u] >> shift) & (bins - 1), to = sBase[d] + sWarp[warp * bins + d] + at[u];
+                if (!last) {
+                    sTile[to] = make_int2(key[u], pos[u]);
+                } else {
+                    a.keyA[to] = key[u];
+                    a.posA[to] = pos[u];
+                    place(key[u], pos[u], to);
+                }
+            }
+        }
+        __syncthreads();  // the caller may read what was stored
+        if (last) break;
+#pragma unroll
+        for (int u = 0; u < kSortSteps; ++u) {
+            if (first + 32 * u >= a.count) continue;
+            key[u] = sTile[first + 32 * u].x;
+            pos[u] = sTile[first + 32 * u].y;
+        }
+    }
+}
+
 // All CTAs of the cluster, 1024 threads each; place(key, position, where) is told of every position in the last pass.
 template <typename Key, typename Place> __device__ __forceinline__ void ClusterSort(const SortArgs &a, unsigned char *shared, Place &&place)
 {
+    if (a.count <= kSortTile) {
+        TileSort<Key>(a, shared, place);
+        return;
+    }
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
@@ -99,26 +233,8 @@ template <typename Key, typename Place> __device__ __forceinline__ void ClusterS
                 all += n;
             }
         }
-        int incl = all;
-#pragma unroll
-        for (int d = 1; d < 32; d <<= 1) {
-            const int t = __shfl_up_sync(0xffffffffu, incl, d);
-            if (lane >= d) incl += t;
-        }
-        if (lane == 31) sScan[warp] = incl;
-        __syncthreads();
-        if (warp == 0) {
-            int w = sScan[lane];
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, w, d);
-                if (lane >= d) w += t;
-            }
-            sScan[lane] = w;
-        }
-        __syncthreads();
+        const int start = SumsBefore(all, sScan) - all;
         if (tid < bins) {
-            const int start = incl - all + (warp > 0 ? sScan[warp - 1] : 0);
             sBase[tid] = start + before;
             if (a.offsets != nullptr && rank == 0 && tid <= a.limit + 1) a.offsets[tid] = start;
             // 2^bits > limit: the end of the last key has a digit of its own unless the digits are used up
@@ -138,40 +254,11 @@ template <typename Key, typename Place> __device__ __forceinline__ void ClusterS
                     pos[u] = p == 0 ? i : __ldcg(posIn + i);
                 }
             }
-            // rank among the warp's positions of the same digit: the lanes of a digit find each other through its word
-            uint32_t *const mask = sMask + warp * bins;
-            uint16_t *const count = sWarp + warp * bins;
 #pragma unroll
-            for (int u = 0; u < kSortSteps; ++u) {
-                const int d = (key[u] >> shift) & (bins - 1);
-                const bool in = key[u] >= 0;
-                if (in) atomicOr(mask + d, 1u << lane);
-                __syncwarp();
-                uint32_t peers = 0;
-                int had = 0;
-                if (in) {
-                    peers = *static_cast<volatile uint32_t *>(mask + d);
-                    had = *static_cast<volatile uint16_t *>(count + d);
-                }
-                const int among = __popc(peers & ((1u << lane) - 1u));
-                __syncwarp();
-                if (in && among == 0) {
-                    mask[d] = 0;
-                    count[d] = (uint16_t)(had + __popc(peers));
-                }
-                __syncwarp();
-                at[u] = had + among;
-            }
+            for (int u = 0; u < kSortSteps; ++u)
+                at[u] = RankInWarp(sMask + warp * bins, sWarp + warp * bins, (key[u] >> shift) & (bins - 1), key[u] >= 0, lane);
             __syncthreads();
-            if (tid < bins) {  // counts become the places of every warp's first
-                int run = 0;
-                for (int w = 0; w < kSortWarps; ++w) {
-                    const int n = sWarp[w * bins + tid];
-                    sWarp[w * bins + tid] = (uint16_t)run;
-                    run += n;
-                }
-                sTile[tid] = run;
-            }
+            if (tid < bins) sTile[tid] = PlacesByWarp(sWarp + tid, bins, kSortWarps);
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < kSortSteps; ++u) {
