@@ -140,7 +140,8 @@ struct aclsparseSpMatDescr {
     b200sp::TileOrderPlan sddmm;  // of the SDDMM products that write this matrix
     mutable std::mutex sddmmMutex;  // held while it is read or written
     mutable b200sp::ExpertsPlan experts;
-    mutable std::mutex expertsMutex;  // held while it is read or written
+    mutable int64_t expertsSized = 0;  // the largest buffer that was asked for its products
+    mutable std::mutex expertsMutex;  // held while they are read or written
     mutable std::mutex copyMutex;  // held while a product that copies into the analysed buffer is enqueued
 };
 

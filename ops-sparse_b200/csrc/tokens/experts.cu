@@ -69,136 +69,27 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
     }
 }
 
+// ---------------------------------------------------------------- operands that do not start on 16 bytes
+
+// Rows of 16-bit elements into rows of a multiple of eight, zeros behind the last: what the copies of the products need.  A thread writes 16
+// bytes; what bounds it are the bytes, read and written once each (and read again by the product).
+__global__ void __launch_bounds__(256) ExpertsAlignKernel(const uint16_t *__restrict__ from, long long rows, int cols, long long ld,
+                                                          uint4 *__restrict__ to)
+{
+    b200sp::WaitForPrevious();
+    const int pieces = (cols + 7) / 8;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (long long)gridDim.x * 256) {
+        const long long r = i / pieces;
+        const int c = (int)(i - r * pieces) * 8;
+        const uint16_t *const row = from + r * ld + c;
+        __align__(16) uint16_t v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = c + u < cols ? __ldg(row + u) : 0;
+        to[i] = *reinterpret_cast<const uint4 *>(v);
+    }
+}
+
 // ---------------------------------------------------------------- products
-
-struct ProductArgs {
-    const int *offsets, *entries, *rows;
-    const void *x, *w, *dy;
-    void *out;
-    long long ldx, ldw, ldy, ldo;
-    int experts, nnz;
-    int n, d;          // rows and columns of an expert's matrix
-    int byEntry;       // X has a row per entry
-    int transposed;    // opW = T
-    Scalars sc;
-};
-
-constexpr int kTile = 64, kDepth = 16;
-
-// Which expert's which tile of 64 entries.  Group `experts` has the entries of no expert.
-__device__ __forceinline__ bool TileOf(const int *offsets, int groups, int tile, int *expert, int *first, int *end)
-{
-    for (int e = 0; e < groups; ++e) {
-        const int lo = __ldg(offsets + e), hi = __ldg(offsets + e + 1), tiles = (hi - lo + kTile - 1) / kTile;
-        if (tile < tiles) {
-            *expert = e;
-            *first = lo + tile * kTile;
-            *end = hi;
-            return true;
-        }
-        tile -= tiles;
-    }
-    return false;
-}
-
-template <typename T, typename Out> __global__ void __launch_bounds__(256) ExpertsSimpleKernel(const ProductArgs a)
-{
-    __shared__ float sX[kDepth][kTile + 4], sW[kDepth][kTile + 4];
-    b200sp::WaitForPrevious();
-    int expert, first, end;
-    if (!TileOf(a.offsets, a.experts + 1, blockIdx.y, &expert, &first, &end)) return;
-    const int cols = a.transposed ? a.n : a.d, depth = a.transposed ? a.d : a.n, c0 = blockIdx.x * kTile;
-    const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    float acc[4][4] = {};
-    if (expert < a.experts) {
-        const T *const w = static_cast<const T *>(a.w) + (long long)expert * a.n * a.ldw;
-        for (int k0 = 0; k0 < depth; k0 += kDepth) {
-            for (int i = tid; i < kTile * kDepth; i += 256) {
-                const int r = i / kDepth, k = k0 + i % kDepth;
-                float v = 0.0f;
-                if (first + r < end && k < depth) {
-                    const long long row = a.byEntry ? __ldg(a.entries + first + r) : __ldg(a.rows + first + r);
-                    v = ToFloat(static_cast<const T *>(a.x)[row * a.ldx + k]);
-                }
-                sX[i % kDepth][r] = v;
-                const int c = a.transposed ? i / kDepth : i % kTile, kw = a.transposed ? i % kDepth : i / kTile;
-                float u = 0.0f;
-                if (c0 + c < cols && k0 + kw < depth)
-                    u = ToFloat(a.transposed ? w[(long long)(c0 + c) * a.ldw + k0 + kw] : w[(long long)(k0 + kw) * a.ldw + c0 + c]);
-                sW[kw][c] = u;
-            }
-            __syncthreads();
-#pragma unroll
-            for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sX[k][ty * 4 + i], sW[k][tx + 16 * j], acc[i][j]);
-            __syncthreads();
-        }
-    }
-    const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int at = first + ty * 4 + i;
-        if (at >= end) continue;
-        Out *const out = static_cast<Out *>(a.out) + __ldg(a.entries + at) * a.ldo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = c0 + tx + 16 * j;
-            if (c >= cols) continue;
-            float v = alpha * acc[i][j];
-            if (expert == a.experts) v = 0.0f;
-            if (beta != 0.0f) v = fmaf(beta, ToFloat(out[c]), v);
-            out[c] = FromFloat<Out>(v);
-        }
-    }
-}
-
-template <typename T, typename Out> __global__ void __launch_bounds__(256) ExpertsSimpleGradKernel(const ProductArgs a)
-{
-    __shared__ float sY[kDepth][kTile + 4], sX[kDepth][kTile + 4];
-    b200sp::WaitForPrevious();
-    const int expert = blockIdx.z, d0 = blockIdx.x * kTile, n0 = blockIdx.y * kTile;
-    const int lo = __ldg(a.offsets + expert), hi = __ldg(a.offsets + expert + 1);
-    const int tid = threadIdx.x, tx = tid % 16, ty = tid / 16;
-    float acc[4][4] = {};
-    for (int k0 = lo; k0 < hi; k0 += kDepth) {
-        for (int i = tid; i < kTile * kDepth; i += 256) {
-            const int k = i / kTile, c = i % kTile;
-            float y = 0.0f, x = 0.0f;
-            if (k0 + k < hi) {
-                const long long entry = __ldg(a.entries + k0 + k), row = a.byEntry ? entry : __ldg(a.rows + k0 + k);
-                if (n0 + c < a.n) y = ToFloat(static_cast<const T *>(a.dy)[entry * a.ldy + n0 + c]);
-                if (d0 + c < a.d) x = ToFloat(static_cast<const T *>(a.x)[row * a.ldx + d0 + c]);
-            }
-            sY[k][c] = y;
-            sX[k][c] = x;
-        }
-        __syncthreads();
-#pragma unroll
-        for (int k = 0; k < kDepth; ++k)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(sY[k][ty * 4 + i], sX[k][tx + 16 * j], acc[i][j]);
-        __syncthreads();
-    }
-    const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (n0 + ty * 4 + i >= a.n) continue;
-        Out *const out = static_cast<Out *>(a.out) + ((long long)expert * a.n + n0 + ty * 4 + i) * a.ldo;
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int c = d0 + tx + 16 * j;
-            if (c >= a.d) continue;
-            float v = lo < hi ? alpha * acc[i][j] : 0.0f;
-            if (beta != 0.0f) v = fmaf(beta, ToFloat(out[c]), v);
-            out[c] = FromFloat<Out>(v);
-        }
-    }
-}
 
 #include "tokens/experts_tensor.cuh"
 
@@ -270,39 +161,66 @@ bool HoldsOrder(const aclsparseSpMatDescr *R, const void *buffer)
            p.cols == R->cols && p.nnz == R->nnz && p.generation != 0 && p.generation == b200sp::BufferGeneration(buffer);
 }
 
-ProductArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, void *buffer, const Scalars &sc)
+MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const void *buffer, const aclsparseDnMatDescr *stacked,
+               const aclsparseDnMatDescr *out, const Scalars &sc)
 {
     const PlanLayout L = PlanLayoutFor(R->nnz, R->cols);
     const char *p = BufferStart(buffer);
-    ProductArgs a{};
+    MmaArgs a{};
     a.offsets = reinterpret_cast<const int *>(p + L.offsets);
     a.entries = reinterpret_cast<const int *>(p + L.entries);
     a.rows = reinterpret_cast<const int *>(p + L.rows);
+    a.out = out->values;
+    a.ldo = out->ld;
+    a.vectors = RowsAligned(out);
     a.experts = (int)R->cols;
-    a.nnz = (int)R->nnz;
+    a.n = (int)(stacked->rows / R->cols);
+    a.d = (int)stacked->cols;
     a.byEntry = rowsOfX == B200SP_ROWS_OF_ENTRIES;
     a.sc = sc;
     return a;
 }
 
-MmaArgs TensorArgsOf(const ProductArgs &a, const aclsparseSpMatDescr *R)
+// Bytes for a copy of an operand whose rows do not start on multiples of 16 bytes.
+size_t AlignedBytes(const aclsparseDnMatDescr *m)
 {
-    MmaArgs t{};
-    t.offsets = a.offsets;
-    t.entries = a.entries;
-    t.rows = a.rows;
-    t.out = a.out;
-    t.dy = a.dy;
-    t.x = a.x;
-    t.ldy = a.ldy;
-    t.ldx = a.ldx;
-    t.ldo = a.ldo;
-    t.experts = (int)R->cols;
-    t.n = a.n;
-    t.d = a.d;
-    t.byEntry = a.byEntry;
-    t.sc = a.sc;
-    return t;
+    return RowsAligned(m) ? 0 : AlignUp((size_t)m->rows * AlignUp((size_t)m->cols, 8) * 2, 256);
+}
+size_t BufferBytes(const aclsparseSpMatDescr *R, const aclsparseDnMatDescr *first, const aclsparseDnMatDescr *second)
+{
+    return PlanLayoutFor(R->nnz, R->cols).total + AlignedBytes(first) + AlignedBytes(second);
+}
+// What the BufferSize calls for this matrix have said at most.
+size_t NoteSize(const aclsparseSpMatDescr *R, size_t bytes)
+{
+    std::lock_guard<std::mutex> lock(R->expertsMutex);
+    R->expertsSized = std::max(R->expertsSized, (int64_t)bytes);
+    return bytes;
+}
+bool Sized(const aclsparseSpMatDescr *R, size_t bytes)
+{
+    std::lock_guard<std::mutex> lock(R->expertsMutex);
+    return (int64_t)bytes <= R->expertsSized;
+}
+
+// An operand as the kernels read it: where it lies, or its copy at `room`, which moves on.
+struct Operand {
+    const void *values;
+    long long ld;
+    cudaError_t error;
+};
+Operand Aligned(const aclsparseDnMatDescr *m, char **room, cudaStream_t stream)
+{
+    const size_t bytes = AlignedBytes(m);
+    if (bytes == 0) return {m->values, m->ld, cudaSuccess};
+    char *const to = *room;
+    *room += bytes;
+    const long long pieces = m->rows * ((m->cols + 7) / 8);
+    const unsigned blocks = (unsigned)std::min<long long>((pieces + 255) / 256, (long long)b200sp_sm_count() * 32);
+    b200sp_note_launches(1);
+    const cudaError_t e = b200sp::LaunchChained(ExpertsAlignKernel, blocks, 256, 0, stream, static_cast<const uint16_t *>(m->values),
+                                                m->rows, (int)m->cols, m->ld, reinterpret_cast<uint4 *>(to));
+    return {to, (long long)AlignUp((size_t)m->cols, 8), e};
 }
 
 }  // namespace
@@ -382,7 +300,7 @@ aclsparseStatus_t b200spExpertsMMBufferSize(aclsparseHandle_t handle, aclsparseO
     if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const aclsparseStatus_t st = CheckMM(opW, rowsOfX, matR, matX, matW, matY);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    *bufferSize = PlanLayoutFor(matR->nnz, matR->cols).total;
+    *bufferSize = NoteSize(matR, BufferBytes(matR, matX, matW));
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 
@@ -394,46 +312,31 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     const aclsparseStatus_t st = CheckMM(opW, rowsOfX, matR, matX, matW, matY);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer) || !Sized(matR, BufferBytes(matR, matX, matW))) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
-    ProductArgs a = ArgsOf(matR, rowsOfX, buffer, ScalarsOf(handle, alpha, beta));
-    a.x = matX->values;
-    a.w = matW->values;
-    a.out = matY->values;
-    a.ldx = matX->ld;
-    a.ldw = matW->ld;
-    a.ldo = matY->ld;
-    a.n = (int)(matW->rows / matR->cols);
-    a.d = (int)matW->cols;
-    a.transposed = opW == ACL_SPARSE_OP_TRANSPOSE;
-    if (RowsAligned(matX) && RowsAligned(matW)) {
-        MmaArgs t = TensorArgsOf(a, matR);
-        t.colsMost = TileColumns(matR->nnz, matR->cols);
-        t.vectors = RowsAligned(matY);
-        CUtensorMap mapW;
-        if (!MapOf(&mapW, matW->valueType, matW->values, a.d, a.n, matW->ld, (int)matR->cols, a.transposed ? kMmaRows : kMmaDepth))
-            return ACL_SPARSE_STATUS_INTERNAL_ERROR;
-        const cudaError_t e = WithType(matX->valueType, [&](auto in) {
-            return WithType(matY->valueType, [&](auto out) {
-                using T = decltype(in);
-                using Out = decltype(out);
-                if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
-                    return a.transposed ? LaunchTensor<T, Out, Mode::kProductT>(t, mapW, handle->stream)
-                                        : LaunchTensor<T, Out, Mode::kProductN>(t, mapW, handle->stream);
-                else
-                    return cudaErrorInvalidValue;  // refused above
-            });
-        });
-        return Finished(e, "b200spExpertsMM");
-    }
-    const dim3 grid((unsigned)((matY->cols + kTile - 1) / kTile), (unsigned)((a.nnz + kTile - 1) / kTile + a.experts + 1));
-    b200sp_note_launches(1);
-    WithType(matX->valueType, [&](auto in) {
-        WithType(matY->valueType, [&](auto out) {
-            if constexpr (sizeof(in) == 2) ExpertsSimpleKernel<decltype(in), decltype(out)><<<grid, 256, 0, handle->stream>>>(a);
+    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, matW, matY, ScalarsOf(handle, alpha, beta));
+    char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
+    const Operand x = Aligned(matX, &room, handle->stream), w = Aligned(matW, &room, handle->stream);
+    if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, "b200spExpertsMM");
+    a.x = x.values;
+    a.ldx = x.ld;
+    a.colsMost = TileColumns(matR->nnz, matR->cols);
+    const bool transposed = opW == ACL_SPARSE_OP_TRANSPOSE;
+    CUtensorMap mapW;
+    if (!MapOf(&mapW, matW->valueType, w.values, a.d, a.n, w.ld, a.experts, transposed ? kMmaRows : kMmaDepth))
+        return ACL_SPARSE_STATUS_INTERNAL_ERROR;
+    const cudaError_t e = WithType(matX->valueType, [&](auto in) {
+        return WithType(matY->valueType, [&](auto out) {
+            using T = decltype(in);
+            using Out = decltype(out);
+            if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
+                return transposed ? LaunchTensor<T, Out, Mode::kProductT>(a, mapW, handle->stream)
+                                  : LaunchTensor<T, Out, Mode::kProductN>(a, mapW, handle->stream);
+            else
+                return cudaErrorInvalidValue;  // refused above
         });
     });
-    return Finished(cudaGetLastError(), "b200spExpertsMM");
+    return Finished(e, "b200spExpertsMM");
 }
 
 aclsparseStatus_t b200spExpertsGradBufferSize(aclsparseHandle_t handle, b200spExpertRows_t rowsOfX, aclsparseConstSpMatDescr_t matR,
@@ -444,7 +347,7 @@ aclsparseStatus_t b200spExpertsGradBufferSize(aclsparseHandle_t handle, b200spEx
     if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const aclsparseStatus_t st = CheckGrad(rowsOfX, matR, dY, matX, dW);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
-    *bufferSize = PlanLayoutFor(matR->nnz, matR->cols).total;
+    *bufferSize = NoteSize(matR, BufferBytes(matR, matX, dY));
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 
@@ -456,42 +359,29 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     const aclsparseStatus_t st = CheckGrad(rowsOfX, matR, dY, matX, dW);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer) || !Sized(matR, BufferBytes(matR, matX, dY))) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
-    ProductArgs a = ArgsOf(matR, rowsOfX, buffer, ScalarsOf(handle, alpha, beta));
-    a.x = matX->values;
-    a.dy = dY->values;
-    a.out = dW->values;
-    a.ldx = matX->ld;
-    a.ldy = dY->ld;
-    a.ldo = dW->ld;
-    a.n = (int)(dW->rows / matR->cols);
-    a.d = (int)dW->cols;
-    if (RowsAligned(matX) && RowsAligned(dY)) {
-        MmaArgs t = TensorArgsOf(a, matR);
-        t.colsMost = kMmaColsMost;
-        t.vectors = RowsAligned(dW);
-        const CUtensorMap none{};
-        const cudaError_t e = WithType(matX->valueType, [&](auto in) {
-            return WithType(dW->valueType, [&](auto out) {
-                using T = decltype(in);
-                using Out = decltype(out);
-                if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
-                    return LaunchTensor<T, Out, Mode::kGrad>(t, none, handle->stream);
-                else
-                    return cudaErrorInvalidValue;  // refused above
-            });
-        });
-        return Finished(e, "b200spExpertsGrad");
-    }
-    const dim3 grid((unsigned)((a.d + kTile - 1) / kTile), (unsigned)((a.n + kTile - 1) / kTile), (unsigned)a.experts);
-    b200sp_note_launches(1);
-    WithType(matX->valueType, [&](auto in) {
-        WithType(dW->valueType, [&](auto out) {
-            if constexpr (sizeof(in) == 2) ExpertsSimpleGradKernel<decltype(in), decltype(out)><<<grid, 256, 0, handle->stream>>>(a);
+    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, dW, dW, ScalarsOf(handle, alpha, beta));
+    char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
+    const Operand x = Aligned(matX, &room, handle->stream), y = Aligned(dY, &room, handle->stream);
+    if (x.error != cudaSuccess || y.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : y.error, "b200spExpertsGrad");
+    a.x = x.values;
+    a.ldx = x.ld;
+    a.dy = y.values;
+    a.ldy = y.ld;
+    a.colsMost = kMmaColsMost;
+    const CUtensorMap none{};
+    const cudaError_t e = WithType(matX->valueType, [&](auto in) {
+        return WithType(dW->valueType, [&](auto out) {
+            using T = decltype(in);
+            using Out = decltype(out);
+            if constexpr (sizeof(T) == 2 && (sizeof(Out) == 4 || std::is_same_v<T, Out>))
+                return LaunchTensor<T, Out, Mode::kGrad>(a, none, handle->stream);
+            else
+                return cudaErrorInvalidValue;  // refused above
         });
     });
-    return Finished(cudaGetLastError(), "b200spExpertsGrad");
+    return Finished(e, "b200spExpertsGrad");
 }
 
 }  // extern "C"

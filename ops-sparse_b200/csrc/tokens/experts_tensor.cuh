@@ -27,7 +27,7 @@ constexpr int kMmaBlockBytes = kMmaDepth * 128;    // MN-major: 64 rows along th
 constexpr int kMmaShared = 192 << 10;              // for stages
 constexpr int kMmaStagesMost = 12;
 template <typename Out> constexpr int kMmaStoreBytes = 4 * 32 * 32 * (int)sizeof(Out);  // 32 x 32 results of each storing warp
-constexpr int kMmaParts = 2, kMmaGatherStages = 6, kMmaGatherWarps = kMmaParts * kMmaGatherStages;  // warps at a stage, stages at a time
+constexpr int kMmaGatherWarps = 12, kMmaPartsMost = 2;  // warps that gather, of them at a stage
 constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
 constexpr int kMmaThreads = 32 * (kMmaFirstGather + kMmaGatherWarps);
 constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
@@ -45,6 +45,7 @@ struct MmaArgs {
     int vectors;           // rows of the output start on 16 bytes
     int colsMost;          // of a tile
     int stages, stageBytes;
+    int parts;             // warps that gather a stage
     Scalars sc;
     long long waitCycles;
     unsigned extraTx;      // 0 outside the wait test: bytes that W's barrier expects beyond those copied; gathering threads do not arrive
@@ -247,7 +248,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
-            BarInit(sFull + s, (kMode != Mode::kGrad) + kMmaParts * (kPair ? 2 : 1));  // W's request, the gathering warps of every CTA
+            BarInit(sFull + s, (kMode != Mode::kGrad) + a.parts * (kPair ? 2 : 1));  // W's request, the gathering warps of every CTA
             BarInit(sEmpty + s, 1);
         }
         for (int i = 0; i < 2; ++i) {
@@ -311,14 +312,14 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         if (failed && rank == 0)  // copies on their way: a bounded chance to land
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
-    } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + kMmaParts * a.stages) {
+    } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + a.parts * a.stages) {
         // Stages are the warps' in turn: one asks for all of its rows, waits for them and says so, while the others are at the stages
         // beside it.  No more warps than stages: whoever is at stage q knows that q - stages has been used up, so that the wait for
         // q + warps - stages can not be answered by the round before it.  (All warps at every stage, a share each, take turns with it: with the arrivals of 256 threads, and a
         // thread that passes them on to the other CTA, a stage's round took 2900 clocks without any copy.)
         // Eight lanes side by side on 128 bytes of a row: lane l has piece l % 8 of rows l / 8, l / 8 + 4, ...
-        const int mine = (warp - kMmaFirstGather) / kMmaParts, part = (warp - kMmaFirstGather) % kMmaParts;
-        const int warps = min(kMmaGatherStages, a.stages), piece = lane & 7, high = lane >> 3;
+        const int mine = (warp - kMmaFirstGather) / a.parts, part = (warp - kMmaFirstGather) % a.parts;
+        const int warps = min(kMmaGatherWarps / a.parts, a.stages), piece = lane & 7, high = lane >> 3;
         const uint32_t place = base + high * 128;
         const uint32_t even = (uint32_t)(piece ^ high) << 4, odd = (uint32_t)(piece ^ (high + 4)) << 4;  // swizzled: rows high, high + 4 of eight
         Ring ring;
@@ -333,12 +334,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         };
         int turn = mine;  // steps until the next of this warp's stages
         if constexpr (kMode != Mode::kGrad) {
-            constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32 / kMmaParts;  // times 32: rows part + kMmaParts * (0, 1, ...) of eight each
+            constexpr int kRows = kMmaColsMost / (kPair ? 2 : 1) / 32 / kMmaPartsMost;  // times 32
             const int depth = kMode == Mode::kProductT ? a.d : a.n;
             const int *const rowOf = a.byEntry ? a.entries : a.rows;
             const char *const x = static_cast<const char *>(a.x);
             const uint32_t pitch = (uint32_t)a.ldx * 2;
-            // Eights of rows belong to the parts in turn: the lane's own, of which it knows the places, are row 8 * (part + kMmaParts * e)
+            // Eights of rows belong to the parts in turn: the lane's own, of which it knows the places, are row 8 * (part + parts * e)
             // + lane % 8 with e = lane / 8, lane / 8 + 4, ...  (What is past the last entry is a copy of row 0, of whose sums nobody asks.)
             uint32_t row[kRows];
             MmaTile next;
@@ -348,7 +349,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 const int share = kPair ? next.wide / 2 : next.wide;
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) {
-                    const int within = 8 * (part + kMmaParts * (4 * i + lane / 8)) + lane % 8, r = rank * share + within;
+                    const int within = 8 * (part + a.parts * (4 * i + lane / 8)) + lane % 8, r = rank * share + within;
                     row[i] = next.steps > 0 && within < share && r < next.many ? (uint32_t)__ldg(rowOf + next.first + r) : 0;
                 }
             };
@@ -359,7 +360,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 uint32_t now[kRows];
 #pragma unroll
                 for (int i = 0; i < kRows; ++i) now[i] = row[i];
-                const int eights = (share / 8 - part + kMmaParts - 1) / kMmaParts;  // of this part
+                const int eights = (share / 8 - part + a.parts - 1) / a.parts;  // of this part
                 look(t + step);
                 for (; turn < m.steps; turn += warps) {
                     if (!free()) {
@@ -375,7 +376,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         for (int j = 0; j < 8; ++j) {
                             if (4 * i + j / 2 >= eights) break;
                             const uint32_t r = __shfl_sync(0xffffffffu, now[i], 4 * j + high);
-                            CopyPiece(at + (4 * i + j / 2) * (1024 * kMmaParts) + (j & 1) * 512 + (j & 1 ? odd : even), from + (uint64_t)r * pitch, left);
+                            CopyPiece(at + (4 * i + j / 2) * (1024 * a.parts) + (j & 1) * 512 + (j & 1 ? odd : even), from + (uint64_t)r * pitch, left);
                         }
                     }
                     asked();
@@ -624,6 +625,8 @@ cudaError_t LaunchTiles(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
 {
     a.stageBytes = kMmaABytes + a.colsMost * 128 / (kPair ? 2 : 1);
     a.stages = std::min(kMmaShared / a.stageBytes, kMmaStagesMost);
+    // Few rows are one warp's, so that more stages are on their way: with two warps at each of six stages a step of a tile of 32 entries takes 300 ns.
+    a.parts = kMode != Mode::kGrad && a.colsMost <= kMmaColsMost / kMmaPartsMost / (kPair ? 2 : 1) ? 1 : kMmaPartsMost;
     a.waitCycles = gExpertsWaitCycles;
     a.extraTx = gExpertsExtraTx;
     const auto kernel = ExpertsTensorKernel<T, Out, kMode, kPair>;
