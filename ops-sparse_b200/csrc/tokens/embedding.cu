@@ -4,6 +4,7 @@
 // dTable.  Neither reuses anything, so both are bound by the bytes of their rows.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "b200sp_tokens.h"
 #include "common/rows.cuh"
@@ -27,7 +28,51 @@ struct EmbedArgs {
     Scalars sc;
 };
 
-constexpr int kEmbedDepth = 4;  // vectors in flight per thread
+// What bounds it is how much is on the way: four vectors a thread, held as they were read.  16,384 rows of 4096 bf16: 47 us, with two or
+// eight vectors 51 and 49, with four held as floats 70.
+constexpr int kEmbedDepth = 4;
+
+// A vector of kN elements of the table's type, as it lies: in words, of which a 16-bit element alone fills half.
+template <typename In, int kN> struct RawRow {
+    static constexpr int kWords = kN * (int)sizeof(In) < 4 ? 1 : kN * (int)sizeof(In) / 4;
+    uint32_t words[kWords];
+    __device__ __forceinline__ void Load(const In *from, int left, bool in)
+    {
+        if constexpr (kN > 1) {
+            if (in && left >= kN) {
+#pragma unroll
+                for (int i = 0; i < kWords; i += 4) {
+                    const uint4 v = __ldg(reinterpret_cast<const uint4 *>(from) + i / 4);
+                    words[i] = v.x, words[i + 1] = v.y, words[i + 2] = v.z, words[i + 3] = v.w;
+                }
+                return;
+            }
+        }
+        constexpr int kEach = 4 / (int)sizeof(In);
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) {
+            words[i] = 0;
+#pragma unroll
+            for (int j = 0; j < kEach && kEach * i + j < kN; ++j)
+                if (in && kEach * i + j < left) words[i] |= Bits(from[kEach * i + j]) << (16 * j);
+        }
+    }
+    __device__ __forceinline__ float At(int i) const
+    {
+        if constexpr (sizeof(In) == 4) return __uint_as_float(words[i]);
+        else return ToFloat(Element(static_cast<uint16_t>(words[i / 2] >> (16 * (i & 1)))));
+    }
+
+private:
+    static __device__ __forceinline__ uint32_t Bits(float v) { return __float_as_uint(v); }
+    static __device__ __forceinline__ uint32_t Bits(__half v) { return __half_as_ushort(v); }
+    static __device__ __forceinline__ uint32_t Bits(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+    static __device__ __forceinline__ In Element(uint16_t v)
+    {
+        if constexpr (std::is_same_v<In, __half>) return __ushort_as_half(v);
+        else return __ushort_as_bfloat16(v);
+    }
+};
 
 template <typename In, typename Out, typename Key, int kN>
 __global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
@@ -38,48 +83,47 @@ __global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
     const int rowsPerWarp = 32 / a.lanes, sub = lane / a.lanes, at = lane % a.lanes;
     const unsigned long long first = ((unsigned long long)blockIdx.x * 8 + (threadIdx.x >> 5)) * kEmbedDepth * rowsPerWarp + sub;
     const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-    float v[kEmbedDepth][kN];
-    long long row[kEmbedDepth];
-    int col[kEmbedDepth];
+    RawRow<In, kN> raw[kEmbedDepth];
+    long long to[kEmbedDepth];  // -1: nothing
+    int left[kEmbedDepth];      // elements of the row from here
 #pragma unroll
     for (int u = 0; u < kEmbedDepth; ++u) {
         const unsigned long long piece = first + (unsigned long long)u * rowsPerWarp;
-        row[u] = -1;
+        to[u] = -1;
         if (piece >= a.pieces) continue;
+        long long row;
+        int col;
         if (a.pieces <= UINT_MAX) {
-            row[u] = (unsigned)piece / a.perRow;
-            col[u] = (int)(((unsigned)piece % a.perRow) * a.lanes + at) * kN;
+            row = (unsigned)piece / a.perRow;
+            col = (int)(((unsigned)piece % a.perRow) * a.lanes + at) * kN;
         } else {
-            row[u] = (long long)(piece / a.perRow);
-            col[u] = (int)(piece % a.perRow * a.lanes + at) * kN;
+            row = (long long)(piece / a.perRow);
+            col = (int)(piece % a.perRow * a.lanes + at) * kN;
         }
-        if (col[u] >= a.width) row[u] = -1;
-        if (row[u] < 0) continue;
-        const Key token = static_cast<const Key *>(a.tokens)[row[u]];
+        left[u] = a.width - col;
+        if (left[u] <= 0) continue;
+        to[u] = row * a.ldOut + col;
+        const Key token = __ldg(static_cast<const Key *>(a.tokens) + row);
         const bool in = token >= 0 && token < (Key)a.vocab;
-        const In *const from = static_cast<const In *>(a.table) + (long long)(in ? token : 0) * a.ldTable + col[u];
-        if (in && col[u] + kN <= a.width) {
-            LoadFloats<In, kN, kVector>(from, v[u]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < kN; ++i) v[u][i] = in && col[u] + i < a.width ? ToFloat(from[i]) : 0.0f;
-        }
+        const In *const from = static_cast<const In *>(a.table) + (long long)(in ? token : 0) * a.ldTable + col;
+        raw[u].Load(from, left[u], in);
     }
 #pragma unroll
     for (int u = 0; u < kEmbedDepth; ++u) {
-        if (row[u] < 0) continue;
-        Out *const to = static_cast<Out *>(a.out) + row[u] * a.ldOut + col[u];
+        if (to[u] < 0) continue;
+        Out *const out = static_cast<Out *>(a.out) + to[u];
+        float v[kN];
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            v[u][i] *= alpha;
-            if (beta != 0.0f && col[u] + i < a.width) v[u][i] = fmaf(beta, ToFloat(to[i]), v[u][i]);
+            v[i] = alpha * raw[u].At(i);
+            if (beta != 0.0f && i < left[u]) v[i] = fmaf(beta, ToFloat(out[i]), v[i]);
         }
-        if (col[u] + kN <= a.width) {
-            StoreFloats<Out, kN, kVector>(to, v[u]);
+        if (left[u] >= kN) {
+            StoreFloats<Out, kN, kVector>(out, v);
         } else {
 #pragma unroll
             for (int i = 0; i < kN; ++i)
-                if (col[u] + i < a.width) to[i] = FromFloat<Out>(v[u][i]);
+                if (i < left[u]) out[i] = FromFloat<Out>(v[i]);
         }
     }
 }
@@ -87,9 +131,12 @@ __global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
 // ---------------------------------------------------------------- the gradient of the table
 
 // The positions are sorted by token (sort.cuh), in the same launch as some zeros of dTable: the sort is one cluster's work
-// and the zeros everyone else's; the other zeros are written beside the sums.  Then a group of lanes takes `chunk` sorted positions and sums their rows of grad, in
+// and the zeros everyone else's; the other zeros are written beside the joins, which are few and wait long.  Then a group of lanes takes `chunk` sorted positions and sums their rows of grad, in
 // that order, one token after the other.  A token whose positions lie in one chunk is finished there; of one that
 // crosses chunks every chunk leaves a partial row, which EmbeddingJoinKernel adds up in their order.
+// 16,384 rows of 2048 bf16, a table of 65,536 rows in f32 (604 MB): 119 us; 164 with a part of the zeros beside the sums, whose reads wait
+// longer then; 199 with all zeros beside the sort, and rows held as floats, eight deep.  (Zeros alone run at 3.8 TB/s in long stretches, 6.3
+// a row per warp.)
 struct GradArgs {
     const void *grad;
     void *table;
@@ -101,7 +148,8 @@ struct GradArgs {
     int pitch;
     int lanes;                    // threads side by side on a row
     int fillFirst;                // with beta = 0: rows that get zeros while the tokens are sorted
-    unsigned sumBlocks, fillBlocks, sumAcross;  // CTAs of EmbeddingSumKernel: of either kind, and side by side on a row
+    unsigned sumBlocks, sumAcross;  // CTAs that sum, and of those side by side on a row
+    unsigned fillBlocks;            // of EmbeddingJoinKernel, CTAs beside them that write zeros
     Scalars sc;
 };
 
@@ -146,6 +194,18 @@ template <typename Out> __device__ __forceinline__ void FillOthers(const GradArg
         }
         for (c += lane; c < a.width; c += 32) row[c] = FromFloat<Out>(0.0f);
     }
+}
+
+// CTAs that sum wait for what they read, CTAs that fill for nothing: they are mixed evenly.  Whether this one fills, and else which of the
+// others it is.
+template <typename Out> __device__ __forceinline__ bool FillsInstead(const GradArgs &a, unsigned *block)
+{
+    const unsigned long long all = (unsigned long long)a.sumBlocks + a.fillBlocks;
+    const unsigned fills = (unsigned)(blockIdx.x * (unsigned long long)a.fillBlocks / all);  // before this one
+    *block = blockIdx.x - fills;
+    if ((blockIdx.x + 1ull) * a.fillBlocks / all == fills) return false;
+    if (a.sc.Beta() == 0.0f) FillOthers<Out>(a, (int)fills);
+    return true;
 }
 
 template <typename Out, typename Key>
@@ -205,21 +265,13 @@ template <typename Out, int kN> __device__ __forceinline__ void FinishRow(const 
     }
 }
 
-constexpr int kGradDepth = 8;  // rows in flight
+constexpr int kGradDepth = 4, kJoinDepth = 8;  // rows, and partial ones, in flight of a thread
 
 template <typename In, typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingSumKernel(const GradArgs a)
 {
     b200sp::WaitForPrevious();
-    // CTAs that sum wait for rows of grad, CTAs that fill for nothing: they are mixed evenly.
-    const unsigned long long all = a.sumBlocks + a.fillBlocks;
-    const unsigned fills = (unsigned)(blockIdx.x * (unsigned long long)a.fillBlocks / all);  // before this one
-    if ((blockIdx.x + 1ull) * a.fillBlocks / all != fills) {
-        if (a.sc.Beta() == 0.0f) FillOthers<Out>(a, (int)fills);
-        return;
-    }
-    const unsigned block = blockIdx.x - fills;
-    const int chunk = (int)(block / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = (int)(block % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
+    const int chunk = (int)(blockIdx.x / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(blockIdx.x % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
     if (chunk >= a.chunks || col >= a.width) return;
     const int lo = chunk * a.chunk, hi = min(a.count, lo + a.chunk);
     const int before = lo > 0 ? __ldg(a.keys + lo - 1) : -1, after = hi < a.count ? __ldg(a.keys + hi) : -1;
@@ -242,31 +294,33 @@ template <typename In, typename Out, int kN> __global__ void __launch_bounds__(2
         for (int i = 0; i < kN; ++i) sum[i] = 0.0f;
         continued = false;
     };
-    for (int e = lo; e < hi; e += kGradDepth) {
-        float v[kGradDepth][kN];
-        int key[kGradDepth];
+    int key[kGradDepth], position[kGradDepth];  // of the rows to come: -1 none
+    auto look = [&](int e) {
 #pragma unroll
         for (int u = 0; u < kGradDepth; ++u) {
-            key[u] = -1;
-            if (e + u >= hi) continue;
-            key[u] = __ldg(a.keys + e + u);
-            const In *const from = static_cast<const In *>(a.grad) + (long long)__ldg(a.positions + e + u) * a.ldGrad + col;
-            if (col + kN <= a.width) {
-                LoadFloats<In, kN, (kN > 1)>(from, v[u]);
-            } else {
-#pragma unroll
-                for (int i = 0; i < kN; ++i) v[u][i] = col + i < a.width ? ToFloat(from[i]) : 0.0f;
-            }
+            key[u] = e + u < hi ? __ldg(a.keys + e + u) : -1;
+            position[u] = e + u < hi ? __ldg(a.positions + e + u) : 0;
         }
+    };
+    look(lo);
+    for (int e = lo; e < hi; e += kGradDepth) {
+        RawRow<In, kN> v[kGradDepth];
+        int token[kGradDepth];
 #pragma unroll
         for (int u = 0; u < kGradDepth; ++u) {
-            if (key[u] < 0) continue;
-            if (key[u] != now) {
+            token[u] = key[u];
+            if (key[u] >= 0) v[u].Load(static_cast<const In *>(a.grad) + (long long)position[u] * a.ldGrad + col, a.width - col, true);
+        }
+        look(e + kGradDepth);
+#pragma unroll
+        for (int u = 0; u < kGradDepth; ++u) {
+            if (token[u] < 0) continue;
+            if (token[u] != now) {
                 flush(false);
-                now = key[u];
+                now = token[u];
             }
 #pragma unroll
-            for (int i = 0; i < kN; ++i) sum[i] += v[u][i];
+            for (int i = 0; i < kN; ++i) sum[i] += v[u].At(i);
         }
     }
     flush(true);
@@ -276,8 +330,10 @@ template <typename In, typename Out, int kN> __global__ void __launch_bounds__(2
 template <typename Out, int kN> __global__ void __launch_bounds__(256) EmbeddingJoinKernel(const GradArgs a)
 {
     b200sp::WaitForPrevious();
-    const int chunk = (int)(blockIdx.x / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
-    const int col = (int)(blockIdx.x % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
+    unsigned block;
+    if (FillsInstead<Out>(a, &block)) return;
+    const int chunk = (int)(block / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
+    const int col = (int)(block % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
     if (chunk >= a.chunks - 1 || col >= a.width) return;
     const int hi = (chunk + 1) * a.chunk, lo = hi - a.chunk;
     const int key = __ldg(a.keys + hi - 1), next = __ldg(a.keys + hi), before = lo > 0 ? __ldg(a.keys + lo - 1) : -1;
@@ -287,11 +343,11 @@ template <typename Out, int kN> __global__ void __launch_bounds__(256) Embedding
 #pragma unroll
     for (int i = 0; i < kN; ++i) sum[i] = at[i];
     bool more = true;
-    for (int c = chunk + 1; more && c < a.chunks; c += kGradDepth) {
-        float v[kGradDepth][kN];
-        int starts[kGradDepth];
+    for (int c = chunk + 1; more && c < a.chunks; c += kJoinDepth) {
+        float v[kJoinDepth][kN];
+        int starts[kJoinDepth];
 #pragma unroll
-        for (int u = 0; u < kGradDepth; ++u) {
+        for (int u = 0; u < kJoinDepth; ++u) {
             const int from = min(c + u, a.chunks - 1);
             starts[u] = c + u < a.chunks ? __ldg(a.keys + from * a.chunk) : -1;
             const float *heads = a.heads + (long long)from * a.pitch + col;
@@ -299,7 +355,7 @@ template <typename Out, int kN> __global__ void __launch_bounds__(256) Embedding
             for (int i = 0; i < kN; ++i) v[u][i] = heads[i];
         }
 #pragma unroll
-        for (int u = 0; u < kGradDepth; ++u) {
+        for (int u = 0; u < kJoinDepth; ++u) {
             more = more && starts[u] == key;  // the chunk begins with this token: its head is a piece of it
 #pragma unroll
             for (int i = 0; i < kN; ++i) sum[i] = more ? sum[i] + v[u][i] : sum[i];
@@ -400,8 +456,8 @@ template <typename In, typename Out, int kN> cudaError_t LaunchSums(GradArgs a, 
     a.sumBlocks = (unsigned)sums;
     a.fillBlocks = (unsigned)others;
     b200sp_note_launches(2);
-    const cudaError_t e = b200sp::LaunchChained(EmbeddingSumKernel<In, Out, kN>, (unsigned)(sums + others), 256, 0, stream, a);
-    return e != cudaSuccess ? e : b200sp::LaunchChained(EmbeddingJoinKernel<Out, kN>, (unsigned)sums, 256, 0, stream, a);
+    const cudaError_t e = b200sp::LaunchChained(EmbeddingSumKernel<In, Out, kN>, (unsigned)sums, 256, 0, stream, a);
+    return e != cudaSuccess ? e : b200sp::LaunchChained(EmbeddingJoinKernel<Out, kN>, (unsigned)(sums + others), 256, 0, stream, a);
 }
 
 // Rows that are filled while the tokens are sorted: what is written in that time.  Rows of less than 1024 bytes all are: to look up whether a

@@ -73,13 +73,18 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
 
 // Rows of 16-bit elements into rows of a multiple of eight, zeros behind the last: what the copies of the products need.  A thread writes 16
 // bytes; what bounds it are the bytes, read and written once each (and read again by the product).
+// offsets: with rowsEach > 0 the rows are those of experts, as many each, and one without entries is left out.
 __global__ void __launch_bounds__(256) ExpertsAlignKernel(const uint16_t *__restrict__ from, long long rows, int cols, long long ld,
-                                                          uint4 *__restrict__ to)
+                                                          uint4 *__restrict__ to, const int *__restrict__ offsets, int rowsEach)
 {
     b200sp::WaitForPrevious();
     const int pieces = (cols + 7) / 8;
     for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < rows * pieces; i += (long long)gridDim.x * 256) {
         const long long r = i / pieces;
+        if (rowsEach > 0) {
+            const int e = (int)(r / rowsEach);
+            if (__ldg(offsets + e) == __ldg(offsets + e + 1)) continue;
+        }
         const int c = (int)(i - r * pieces) * 8;
         const uint16_t *const row = from + r * ld + c;
         __align__(16) uint16_t v[8];
@@ -209,7 +214,7 @@ struct Operand {
     long long ld;
     cudaError_t error;
 };
-Operand Aligned(const aclsparseDnMatDescr *m, char **room, cudaStream_t stream)
+Operand Aligned(const aclsparseDnMatDescr *m, char **room, cudaStream_t stream, const int *offsets = nullptr, int rowsEach = 0)
 {
     const size_t bytes = AlignedBytes(m);
     if (bytes == 0) return {m->values, m->ld, cudaSuccess};
@@ -219,7 +224,7 @@ Operand Aligned(const aclsparseDnMatDescr *m, char **room, cudaStream_t stream)
     const unsigned blocks = (unsigned)std::min<long long>((pieces + 255) / 256, (long long)b200sp_sm_count() * 32);
     b200sp_note_launches(1);
     const cudaError_t e = b200sp::LaunchChained(ExpertsAlignKernel, blocks, 256, 0, stream, static_cast<const uint16_t *>(m->values),
-                                                m->rows, (int)m->cols, m->ld, reinterpret_cast<uint4 *>(to));
+                                                m->rows, (int)m->cols, m->ld, reinterpret_cast<uint4 *>(to), offsets, rowsEach);
     return {to, (long long)AlignUp((size_t)m->cols, 8), e};
 }
 
@@ -316,7 +321,7 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     const OnDevice device(handle);
     MmaArgs a = ArgsOf(matR, rowsOfX, buffer, matW, matY, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
-    const Operand x = Aligned(matX, &room, handle->stream), w = Aligned(matW, &room, handle->stream);
+    const Operand x = Aligned(matX, &room, handle->stream), w = Aligned(matW, &room, handle->stream, a.offsets, a.n);
     if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, "b200spExpertsMM");
     a.x = x.values;
     a.ldx = x.ld;

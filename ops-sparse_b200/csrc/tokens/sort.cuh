@@ -218,32 +218,10 @@ template <typename Key, typename Place> __device__ __forceinline__ void ClusterS
         const bool fromA = (a.passes - p) % 2 == 0;
         const int *const keyIn = fromA ? a.keyA : a.keyB, *const posIn = fromA ? a.posA : a.posB;
         int *const keyOut = fromA ? a.keyB : a.keyA, *const posOut = fromA ? a.posB : a.posA;
-        for (int i = tid; i < bins; i += kSortThreads) sCount[i] = 0;
-        __syncthreads();
-        for (int i = lo + tid; i < hi; i += kSortThreads) {
-            const int k = p == 0 ? SortKey<Key>(a, i) : __ldcg(keyIn + i);
-            atomicAdd(sCount + ((k >> shift) & (bins - 1)), 1);
-        }
-        cluster.sync();
-        int all = 0, before = 0;  // of digit tid
-        if (tid < bins) {
-            for (int c = 0; c < ctas; ++c) {
-                const int n = cluster.map_shared_rank(sCount, c)[tid];
-                before += c < rank ? n : 0;
-                all += n;
-            }
-        }
-        const int start = SumsBefore(all, sScan) - all;
-        if (tid < bins) {
-            sBase[tid] = start + before;
-            if (a.offsets != nullptr && rank == 0 && tid <= a.limit + 1) a.offsets[tid] = start;
-            // 2^bits > limit: the end of the last key has a digit of its own unless the digits are used up
-            if (a.offsets != nullptr && rank == 0 && tid == a.limit && a.limit + 1 == bins) a.offsets[bins] = a.count;
-        }
-        for (int tile = lo; tile < hi; tile += kSortTile) {
+        int key[kSortSteps], pos[kSortSteps], at[kSortSteps];
+        // The tile's positions, and their ranks among the warps' of the same digit; then sTile has the tile's counts.
+        auto rankTile = [&](int tile) {
             for (int i = tid; i < kSortWarps * bins / 2; i += kSortThreads) reinterpret_cast<uint32_t *>(sWarp)[i] = 0;
-            __syncthreads();
-            int key[kSortSteps], pos[kSortSteps], at[kSortSteps];
             const int first = tile + warp * (32 * kSortSteps) + lane;
 #pragma unroll
             for (int u = 0; u < kSortSteps; ++u) {
@@ -254,11 +232,47 @@ template <typename Key, typename Place> __device__ __forceinline__ void ClusterS
                     pos[u] = p == 0 ? i : __ldcg(posIn + i);
                 }
             }
+            __syncthreads();
 #pragma unroll
             for (int u = 0; u < kSortSteps; ++u)
                 at[u] = RankInWarp(sMask + warp * bins, sWarp + warp * bins, (key[u] >> shift) & (bins - 1), key[u] >= 0, lane);
             __syncthreads();
             if (tid < bins) sTile[tid] = PlacesByWarp(sWarp + tid, bins, kSortWarps);
+        };
+        // A share of one tile is read once; of a longer one the digits are counted first.
+        const bool once = hi - lo <= kSortTile;
+        if (once) {
+            rankTile(lo);
+            if (tid < bins) sCount[tid] = sTile[tid];
+        } else {
+            for (int i = tid; i < bins; i += kSortThreads) sCount[i] = 0;
+            __syncthreads();
+            for (int i = lo + tid; i < hi; i += kSortThreads) {
+                const int k = p == 0 ? SortKey<Key>(a, i) : __ldcg(keyIn + i);
+                atomicAdd(sCount + ((k >> shift) & (bins - 1)), 1);
+            }
+        }
+        cluster.sync();
+        int all = 0, before = 0;  // of digit tid
+        if (tid < bins) {
+            int n[kSortMaxCtas];
+#pragma unroll
+            for (int c = 0; c < kSortMaxCtas; ++c) n[c] = c < ctas ? cluster.map_shared_rank(sCount, c)[tid] : 0;
+#pragma unroll
+            for (int c = 0; c < kSortMaxCtas; ++c) {
+                before += c < rank ? n[c] : 0;
+                all += n[c];
+            }
+        }
+        const int start = SumsBefore(all, sScan) - all;
+        if (tid < bins) {
+            sBase[tid] = start + before;
+            if (a.offsets != nullptr && rank == 0 && tid <= a.limit + 1) a.offsets[tid] = start;
+            // 2^bits > limit: the end of the last key has a digit of its own unless the digits are used up
+            if (a.offsets != nullptr && rank == 0 && tid == a.limit && a.limit + 1 == bins) a.offsets[bins] = a.count;
+        }
+        for (int tile = lo; tile < hi; tile += kSortTile) {
+            if (!once) rankTile(tile);
             __syncthreads();
 #pragma unroll
             for (int u = 0; u < kSortSteps; ++u) {
