@@ -13,6 +13,7 @@
  * rounded once: the same inputs give the same bits.  Values that f16 cannot hold become infinite (SpMM clamps them; a
  * gradient has to show that it overflowed).  Calls enqueue on the handle's stream, wait for nothing, allocate nothing,
  * and may be captured.  A handle is used on the device that it was created on, whatever device is current.
+ * An output overlaps no input, unless it says so.  At most 2^31 - 2^20 tokens or entries of R.
  * Column-major operands, index bases of one and 64-bit CSR indices are ACL_SPARSE_STATUS_NOT_SUPPORTED.
  */
 #ifndef B200SP_TOKENS_H_
@@ -98,7 +99,10 @@ typedef enum b200spExpertRows_t {
  * written.  Nothing is waited for: it may be captured with the products that follow. */
 aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, void *buffer);
 
-/* Y[i] = alpha * X[row of entry i] * op(W of its expert) + beta * Y[i], a row of Y for every entry of R.
+/* Operands of the products whose rows do not start on 16 bytes are copied into the buffer first, in every call: the BufferSize calls count
+ * the room for the operands they are given.
+ *
+ * Y[i] = alpha * X[row of entry i] * op(W of its expert) + beta * Y[i], a row of Y for every entry of R.
  * opW = T: X has d columns, Y n (a layer whose weights lie as n x d); opW = N: X has n columns, Y d (the
  * gradient of that layer's input rows).  `buffer`: what b200spExpertsPreprocess wrote, with as many bytes as
  * the BufferSize call says; one buffer serves several products with the same R, one at a time, with the largest size. */

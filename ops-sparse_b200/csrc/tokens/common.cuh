@@ -1,6 +1,7 @@
 // What the token operators (include/b200sp_tokens.h) share: element types, scalars, argument checks, the handle's device.
 #pragma once
 
+#include <atomic>
 #include <cstdint>
 
 #include <cuda_bf16.h>
@@ -134,6 +135,19 @@ inline uint64_t NoteWrite(const void *buffer) noexcept
     } catch (...) {
         return 0;
     }
+}
+
+// Lets a kernel use `bytes` of shared memory on the current device, where no call has done so yet.
+template <auto kKernel> cudaError_t AllowShared(int bytes)
+{
+    static std::atomic<bool> done[64] = {};
+    int device = 0;
+    const cudaError_t got = cudaGetDevice(&device);
+    if (got != cudaSuccess || device < 0 || device >= 64) return cudaErrorInvalidDevice;
+    if (done[device].load(std::memory_order_relaxed)) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done[device].store(true, std::memory_order_relaxed);
+    return e;
 }
 
 inline aclsparseStatus_t Finished(cudaError_t e, const char *call)

@@ -273,7 +273,7 @@ template <typename In, typename Out, int kN> __global__ void __launch_bounds__(2
     const int chunk = (int)(blockIdx.x / a.sumAcross) * (256 / a.lanes) + threadIdx.x / a.lanes;
     const int col = (int)(blockIdx.x % a.sumAcross * a.lanes + threadIdx.x % a.lanes) * kN;
     if (chunk >= a.chunks || col >= a.width) return;
-    const int lo = chunk * a.chunk, hi = min(a.count, lo + a.chunk);
+    const int lo = chunk * a.chunk, hi = (int)min((long long)a.count, (long long)lo + a.chunk);
     const int before = lo > 0 ? __ldg(a.keys + lo - 1) : -1, after = hi < a.count ? __ldg(a.keys + hi) : -1;
     float sum[kN];
 #pragma unroll
@@ -370,7 +370,7 @@ aclsparseStatus_t CheckTokens(const aclsparseDnVecDescr *tokens)
 {
     if (tokens == nullptr || tokens->magic != b200sp::kDnVecMagic) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (tokens->valueType != ACL_INT32 && tokens->valueType != ACL_INT64) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (tokens->size > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (tokens->size > kMostSorted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (reinterpret_cast<uintptr_t>(tokens->values) % (tokens->valueType == ACL_INT64 ? 8 : 4) != 0) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;
 }
@@ -471,7 +471,7 @@ int FillFirst(long long vocab, long long rowBytes)
 template <typename Out, typename Key> cudaError_t LaunchSort(const SortArgs &s, const GradArgs &a, cudaStream_t stream)
 {
     const int size = SortCtas(a.count), shared = SortShared(s.digitBits, a.count <= kSortTile && s.passes > 1);
-    const cudaError_t set = cudaFuncSetAttribute(EmbeddingSortKernel<Out, Key>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSharedMost);
+    const cudaError_t set = AllowShared<EmbeddingSortKernel<Out, Key>>(kSortSharedMost);
     if (set != cudaSuccess) return set;
     // one cluster sorts; the others fill the table, if it has to be (one CTA per SM: what the sort needs of shared memory)
     const bool fills = a.sc.betaAt != nullptr || a.sc.beta == 0.0f;

@@ -107,7 +107,7 @@ aclsparseStatus_t CheckRouted(const aclsparseSpMatDescr *R)
     const aclsparseStatus_t idx = b200sp::CheckExecIndexTypes(R->offsetType, R->indexType);
     if (idx != ACL_SPARSE_STATUS_SUCCESS) return idx;
     if (R->base != ACL_SPARSE_INDEX_BASE_ZERO) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz >= INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz > kMostSorted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (R->rows == 0 || R->cols == 0 || R->nnz == 0) return ACL_SPARSE_STATUS_INVALID_VALUE;  // no dense operand has as few rows
     if (R->offsets == nullptr || R->indices == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;
@@ -272,7 +272,7 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
     s.keyB = reinterpret_cast<int *>(p + L.keyB);
     s.posB = reinterpret_cast<int *>(p + L.posB);
     s.offsets = s.passes == 1 ? offsets : nullptr;
-    cudaError_t e = cudaFuncSetAttribute(ExpertsOrderKernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSortSharedMost);
+    cudaError_t e = AllowShared<ExpertsOrderKernel>(kSortSharedMost);
     if (e == cudaSuccess) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)SortCtas(s.count));

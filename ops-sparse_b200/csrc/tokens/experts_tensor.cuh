@@ -630,7 +630,7 @@ cudaError_t LaunchTiles(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
     a.waitCycles = gExpertsWaitCycles;
     a.extraTx = gExpertsExtraTx;
     const auto kernel = ExpertsTensorKernel<T, Out, kMode, kPair>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMmaShared + kMmaStoreBytes<Out> + 1024);
+    const cudaError_t e = AllowShared<ExpertsTensorKernel<T, Out, kMode, kPair>>(kMmaShared + kMmaStoreBytes<Out> + 1024);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(b200sp_sm_count() / 2 * 2));

@@ -103,6 +103,10 @@ GRADIENT = [  # count, vocab, width, grad, table, index, alpha, beta, pad, shift
     (20000, 1500000, 4, "f32", "f32", torch.int64, 1.0, 0.0, 0, 0, 0.5),  # three passes of the sort
     (70001, 1023, 8, "f16", "f32", torch.int32, 1.0, 0.0, 0, 0, 1),
     (70001, 1024, 8, "bf16", "f32", torch.int32, 1.0, 0.0, 0, 0, 1),  # the first table that takes two
+    (4096, 2 ** 19 + 1, 3, "f32", "f32", torch.int32, 1.0, 0.0, 0, 0, 0),  # a tile's worth in three passes
+    (3000, 40000, 512, "bf16", "f32", torch.int64, 1.0, 0.0, 0, 0, 0.5),  # zeros in two kernels
+    (3000, 40000, 513, "f16", "f32", torch.int64, 2.0, 0.0, 2, 1, 0.5),
+    (300, 40000, 1030, "f32", "f16", torch.int32, 1.0, 0.5, 2, 0, 0.5),
 ]
 
 
@@ -357,6 +361,12 @@ PRODUCTS = [  # tokens, experts, mean, n, d, type, out, transpose, rows, alpha, 
     (64, 1024, 3, 24, 40, "bf16", "bf16", True, "tokens", 1.0, 0.0, 0, 0),  # two passes of the sort
     (30, 300, 2, 40, 2056, "f16", "f16", True, "tokens", 1.0, 0.0, 0, 0),
     (5000, 4, 2, 40, 64, "bf16", "bf16", True, "tokens", 1.0, 0.0, 0, 0),
+    (1, 5, 3, 1024, 2048, "bf16", "bf16", True, "tokens", 1.0, 0.0, 0, 0),
+    (20, 64, 4, 256, 1024, "f16", "f16", True, "tokens", 1.0, 0.0, 0, 0),
+    (3000, 6, 3, 1100, 600, "bf16", "bf16", True, "tokens", 1.0, 0.0, 4, 0),  # every CTA has several tiles
+    (3000, 6, 3, 1100, 600, "bf16", "f32", False, "entries", 1.0, 0.0, 4, 0),
+    (3000, 6, 3, 1100, 600, "f16", "f16", False, "tokens", 1.0, 1.0, 0, 0),
+    (2500, 33, 4, 128, 1000, "bf16", "bf16", True, "entries", 1.0, 0.0, 0, 0),  # one CTA a tile of 256 entries
 ]
 
 
@@ -401,6 +411,8 @@ GRADIENTS = [  # tokens, experts, mean, n, d, type, out, rows, alpha, beta, pad,
     (900, 3, 4, 24, 600, "bf16", "bf16", "entries", 1.0, 0.0, 0, 0),
     (64, 1024, 3, 24, 40, "bf16", "bf16", "tokens", 1.0, 0.0, 0, 0),
     (5000, 2, 2, 40, 64, "f16", "f16", "tokens", 0.1, 0.0, 0, 0),
+    (3000, 6, 3, 1100, 600, "bf16", "bf16", "tokens", 1.0, 0.0, 4, 0),
+    (2000, 40, 3, 300, 1032, "bf16", "f32", "entries", 1.0, 0.0, 0, 0),
 ]
 
 
@@ -462,6 +474,25 @@ def test_experts_keep_their_neighbours_infinities(pkg, handle):
     hit[columns[(token == 5) | (token == 77)].long()] = True
     hit[columns[11].long()] = True
     assert torch.equal(~dw.view(experts, -1).isfinite().all(1), hit)
+
+
+def test_products_refuse_a_buffer_sized_for_other_operands(pkg, handle):
+    """Room for the copy of an operand that starts on no multiple of 16 bytes has to have been asked for."""
+    from ops_sparse_b200 import api
+    g = gen(6)
+    offsets, columns = ragged(g, 20, 4, 2)
+    nnz = len(columns)
+    R = api.CsrMatrix(offsets, columns, torch.empty(nnz, device="cuda"), 20, 4)
+    X, W, Y = mat(api, matrix(g, 20, 32, "bf16")[0]), mat(api, matrix(g, 64, 32, "bf16")[0]), mat(api, torch.empty(nnz, 16, dtype=torch.bfloat16, device="cuda"))
+    odd = mat(api, matrix(g, 20, 32, "bf16", shift=1)[0])
+    buffer = torch.empty(api.experts_buffer_size(handle, R, X, W, Y) + 20 * 32 * 2 + 256, dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, X, W, Y, buffer=buffer)
+    with pytest.raises(pkg.AclSparseError, match="INVALID_VALUE"):
+        api.experts_mm(handle, R, odd, W, Y, buffer=buffer)
+    assert api.experts_buffer_size(handle, R, odd, W, Y) <= buffer.numel()
+    api.experts_mm(handle, R, odd, W, Y, buffer=buffer)
+    torch.cuda.synchronize()
 
 
 def test_products_want_the_order_in_their_buffer(pkg, handle):

@@ -70,6 +70,9 @@ def test_embedding_refusals(pkg):
     assert call(k=_vec(pkg, 7, S.ACL_INT64, FAKE + 4)) == bad  # not on the type's boundary
     assert call(t=_mat(pkg, 100, 64, at=FAKE + 1)) == bad
     assert call(t=_mat(pkg, (1 << 31) - 1, 64)) == no
+    many = (1 << 31) - (1 << 20) + 1
+    assert call(k=_vec(pkg, many, S.ACL_INT32), o=_mat(pkg, many, 64)) == no
+    assert call(t=_mat(pkg, 100, 64, ld=1 << 31)) == no
     size = c_size_t()
     g = pkg.lib().b200spEmbeddingGradBufferSize
     assert g(_h(), out, tokens, table, None) == bad
