@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     const int now = entry;
                     if (c0 + 32 + lane < m.many) entry = __ldg(a.entries + m.first + c0 + 32 + lane);
                     Out *const out = static_cast<Out *>(a.out);
-                    if (a.vectors && beta == 0.0f && f0 + 32 <= features) {
+                    if (a.vectors && beta == 0.0f) {
                         // Through shared memory, so that 16 bytes of a row are stored at once and a row's 32 columns side by side.
                         constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
 #pragma unroll
@@ -518,48 +518,74 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                             const int c = (32 * i + lane) / kPieces, at = lane % kPieces * kN;
                             const long long row = __shfl_sync(0xffffffffu, now, c);
                             const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + 32 * c + at);
-                            if (c < live) *reinterpret_cast<uint4 *>(out + row * a.ldo + f0 + at) = piece;
+                            Out *const to = out + row * a.ldo + f0 + at;
+                            if (c < live && f0 + at + kN <= features) *reinterpret_cast<uint4 *>(to) = piece;
+                            else if (c < live)  // the last columns
+                                for (int j = 0; f0 + at + j < features; ++j) to[j] = sOut[32 * c + at + j];
                         }
                         __syncwarp();
                     } else {
+                        // A column a lane.  What is read is asked for before anything is stored.
+                        const bool in = f0 + lane < features;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const long long row = __shfl_sync(0xffffffffu, now, i);
-                            if (i >= live || f0 + lane >= features) continue;
-                            Out *const to = out + row * a.ldo + f0 + lane;
-                            float u = by * v[i];
-                            if (beta != 0.0f) u = fmaf(beta, ToFloat(*to), u);
-                            *to = FromFloat<Out>(u);
+                        for (int g = 0; g < 32; g += 8) {
+                            float old[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const long long row = __shfl_sync(0xffffffffu, now, g + i);
+                                old[i] = beta != 0.0f && in && g + i < live ? ToFloat(out[row * a.ldo + f0 + lane]) : 0.0f;
+                            }
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) {
+                                const long long row = __shfl_sync(0xffffffffu, now, g + i);
+                                const float u = beta != 0.0f ? fmaf(beta, old[i], by * v[g + i]) : by * v[g + i];
+                                if (in && g + i < live) out[row * a.ldo + f0 + lane] = FromFloat<Out>(u);
+                            }
                         }
                     }
                 } else {
                     constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
                     Out *const out = static_cast<Out *>(a.out) + ((long long)m.expert * a.n + f0) * a.ldo + m.first + c0;
-                    if (a.vectors && beta == 0.0f && live == 32) {
-                        // The lane's row, its pieces exchanged so that neither side meets in a bank; then pieces of a row side by side.
+                    if (beta == 0.0f) {
+                        // The lane's row, its pieces exchanged so that neither side meets in a bank; then pieces of a row side by side, or where
+                        // rows do not start on 16 bytes a row at a time.
+                        auto pieceOf = [&](int r, int at) { return sOut + 32 * r + kN * (at ^ (r * kPieces / 8 & (kPieces - 1))); };
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i) {
                             float u[kN];
 #pragma unroll
                             for (int j = 0; j < kN; ++j) u[j] = by * v[kN * i + j];
-                            StoreFloats<Out, kN, true>(sOut + 32 * lane + kN * (i ^ (lane * kPieces / 8 & (kPieces - 1))), u);
+                            StoreFloats<Out, kN, true>(pieceOf(lane, i), u);
                         }
                         __syncwarp();
+                        if (a.vectors) {
 #pragma unroll
-                        for (int i = 0; i < kPieces; ++i) {
-                            const int r = (32 * i + lane) / kPieces, at = lane % kPieces;
-                            const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + 32 * r + kN * (at ^ (r * kPieces / 8 & (kPieces - 1))));
-                            if (f0 + r < features) *reinterpret_cast<uint4 *>(out + r * a.ldo + kN * at) = piece;
+                            for (int i = 0; i < kPieces; ++i) {
+                                const int r = (32 * i + lane) / kPieces, at = lane % kPieces;
+                                const uint4 piece = *reinterpret_cast<const uint4 *>(pieceOf(r, at));
+                                Out *const to = out + r * a.ldo + kN * at;
+                                if (f0 + r < features && kN * (at + 1) <= live) *reinterpret_cast<uint4 *>(to) = piece;
+                                else if (f0 + r < features)  // the last columns
+                                    for (int j = 0; kN * at + j < live; ++j) to[j] = pieceOf(r, at)[j];
+                            }
+                        } else {
+#pragma unroll 8
+                            for (int r = 0; r < 32; ++r) {
+                                const Out one = pieceOf(r, lane / kN)[lane % kN];
+                                if (f0 + r < features && lane < live) out[r * a.ldo + lane] = one;
+                            }
                         }
                         __syncwarp();
                     } else if (f0 + lane < features) {
                         Out *const to = out + lane * a.ldo;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            if (i >= live) continue;
-                            float u = by * v[i];
-                            if (beta != 0.0f) u = fmaf(beta, ToFloat(to[i]), u);
-                            to[i] = FromFloat<Out>(u);
+                        for (int g = 0; g < 32; g += 8) {
+                            float old[8];
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) old[i] = beta != 0.0f && g + i < live ? ToFloat(to[g + i]) : 0.0f;
+#pragma unroll
+                            for (int i = 0; i < 8; ++i)
+                                if (g + i < live) to[g + i] = FromFloat<Out>(beta != 0.0f ? fmaf(beta, old[i], by * v[g + i]) : by * v[g + i]);
                         }
                     }
                 }
