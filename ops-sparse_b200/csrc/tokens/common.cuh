@@ -25,6 +25,19 @@ template <> __device__ __forceinline__ float FromFloat<float>(float v) { return 
 template <> __device__ __forceinline__ __half FromFloat<__half>(float v) { return __float2half_rn(v); }
 template <> __device__ __forceinline__ __nv_bfloat16 FromFloat<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Two neighbours in a word.
+template <typename T> __device__ __forceinline__ uint32_t TwoFromFloats(float a, float b);
+template <> __device__ __forceinline__ uint32_t TwoFromFloats<__half>(float a, float b)
+{
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+template <> __device__ __forceinline__ uint32_t TwoFromFloats<__nv_bfloat16>(float a, float b)
+{
+    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 // alpha and beta of a call: values, or device pointers to them.
 struct Scalars {
     float alpha, beta;
@@ -65,12 +78,15 @@ template <typename T, int kN, bool kVector> __device__ __forceinline__ void Stor
 {
     if constexpr (kVector) {
         static_assert(kN * sizeof(T) % 16 == 0);
-        uint4 raw[kN * sizeof(T) / 16];
-        T *e = reinterpret_cast<T *>(raw);
+        uint32_t words[kN * sizeof(T) / 4];
 #pragma unroll
-        for (int i = 0; i < kN; ++i) e[i] = FromFloat<T>(v[i]);
+        for (int i = 0; i < (int)(kN * sizeof(T) / 4); ++i) {
+            if constexpr (sizeof(T) == 4) words[i] = __float_as_uint(v[i]);
+            else words[i] = TwoFromFloats<T>(v[2 * i], v[2 * i + 1]);
+        }
 #pragma unroll
-        for (int i = 0; i < (int)(kN * sizeof(T) / 16); ++i) *(reinterpret_cast<uint4 *>(at) + i) = raw[i];
+        for (int i = 0; i < (int)(kN * sizeof(T) / 16); ++i)
+            *(reinterpret_cast<uint4 *>(at) + i) = make_uint4(words[4 * i], words[4 * i + 1], words[4 * i + 2], words[4 * i + 3]);
     } else {
 #pragma unroll
         for (int i = 0; i < kN; ++i) at[i] = FromFloat<T>(v[i]);
