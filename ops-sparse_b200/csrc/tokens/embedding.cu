@@ -86,20 +86,30 @@ __global__ void __launch_bounds__(256) EmbeddingKernel(const EmbedArgs a)
     RawRow<In, kN> raw[kEmbedDepth];
     long long to[kEmbedDepth];  // -1: nothing
     int left[kEmbedDepth];      // elements of the row from here
+    // Rows of several pieces have all lanes on each: one division, then a piece further every time.
+    long long row;
+    unsigned within;
+    if (a.perRow == 1) {
+        row = (long long)first;
+        within = 0;
+    } else if (a.pieces <= UINT_MAX) {
+        row = (unsigned)first / a.perRow;
+        within = (unsigned)first % a.perRow;
+    } else {
+        row = (long long)(first / a.perRow);
+        within = (unsigned)(first % a.perRow);
+    }
 #pragma unroll
     for (int u = 0; u < kEmbedDepth; ++u) {
-        const unsigned long long piece = first + (unsigned long long)u * rowsPerWarp;
-        to[u] = -1;
-        if (piece >= a.pieces) continue;
-        long long row;
-        int col;
-        if (a.pieces <= UINT_MAX) {
-            row = (unsigned)piece / a.perRow;
-            col = (int)(((unsigned)piece % a.perRow) * a.lanes + at) * kN;
-        } else {
-            row = (long long)(piece / a.perRow);
-            col = (int)(piece % a.perRow * a.lanes + at) * kN;
+        if (u > 0 && a.perRow == 1) {
+            row += rowsPerWarp;
+        } else if (u > 0 && ++within == a.perRow) {
+            within = 0;
+            ++row;
         }
+        to[u] = -1;
+        if (first + (unsigned long long)u * rowsPerWarp >= a.pieces) continue;
+        const int col = (int)(within * a.lanes + at) * kN;
         left[u] = a.width - col;
         if (left[u] <= 0) continue;
         to[u] = row * a.ldOut + col;
