@@ -110,6 +110,7 @@ aclsparseStatus_t CheckRouted(const aclsparseSpMatDescr *R)
     if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz > kMostSorted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (R->rows == 0 || R->cols == 0 || R->nnz == 0) return ACL_SPARSE_STATUS_INVALID_VALUE;  // no dense operand has as few rows
     if (R->offsets == nullptr || R->indices == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!OnBoundary(R->offsets, 4) || !OnBoundary(R->indices, 4)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 

@@ -5,14 +5,17 @@
 // at full width; the accumulator's lanes are then columns of Y, and a store is 32 of them for one entry.
 // The gradient's tile is 128 rows of dW by up to 256 of its columns, summed over the expert's entries.
 //
-// One CTA per SM walks over the tiles of all experts.  One thread requests W by TMA; eight warps gather the rows of X (and
-// dY), which may lie anywhere, by cp.async, a stage each in turn, so that nothing is laid out in between; one thread starts the products, four warps
-// empty the accumulators, of which there are two: the next tile is summed meanwhile.  (Rows by TMA, tile::gather4, come at one
-// row of 128 bytes in 18 clocks and SM: 8192 tokens, four of 32 experts, 2048 x 2048: 1250 us.)
+// One CTA per SM, or a pair of CTAs on tiles twice as high, walks over the tiles of all experts.  One warp requests W by TMA; twelve gather
+// the rows of X (and dY), which may lie anywhere, by cp.async, so that nothing is laid out in between; one starts the products, four
+// empty the accumulators, of which there are two: the next tile is summed meanwhile.
+// What bounds it: with many entries the tensor cores (71 % of the cycles) and what comes from L2, 32 KB a step and SM at some 58 bytes a clock,
+// where the products of a step take 450; with few the weights, once from DRAM.  One B200: 8192 tokens, four of 32 experts, 2048 x 2048, bf16
+// (275 GFLOP) 223 us; 16 tokens, 8 of 64 experts, 2048 x 1024 40 us (0.9 of the copy rate).  The same by rows of X from TMA
+// (tile::gather4: 18 clocks a row of 128 bytes and SM) 1250, by one CTA a tile 380.
 // Operands arrive in rows of 128 bytes, swizzled: K-major where those run along the sum (X; W with opW = T), MN-major
 // where they run along the tile (W with opW = N; both of the gradient's).
 //
-// Every wait is bounded.  One that ran out ends its warp's work, raises the flag of b200spExpertsError and leaves rows of the
+// Every wait is bounded.  One that ran out ends its warp's work, raises the flag of b200sp_experts_error and leaves rows of the
 // output unwritten; nothing waits for ever, and tensor memory is freed when copies and products in flight have had time to
 // land.
 #pragma once
@@ -69,6 +72,8 @@ __device__ __forceinline__ uint32_t LeadersBar(uint64_t *bar)
     asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(at) : "r"(Shared(bar)));
     return at;
 }
+// Of this CTA or another one of the cluster.  What it orders is read from the arriving CTA's own memories by the tensor cores: tensor memory, or
+// shared memory that a proxy fence has handed over.  (A release at cluster scope waits for every access of the SM, 1600 clocks.)
 __device__ __forceinline__ void BarArriveAt(uint32_t bar)
 {
     asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
@@ -195,7 +200,6 @@ template <Mode kMode, bool kPair> struct Tiles {
     static constexpr int kUnit = kMode != Mode::kGrad ? 16 : kPair ? 128 : 64;
 
     __device__ __forceinline__ int Groups() const { return kMode == Mode::kGrad ? a.experts : a.experts + 1; }
-    __device__ __forceinline__ int Features() const { return kMode == Mode::kProductN ? a.d : a.n; }
     // Tiles of `count` entries side by side, nearly equal.
     __device__ __forceinline__ int Across(int count) const { return (count + a.colsMost - 1) / a.colsMost; }
     __device__ __forceinline__ int Count(int lo, int hi) const
@@ -313,10 +317,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
     } else if (warp >= kMmaFirstGather && warp < kMmaFirstGather + a.parts * a.stages) {
-        // Stages are the warps' in turn: one asks for all of its rows, waits for them and says so, while the others are at the stages
-        // beside it.  No more warps than stages: whoever is at stage q knows that q - stages has been used up, so that the wait for
-        // q + warps - stages can not be answered by the round before it.  (All warps at every stage, a share each, take turns with it: with the arrivals of 256 threads, and a
-        // thread that passes them on to the other CTA, a stage's round took 2900 clocks without any copy.)
+        // Stages are the warps' in turn, one's or a pair of warps': they ask for all of its rows, wait for them and say so, while the others are
+        // at the stages beside it.  No more turns than stages: whoever is at stage q knows that q - stages has been used up, so that the
+        // wait for q + turns - stages can not be answered by the round before it.  (All warps at every stage, a share each, and an arrival
+        // of every thread: a stage's round took 2900 clocks without any copy.)
         // Eight lanes side by side on 128 bytes of a row: lane l has piece l % 8 of rows l / 8, l / 8 + 4, ...
         const int mine = (warp - kMmaFirstGather) / a.parts, part = (warp - kMmaFirstGather) % a.parts;
         const int warps = min(kMmaGatherWarps / a.parts, a.stages), piece = lane & 7, high = lane >> 3;
@@ -582,10 +586,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         for (int g = 0; g < 32; g += 8) {
                             float old[8];
 #pragma unroll
-                            for (int i = 0; i < 8; ++i) old[i] = beta != 0.0f && g + i < live ? ToFloat(to[g + i]) : 0.0f;
+                            for (int i = 0; i < 8; ++i) old[i] = g + i < live ? ToFloat(to[g + i]) : 0.0f;
 #pragma unroll
                             for (int i = 0; i < 8; ++i)
-                                if (g + i < live) to[g + i] = FromFloat<Out>(beta != 0.0f ? fmaf(beta, old[i], by * v[g + i]) : by * v[g + i]);
+                                if (g + i < live) to[g + i] = FromFloat<Out>(fmaf(beta, old[i], by * v[g + i]));
                         }
                     }
                 }
@@ -634,7 +638,8 @@ inline bool MapOf(CUtensorMap *map, aclDataType type, const void *at, long long 
 }
 
 // Entries of a tile: as many as an expert has on average, half as much again for the uneven ones, so that the weights of most experts are
-// read by one tile a column block, and stages are no larger than that wants.
+// read by one tile a column block, and stages are no larger than that wants.  32 experts of 2048 x 2048, four a token, us with tiles of 256, 128
+// (pairs of CTAs) and 64 entries: 64 tokens 54, 53, 54; 512 tokens 64, 62, 81; 1024 tokens 69, 79, 117; 4096 tokens 135, 182, 353.
 inline int TileColumns(long long nnz, long long experts)
 {
     const long long want = (nnz * 3 + 2 * experts - 1) / (2 * experts);
@@ -676,7 +681,8 @@ cudaError_t LaunchTiles(MmaArgs a, const CUtensorMap &mapW, cudaStream_t stream)
 }
 
 // A pair of CTAs on a tile of 256 columns reads half as much of X (or of both operands of a gradient) per product.  That counts where there are
-// products enough to be bound by them.
+// products enough to be bound by them: 1024 tokens as above 69 us, by single CTAs 84, 4096 tokens 135 and 178; gradients of 4096 entries of 1024 x
+// 2048 87 and 102.  With few entries there is nothing in it (64 tokens 54 and 54).
 template <typename T, typename Out, Mode kMode>
 cudaError_t LaunchTensor(const MmaArgs &a, const CUtensorMap &mapW, cudaStream_t stream)
 {

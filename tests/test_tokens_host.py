@@ -30,10 +30,10 @@ def _vec(pkg, size, kind, at=FAKE):
     return d
 
 
-def _csr(pkg, rows, cols, nnz, kind=None, offsets=0, base=0):
+def _csr(pkg, rows, cols, nnz, kind=None, offsets=0, base=0, at=FAKE):
     d = c_void_p()
     kind = pkg.ACL_FLOAT if kind is None else kind
-    assert pkg.lib().aclsparseCreateCsr(byref(d), rows, cols, nnz, c_void_p(FAKE), c_void_p(FAKE), c_void_p(FAKE), offsets, offsets, base, kind) == 0
+    assert pkg.lib().aclsparseCreateCsr(byref(d), rows, cols, nnz, c_void_p(at), c_void_p(at), c_void_p(at), offsets, offsets, base, kind) == 0
     return d
 
 
@@ -118,6 +118,7 @@ def test_route_refusals(pkg):
     assert call(R=_csr(pkg, 10, 64, 80, S.ACL_INT32)) == no and call(R=_csr(pkg, 10, 64, 80, offsets=1)) == no
     assert call(R=_csr(pkg, 10, 64, 80, base=1)) == no
     assert call(x=_mat(pkg, 10, 1025), R=_csr(pkg, 10, 1025, 80)) == no
+    assert call(b=_vec(pkg, 64, S.ACL_FLOAT, FAKE + 2)) == bad and call(R=_csr(pkg, 10, 64, 80, at=FAKE + 2)) == bad  # not on the types' boundaries
     assert call(b=_vec(pkg, 63, S.ACL_FLOAT)) == bad and call(b=_vec(pkg, 64, S.ACL_BF16)) == no
     many = _rule(pkg, groups=64, groups_kept=64)
     assert f(_h(), many.address, x, None, R) == no
@@ -125,7 +126,7 @@ def test_route_refusals(pkg):
     d = _vec(pkg, 80, S.ACL_FLOAT)
     assert g(None, rule.address, x, R, d, x) == S.ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR
     assert g(_h(), rule.address, x, R, None, x) == bad and g(_h(), rule.address, x, R, d, None) == bad
-    assert g(_h(), rule.address, x, R, _vec(pkg, 79, S.ACL_FLOAT), x) == bad
+    assert g(_h(), rule.address, x, R, _vec(pkg, 79, S.ACL_FLOAT), x) == bad and g(_h(), rule.address, x, R, _vec(pkg, 80, S.ACL_FLOAT, FAKE + 2), x) == bad
     assert g(_h(), rule.address, x, R, _vec(pkg, 80, S.ACL_INT32), x) == no
     assert g(_h(), rule.address, x, R, d, _mat(pkg, 10, 64, S.ACL_FLOAT)) == no
     assert g(_h(), rule.address, x, R, d, _mat(pkg, 9, 64)) == bad
@@ -155,6 +156,7 @@ def test_experts_refusals(pkg):
     assert mm(X=_mat(pkg, 10, 32, S.ACL_FLOAT)) == no and mm(W=_mat(pkg, 4 * 48, 32, S.ACL_FLOAT16)) == no
     assert mm(X=_mat(pkg, 10, 32, order=1)) == no
     assert mm(R=_csr(pkg, 10, 4, 20, offsets=1)) == no and mm(R=_csr(pkg, 10, 4, 20, base=1)) == no
+    assert mm(R=_csr(pkg, 10, 4, 20, at=FAKE + 1)) == bad
     assert mm(R=_csr(pkg, 10, 1025, 20), W=_mat(pkg, 1025, 32), Y=_mat(pkg, 20, 1)) == no
     assert L.b200spExpertsMM(None, 1, 0, None, R, X, W, None, Y, None) == S.ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR
     assert L.b200spExpertsMM(_h(), 1, 0, None, R, X, W, None, Y, None) == S.ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES
