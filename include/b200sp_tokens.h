@@ -13,6 +13,7 @@
  * rounded once: the same inputs give the same bits.  Values that f16 cannot hold become infinite (SpMM clamps them; a
  * gradient has to show that it overflowed).  Calls enqueue on the handle's stream, wait for nothing, allocate nothing,
  * and may be captured.  A handle is used on the device that it was created on, whatever device is current.
+ * (A call on no tokens can not be described: aclsparseCreateDnMat refuses a matrix of no rows.)
  * An output overlaps no input, unless it says so.  At most 2^31 - 2^20 tokens or entries of R.
  * Column-major operands, index bases of one and 64-bit CSR indices are ACL_SPARSE_STATUS_NOT_SUPPORTED.
  */

@@ -704,6 +704,21 @@ def test_scalars_on_the_device(pkg, handle):
         ref.close(grad, want, (many + 4) * F32 * size)
     api.embedding(handle, mat(api, table), api.DnVec(tokens), mat(api, out), None, None)
     assert torch.equal(out, table[tokens])
+    offsets, columns = ragged(g, 40, 3, 2)
+    nnz = len(columns)
+    x, w, y, dw = (matrix(g, *s)[0] for s in ((40, 48, "bf16"), (3 * 72, 48, "bf16"), (nnz, 72, "bf16"), (3 * 72, 48, "f32")))
+    R = api.CsrMatrix(offsets, columns, torch.empty(nnz, device="cuda"), 40, 3)
+    X, W, Y, DW = mat(api, x), mat(api, w), mat(api, y), mat(api, dw)
+    buffer = torch.empty(max(api.experts_buffer_size(handle, R, X, W, Y), api.experts_grad_buffer_size(handle, R, Y, X, DW)), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    for b in (0.0, 0.5):
+        beta = torch.tensor([b], device="cuda")
+        want, size, many = ref.experts_grad(offsets, columns, y, x, 3, False, 1.5, b, dw.view(3, 72, 48))
+        api.experts_grad(handle, R, Y, X, DW, alpha, beta, buffer=buffer)
+        ref.close(dw.view(3, 72, 48), want, ref.rounding(dw.dtype, want) + size * (many + 4) * 2 * F32)
+        want, size = ref.experts_mm(offsets, columns, x, w.view(3, 72, 48), 3, True, False, 1.5, b, y)
+        api.experts_mm(handle, R, X, W, Y, alpha, beta, buffer=buffer)
+        ref.close(y, want, ref.rounding(y.dtype, want) + size * 52 * 2 * F32)
     handle.set_pointer_mode_device(False)
 
 
@@ -738,3 +753,44 @@ def test_experts_wait_that_runs_out(pkg, handle):
     assert L.b200sp_experts_error() == 0
     want, size = ref.experts_mm(offsets, columns, x, w.view(4, 128, 64), 4, True, False, 1.0, 0.0, y)
     ref.close(y, want, ref.rounding(y.dtype, want) + size * 68 * 2 * F32)
+
+
+def test_tables_and_weights_beyond_32_bits(pkg, handle):
+    """More than 2^31 elements and 2^32 bytes: the last rows of a table, its gradient, the last of the experts."""
+    from ops_sparse_b200 import api
+    g = gen(9)
+    vocab, width = 270001, 8192
+    table = torch.empty(vocab, width, dtype=torch.float16, device="cuda")
+    assert table.numel() > 2 ** 31
+    tokens = torch.tensor([vocab - 1, 0, vocab - 2, vocab - 1, 262145], device="cuda")
+    table[tokens] = torch.randn(5, width, generator=g, device="cuda").half()
+    out = torch.empty(5, width, dtype=torch.float16, device="cuda")
+    api.embedding(handle, mat(api, table), api.DnVec(tokens), mat(api, out))
+    assert torch.equal(out, table[tokens])
+    table.fill_(3.0)
+    api.embedding_grad(handle, mat(api, out), api.DnVec(tokens), mat(api, table))
+    want = torch.zeros(vocab, dtype=torch.bool, device="cuda")
+    want[tokens] = True
+    assert torch.equal((table != 0).any(1), want)
+    assert torch.equal(table[vocab - 1], (out[0].float() + out[3].float()).half()) and torch.equal(table[262145], out[4])
+    del table
+    experts, n, d = 34, 8192, 8192
+    w = torch.empty(experts * n, d, dtype=torch.bfloat16, device="cuda")
+    assert w.numel() > 2 ** 31
+    w[-n:] = torch.randn(n, d, generator=g, device="cuda").bfloat16() / 64
+    x = torch.randn(3, d, generator=g, device="cuda").bfloat16()
+    R = api.CsrMatrix(torch.arange(4, dtype=torch.int32, device="cuda"), torch.full((3,), experts - 1, dtype=torch.int32, device="cuda"),
+                      torch.empty(3, device="cuda"), 3, experts)
+    y = torch.empty(3, n, dtype=torch.float32, device="cuda")
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    buffer = torch.empty(api.experts_buffer_size(handle, R, X, W, Y), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, X, W, Y, buffer=buffer)
+    last = w[-n:].double()
+    ref.close(y, x.double() @ last.T, (x.double().abs() @ last.abs().T) * (d + 4) * 2 * F32)
+    dy = torch.randn(3, n, generator=g, device="cuda").bfloat16()
+    w.fill_(2.0)
+    api.experts_grad(handle, R, mat(api, dy), X, W, buffer=buffer)
+    assert (w[:-n] == 0).all()
+    want = dy.double().T @ x.double()
+    ref.close(w[-n:], want, ref.rounding(w.dtype, want) + 14 * F32 * (dy.double().abs().T @ x.double().abs()))
