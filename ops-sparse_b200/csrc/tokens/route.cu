@@ -88,10 +88,11 @@ __device__ __forceinline__ unsigned long long MaxKey(unsigned long long v)
 
 // Scores of the lanes' logits (masked: -infinity), 0 for the masked.  In f32 a sigmoid is taken from the fast exponential and division: it
 // serves the choice alone.  *error: how far they may be from exact ones.
-//   sigmoid: __expf is off by 2 + 1.16 |x| units of 2^-23 relative to e^-x, of which p (1 - p) <= p / (1 + |x|) reaches p: less
-//   than 4 of p with the division's 2 and the addition; 8 are allowed.
-//   softmax: expf is off by 2, the difference of the logits by |x - most| / 2 (of which p |x - most| <= 0.4 reaches p), a sum of kPer +
-//   5 additions by half of that, at most 24 units of p <= the largest score; 32 are allowed.
+//   sigmoid: __expf is off by 2 + 1.17 |x| units of 2^-23 relative to e^-x, of which p (1 - p) times reaches p: with p (1 - p) <= 1/4 and
+//   p (1 - p) |x| < 0.23 less than one unit; the addition and the division bring three more; 8 are allowed.
+//   softmax: expf is off by 2 units relative to p, the difference of the logits by |x - most| / 2 (p |x - most| <= 0.4 of the largest score), a
+//   sum of kPer + 5 additions by half of that many, the reciprocal and the product by one: at most 24 of the largest score; 32 are
+//   allowed.
 template <typename Real, int kPer>
 __device__ __forceinline__ void Scores(const RouteArgs &a, const float (&x)[kPer], Real (&p)[kPer], float *most, Real *inverse, float *error)
 {
@@ -187,7 +188,7 @@ __device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer
         const float least = ValueOf(__reduce_min_sync(kAll, kept ? key : ~0u));
         const float other = ValueOf(__reduce_max_sync(kAll, lane < a.groups && !kept ? key : KeyOf(-INFINITY)));
         // two scores each, and three additions that round
-        unsure = least - other <= 4 * error + 4.8e-7f * (fabsf(least) + fabsf(other));
+        unsure = other > -INFINITY && least - other <= 4 * error + 4.8e-7f * (fabsf(least) + fabsf(other));
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
@@ -279,7 +280,7 @@ template <typename In, typename Out, int kPer> __global__ void __launch_bounds__
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         x[j] = 32 * j + lane < a.experts ? ToFloat(row[32 * j + lane]) : -INFINITY;
-        if (!(x[j] > -INFINITY)) x[j] = -INFINITY;  // NaN, too
+        x[j] = fmaxf(x[j], -INFINITY);  // NaN is masked, too
         sLogits[32 * j + lane] = x[j];
     }
     __syncwarp();
