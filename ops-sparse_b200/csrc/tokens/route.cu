@@ -366,7 +366,7 @@ __device__ __forceinline__ float LoadAs(const void *p, long long i, int type)
     return static_cast<const float *>(p)[i];
 }
 
-// Lane i has entry i of the token's row.  With q the weights over scale and g their gradients (times scale):
+// Lane i has entry i of the token's row.  With q the weights over scale and g their gradients, scale times
 //   softmax, renormalised   dx = q (g - sum g q): the softmax of the chosen logits alone
 //   sigmoid, renormalised   dx = (g - sum g q) / (sum s) * s (1 - s)
 //   sigmoid                 dx = g s (1 - s)
@@ -387,7 +387,7 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
         col = __ldg(a.columns + i);
         if (col < 0 || col >= a.experts || LoadAs(a.values, i, a.valueType) == 0.0f) col = -1;
         if (col >= 0) {
-            g = a.scale * LoadAs(a.grad, i, a.gradType);
+            g = LoadAs(a.grad, i, a.gradType);
             x = ToFloat(row[col]);
             if (!(x > -INFINITY)) col = -1, g = 0.0f, x = -INFINITY;
         }
@@ -413,7 +413,7 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
         const float p = col < 0 ? 0.0f : (x == m ? 1.0f : expf(x - m)) * inv;
         const float dot = WarpSum(g * p);
 #pragma unroll
-        for (int j = 0; j < kPer; ++j) sRow[32 * j + lane] = -v[j] * inv * dot;
+        for (int j = 0; j < kPer; ++j) sRow[32 * j + lane] = -a.scale * v[j] * inv * dot;
         dx = p * (g - dot);
     } else {
 #pragma unroll
@@ -422,8 +422,8 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
             const float s = col < 0 ? 0.0f : 1.0f / (1.0f + expf(-x));
             const float rest = col < 0 ? 0.0f : 1.0f / (1.0f + expf(x));  // 1 - s, exactly enough where s is near 1
             if (a.renormalise) {
-                const float sum = WarpSum(s), inv = sum > 0 ? 1.0f / sum : 0.0f;
-                g = (g - WarpSum(g * s) * inv) * inv;
+                const float sum = WarpSum(s), dot = WarpSum(g * s);
+                g = sum > 0 ? (g - dot / sum) / sum : 0.0f;
             }
             dx = g * s * rest;
         } else {
@@ -434,7 +434,7 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
         }
     }
     __syncwarp();
-    if (col >= 0) sRow[col] = dx;
+    if (col >= 0) sRow[col] = a.scale * dx;
     __syncwarp();
     T *const out = static_cast<T *>(a.out) + token * a.ldOut;
 #pragma unroll
