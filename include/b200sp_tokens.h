@@ -126,8 +126,9 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
                                     aclsparseConstDnMatDescr_t matX, const void *beta, aclsparseDnMatDescr_t dW,
                                     void *buffer);
 
-/* 1 if a bounded wait of the experts' kernels ran out since the flag was cleared (never observed outside the test that
- * provokes it): rows of an output are unwritten then.  Both synchronise the device. */
+/* What went wrong in an experts' product since the flag was cleared.  1: a bounded wait ran out (never observed outside the test that
+ * provokes it), rows of the output are unwritten; 2: its buffer held no order, because the b200spExpertsPreprocess that belongs to it
+ * was captured and not replayed yet, and the output is untouched.  Both calls synchronise the device. */
 int b200sp_experts_error(void);
 int b200sp_experts_error_clear(void);
 /* For tests of that path: later products wait at most wait_cycles SM clocks (0 = the default, about two seconds) and expect

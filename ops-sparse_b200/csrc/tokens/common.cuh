@@ -14,6 +14,9 @@
 
 namespace b200sp_tokens {
 
+// Positions, columns: what a loop counts to, so that a step further is still an int.
+constexpr long long kMostCounted = (1ll << 31) - (1 << 20);
+
 inline size_t AlignUp(size_t v, size_t a) { return (v + a - 1) / a * a; }
 inline bool OnBoundary(const void *p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
 inline bool Aligned16(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
@@ -108,7 +111,7 @@ inline aclsparseStatus_t CheckDense(const aclsparseDnMatDescr *m)
 {
     if (m == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (m->order != ACL_SPARSE_ORDER_ROW || !IsFloatType(m->valueType)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (m->rows > INT32_MAX || m->cols > INT32_MAX || m->ld > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (m->rows > INT32_MAX || m->cols > kMostCounted || m->ld > INT32_MAX) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (m->values == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (!OnBoundary(m->values, BytesOf(m->valueType))) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;

@@ -380,7 +380,7 @@ aclsparseStatus_t CheckTokens(const aclsparseDnVecDescr *tokens)
 {
     if (tokens == nullptr || tokens->magic != b200sp::kDnVecMagic) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (tokens->valueType != ACL_INT32 && tokens->valueType != ACL_INT64) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (tokens->size > kMostSorted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (tokens->size > kMostCounted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (!OnBoundary(tokens->values, tokens->valueType == ACL_INT64 ? 8 : 4)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     return ACL_SPARSE_STATUS_SUCCESS;
 }

@@ -16,8 +16,8 @@ using namespace b200sp_tokens;
 
 constexpr int kMaxExperts = 1024;
 
-// The buffer: where every expert's entries begin (one more group: entries of no expert), the entries by expert and the
-// rows of R that they lie in; and the sort's own arrays.
+// The buffer: what R it is the order of; where every expert's entries begin (one more group: entries of no expert), the entries by
+// expert and the rows of R that they lie in; and the sort's own arrays.
 struct PlanLayout {
     size_t offsets, entries, rows, keyA, keyB, posB, total;
 };
@@ -25,8 +25,8 @@ PlanLayout PlanLayoutFor(long long nnz, long long experts)
 {
     PlanLayout L;
     const size_t words = AlignUp(sizeof(int) * (size_t)nnz, 256);
-    L.offsets = 0;
-    L.entries = AlignUp(sizeof(int) * (size_t)(experts + 2), 256);
+    L.offsets = 256;  // the header lies before
+    L.entries = L.offsets + AlignUp(sizeof(int) * (size_t)(experts + 2), 256);
     L.rows = L.entries + words;
     L.keyA = L.rows + words;
     L.keyB = L.keyA + words;
@@ -35,13 +35,20 @@ PlanLayout PlanLayoutFor(long long nnz, long long experts)
     return L;
 }
 
+// A product follows the order only if the buffer starts with this: the sizes that its entries and rows are below.  A Preprocess that was
+// captured and has not been replayed yet has written nothing.
+constexpr int kOrderMark = 0x45585031;
+inline int4 HeaderOf(long long nnz, long long experts, long long rows) { return make_int4(kOrderMark, (int)nnz, (int)experts, (int)rows); }
+
 // ---------------------------------------------------------------- the order of the entries
 
 __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const SortArgs s, const int *__restrict__ rowPtr, int rows,
-                                                                     int *__restrict__ rowOf, int *__restrict__ offsets)
+                                                                     int *__restrict__ rowOf, int *__restrict__ offsets, int4 *header,
+                                                                     const int4 mark)
 {
     extern __shared__ unsigned char sSort[];
     b200sp::WaitForPrevious();
+    if (blockIdx.x == 0 && threadIdx.x == 0) *header = mark;
     ClusterSort<int>(s, sSort, [&](int, int entry, int to) {
         // rows are of about the same length: the first guess is nearly always right
         int r = (int)((long long)entry * rows / s.count);
@@ -107,7 +114,7 @@ aclsparseStatus_t CheckRouted(const aclsparseSpMatDescr *R)
     const aclsparseStatus_t idx = b200sp::CheckExecIndexTypes(R->offsetType, R->indexType);
     if (idx != ACL_SPARSE_STATUS_SUCCESS) return idx;
     if (R->base != ACL_SPARSE_INDEX_BASE_ZERO) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz > kMostSorted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz > kMostCounted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
     if (R->rows == 0 || R->cols == 0 || R->nnz == 0) return ACL_SPARSE_STATUS_INVALID_VALUE;  // no dense operand has as few rows
     if (R->offsets == nullptr || R->indices == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
     if (!OnBoundary(R->offsets, 4) || !OnBoundary(R->indices, 4)) return ACL_SPARSE_STATUS_INVALID_VALUE;
@@ -173,6 +180,8 @@ MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const v
     const PlanLayout L = PlanLayoutFor(R->nnz, R->cols);
     const char *p = BufferStart(buffer);
     MmaArgs a{};
+    a.header = reinterpret_cast<const int4 *>(p);
+    a.mark = HeaderOf(R->nnz, R->cols, R->rows);
     a.offsets = reinterpret_cast<const int *>(p + L.offsets);
     a.entries = reinterpret_cast<const int *>(p + L.entries);
     a.rows = reinterpret_cast<const int *>(p + L.rows);
@@ -290,7 +299,8 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
         cfg.numAttrs = 2;
         b200sp_note_launches(1);
         e = cudaLaunchKernelEx(&cfg, ExpertsOrderKernel, s, static_cast<const int *>(matR->offsets), (int)matR->rows,
-                               reinterpret_cast<int *>(p + L.rows), offsets);
+                               reinterpret_cast<int *>(p + L.rows), offsets, reinterpret_cast<int4 *>(p),
+                               HeaderOf(matR->nnz, matR->cols, matR->rows));
     }
     std::lock_guard<std::mutex> lock(matR->expertsMutex);
     matR->experts = {};

@@ -38,6 +38,8 @@ constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
 enum class Mode { kProductT, kProductN, kGrad };
 
 struct MmaArgs {
+    const int4 *header;    // has to be `mark`, or nothing of the rest is looked at
+    int4 mark;
     const int *offsets, *entries, *rows;
     void *out;
     long long ldo;
@@ -55,6 +57,7 @@ struct MmaArgs {
 };
 
 __device__ int gExpertsError = 0;
+constexpr int kWaitRanOut = 1, kNoOrder = 2;
 
 __device__ __forceinline__ uint32_t Shared(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void BarInit(uint64_t *bar, int count)
@@ -266,7 +269,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     const Tiles<kMode, kPair> tiles{a, sStart, sOffset,
                                     ((kMode == Mode::kProductN ? a.d : a.n) + Tiles<kMode, kPair>::kHigh - 1) / Tiles<kMode, kPair>::kHigh};
     const int groups = tiles.Groups();
-    for (int e = tid; e <= groups; e += kMmaThreads) sOffset[e] = __ldg(a.offsets + e);
+    const int4 found = __ldg(a.header);
+    const bool ordered = found.x == a.mark.x && found.y == a.mark.y && found.z == a.mark.z && found.w == a.mark.w;
+    for (int e = tid; e <= groups; e += kMmaThreads) sOffset[e] = ordered ? __ldg(a.offsets + e) : 0;
     __syncthreads();
     if (warp == 0) {
         int run = 0;
@@ -287,7 +292,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sTmem;
-    const int all = sStart[groups];
+    const int all = ordered ? sStart[groups] : 0;
+    if (!ordered && tid == 0 && blockIdx.x == 0) atomicMax(&gExpertsError, kNoOrder);
     bool failed = false;
 
     if (kMode != Mode::kGrad && warp == 0) {
@@ -597,7 +603,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
         }
     }
     __syncwarp();
-    if (failed) atomicExch(&gExpertsError, 1);
+    if (failed) atomicMax(&gExpertsError, kWaitRanOut);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.

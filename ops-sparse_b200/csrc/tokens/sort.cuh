@@ -23,7 +23,6 @@ constexpr int kSortSteps = 4;                            // positions per thread
 constexpr int kSortTile = kSortThreads * kSortSteps;
 constexpr int kSortMaxBits = 10;
 constexpr int kSortMaxCtas = 8;                          // the portable cluster size
-constexpr long long kMostSorted = (1ll << 31) - (1 << 20);  // positions: a loop's step further is still an int
 
 struct SortArgs {
     const void *keys;     // int32 or int64, the caller's

@@ -476,6 +476,41 @@ def test_experts_keep_their_neighbours_infinities(pkg, handle):
     assert torch.equal(~dw.view(experts, -1).isfinite().all(1), hit)
 
 
+def test_a_captured_order_is_none_until_it_is_replayed(pkg, device):
+    """Preprocess in a graph, a product outside of it: before the first replay there is nothing to follow, whatever the buffer holds."""
+    from ops_sparse_b200 import api
+    L = pkg.lib()
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        h = api.Handle(stream)
+        g = gen(12)
+        offsets, columns = ragged(g, 60, 5, 2)
+        nnz = len(columns)
+        x, w = matrix(g, 60, 64, "bf16")[0], matrix(g, 5 * 136, 64, "bf16")[0]
+        y, dw = torch.full((nnz, 136), 5.0, dtype=torch.bfloat16, device="cuda"), torch.full((5 * 136, 64), 5.0, dtype=torch.bfloat16, device="cuda")
+        R = api.CsrMatrix(offsets, columns, torch.empty(nnz, device="cuda"), 60, 5)
+        X, W, Y, DW = mat(api, x), mat(api, w), mat(api, y), mat(api, dw)
+        size = max(api.experts_buffer_size(h, R, X, W, Y), api.experts_grad_buffer_size(h, R, Y, X, DW))
+        buffer = torch.full((size,), 127, dtype=torch.uint8, device="cuda")
+        graph = torch.cuda.CUDAGraph()
+        stream.synchronize()
+        with torch.cuda.graph(graph, stream=stream):
+            api.experts_preprocess(h, R, buffer)
+        for call in (lambda: api.experts_mm(h, R, X, W, Y, buffer=buffer), lambda: api.experts_grad(h, R, Y, X, DW, buffer=buffer)):
+            call()
+            stream.synchronize()
+            assert L.b200sp_experts_error() == 2 and L.b200sp_experts_error_clear() == 0
+        assert (y == 5).all() and (dw == 5).all()
+        graph.replay()
+        api.experts_mm(h, R, X, W, Y, buffer=buffer)
+        stream.synchronize()
+        assert L.b200sp_experts_error() == 0
+        want, size = ref.experts_mm(offsets, columns, x, w.view(5, 136, 64), 5, True, False, 1.0, 0.0, y)
+        ref.close(y, want, ref.rounding(y.dtype, want) + size * 68 * 2 * F32)
+        del graph
+    h.close()
+
+
 def test_products_refuse_a_buffer_sized_for_other_operands(pkg, handle):
     """Room for the copy of an operand that starts on no multiple of 16 bytes has to have been asked for."""
     from ops_sparse_b200 import api

@@ -72,7 +72,7 @@ def test_embedding_refusals(pkg):
     assert call(t=_mat(pkg, (1 << 31) - 1, 64)) == no
     many = (1 << 31) - (1 << 20) + 1
     assert call(k=_vec(pkg, many, S.ACL_INT32), o=_mat(pkg, many, 64)) == no
-    assert call(t=_mat(pkg, 100, 64, ld=1 << 31)) == no
+    assert call(t=_mat(pkg, 100, 64, ld=1 << 31)) == no and call(t=_mat(pkg, 1, many)) == no
     size = c_size_t()
     g = pkg.lib().b200spEmbeddingGradBufferSize
     assert g(_h(), out, tokens, table, None) == bad
