@@ -304,23 +304,28 @@ template <typename In, typename Out, int kPer> __global__ void __launch_bounds__
     int at = 0;
     const uint32_t nothing = KeyOf(-INFINITY);
     Chosen c{-1, false};
-    uint32_t top = 0;
+    uint32_t top = 0, taken = 0;  // of the last one, of the lane's
     unsigned e = 0;
     for (int i = 0; i < a.k; ++i) {
         top = __reduce_max_sync(kAll, head.x);
         e = __reduce_min_sync(kAll, head.x == top ? head.y : ~0u);
-        if (lane == i) c = {(int)e, top == nothing};
+        if (lane == i) c = {(int)e, top == nothing}, taken = top;
         if (head.y == e && head.x != 0) head = sList[at], at += 32;
     }
     if (a.bias != nullptr) {
-        // Neighbours of the last one taken, but for its equals in exact arithmetic too.
+        // Experts left out as near the last one taken as f32 tells: the choice is certain only where they, and those taken that are as near,
+        // all have its logit and bias.  (Equals of the last that are left out may be above another one taken.)
         const float last = ValueOf(top), room = 2 * error + 4.8e-7f * fabsf(last);
         const uint32_t near = top == nothing ? ~0u : KeyOf(last - room);
-        while (__any_sync(kAll, head.x > nothing && head.x >= near)) {
-            if (head.x > nothing && head.x >= near) {
-                unsure |= !(sLogits[head.y] == sLogits[e] && __ldg(a.bias + head.y) == __ldg(a.bias + e));
-                head = sList[at], at += 32;
-            }
+        const auto differs = [&](unsigned other) { return !(sLogits[other] == sLogits[e] && __ldg(a.bias + other) == __ldg(a.bias + e)); };
+        if (__any_sync(kAll, head.x > nothing && head.x >= near)) {
+            unsure |= lane < a.k && taken <= KeyOf(last + room) && differs(c.expert);
+            do {
+                if (head.x > nothing && head.x >= near) {
+                    unsure |= differs(head.y);
+                    head = sList[at], at += 32;
+                }
+            } while (__any_sync(kAll, head.x > nothing && head.x >= near));
         }
     }
     if (__any_sync(kAll, unsure)) c = ChooseExactly<kPer>(a, sLogits, sRows[warp], lane);

@@ -1,0 +1,41 @@
+"""GPU: token operators at their borders -- values that f32 cannot tell apart, weights that underflow, loops and offsets at the
+last sizes that are taken, orders that are out of date."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import token_reference as ref
+from test_tokens_gpu import check_route, gen, mat, matrix, ragged, routed
+from token_reference import DTYPE, F32
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the choice
+
+def test_route_three_saturated_scores(pkg, handle):
+    """Scores that are all 1 in f32: the one left out equals the last one taken, the first one taken lies below both."""
+    from ops_sparse_b200 import api
+    R = check_route(api, handle, torch.tensor([[20.0, 21.0, 21.0]], device="cuda"), torch.zeros(3, device="cuda"), 2, score="sigmoid")
+    assert R.col_ind.tolist() == [1, 2]
+
+
+@pytest.mark.parametrize("score,high", [("sigmoid", 20.0), ("softmax", 0.0)])
+@pytest.mark.parametrize("level", [0.0, 0.25])
+@pytest.mark.parametrize("experts,k,groups", [(12, 4, 1), (64, 8, 4), (300, 10, 1)])
+def test_route_equals_of_the_last_beside_near_ones(pkg, handle, score, high, level, experts, k, groups):
+    """Few different logits, one bias for all, scores closer than a step of the selection values: a sigmoid near 1, or a softmax beside an
+    expert that is larger by e^30.  In the second half of the rows all that are left out equal the last one taken, while lower ones have been taken."""
+    from ops_sparse_b200 import api
+    g = gen(experts + k)
+    x = high + 0.5 * torch.randint(0, 4, (200, experts), generator=g, device="cuda").float()
+    x[100:] = high + 1.0
+    x[100:, :k - 1] -= 0.5 * torch.randint(0, 2, (100, k - 1), generator=g, device="cuda")
+    if score == "softmax":
+        x[torch.arange(200, device="cuda"), torch.randint(0, experts, (200,), generator=g, device="cuda")] = 30.0
+    bias = torch.full((experts,), level, device="cuda")
+    bias[experts // 2 if groups > 1 else experts:] -= 5.0  # which groups are kept is clear
+    check_route(api, handle, x.bfloat16(), bias, k, score=score, groups=groups, kept=max(groups // 2, 1))
