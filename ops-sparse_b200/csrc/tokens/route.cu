@@ -183,12 +183,15 @@ __device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer
     const bool kept = lane < a.groups && place < a.kept;
     const unsigned open = __ballot_sync(kAll, kept);
     if (sizeof(Real) == 4 && (a.bias != nullptr || sums)) {
-        // the last group kept, and the first that is not
+        // The last group kept, and the first that is not.  Off are two scores of each, and by half a unit of 2^-23 what rounds: the two values
+        // and their sum.  A value with its bias may be far larger than the sum, and any group the one that is off: the largest terms count.
         const uint32_t key = KeyOf((float)mine);
         const float least = ValueOf(__reduce_min_sync(kAll, kept ? key : ~0u));
         const float other = ValueOf(__reduce_max_sync(kAll, lane < a.groups && !kept ? key : KeyOf(-INFINITY)));
-        // two scores each, and three additions that round
-        unsure = other > -INFINITY && least - other <= 4 * error + 4.8e-7f * (fabsf(least) + fabsf(other));
+        const bool finite = first > nothing && first < (Real)INFINITY;  // infinite ones are exact
+        const float terms = finite ? fabsf((float)first) + (sums && second > nothing ? fabsf((float)second) : 0.0f) : 0.0f;
+        const float most = __uint_as_float(__reduce_max_sync(kAll, __float_as_uint(terms)));
+        unsure = other > -INFINITY && !(least - other > 4 * error + 4.8e-7f * most);
     }
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {

@@ -39,3 +39,13 @@ def test_route_equals_of_the_last_beside_near_ones(pkg, handle, score, high, lev
     bias = torch.full((experts,), level, device="cuda")
     bias[experts // 2 if groups > 1 else experts:] -= 5.0  # which groups are kept is clear
     check_route(api, handle, x.bfloat16(), bias, k, score=score, groups=groups, kept=max(groups // 2, 1))
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size,tokens", [(300.0, 1000), (64.0, 3000)])
+def test_route_group_sums_of_large_opposite_biases(pkg, handle, score, size, tokens):
+    """The sum of a group's two best is near 1, its terms are not: what is rounded are the terms.  All experts of the kept groups are taken."""
+    from ops_sparse_b200 import api
+    x = (1e-4 if score == "sigmoid" else 0.5) * torch.randn(tokens, 64, generator=gen(31), device="cuda")
+    bias = torch.tensor([size, -size], device="cuda").repeat(32)
+    check_route(api, handle, x, bias, 32, score=score, groups=32, kept=16, group_score="top2")
