@@ -332,16 +332,22 @@ template <typename In, typename Out, int kPer> __global__ void __launch_bounds__
         }
     }
     if (__any_sync(kAll, unsure)) c = ChooseExactly<kPer>(a, sLogits, sRows[warp], lane);
-    // the weights, of the experts taken alone; their places by column
+    // The weights, of the experts taken alone; their places by column.  Those that are renormalised may share a factor, e^-x of the largest
+    // logit taken (a sigmoid, e^x / (1 + e^x), where that x is negative): scores below the least f32 still have their quotients.
     float w = 0.0f;
-    if (c.expert >= 0 && !c.weightless) {
-        const float own = sLogits[c.expert];
-        w = a.sigmoid ? 1.0f / (1.0f + expf(-own)) : (own == most ? 1.0f : expf(own - most)) * inverse;
+    const bool weighs = c.expert >= 0 && !c.weightless;
+    const float own = weighs ? sLogits[c.expert] : -INFINITY;
+    const float largest = a.renormalise ? ValueOf(__reduce_max_sync(kAll, KeyOf(own))) : a.sigmoid ? 0.0f : most;
+    if (weighs) {
+        if (a.sigmoid) w = expf(fminf(own, 0.0f) - fminf(largest, 0.0f)) / (1.0f + expf(-fabsf(own)));
+        else w = own == largest ? 1.0f : expf(own - largest);
     }
     float by = a.scale;
     if (a.renormalise) {
         const float sum = WarpSum(w);
         by = sum > 0 ? a.scale / sum : 0.0f;
+    } else if (!a.sigmoid) {
+        w *= inverse;
     }
     int to = 0;
     for (int i = 0; i < a.k; ++i) to += __shfl_sync(kAll, c.expert, i) < c.expert;

@@ -49,3 +49,30 @@ def test_route_group_sums_of_large_opposite_biases(pkg, handle, score, size, tok
     x = (1e-4 if score == "sigmoid" else 0.5) * torch.randn(tokens, 64, generator=gen(31), device="cuda")
     bias = torch.tensor([size, -size], device="cuda").repeat(32)
     check_route(api, handle, x, bias, 32, score=score, groups=32, kept=16, group_score="top2")
+
+
+# ---------------------------------------------------------------- weights that underflow
+
+FAR = [[-100.0, -101.0, -math.inf, -103.5], [-88.0, -89.0, -95.0, -400.0], [-90.0, -90.0, -90.0, -90.0], [3.0, -60.0, -95.0, -100.0],
+       [-700.0, -699.0, -698.5, -702.0], [-0.5, -88.5, -89.0, 0.25]]
+
+
+@pytest.mark.parametrize("x", ["f32", "bf16"])
+@pytest.mark.parametrize("k", [2, 4])
+def test_renormalised_weights_of_vanishing_sigmoids(pkg, handle, x, k):
+    """Scores below the least f32: their quotients are not."""
+    from ops_sparse_b200 import api
+    check_route(api, handle, torch.tensor(FAR, device="cuda").to(DTYPE[x]), None, k, score="sigmoid", scale=2.0)
+    R = routed(api, 1, 2, 2)
+    api.route(handle, api.RouteRule(score="sigmoid"), mat(api, torch.tensor([[-10001.0, -10000.0]], device="cuda")), None, R)
+    want = torch.softmax(torch.tensor([[0.0, 1.0]], dtype=torch.float64), 1)  # e^x / (1 + e^x) is e^x there
+    ref.close(R.values.view(1, 2), want, want * 16 * F32)
+
+
+def test_renormalised_weights_far_below_the_largest_logit(pkg, handle):
+    """A softmax whose largest logit is not among the chosen, which a bias or a group brings about."""
+    from ops_sparse_b200 import api
+    x = torch.tensor([[0.0, -120.0, -121.0, -300.0], [50.0, -60.0, -60.0, -61.5], [5.0, 2.0, 3.0, -200.0]], device="cuda")
+    R = check_route(api, handle, x, torch.tensor([0.0, 2.0, 2.0, 0.5], device="cuda"), 2)
+    assert R.col_ind.tolist() == [1, 2] * 3
+    check_route(api, handle, x, torch.tensor([0.0, 0.0, 2.0, 1.5], device="cuda"), 2, groups=2, kept=1, group_score="top2")
