@@ -382,7 +382,7 @@ __device__ __forceinline__ float LoadAs(const void *p, long long i, int type)
 
 // Lane i has entry i of the token's row.  With q the weights over scale and g their gradients, scale times
 //   softmax, renormalised   dx = q (g - sum g q): the softmax of the chosen logits alone
-//   sigmoid, renormalised   dx = (g - sum g q) / (sum s) * s (1 - s)
+//   sigmoid, renormalised   dx = q (g - sum g q) (1 - s)
 //   sigmoid                 dx = g s (1 - s)
 //   softmax                 dx = p (g - sum g p) for the chosen, -p sum g p for the others
 template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWarps<kPer>) RouteGradKernel(const RouteGradArgs a)
@@ -433,13 +433,16 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
 #pragma unroll
         for (int j = 0; j < kPer; ++j) sRow[32 * j + lane] = 0.0f;
         if (a.sigmoid) {
-            const float s = col < 0 ? 0.0f : 1.0f / (1.0f + expf(-x));
-            const float rest = col < 0 ? 0.0f : 1.0f / (1.0f + expf(x));  // 1 - s, exactly enough where s is near 1
+            // the scores as the weights are taken from them: without the factor e^(largest) where that is small
+            const float largest = a.renormalise ? WarpMax(x) : 0.0f;
+            const float s = col < 0 ? 0.0f : expf(fminf(x, 0.0f) - fminf(largest, 0.0f)) / (1.0f + expf(-fabsf(x)));
+            const float rest = col < 0 ? 0.0f : 1.0f / (1.0f + expf(x));  // 1 - the score, exactly enough where that is near 1
             if (a.renormalise) {
-                const float sum = WarpSum(s), dot = WarpSum(g * s);
-                g = sum > 0 ? (g - dot / sum) / sum : 0.0f;
+                const float sum = WarpSum(s), q = sum > 0 ? s / sum : 0.0f;
+                dx = q * (g - WarpSum(g * q)) * rest;
+            } else {
+                dx = g * s * rest;
             }
-            dx = g * s * rest;
         } else {
             const float m = WarpMax(x);
             const float e = col < 0 ? 0.0f : x == m ? 1.0f : expf(x - m);

@@ -76,3 +76,27 @@ def test_renormalised_weights_far_below_the_largest_logit(pkg, handle):
     R = check_route(api, handle, x, torch.tensor([0.0, 2.0, 2.0, 0.5], device="cuda"), 2)
     assert R.col_ind.tolist() == [1, 2] * 3
     check_route(api, handle, x, torch.tensor([0.0, 0.0, 2.0, 1.5], device="cuda"), 2, groups=2, kept=1, group_score="top2")
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("grad", ["f32", "bf16"])
+def test_gradient_of_renormalised_weights_that_vanish(pkg, handle, score, grad):
+    from ops_sparse_b200 import api
+    x = torch.tensor(FAR, device="cuda")
+    rule = {"score": score, "scale": 1.5}
+    columns, weights = ref.route(x, None, 3, **rule)
+    values = weights.float().cuda()  # as if they had been kept: none is 0 but that of the masked
+    offsets = torch.arange(0, 3 * len(FAR) + 1, 3, dtype=torch.int32, device="cuda")
+    R = api.CsrMatrix(offsets, columns.flatten().cuda(), values.flatten(), len(FAR), 4)
+    d = torch.randn(3 * len(FAR), generator=gen(7), device="cuda").to(DTYPE[grad])
+    out = torch.full_like(x, math.nan)
+    api.route_grad(handle, api.RouteRule(**rule), mat(api, x), R, api.DnVec(d), mat(api, out))
+    # dx = scale * q (g - sum g q) (1 - s for a sigmoid), q the weights over scale; each term with the errors of q: an exponential of a
+    # difference of up to 302 and of x, to two units each, three additions, a division
+    q, g = (weights / 1.5), d.double().cpu().view(-1, 3)
+    chosen = x.double().cpu().gather(1, columns.long())
+    rest = 1 / (1 + chosen.exp()) if score == "sigmoid" else 1.0
+    want = torch.zeros(x.shape, dtype=torch.float64).scatter_(1, columns.long(), 1.5 * q * rest * (g - (g * q).sum(1, keepdim=True)))
+    size = torch.zeros_like(want).scatter_(1, columns.long(), 1.5 * q * 2 * g.abs().amax(1, keepdim=True))
+    ref.close(out, want, (size * (2 * 302 + 24) * F32).clamp_min(1e-37))
+    assert (want[0].abs() > 1e-3).sum() >= 2
