@@ -181,7 +181,7 @@ template <typename Out> __device__ __forceinline__ void FillTable(const GradArgs
         if (block == 0 && rest < elements) table[rest] = FromFloat<Out>(0.0f);
         return;
     }
-    for (int r = block; r < a.fillFirst; r += blocks)
+    for (long long r = block; r < a.fillFirst; r += blocks)  // a step past the last of 2^31 - 2 rows is no int
         for (int c = threadIdx.x; c < a.width; c += blockDim.x) table[r * a.ldTable + c] = FromFloat<Out>(0.0f);
 }
 
@@ -249,8 +249,8 @@ template <typename Out> __global__ void __launch_bounds__(256) EmbeddingScaleKer
     b200sp::WaitForPrevious();
     const float beta = a.sc.Beta();
     if (beta == 0.0f || beta == 1.0f) return;
-    for (int r = blockIdx.x; r < a.vocab; r += gridDim.x) {
-        const int at = LowerBound(a.keys, a.count, r);
+    for (long long r = blockIdx.x; r < a.vocab; r += gridDim.x) {
+        const int at = LowerBound(a.keys, a.count, (int)r);
         if (at < a.count && __ldg(a.keys + at) == r) continue;
         Out *const row = static_cast<Out *>(a.table) + r * a.ldTable;
         for (int c = threadIdx.x; c < a.width; c += 256) row[c] = FromFloat<Out>(beta * ToFloat(row[c]));

@@ -100,3 +100,24 @@ def test_gradient_of_renormalised_weights_that_vanish(pkg, handle, score, grad):
     size = torch.zeros_like(want).scatter_(1, columns.long(), 1.5 * q * 2 * g.abs().amax(1, keepdim=True))
     ref.close(out, want, (size * (2 * 302 + 24) * F32).clamp_min(1e-37))
     assert (want[0].abs() > 1e-3).sum() >= 2
+
+
+# ---------------------------------------------------------------- loops at the last sizes that are taken
+
+def test_table_gradient_of_the_most_rows(pkg, handle):
+    """2^31 - 2 rows, the largest table that is taken: a step past the last row is no int.  Scaled rows, and zeros of rows with a gap behind."""
+    from ops_sparse_b200 import api
+    vocab = 2 ** 31 - 2
+    tokens, d = torch.tensor([vocab - 1, 3, vocab - 1], device="cuda"), torch.tensor([[1.0], [2.0], [4.0]], device="cuda").half()
+    memory = torch.full((2 * vocab,), 3.0, dtype=torch.float16, device="cuda")
+    table = memory[:vocab]
+    api.embedding_grad(handle, mat(api, d), api.DnVec(tokens), api.DnMat(table, vocab, 1, 1), beta=0.5)
+    assert table[-1] == 6.5 and table[3] == 3.5
+    table[-1] = table[3] = 1.5
+    assert (table == 1.5).all() and (memory[vocab:] == 3.0).all()
+    memory.fill_(3.0)
+    api.embedding_grad(handle, mat(api, d), api.DnVec(tokens), api.DnMat(memory, vocab, 1, 2))
+    table = memory.view(vocab, 2)
+    assert table[-1].tolist() == [5.0, 3.0] and table[3].tolist() == [2.0, 3.0]
+    table[-1, 0] = table[3, 0] = 0.0
+    assert (table[:, 0] == 0).all() and (table[:, 1] == 3.0).all()
