@@ -236,7 +236,7 @@ __device__ __forceinline__ int LowerBound(const int *keys, int count, int key)
 {
     int lo = 0, hi = count;
     while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
+        const int mid = lo + ((hi - lo) >> 1);
         if (__ldg(keys + mid) < key) lo = mid + 1;
         else hi = mid;
     }

@@ -121,3 +121,15 @@ def test_table_gradient_of_the_most_rows(pkg, handle):
     assert table[-1].tolist() == [5.0, 3.0] and table[3].tolist() == [2.0, 3.0]
     table[-1, 0] = table[3, 0] = 0.0
     assert (table[:, 0] == 0).all() and (table[:, 1] == 3.0).all()
+
+
+def test_table_gradient_of_more_than_a_billion_tokens(pkg, handle):
+    """Past 2^30 positions the sum of two of them is no int: rows whose tokens would come behind all that occur are looked for there."""
+    from ops_sparse_b200 import api
+    count = 2 ** 30 + 4097
+    tokens = torch.full((count,), 5, dtype=torch.int32, device="cuda")
+    d = torch.zeros(count, 1, dtype=torch.float16, device="cuda")
+    d[::1 << 20] = 1.0  # 1025 of them
+    table = torch.full((8, 1), 3.0, device="cuda")
+    api.embedding_grad(handle, mat(api, d), api.DnVec(tokens), mat(api, table), alpha=2.0, beta=0.5)
+    assert table.flatten().tolist() == [1.5] * 5 + [2051.5] + [1.5] * 2
