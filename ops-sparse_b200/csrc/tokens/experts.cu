@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
         for (int e = threadIdx.x; e <= s.limit + 1; e += kSortThreads) {
             int lo = 0, hi = s.count;
             while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
+                const int mid = lo + ((hi - lo) >> 1);
                 if (__ldcg(s.keyA + mid) < e) lo = mid + 1;
                 else hi = mid;
             }

@@ -133,3 +133,25 @@ def test_table_gradient_of_more_than_a_billion_tokens(pkg, handle):
     table = torch.full((8, 1), 3.0, device="cuda")
     api.embedding_grad(handle, mat(api, d), api.DnVec(tokens), mat(api, table), alpha=2.0, beta=0.5)
     assert table.flatten().tolist() == [1.5] * 5 + [2051.5] + [1.5] * 2
+
+
+def test_experts_of_more_than_a_billion_entries(pkg, handle):
+    """1024 experts (two passes of the sort, experts' first places by search) and more than 2^30 entries."""
+    from ops_sparse_b200 import api
+    tokens, each, experts = 1024, 2 ** 20 + 2, 1024
+    nnz = tokens * each
+    columns = torch.tensor([3, experts - 1], dtype=torch.int32, device="cuda").repeat(nnz // 2)
+    offsets = each * torch.arange(tokens + 1, dtype=torch.int32, device="cuda")
+    R = api.CsrMatrix(offsets, columns, torch.empty(1, device="cuda"), tokens, experts, nnz)
+    x, w = torch.zeros(tokens, 8, dtype=torch.bfloat16, device="cuda"), torch.zeros(experts, 8, dtype=torch.bfloat16, device="cuda")
+    x[:, 0] = (torch.arange(tokens, device="cuda") % 8).bfloat16()
+    w[3, 0], w[-1, 0] = 1.0, 2.0
+    y = torch.full((nnz, 1), 9.0, dtype=torch.bfloat16, device="cuda")
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    buffer = torch.empty(api.experts_buffer_size(handle, R, X, W, Y), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, X, W, Y, buffer=buffer)
+    torch.cuda.synchronize()
+    assert pkg.lib().b200sp_experts_error() == 0
+    y = y.view(tokens, each // 2, 2)
+    assert (y[:, :, 0] == x[:, :1]).all() and (y[:, :, 1] == 2 * x[:, :1]).all()
