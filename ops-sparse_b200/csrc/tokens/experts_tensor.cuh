@@ -378,8 +378,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                         break;
                     }
                     const uint32_t at = place + ring.stage * a.stageBytes + kMmaABytes + part * 1024;
-                    const int col = turn * kMmaDepth + 8 * piece, left = max(0, min(16, 2 * (depth - col)));  // bytes of the piece
-                    const char *const from = x + (left > 0 ? 2 * col : 0);
+                    const int col = turn * kMmaDepth + 8 * piece, left = 2 * max(0, min(8, depth - col));  // bytes of the piece
+                    const char *const from = x + (left > 0 ? 2ll * col : 0);
 #pragma unroll
                     for (int i = 0; i < kRows; ++i) {
 #pragma unroll
@@ -402,9 +402,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 constexpr int kBlocksY = kMmaRows / 64, kBlocksX = kMmaColsMost / (kPair ? 2 : 1) / 64;
                 int leftY[kBlocksY], leftX[kBlocksX];
 #pragma unroll
-                for (int b = 0; b < kBlocksY; ++b) leftY[b] = max(0, min(16, 2 * (a.n - f0 - 8 * piece - 64 * b)));
+                for (int b = 0; b < kBlocksY; ++b) leftY[b] = 2 * max(0, min(8, a.n - f0 - 8 * piece - 64 * b));
 #pragma unroll
-                for (int b = 0; b < kBlocksX; ++b) leftX[b] = max(0, min(16, 2 * (a.d - c0 - 8 * piece - 64 * b)));
+                for (int b = 0; b < kBlocksX; ++b) leftX[b] = 2 * max(0, min(8, a.d - c0 - 8 * piece - 64 * b));
                 const char *const y = static_cast<const char *>(a.dy) + 2ll * (f0 + 8 * piece), *const x = static_cast<const char *>(a.x) + 2ll * (c0 + 8 * piece);
                 const uint32_t pitchY = (uint32_t)a.ldy * 2, pitchX = (uint32_t)a.ldx * 2;
                 int rowY, rowX;

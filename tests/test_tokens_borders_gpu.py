@@ -155,3 +155,27 @@ def test_experts_of_more_than_a_billion_entries(pkg, handle):
     assert pkg.lib().b200sp_experts_error() == 0
     y = y.view(tokens, each // 2, 2)
     assert (y[:, :, 0] == x[:, :1]).all() and (y[:, :, 1] == 2 * x[:, :1]).all()
+
+
+def test_experts_of_more_than_a_billion_columns(pkg, handle):
+    """Past 2^30 columns twice a column is no int: gradients of an expert that is one row of so many, or one column."""
+    from ops_sparse_b200 import api
+    wide = 2 ** 30 + 72
+    one = torch.tensor([[3.0]], dtype=torch.bfloat16, device="cuda").expand(1, 8).contiguous()
+    long = torch.zeros(1, wide, dtype=torch.bfloat16, device="cuda")
+    spots = [0, 5, 2 ** 29 + 1, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 71]
+    long[0, spots] = torch.arange(1, 7, device="cuda").bfloat16()
+    R = api.CsrMatrix(torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty(1, device="cuda"), 1, 1)
+    for dy, x in ((one, long), (long, one)):  # dW of 8 x wide, of wide x 8
+        dw = torch.full((dy.shape[1], x.shape[1]), 9.0, dtype=torch.bfloat16, device="cuda")
+        DY, X, DW = mat(api, dy), mat(api, x), mat(api, dw)
+        buffer = torch.empty(api.experts_grad_buffer_size(handle, R, DY, X, DW), dtype=torch.uint8, device="cuda")
+        api.experts_preprocess(handle, R, buffer)
+        api.experts_grad(handle, R, DY, X, DW, buffer=buffer)
+        torch.cuda.synchronize()
+        assert pkg.lib().b200sp_experts_error() == 0
+        if x is long:
+            assert all(torch.equal(row, 3 * long[0]) for row in dw)
+        else:
+            assert all(torch.equal(dw[:, c], 3 * long[0]) for c in range(8))
+        del dw, DW
