@@ -34,6 +34,8 @@ constexpr int kMmaGatherWarps = 12, kMmaPartsMost = 2;  // warps that gather, of
 constexpr int kMmaFirstGather = 6;                 // warp 0 requests W, 1 multiplies, 2 ... 5 store, 6 ... gather
 constexpr int kMmaThreads = 32 * (kMmaFirstGather + kMmaGatherWarps);
 constexpr long long kMmaWaitCycles = 4'000'000'000;  // two seconds
+// A tile's results may take longer, by its steps: all SMs at once ask DRAM for 48 KB a step, some 2000 clocks, where nothing comes from L2.
+constexpr long long kMmaStepCycles = 4096;
 
 enum class Mode { kProductT, kProductN, kGrad };
 
@@ -492,7 +494,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             const MmaTile m = tiles.At(t);
             const int acc = tile & 1, turn = tile >> 1;
             if (m.steps > 0) {
-                if (!BarWaitWarp(sDone + acc, (uint32_t)turn & 1u, a.waitCycles)) {
+                if (!BarWaitWarp(sDone + acc, (uint32_t)turn & 1u, a.waitCycles + m.steps * kMmaStepCycles)) {
                     failed = true;
                     break;
                 }

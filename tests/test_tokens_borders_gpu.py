@@ -179,3 +179,54 @@ def test_experts_of_more_than_a_billion_columns(pkg, handle):
         else:
             assert all(torch.equal(dw[:, c], 3 * long[0]) for c in range(8))
         del dw, DW
+
+
+def _waits(pkg):
+    import ctypes
+    f = pkg.lib().b200sp_experts_wait_test
+    f.argtypes, f.restype = [ctypes.c_longlong, ctypes.c_uint], None
+    return f
+
+
+def test_a_long_sum_is_no_wait_that_runs_out(pkg, handle):
+    """The results of a tile may take as long as its steps: with a limit of 400,000 clocks, an expert of 300,000 entries (4688 steps)."""
+    from ops_sparse_b200 import api
+    nnz = 300000
+    g = gen(3)
+    R = api.CsrMatrix(torch.arange(nnz + 1, dtype=torch.int32, device="cuda"), torch.zeros(nnz, dtype=torch.int32, device="cuda"), torch.empty(1, device="cuda"),
+                      nnz, 1, nnz)
+    x, dy = (torch.randint(-1, 2, (nnz, 64), generator=g, device="cuda").bfloat16() for _ in range(2))
+    dw = torch.empty(64, 64, device="cuda")
+    X, DY, DW = mat(api, x), mat(api, dy), mat(api, dw)
+    buffer = torch.empty(api.experts_grad_buffer_size(handle, R, DY, X, DW), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    torch.cuda.synchronize()
+    waits = _waits(pkg)
+    try:
+        waits(400_000, 0)
+        api.experts_grad(handle, R, DY, X, DW, buffer=buffer)
+        torch.cuda.synchronize()
+    finally:
+        waits(0, 0)
+    error = pkg.lib().b200sp_experts_error()
+    pkg.lib().b200sp_experts_error_clear()
+    assert error == 0
+    assert torch.equal(dw.double(), dy.double().T @ x.double())  # whole numbers below 2^24
+
+
+def test_a_sum_over_more_than_a_billion_columns(pkg, handle):
+    """2^24 steps in one tile: seconds, but no wait that runs out; columns past 2^30."""
+    from ops_sparse_b200 import api
+    wide = 2 ** 30 + 72
+    x, w = torch.zeros(1, wide, dtype=torch.bfloat16, device="cuda"), torch.zeros(1, wide, dtype=torch.bfloat16, device="cuda")
+    spots = [0, 5, 2 ** 29 + 1, 2 ** 30 - 1, 2 ** 30, 2 ** 30 + 71]
+    x[0, spots], w[0, spots] = torch.arange(1, 7, device="cuda").bfloat16(), torch.tensor([1.0, 8, 64, 512, 4096, 32768], device="cuda").bfloat16()
+    R = api.CsrMatrix(torch.tensor([0, 1], dtype=torch.int32, device="cuda"), torch.zeros(1, dtype=torch.int32, device="cuda"), torch.empty(1, device="cuda"), 1, 1)
+    y = torch.full((1, 1), 9.0, device="cuda")
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    buffer = torch.empty(api.experts_buffer_size(handle, R, X, W, Y), dtype=torch.uint8, device="cuda")
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, X, W, Y, buffer=buffer)
+    torch.cuda.synchronize()
+    assert pkg.lib().b200sp_experts_error() == 0
+    assert y.item() == 1 + 16 + 192 + 2048 + 20480 + 196608
