@@ -245,12 +245,15 @@ extern "C" {
 int b200sp_experts_error(void)
 {
     int flag = 0;
+    if (cudaDeviceSynchronize() != cudaSuccess) return -1;  // the copy alone waits for no stream that the default one does not wait for
     return cudaMemcpyFromSymbol(&flag, gExpertsError, sizeof(flag)) == cudaSuccess ? flag : -1;
 }
 
 int b200sp_experts_error_clear(void)
 {
     const int zero = 0;
+    const cudaError_t e = cudaDeviceSynchronize();
+    if (e != cudaSuccess) return (int)e;
     return (int)cudaMemcpyToSymbol(gExpertsError, &zero, sizeof(zero));
 }
 

@@ -230,3 +230,35 @@ def test_a_sum_over_more_than_a_billion_columns(pkg, handle):
     torch.cuda.synchronize()
     assert pkg.lib().b200sp_experts_error() == 0
     assert y.item() == 1 + 16 + 192 + 2048 + 20480 + 196608
+
+
+def test_the_error_flag_waits_for_other_streams(pkg, device):
+    """Asked, or cleared, right after a product on a stream that the default one does not wait for."""
+    from ops_sparse_b200 import api
+    stream = torch.cuda.Stream()
+    L, waits = pkg.lib(), _waits(pkg)
+    with torch.cuda.stream(stream):
+        h = api.Handle(stream)
+        g = gen(4)
+        offsets, columns = ragged(g, 50, 4, 2, wild=0)
+        x, w = matrix(g, 50, 64, "bf16")[0], matrix(g, 4 * 128, 64, "bf16")[0]
+        y = torch.empty(len(columns), 128, dtype=torch.bfloat16, device="cuda")
+        R = api.CsrMatrix(offsets, columns, torch.empty(len(columns), device="cuda"), 50, 4)
+        X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+        buffer = torch.empty(api.experts_buffer_size(h, R, X, W, Y), dtype=torch.uint8, device="cuda")
+        api.experts_preprocess(h, R, buffer)
+        torch.cuda.synchronize()
+        try:
+            waits(200_000_000, 16)  # a tenth of a second
+            api.experts_mm(h, R, X, W, Y, buffer=buffer)
+            asked = L.b200sp_experts_error()
+            L.b200sp_experts_error_clear()
+            api.experts_mm(h, R, X, W, Y, buffer=buffer)
+            L.b200sp_experts_error_clear()
+        finally:
+            waits(0, 0)
+        torch.cuda.synchronize()
+        left = L.b200sp_experts_error()
+        L.b200sp_experts_error_clear()
+        assert asked == 1 and left == 0
+    h.close()
