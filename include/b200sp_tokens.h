@@ -97,7 +97,8 @@ typedef enum b200spExpertRows_t {
 } b200spExpertRows_t;
 
 /* Orders the entries of R by expert in `buffer`; wanted again when R's offsets or columns change, or when the buffer has been
- * written.  Nothing is waited for: it may be captured with the products that follow. */
+ * written.  After a b200spRoute into R products are refused (ACL_SPARSE_STATUS_INVALID_VALUE) until it has been called again.
+ * Nothing is waited for: it may be captured with the products that follow. */
 aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, void *buffer);
 
 /* Operands of the products whose rows do not start on 16 bytes are copied into the buffer first, in every call: the BufferSize calls count

@@ -520,6 +520,11 @@ aclsparseStatus_t b200spRoute(aclsparseHandle_t handle, const b200spRouteRule *r
                 (int)matR->cols, (int)(matR->nnz / matR->rows), rule->score == B200SP_ROUTE_SIGMOID, rule->groups, rule->groupsKept,
                 rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, 0, 0, 0, static_cast<int *>(matR->offsets),
                 static_cast<int *>(matR->indices), matR->values};
+    {
+        // R's columns are written: no buffer holds their order any more
+        std::lock_guard<std::mutex> lock(matR->expertsMutex);
+        matR->experts = {};
+    }
     if (a.kept == a.groups) a.groups = a.kept = 1;  // all are kept
     a.groupSize = a.experts / a.groups;
     a.perGroup = ((1u << 20) + a.groupSize - 1) / a.groupSize;

@@ -262,3 +262,41 @@ def test_the_error_flag_waits_for_other_streams(pkg, device):
         L.b200sp_experts_error_clear()
         assert asked == 1 and left == 0
     h.close()
+
+
+# ---------------------------------------------------------------- orders that are out of date
+
+def small(pkg, api, handle, g, tokens=40, experts=6, k=2, n=24, d=32):
+    """R as b200spRoute leaves it, the operands of a product, a buffer of its size."""
+    R = routed(api, tokens, experts, k)
+    logits = torch.randn(tokens, experts, generator=g, device="cuda")
+    x, w = matrix(g, tokens, d, "bf16")[0], matrix(g, experts * n, d, "bf16")[0]
+    y = torch.full((tokens * k, n), 5.0, dtype=torch.bfloat16, device="cuda")
+    operands = mat(api, x), mat(api, w), mat(api, y)
+    buffer = torch.empty(api.experts_buffer_size(handle, R, *operands), dtype=torch.uint8, device="cuda")
+
+    def check():
+        torch.cuda.synchronize()
+        assert pkg.lib().b200sp_experts_error() == 0
+        want, size = ref.experts_mm(R.row_ptr, R.col_ind, x, w.view(experts, n, d), experts, True, False, 1.0, 0.0, y)
+        ref.close(y, want, ref.rounding(y.dtype, want) + size * (d + 4) * 2 * F32)
+
+    return R, logits, operands, buffer, y, check
+
+
+def test_routing_anew_ends_the_order(pkg, handle):
+    from ops_sparse_b200 import api
+    g = gen(21)
+    R, logits, operands, buffer, _, check = small(pkg, api, handle, g)
+    rule = api.RouteRule()
+    api.route(handle, rule, mat(api, logits), None, R)
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, *operands, buffer=buffer)
+    check()
+    logits.neg_()
+    api.route(handle, rule, mat(api, logits), None, R)
+    with pytest.raises(pkg.AclSparseError, match="INVALID_VALUE"):
+        api.experts_mm(handle, R, *operands, buffer=buffer)
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_mm(handle, R, *operands, buffer=buffer)
+    check()
