@@ -102,7 +102,8 @@ typedef enum b200spExpertRows_t {
 aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, void *buffer);
 
 /* Operands of the products whose rows do not start on 16 bytes are copied into the buffer first, in every call: the BufferSize calls count
- * the room for the operands they are given.
+ * the room for the operands they are given.  A product that copies is refused (ACL_SPARSE_STATUS_INVALID_VALUE) unless so much has been
+ * asked for through R's own descriptor; that a buffer has the size that was asked for is the caller's to see to, for every buffer.
  *
  * Y[i] = alpha * X[row of entry i] * op(W of its expert) + beta * Y[i], a row of Y for every entry of R.
  * opW = T: X has d columns, Y n (a layer whose weights lie as n x d); opW = N: X has n columns, Y d (the

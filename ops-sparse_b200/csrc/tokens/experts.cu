@@ -212,10 +212,12 @@ size_t NoteSize(const aclsparseSpMatDescr *R, size_t bytes)
     R->expertsSized = std::max(R->expertsSized, (int64_t)bytes);
     return bytes;
 }
-bool Sized(const aclsparseSpMatDescr *R, size_t bytes)
+// Whether the buffer may be taken to have room for copies of the operands, if any: what Preprocess writes it has.
+bool HasRoom(const aclsparseSpMatDescr *R, const aclsparseDnMatDescr *first, const aclsparseDnMatDescr *second)
 {
+    if (AlignedBytes(first) + AlignedBytes(second) == 0) return true;
     std::lock_guard<std::mutex> lock(R->expertsMutex);
-    return (int64_t)bytes <= R->expertsSized;
+    return (int64_t)BufferBytes(R, first, second) <= R->expertsSized;
 }
 
 // An operand as the kernels read it: where it lies, or its copy at `room`, which moves on.
@@ -331,7 +333,7 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     const aclsparseStatus_t st = CheckMM(opW, rowsOfX, matR, matX, matW, matY);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer) || !Sized(matR, BufferBytes(matR, matX, matW))) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer) || !HasRoom(matR, matX, matW)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
     MmaArgs a = ArgsOf(matR, rowsOfX, buffer, matW, matY, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
@@ -378,7 +380,7 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     const aclsparseStatus_t st = CheckGrad(rowsOfX, matR, dY, matX, dW);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer) || !Sized(matR, BufferBytes(matR, matX, dY))) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer) || !HasRoom(matR, matX, dY)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
     MmaArgs a = ArgsOf(matR, rowsOfX, buffer, dW, dW, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;

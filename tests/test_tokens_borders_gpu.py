@@ -300,3 +300,22 @@ def test_routing_anew_ends_the_order(pkg, handle):
     api.experts_preprocess(handle, R, buffer)
     api.experts_mm(handle, R, *operands, buffer=buffer)
     check()
+
+
+def test_a_matrix_made_anew_takes_a_buffer_of_the_known_size(pkg, handle):
+    """Room has to have been asked for through the same descriptor for operands that are copied alone."""
+    from ops_sparse_b200 import api
+    g = gen(22)
+    R, logits, operands, buffer, _, check = small(pkg, api, handle, g)
+    api.route(handle, api.RouteRule(), mat(api, logits), None, R)
+    again = api.CsrMatrix(R.row_ptr, R.col_ind, R.values, R.rows, R.cols)
+    api.experts_preprocess(handle, again, buffer)
+    api.experts_mm(handle, again, *operands, buffer=buffer)
+    check()
+    dw = torch.empty(6 * 24, 32, device="cuda")
+    api.experts_grad(handle, again, operands[2], operands[0], mat(api, dw), buffer=buffer)
+    want, size, many = ref.experts_grad(R.row_ptr, R.col_ind, operands[2].values, operands[0].values, 6, False, 1.0, 0.0, dw.view(6, 24, 32))
+    ref.close(dw.view(6, 24, 32), want, ref.rounding(dw.dtype, want) + size * (many + 4) * 2 * F32)
+    odd = mat(api, matrix(g, 40, 32, "bf16", shift=1)[0])
+    with pytest.raises(pkg.AclSparseError, match="INVALID_VALUE"):
+        api.experts_mm(handle, again, odd, *operands[1:], buffer=buffer)
