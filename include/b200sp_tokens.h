@@ -129,9 +129,9 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
                                     void *buffer);
 
 /* What went wrong in an experts' product since the flag was cleared.  1: a bounded wait ran out (never observed outside the test that
- * provokes it), rows of the output are unwritten; 2: its buffer held no order, because the b200spExpertsPreprocess that belongs to it
- * was captured and not replayed yet, and the output is untouched.  Both calls are for the current device, which has to be that of the
- * product's handle, and synchronise it (not during a capture); b200sp_experts_error is -1 if that fails. */
+ * provokes it), rows of the output are unwritten; 2: its buffer held no order, or one of earlier columns, because the b200spExpertsPreprocess
+ * that belongs to it was captured and not replayed yet, and the output is untouched.  Both calls are for the current device, which has to be
+ * that of the product's handle, and synchronise it (not during a capture); b200sp_experts_error is -1 if that fails. */
 int b200sp_experts_error(void);
 int b200sp_experts_error_clear(void);
 /* For tests of that path: later products wait at most wait_cycles SM clocks (0 = the default, about two seconds) and expect

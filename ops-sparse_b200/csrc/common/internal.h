@@ -89,6 +89,9 @@ struct ExpertsPlan {
     const void *offsets = nullptr, *indices = nullptr;
     int64_t rows = 0, cols = 0, nnz = 0;
     uint64_t generation = 0;
+    uint64_t number = 0;    // what the buffer begins with
+    bool captured = false;  // it is there from the graph's first replay on
+    bool stale = false;     // the columns are others
 };
 
 // Every library call that writes an analysis or scratch data into a caller buffer stamps that buffer with a new

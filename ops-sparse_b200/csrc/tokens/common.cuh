@@ -170,6 +170,15 @@ template <auto kKernel> cudaError_t AllowShared(int bytes)
     return e;
 }
 
+// Whether calls on the stream are recorded and not run.
+inline bool Captures(cudaStream_t stream)
+{
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream, &capture) == cudaSuccess) return capture != cudaStreamCaptureStatusNone;
+    (void)cudaGetLastError();
+    return false;
+}
+
 inline aclsparseStatus_t Finished(cudaError_t e, const char *call)
 {
     if (e == cudaSuccess) return ACL_SPARSE_STATUS_SUCCESS;

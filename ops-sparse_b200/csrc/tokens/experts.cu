@@ -35,8 +35,10 @@ PlanLayout PlanLayoutFor(long long nnz, long long experts)
     return L;
 }
 
-// A product follows the order only if the buffer starts with this: the sizes that its entries and rows are below.  A Preprocess that was
-// captured and has not been replayed yet has written nothing.
+// A product follows the order only if the buffer starts with this: the sizes that its entries and rows are below, then a number of the order.
+// A Preprocess that was captured and has not been replayed yet has written nothing: an eager product after it wants its number.  (Others do
+// not: a graph's products follow the order that is there when they are replayed, whoever made it last.)  All that order the entries of one R
+// in one buffer write the same number, so that any of them may have been the last to run, until an eager b200spRoute gives R other columns.
 constexpr int kOrderMark = 0x45585031;
 inline int4 HeaderOf(long long nnz, long long experts, long long rows) { return make_int4(kOrderMark, (int)nnz, (int)experts, (int)rows); }
 
@@ -44,11 +46,14 @@ inline int4 HeaderOf(long long nnz, long long experts, long long rows) { return 
 
 __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const SortArgs s, const int *__restrict__ rowPtr, int rows,
                                                                      int *__restrict__ rowOf, int *__restrict__ offsets, int4 *header,
-                                                                     const int4 mark)
+                                                                     const int4 mark, const uint64_t number)
 {
     extern __shared__ unsigned char sSort[];
     b200sp::WaitForPrevious();
-    if (blockIdx.x == 0 && threadIdx.x == 0) *header = mark;
+    if (blockIdx.x == 0 && threadIdx.x == 0) {
+        header[0] = mark;
+        *reinterpret_cast<uint64_t *>(header + 1) = number;
+    }
     ClusterSort<int>(s, sSort, [&](int, int entry, int to) {
         // rows are of about the same length: the first guess is nearly always right
         int r = (int)((long long)entry * rows / s.count);
@@ -165,16 +170,22 @@ aclsparseStatus_t CheckGrad(b200spExpertRows_t rowsOfX, const aclsparseSpMatDesc
 
 char *BufferStart(const void *buffer) { return reinterpret_cast<char *>(AlignUp(reinterpret_cast<uintptr_t>(buffer), 256)); }
 
-// Whether the buffer still holds the order of R's entries.
-bool HoldsOrder(const aclsparseSpMatDescr *R, const void *buffer)
+// Whether the buffer is the one that R's entries were ordered in last, and no other call has written it since.
+bool SameBuffer(const aclsparseSpMatDescr *R, const void *buffer)
 {
-    std::lock_guard<std::mutex> lock(R->expertsMutex);
     const b200sp::ExpertsPlan &p = R->experts;
     return buffer != nullptr && p.buffer == buffer && p.offsets == R->offsets && p.indices == R->indices && p.rows == R->rows &&
            p.cols == R->cols && p.nnz == R->nnz && p.generation != 0 && p.generation == b200sp::BufferGeneration(buffer);
 }
+// Whether the buffer still holds the order of R's entries; the number that it has to have, 0: any.
+bool HoldsOrder(const aclsparseSpMatDescr *R, const void *buffer, cudaStream_t stream, uint64_t *number)
+{
+    std::lock_guard<std::mutex> lock(R->expertsMutex);
+    *number = R->experts.captured && !Captures(stream) ? R->experts.number : 0;
+    return SameBuffer(R, buffer) && !R->experts.stale;
+}
 
-MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const void *buffer, const aclsparseDnMatDescr *stacked,
+MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const void *buffer, uint64_t number, const aclsparseDnMatDescr *stacked,
                const aclsparseDnMatDescr *out, const Scalars &sc)
 {
     const PlanLayout L = PlanLayoutFor(R->nnz, R->cols);
@@ -182,6 +193,7 @@ MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const v
     MmaArgs a{};
     a.header = reinterpret_cast<const int4 *>(p);
     a.mark = HeaderOf(R->nnz, R->cols, R->rows);
+    a.number = number;
     a.offsets = reinterpret_cast<const int *>(p + L.offsets);
     a.entries = reinterpret_cast<const int *>(p + L.entries);
     a.rows = reinterpret_cast<const int *>(p + L.rows);
@@ -272,7 +284,9 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
     const OnDevice device(handle);
-    const uint64_t generation = NoteWrite(buffer);
+    std::lock_guard<std::mutex> lock(matR->expertsMutex);
+    const uint64_t before = SameBuffer(matR, buffer) ? matR->experts.number : 0;
+    const uint64_t generation = NoteWrite(buffer), number = before != 0 ? before : generation;  // generations are given once
     if (generation == 0) return ACL_SPARSE_STATUS_ALLOC_FAILED;
     const PlanLayout L = PlanLayoutFor(matR->nnz, matR->cols);
     char *const p = BufferStart(buffer);
@@ -305,11 +319,11 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
         b200sp_note_launches(1);
         e = cudaLaunchKernelEx(&cfg, ExpertsOrderKernel, s, static_cast<const int *>(matR->offsets), (int)matR->rows,
                                reinterpret_cast<int *>(p + L.rows), offsets, reinterpret_cast<int4 *>(p),
-                               HeaderOf(matR->nnz, matR->cols, matR->rows));
+                               HeaderOf(matR->nnz, matR->cols, matR->rows), number);
     }
-    std::lock_guard<std::mutex> lock(matR->expertsMutex);
     matR->experts = {};
-    if (e == cudaSuccess) matR->experts = {buffer, matR->offsets, matR->indices, matR->rows, matR->cols, matR->nnz, generation};
+    if (e == cudaSuccess)
+        matR->experts = {buffer, matR->offsets, matR->indices, matR->rows, matR->cols, matR->nnz, generation, number, Captures(handle->stream), false};
     return Finished(e, "b200spExpertsPreprocess");
 }
 
@@ -333,9 +347,10 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     const aclsparseStatus_t st = CheckMM(opW, rowsOfX, matR, matX, matW, matY);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer) || !HasRoom(matR, matX, matW)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoom(matR, matX, matW)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
-    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, matW, matY, ScalarsOf(handle, alpha, beta));
+    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, number, matW, matY, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
     const Operand x = Aligned(matX, &room, handle->stream), w = Aligned(matW, &room, handle->stream, a.offsets, a.n);
     if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, "b200spExpertsMM");
@@ -380,9 +395,10 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     const aclsparseStatus_t st = CheckGrad(rowsOfX, matR, dY, matX, dW);
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
-    if (!HoldsOrder(matR, buffer) || !HasRoom(matR, matX, dY)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoom(matR, matX, dY)) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
-    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, dW, dW, ScalarsOf(handle, alpha, beta));
+    MmaArgs a = ArgsOf(matR, rowsOfX, buffer, number, dW, dW, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
     const Operand x = Aligned(matX, &room, handle->stream), y = Aligned(dY, &room, handle->stream);
     if (x.error != cudaSuccess || y.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : y.error, "b200spExpertsGrad");

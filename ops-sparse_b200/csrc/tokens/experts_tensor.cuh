@@ -40,8 +40,9 @@ constexpr long long kMmaStepCycles = 4096;
 enum class Mode { kProductT, kProductN, kGrad };
 
 struct MmaArgs {
-    const int4 *header;    // has to be `mark`, or nothing of the rest is looked at
+    const int4 *header;    // has to be `mark`, and `number` unless that is 0, or nothing of the rest is looked at
     int4 mark;
+    uint64_t number;
     const int *offsets, *entries, *rows;
     void *out;
     long long ldo;
@@ -272,7 +273,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                                     ((kMode == Mode::kProductN ? a.d : a.n) + Tiles<kMode, kPair>::kHigh - 1) / Tiles<kMode, kPair>::kHigh};
     const int groups = tiles.Groups();
     const int4 found = __ldg(a.header);
-    const bool ordered = found.x == a.mark.x && found.y == a.mark.y && found.z == a.mark.z && found.w == a.mark.w;
+    const bool ordered = found.x == a.mark.x && found.y == a.mark.y && found.z == a.mark.z && found.w == a.mark.w &&
+                         (a.number == 0 || __ldg(reinterpret_cast<const unsigned long long *>(a.header + 1)) == a.number);
     for (int e = tid; e <= groups; e += kMmaThreads) sOffset[e] = ordered ? __ldg(a.offsets + e) : 0;
     __syncthreads();
     if (warp == 0) {

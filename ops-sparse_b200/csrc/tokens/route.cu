@@ -521,9 +521,10 @@ aclsparseStatus_t b200spRoute(aclsparseHandle_t handle, const b200spRouteRule *r
                 rule->groupScore == B200SP_GROUP_TOP2, rule->renormalise, rule->scale, 0, 0, 0, static_cast<int *>(matR->offsets),
                 static_cast<int *>(matR->indices), matR->values};
     {
-        // R's columns are written: no buffer holds their order any more
+        // R's columns are written: no buffer holds their order any more.  (A captured call has not written them yet.)
         std::lock_guard<std::mutex> lock(matR->expertsMutex);
-        matR->experts = {};
+        if (Captures(handle->stream)) matR->experts.stale = true;
+        else matR->experts = {};
     }
     if (a.kept == a.groups) a.groups = a.kept = 1;  // all are kept
     a.groupSize = a.experts / a.groups;

@@ -319,3 +319,87 @@ def test_a_matrix_made_anew_takes_a_buffer_of_the_known_size(pkg, handle):
     odd = mat(api, matrix(g, 40, 32, "bf16", shift=1)[0])
     with pytest.raises(pkg.AclSparseError, match="INVALID_VALUE"):
         api.experts_mm(handle, again, odd, *operands[1:], buffer=buffer)
+
+
+def test_a_captured_order_is_not_the_one_before_it(pkg, device):
+    """A buffer that holds an order, an order of other columns captured but not replayed: an eager product does not follow the old one."""
+    from ops_sparse_b200 import api
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        h = api.Handle(stream)
+        R, logits, operands, buffer, y, check = small(pkg, api, h, gen(23))
+        rule, L = api.RouteRule(), mat(api, logits)
+        api.route(h, rule, L, None, R)
+        api.experts_preprocess(h, R, buffer)
+        api.experts_mm(h, R, *operands, buffer=buffer)
+        check()
+        logits.neg_()
+        api.route(h, rule, L, None, R)
+        stream.synchronize()
+        graph, both = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            api.experts_preprocess(h, R, buffer)
+        y.fill_(5.0)
+        api.experts_mm(h, R, *operands, buffer=buffer)
+        stream.synchronize()
+        error = pkg.lib().b200sp_experts_error()
+        pkg.lib().b200sp_experts_error_clear()
+        assert error == 2 and (y == 5).all()
+        graph.replay()
+        api.experts_mm(h, R, *operands, buffer=buffer)
+        check()
+        # products in graphs follow what the buffer holds when they are replayed: of the same graph, or of eager calls
+        with torch.cuda.graph(both, stream=stream):
+            api.route(h, rule, L, None, R)
+            api.experts_preprocess(h, R, buffer)
+            api.experts_mm(h, R, *operands, buffer=buffer)
+        alone = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(alone, stream=stream):
+            api.experts_mm(h, R, *operands, buffer=buffer)
+        for _ in range(2):
+            logits.mul_(-1.5)
+            both.replay()
+            check()
+            api.experts_mm(h, R, *operands, buffer=buffer)
+            check()
+        logits.neg_()
+        api.route(h, rule, L, None, R)
+        api.experts_preprocess(h, R, buffer)
+        alone.replay()
+        check()
+        graph.replay()
+        api.experts_mm(h, R, *operands, buffer=buffer)  # an eager order before, whatever graph wrote the same since
+        check()
+        del graph, both, alone
+    h.close()
+
+
+def test_graphs_that_order_the_same_entries_in_turn(pkg, device):
+    """Two graphs that route, order and multiply; eager products after either of them, the first captured replayed last."""
+    from ops_sparse_b200 import api
+    stream = torch.cuda.Stream()
+    with torch.cuda.stream(stream):
+        h = api.Handle(stream)
+        R, logits, operands, buffer, y, check = small(pkg, api, h, gen(24))
+        rule, L = api.RouteRule(score="sigmoid"), mat(api, logits)
+        api.route(h, rule, L, None, R)
+        api.experts_preprocess(h, R, buffer)
+        api.experts_mm(h, R, *operands, buffer=buffer)
+        check()
+        graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+        for graph in graphs:
+            with torch.cuda.graph(graph, stream=stream):
+                api.route(h, rule, L, None, R)
+                with pytest.raises(pkg.AclSparseError, match="INVALID_VALUE"):
+                    api.experts_mm(h, R, *operands, buffer=buffer)
+                api.experts_preprocess(h, R, buffer)
+                api.experts_mm(h, R, *operands, buffer=buffer)
+        for graph in (graphs[1], graphs[0], graphs[1], graphs[0]):
+            logits.mul_(-1.25)
+            graph.replay()
+            check()
+            y.fill_(5.0)
+            api.experts_mm(h, R, *operands, buffer=buffer)
+            check()
+        del graphs
+    h.close()
