@@ -395,6 +395,8 @@ def embedding_grad(handle: Handle, grad: DnMat, tokens: DnVec, d_table: DnMat, a
 
 def route(handle: Handle, rule: RouteRule, logits: DnMat, bias: DnVec | None, R: CsrMatrix) -> None:
     """Writes R (tokens x experts, the same number of entries in every row): offsets, ascending columns and values."""
+    if bias is not None and not bias._d:
+        raise ValueError("route: the bias has been closed")  # its NULL would say that there is none
     status = lib().b200spRoute(handle._h, rule.address, logits._d, None if bias is None else bias._d, R._d)
     if status:
         check(status, "b200spRoute")
