@@ -86,6 +86,24 @@ __device__ __forceinline__ unsigned long long MaxKey(unsigned long long v)
     return (unsigned long long)high << 32 | low;
 }
 
+// The largest of the warp's, no NaN among them.
+__device__ __forceinline__ float LargestOf(float v) { return ValueOf(__reduce_max_sync(kAll, KeyOf(v))); }
+
+__device__ __forceinline__ float Sigmoid(float x)
+{
+    const float e = expf(-fabsf(x));
+    return (x >= 0.0f ? 1.0f : e) / (1.0f + e);
+}
+
+// Scores that are divided by their sum may share any factor.  Where the sum is small (by sigmoids, or by exponentials of the difference to
+// the row's largest logit) they are taken relative to the largest logit among them: scores below the least f32 still have quotients.
+// Above, what is lost is below the least f32 of the quotients, too.
+constexpr float kSmall = 0.25f;
+__device__ __forceinline__ float FarScore(float x, bool sigmoid, float largest)  // a sigmoid below kSmall: x is negative
+{
+    return (x == largest ? 1.0f : expf(x - largest)) / (sigmoid ? 1.0f + expf(x) : 1.0f);
+}
+
 // Scores of the lanes' logits (masked: -infinity), 0 for the masked.  In f32 a sigmoid is taken from the fast exponential and division: it
 // serves the choice alone.  *error: how far they may be from exact ones.
 //   sigmoid: __expf is off by 2 + 1.17 |x| units of 2^-23 relative to e^-x, of which p (1 - p) times reaches p: with p (1 - p) <= 1/4 and
@@ -332,19 +350,19 @@ template <typename In, typename Out, int kPer> __global__ void __launch_bounds__
         }
     }
     if (__any_sync(kAll, unsure)) c = ChooseExactly<kPer>(a, sLogits, sRows[warp], lane);
-    // The weights, of the experts taken alone; their places by column.  Those that are renormalised may share a factor, e^-x of the largest
-    // logit taken (a sigmoid, e^x / (1 + e^x), where that x is negative): scores below the least f32 still have their quotients.
-    float w = 0.0f;
+    // the weights, of the experts taken alone; their places by column
     const bool weighs = c.expert >= 0 && !c.weightless;
     const float own = weighs ? sLogits[c.expert] : -INFINITY;
-    const float largest = a.renormalise ? ValueOf(__reduce_max_sync(kAll, KeyOf(own))) : a.sigmoid ? 0.0f : most;
-    if (weighs) {
-        if (a.sigmoid) w = expf(fminf(own, 0.0f) - fminf(largest, 0.0f)) / (1.0f + expf(-fabsf(own)));
-        else w = own == largest ? 1.0f : expf(own - largest);
-    }
+    float w = 0.0f;
+    if (weighs) w = a.sigmoid ? Sigmoid(own) : own == most ? 1.0f : expf(own - most);
     float by = a.scale;
     if (a.renormalise) {
-        const float sum = WarpSum(w);
+        float sum = WarpSum(w);
+        if (sum < kSmall) {
+            const float largest = LargestOf(own);
+            if (weighs) w = FarScore(own, a.sigmoid, largest);
+            sum = WarpSum(w);
+        }
         by = sum > 0 ? a.scale / sum : 0.0f;
     } else if (!a.sigmoid) {
         w *= inverse;
@@ -433,13 +451,16 @@ template <typename T, int kPer> __global__ void __launch_bounds__(32 * kRouteWar
 #pragma unroll
         for (int j = 0; j < kPer; ++j) sRow[32 * j + lane] = 0.0f;
         if (a.sigmoid) {
-            // the scores as the weights are taken from them: without the factor e^(largest) where that is small
-            const float largest = a.renormalise ? WarpMax(x) : 0.0f;
-            const float s = col < 0 ? 0.0f : expf(fminf(x, 0.0f) - fminf(largest, 0.0f)) / (1.0f + expf(-fabsf(x)));
+            float s = col < 0 ? 0.0f : Sigmoid(x);
             const float rest = col < 0 ? 0.0f : 1.0f / (1.0f + expf(x));  // 1 - the score, exactly enough where that is near 1
             if (a.renormalise) {
-                const float sum = WarpSum(s), q = sum > 0 ? s / sum : 0.0f;
-                dx = q * (g - WarpSum(g * q)) * rest;
+                float sum = WarpSum(s), dot = WarpSum(g * s);
+                if (sum < kSmall) {
+                    const float largest = LargestOf(x);
+                    if (col >= 0) s = FarScore(x, true, largest);
+                    sum = WarpSum(s), dot = WarpSum(g * s);
+                }
+                dx = sum > 0 ? (g - dot / sum) / sum * s * rest : 0.0f;
             } else {
                 dx = g * s * rest;
             }
