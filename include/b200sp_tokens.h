@@ -14,7 +14,7 @@
  * gradient has to show that it overflowed).  Calls enqueue on the handle's stream, wait for nothing, allocate nothing,
  * and may be captured.  A handle is used on the device that it was created on, whatever device is current.
  * (A call on no tokens can not be described: aclsparseCreateDnMat refuses a matrix of no rows.)
- * An output overlaps no input, unless it says so.  At most 2^31 - 2^20 tokens or entries of R.
+ * An output overlaps no input, unless it says so.  At most 2^31 - 2^20 tokens, columns or entries of R, and tables of 2^31 - 2 rows.
  * Column-major operands, index bases of one and 64-bit CSR indices are ACL_SPARSE_STATUS_NOT_SUPPORTED.
  */
 #ifndef B200SP_TOKENS_H_
@@ -70,8 +70,8 @@ typedef struct b200spRouteRule {
  *
  * An expert's selection value is p + bias with a bias, where p is its score, and without one the logit itself: both
  * scores ascend with it.  The groupsKept groups of the highest group score are kept, then the k experts of the
- * highest selection value taken; what is equal goes to the lower index.  The order is that of exact arithmetic: values
- * that f32 cannot tell apart are compared in f64.  An expert with a logit or bias of -infinity or NaN is masked: no score,
+ * highest selection value taken; what is equal goes to the lower index.  The order is that of f64 arithmetic: values
+ * that f32 might not tell apart are compared in f64.  An expert with a logit or bias of -infinity or NaN is masked: no score,
  * and taken only where fewer than k others are left in the kept groups, the lowest index first; experts of groups that are
  * not kept are treated alike.  Such entries have weight 0.  The other weights are p, over their sum if renormalise,
  * times scale; the bias is in none of them.
@@ -134,8 +134,8 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
  * that of the product's handle, and synchronise it (not during a capture); b200sp_experts_error is -1 if that fails. */
 int b200sp_experts_error(void);
 int b200sp_experts_error_clear(void);
-/* For tests of that path: later products wait at most wait_cycles SM clocks (0 = the default, about two seconds) and expect
- * extra_tx bytes more than they copy on every barrier, so that with extra_tx > 0 every wait runs out. */
+/* For tests of that path: later products wait at most wait_cycles SM clocks (0 = the default, about two seconds; for a tile's results 4096 more
+ * for each of its steps of 64 terms) and expect extra_tx bytes more than they copy on every barrier, so that with extra_tx > 0 every wait runs out. */
 void b200sp_experts_wait_test(long long wait_cycles, unsigned extra_tx);
 
 #ifdef __cplusplus

@@ -84,7 +84,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
 // ---------------------------------------------------------------- operands that do not start on 16 bytes
 
 // Rows of 16-bit elements into rows of a multiple of eight, zeros behind the last: what the copies of the products need.  A thread writes 16
-// bytes; what bounds it are the bytes, read and written once each (and read again by the product).
+// bytes, read two at a time, which is what bounds it: 2048 tokens, four of 64 experts, 1001 x 777 take 127 us, 1008 x 784 without copies 35.
 // offsets: with rowsEach > 0 the rows are those of experts, as many each, and one without entries is left out.
 __global__ void __launch_bounds__(256) ExpertsAlignKernel(const uint16_t *__restrict__ from, long long rows, int cols, long long ld,
                                                           uint4 *__restrict__ to, const int *__restrict__ offsets, int rowsEach)

@@ -6,7 +6,8 @@
 // count the digits of the share in shared memory; read the other CTAs' counts through the cluster, which gives every digit's
 // first place; then rank tile by tile (by warp, step and lane, which is the order in memory) and store.  Passes meet at
 // cluster barriers.  Nothing is atomic across CTAs, so the result is unique and the same in every run.
-// One B200: 128 entries by 64 experts 5.5 us, 32,768 by 32 some 13 (one pass); 16,384 tokens of a table of 65,536 rows (two passes) less than 20,
+// One B200: 128 entries by 64 experts 5 us, 32,768 some 13, 131,072 40 and 1,048,576 285 (one pass; from 32,768 on time grows with the count, since
+// the cluster is as large as it gets); 16,384 tokens of a table of 65,536 rows (two passes) less than 20,
 // with 64 MB of zeros written beside them.  What bounds it is latency: loads, barriers and the cluster's reads one after the other.
 #pragma once
 
