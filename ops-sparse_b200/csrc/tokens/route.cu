@@ -9,6 +9,7 @@
 // f64.
 // What bounds it are instructions, some 1230 a token: 16,384 tokens, 8 of 256 experts in groups, with a bias 26 us (17.9 MB; 74 % of the issue
 // slots), without groups 20, without either 16; the largest of all lanes' experts looked for in every round 52.
+#include <cfloat>
 #include <cmath>
 
 #include "b200sp_tokens.h"
@@ -38,9 +39,11 @@ struct RouteArgs {
 template <typename Real> struct Limits;
 template <> struct Limits<float> {
     static __device__ __forceinline__ float Lowest() { return -INFINITY; }
+    static __device__ __forceinline__ float Least() { return -FLT_MAX; }
 };
 template <> struct Limits<double> {
     static __device__ __forceinline__ double Lowest() { return -(double)INFINITY; }
+    static __device__ __forceinline__ double Least() { return -DBL_MAX; }
 };
 
 __device__ __forceinline__ float Exp(float v) { return expf(v); }
@@ -190,7 +193,8 @@ __device__ __forceinline__ bool Values(const RouteArgs &a, const float (&x)[kPer
         first = Larger(first, f);
     }
     __syncwarp();  // the values may be written again
-    const Real value = sums && second > nothing ? first + second : first;
+    // two of the lowest f32 are no masked group
+    const Real value = sums && second > nothing ? Larger(first + second, Limits<Real>::Least()) : first;
     // lane g < groups: group g
     const Real own = __shfl_sync(kAll, value, (lane * wide) & 31), mine = lane < a.groups ? own : nothing;
     int place = 0;

@@ -51,6 +51,24 @@ def test_route_group_sums_of_large_opposite_biases(pkg, handle, score, size, tok
     check_route(api, handle, x, bias, 32, score=score, groups=32, kept=16, group_score="top2")
 
 
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_groups_of_the_lowest_biases(pkg, handle, score):
+    """A bias of f32's lowest value masks nothing: a group whose two best have it is behind others, and before groups of masked experts."""
+    from ops_sparse_b200 import api
+    g = gen(37)
+    lowest = torch.finfo(torch.float32).min
+    x = torch.randn(400, 32, generator=g, device="cuda")
+    x[:200, :8] = -math.inf  # the first groups are masked
+    x[200:300, torch.randint(0, 32, (16,), generator=g, device="cuda")] = -math.inf
+    bias = torch.where(torch.rand(32, generator=g, device="cuda") < 0.25, 0.5, lowest)
+    check_route(api, handle, x, torch.full((32,), lowest, device="cuda"), 6, score=score, groups=8, kept=4, group_score="top2")
+    check_route(api, handle, x, bias, 6, score=score, groups=8, kept=5, group_score="top2")
+    check_route(api, handle, x, bias, 6, score=score, groups=8, kept=5, group_score="max")
+    x[:200, 2:8] = 0.25 * torch.randint(0, 3, (200, 6), generator=g, device="cuda")
+    # groups of two, the first masked; all experts of the kept ones are taken, so that no other comparison asks for f64
+    check_route(api, handle, x[:200, :8], torch.full((8,), lowest, device="cuda"), 4, score=score, groups=4, kept=2, group_score="top2")
+
+
 # ---------------------------------------------------------------- weights that underflow
 
 FAR = [[-100.0, -101.0, -math.inf, -103.5], [-88.0, -89.0, -95.0, -400.0], [-90.0, -90.0, -90.0, -90.0], [3.0, -60.0, -95.0, -100.0],
