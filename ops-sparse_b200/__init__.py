@@ -36,6 +36,8 @@ ACL_SPARSE_POINTER_MODE_HOST, ACL_SPARSE_POINTER_MODE_DEVICE = 0, 1
 B200SP_ROUTE_SOFTMAX, B200SP_ROUTE_SIGMOID = 0, 1
 B200SP_GROUP_MAX, B200SP_GROUP_TOP2 = 0, 1
 B200SP_ROWS_OF_TOKENS, B200SP_ROWS_OF_ENTRIES = 0, 1
+# include/b200sp_rows.h
+B200SP_WEIGHTS_NONE, B200SP_WEIGHTS_OF_R = 0, 1
 
 STATUS_NAMES = [
     "SUCCESS", "NOT_INITIALIZED", "ALLOC_FAILED", "INVALID_VALUE", "ARCH_MISMATCH", "EXECUTION_FAILED",
@@ -162,6 +164,17 @@ _SIGNATURES = {
     "b200spExpertsMM": [P, c_int, c_int, P, P, P, P, P, P, P],
     "b200spExpertsGradBufferSize": [P, c_int, P, P, P, P, POINTER(c_size_t)],
     "b200spExpertsGrad": [P, c_int, P, P, P, P, P, P, P],
+    # rows in the order of the experts and in 8 bits (include/b200sp_rows.h)
+    "b200spExpertsOrderBufferSize": [P, P, POINTER(c_size_t)],
+    "b200spExpertsDispatch": [P, P, P, P, P, P, P, P],
+    "b200spExpertsCombine": [P, c_int, P, P, P, P, P, P],
+    "b200spExpertsCombineGrad": [P, P, P, P, P, P, P, P, P],
+    "b200spQuantiseRows": [P, P, P, P],
+    "b200spExpertsQuantise": [P, P, P, P, P, P, P],
+    "b200spScaledMMBufferSize": [P, P, P, P, POINTER(c_size_t)],
+    "b200spScaledMM": [P, P, P, P, P, P, P, P, P],
+    "b200spExpertsScaledMMBufferSize": [P, P, P, P, P, POINTER(c_size_t)],
+    "b200spExpertsScaledMM": [P, P, P, P, P, P, P, P, P, P],
     # multi-GPU helpers (include/b200sp_mg.h)
     "b200spMgPartitionRows": [P, c_int64, c_int32, POINTER(c_int64)],
 }
@@ -196,11 +209,14 @@ def __getattr__(name: str):
 
 
 from .api import (  # noqa: E402  (needs the names above)
-    CsrMatrix, DnMat, DnVec, Handle, RouteRule, acl_type_of, embedding, embedding_grad, experts_grad, experts_mm,
-    experts_preprocess, route, route_grad, spmm, spmv,
+    CsrMatrix, DnMat, DnVec, Handle, RouteRule, acl_type_of, embedding, embedding_grad, experts_combine,
+    experts_combine_grad, experts_dispatch, experts_grad, experts_mm, experts_preprocess, experts_quantise,
+    experts_scaled_mm, quantise_rows, route, route_grad, scaled_mm, spmm, spmv,
 )
 
 __all__ = [
     "lib", "check", "AclSparseError", "Handle", "CsrMatrix", "DnVec", "DnMat", "spmv", "spmm", "acl_type_of",
     "RouteRule", "embedding", "embedding_grad", "route", "route_grad", "experts_preprocess", "experts_mm", "experts_grad",
+    "experts_dispatch", "experts_combine", "experts_combine_grad", "quantise_rows", "experts_quantise", "scaled_mm",
+    "experts_scaled_mm",
 ]

@@ -17,7 +17,8 @@ from . import (
     ACL_SPARSE_INDEX_BASE_ZERO, ACL_SPARSE_SPMVOP_ALG_DEFAULT, ACL_SPARSE_SPMVOP_ALG2,
     ACL_SPARSE_OP_NON_TRANSPOSE, ACL_SPARSE_ORDER_COL, ACL_SPARSE_ORDER_ROW, ACL_SPARSE_POINTER_MODE_DEVICE,
     ACL_SPARSE_OP_TRANSPOSE, ACL_SPARSE_SPMM_ALG_DEFAULT, ACL_SPARSE_SPMV_ALG_DEFAULT, B200SP_GROUP_MAX, B200SP_GROUP_TOP2,
-    B200SP_ROUTE_SIGMOID, B200SP_ROUTE_SOFTMAX, B200SP_ROWS_OF_ENTRIES, B200SP_ROWS_OF_TOKENS, check, lib,
+    B200SP_ROUTE_SIGMOID, B200SP_ROUTE_SOFTMAX, B200SP_ROWS_OF_ENTRIES, B200SP_ROWS_OF_TOKENS, B200SP_WEIGHTS_NONE,
+    B200SP_WEIGHTS_OF_R, check, lib,
 )
 
 _ACL_OF = {
@@ -452,3 +453,105 @@ def experts_grad(handle: Handle, R: CsrMatrix, dY: DnMat, X: DnMat, dW: DnMat, a
                                      None if buffer is None else buffer.data_ptr())
     if status:
         check(status, "b200spExpertsGrad")
+
+
+# ---- rows in the order of the experts and in 8 bits (include/b200sp_rows.h) ----
+
+def _optional(what, name: str):
+    """The descriptor of an argument that may be None.  (A closed one is refused: its NULL would say that there is none.)"""
+    if what is None:
+        return None
+    if not what._d:
+        raise ValueError(f"{name} has been closed")
+    return what._d
+
+
+def _address(buffer: torch.Tensor | None):
+    return None if buffer is None else buffer.data_ptr()
+
+
+def experts_order_buffer_size(handle: Handle, R: CsrMatrix) -> int:
+    """For experts_preprocess and the calls below but experts_scaled_mm."""
+    size = c_size_t()
+    check(lib().b200spExpertsOrderBufferSize(handle.raw, R.raw, byref(size)), "b200spExpertsOrderBufferSize")
+    return size.value
+
+
+def experts_dispatch(handle: Handle, R: CsrMatrix, X: DnMat, S: DnMat, alpha=1.0, beta=0.0, offsets: DnVec | None = None,
+                     buffer: torch.Tensor | None = None) -> None:
+    """S[place of entry i] = alpha * X[token of entry i] + beta * S[place]: the tokens' rows in the order of the experts.
+    offsets: takes the first row of every expert and the end of the last one's, int32."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsDispatch(handle._h, a, R._d, X._d, b, S._d, _optional(offsets, "experts_dispatch: offsets"),
+                                         _address(buffer))
+    if status:
+        check(status, "b200spExpertsDispatch")
+
+
+def experts_combine(handle: Handle, R: CsrMatrix, S: DnMat, out: DnMat, alpha=1.0, beta=0.0, weighted: bool = True,
+                    buffer: torch.Tensor | None = None) -> None:
+    """out[t] = alpha * sum over the entries i of token t of (R's value i if weighted, else 1) * S[place of i] + beta * out[t].
+    Without weights it is the gradient of experts_dispatch."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsCombine(handle._h, B200SP_WEIGHTS_OF_R if weighted else B200SP_WEIGHTS_NONE, a, R._d, S._d,
+                                        b, out._d, _address(buffer))
+    if status:
+        check(status, "b200spExpertsCombine")
+
+
+def experts_combine_grad(handle: Handle, R: CsrMatrix, d_out: DnMat, S: DnMat | None, d_S: DnMat,
+                         d_values: DnVec | None = None, alpha=1.0, beta=0.0, buffer: torch.Tensor | None = None) -> None:
+    """Gradients of the weighted experts_combine: of the rows, and with S and d_values of R's values."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsCombineGrad(handle._h, a, R._d, d_out._d, _optional(S, "experts_combine_grad: S"), b, d_S._d,
+                                            _optional(d_values, "experts_combine_grad: d_values"), _address(buffer))
+    if status:
+        check(status, "b200spExpertsCombineGrad")
+
+
+def quantise_rows(handle: Handle, X: DnMat, Q: DnMat, scales: DnVec) -> None:
+    """Q = X in whole numbers of up to 127 (int8), every row by its largest absolute value, and the rows' scales."""
+    status = lib().b200spQuantiseRows(handle._h, X._d, Q._d, scales._d)
+    if status:
+        check(status, "b200spQuantiseRows")
+
+
+def experts_quantise(handle: Handle, R: CsrMatrix, X: DnMat, Q: DnMat, scales: DnVec, offsets: DnVec | None = None,
+                     buffer: torch.Tensor | None = None) -> None:
+    """quantise_rows of every token's row into the rows of its entries in the order of the experts."""
+    status = lib().b200spExpertsQuantise(handle._h, R._d, X._d, Q._d, scales._d, _optional(offsets, "experts_quantise: offsets"),
+                                         _address(buffer))
+    if status:
+        check(status, "b200spExpertsQuantise")
+
+
+def scaled_mm_buffer_size(handle: Handle, X: DnMat, W: DnMat, Y: DnMat) -> int:
+    """0 where the rows of X and W start on 16 bytes: no buffer is needed then."""
+    size = c_size_t()
+    check(lib().b200spScaledMMBufferSize(handle.raw, X.raw, W.raw, Y.raw, byref(size)), "b200spScaledMMBufferSize")
+    return size.value
+
+
+def scaled_mm(handle: Handle, X: DnMat, x_scales: DnVec, W: DnMat, w_scales: DnVec, Y: DnMat, alpha=1.0, beta=0.0,
+              buffer: torch.Tensor | None = None) -> None:
+    """Y[i][j] = alpha * x_scales[i] * w_scales[j] * <X[i], W[j]> + beta * Y[i][j]; X and W int8."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spScaledMM(handle._h, a, X._d, x_scales._d, W._d, w_scales._d, b, Y._d, _address(buffer))
+    if status:
+        check(status, "b200spScaledMM")
+
+
+def experts_scaled_mm_buffer_size(handle: Handle, R: CsrMatrix, X: DnMat, W: DnMat, Y: DnMat) -> int:
+    size = c_size_t()
+    check(lib().b200spExpertsScaledMMBufferSize(handle.raw, R.raw, X.raw, W.raw, Y.raw, byref(size)),
+          "b200spExpertsScaledMMBufferSize")
+    return size.value
+
+
+def experts_scaled_mm(handle: Handle, R: CsrMatrix, X: DnMat, x_scales: DnVec, W: DnMat, w_scales: DnVec, Y: DnMat, alpha=1.0,
+                      beta=0.0, buffer: torch.Tensor | None = None) -> None:
+    """scaled_mm of every expert's rows, in the order of the experts, by its own matrix; W: the experts' matrices stacked."""
+    a, b = _float_scalars(handle, alpha, beta)
+    status = lib().b200spExpertsScaledMM(handle._h, a, R._d, X._d, x_scales._d, W._d, w_scales._d, b, Y._d, _address(buffer))
+    if status:
+        check(status, "b200spExpertsScaledMM")

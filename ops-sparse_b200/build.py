@@ -40,6 +40,7 @@ SOURCES = [
     "tokens/embedding.cu",
     "tokens/route.cu",
     "tokens/experts.cu",
+    "tokens/scaled.cu",
     "mg/partition.cpp",
     "mg/exchange.cu",
 ]

@@ -6,47 +6,24 @@
 #include <algorithm>
 #include <type_traits>
 
+#include "b200sp_rows.h"
 #include "b200sp_tokens.h"
 #include "tokens/common.cuh"
+#include "tokens/experts_plan.cuh"
+#include "tokens/rows.cuh"
 #include "tokens/sort.cuh"
+#include "tokens/tensor.cuh"
 
 namespace {
 
 using namespace b200sp_tokens;
 
-constexpr int kMaxExperts = 1024;
-
-// The buffer: what R it is the order of; where every expert's entries begin (one more group: entries of no expert), the entries by
-// expert and the rows of R that they lie in; and the sort's own arrays.
-struct PlanLayout {
-    size_t offsets, entries, rows, keyA, keyB, posB, total;
-};
-PlanLayout PlanLayoutFor(long long nnz, long long experts)
-{
-    PlanLayout L;
-    const size_t words = AlignUp(sizeof(int) * (size_t)nnz, 256);
-    L.offsets = 256;  // the header lies before
-    L.entries = L.offsets + AlignUp(sizeof(int) * (size_t)(experts + 2), 256);
-    L.rows = L.entries + words;
-    L.keyA = L.rows + words;
-    L.keyB = L.keyA + words;
-    L.posB = L.keyB + words;
-    L.total = L.posB + words + 256;  // any address is accepted
-    return L;
-}
-
-// A product follows the order only if the buffer starts with this: the sizes that its entries and rows are below, then a number of the order.
-// A Preprocess that was captured and has not been replayed yet has written nothing: an eager product after it wants its number.  (Others do
-// not: a graph's products follow the order that is there when they are replayed, whoever made it last.)  All that order the entries of one R
-// in one buffer write the same number, so that any of them may have been the last to run, until an eager b200spRoute gives R other columns.
-constexpr int kOrderMark = 0x45585031;
-inline int4 HeaderOf(long long nnz, long long experts, long long rows) { return make_int4(kOrderMark, (int)nnz, (int)experts, (int)rows); }
-
 // ---------------------------------------------------------------- the order of the entries
 
 __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const SortArgs s, const int *__restrict__ rowPtr, int rows,
-                                                                     int *__restrict__ rowOf, int *__restrict__ offsets, int4 *header,
-                                                                     const int4 mark, const uint64_t number)
+                                                                     int *__restrict__ rowOf, int *__restrict__ placeOf,
+                                                                     int *__restrict__ offsets, int4 *header, const int4 mark,
+                                                                     const uint64_t number)
 {
     extern __shared__ unsigned char sSort[];
     b200sp::WaitForPrevious();
@@ -67,6 +44,7 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
             r = lo;
         }
         rowOf[to] = r;
+        placeOf[entry] = to;
     });
     if (s.passes > 1 && blockIdx.x == 0) {
         for (int e = threadIdx.x; e <= s.limit + 1; e += kSortThreads) {
@@ -110,21 +88,11 @@ __global__ void __launch_bounds__(256) ExpertsAlignKernel(const uint16_t *__rest
 
 #include "tokens/experts_tensor.cuh"
 
-// ---------------------------------------------------------------- host
+// ---------------------------------------------------------------- rows in the order of the experts
 
-aclsparseStatus_t CheckRouted(const aclsparseSpMatDescr *R)
-{
-    if (R == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (R->format != ACL_SPARSE_FORMAT_CSR) return ACL_SPARSE_STATUS_MATRIX_TYPE_NOT_SUPPORTED;
-    const aclsparseStatus_t idx = b200sp::CheckExecIndexTypes(R->offsetType, R->indexType);
-    if (idx != ACL_SPARSE_STATUS_SUCCESS) return idx;
-    if (R->base != ACL_SPARSE_INDEX_BASE_ZERO) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (R->cols > kMaxExperts || R->rows >= INT32_MAX || R->nnz > kMostCounted) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
-    if (R->rows == 0 || R->cols == 0 || R->nnz == 0) return ACL_SPARSE_STATUS_INVALID_VALUE;  // no dense operand has as few rows
-    if (R->offsets == nullptr || R->indices == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    if (!OnBoundary(R->offsets, 4) || !OnBoundary(R->indices, 4)) return ACL_SPARSE_STATUS_INVALID_VALUE;
-    return ACL_SPARSE_STATUS_SUCCESS;
-}
+#include "tokens/experts_rows.cuh"
+
+// ---------------------------------------------------------------- host
 
 bool Is16(aclDataType t) { return t == ACL_FLOAT16 || t == ACL_BF16; }
 
@@ -168,23 +136,6 @@ aclsparseStatus_t CheckGrad(b200spExpertRows_t rowsOfX, const aclsparseSpMatDesc
     return ACL_SPARSE_STATUS_SUCCESS;
 }
 
-char *BufferStart(const void *buffer) { return reinterpret_cast<char *>(AlignUp(reinterpret_cast<uintptr_t>(buffer), 256)); }
-
-// Whether the buffer is the one that R's entries were ordered in last, and no other call has written it since.
-bool SameBuffer(const aclsparseSpMatDescr *R, const void *buffer)
-{
-    const b200sp::ExpertsPlan &p = R->experts;
-    return buffer != nullptr && p.buffer == buffer && p.offsets == R->offsets && p.indices == R->indices && p.rows == R->rows &&
-           p.cols == R->cols && p.nnz == R->nnz && p.generation != 0 && p.generation == b200sp::BufferGeneration(buffer);
-}
-// Whether the buffer still holds the order of R's entries; the number that it has to have, 0: any.
-bool HoldsOrder(const aclsparseSpMatDescr *R, const void *buffer, cudaStream_t stream, uint64_t *number)
-{
-    std::lock_guard<std::mutex> lock(R->expertsMutex);
-    *number = R->experts.captured && !Captures(stream) ? R->experts.number : 0;
-    return SameBuffer(R, buffer) && !R->experts.stale;
-}
-
 MmaArgs ArgsOf(const aclsparseSpMatDescr *R, b200spExpertRows_t rowsOfX, const void *buffer, uint64_t number, const aclsparseDnMatDescr *stacked,
                const aclsparseDnMatDescr *out, const Scalars &sc)
 {
@@ -217,21 +168,6 @@ size_t BufferBytes(const aclsparseSpMatDescr *R, const aclsparseDnMatDescr *firs
 {
     return PlanLayoutFor(R->nnz, R->cols).total + AlignedBytes(first) + AlignedBytes(second);
 }
-// What the BufferSize calls for this matrix have said at most.
-size_t NoteSize(const aclsparseSpMatDescr *R, size_t bytes)
-{
-    std::lock_guard<std::mutex> lock(R->expertsMutex);
-    R->expertsSized = std::max(R->expertsSized, (int64_t)bytes);
-    return bytes;
-}
-// Whether the buffer may be taken to have room for copies of the operands, if any: what Preprocess writes it has.
-bool HasRoom(const aclsparseSpMatDescr *R, const aclsparseDnMatDescr *first, const aclsparseDnMatDescr *second)
-{
-    if (AlignedBytes(first) + AlignedBytes(second) == 0) return true;
-    std::lock_guard<std::mutex> lock(R->expertsMutex);
-    return (int64_t)BufferBytes(R, first, second) <= R->expertsSized;
-}
-
 // An operand as the kernels read it: where it lies, or its copy at `room`, which moves on.
 struct Operand {
     const void *values;
@@ -318,8 +254,8 @@ aclsparseStatus_t b200spExpertsPreprocess(aclsparseHandle_t handle, aclsparseCon
         cfg.numAttrs = 2;
         b200sp_note_launches(1);
         e = cudaLaunchKernelEx(&cfg, ExpertsOrderKernel, s, static_cast<const int *>(matR->offsets), (int)matR->rows,
-                               reinterpret_cast<int *>(p + L.rows), offsets, reinterpret_cast<int4 *>(p),
-                               HeaderOf(matR->nnz, matR->cols, matR->rows), number);
+                               reinterpret_cast<int *>(p + L.rows), reinterpret_cast<int *>(p + L.places), offsets,
+                               reinterpret_cast<int4 *>(p), HeaderOf(matR->nnz, matR->cols, matR->rows), number);
     }
     matR->experts = {};
     if (e == cudaSuccess)
@@ -348,7 +284,7 @@ aclsparseStatus_t b200spExpertsMM(aclsparseHandle_t handle, aclsparseOperation_t
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
     uint64_t number;
-    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoom(matR, matX, matW)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoomFor(matR, AlignedBytes(matX) + AlignedBytes(matW))) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
     MmaArgs a = ArgsOf(matR, rowsOfX, buffer, number, matW, matY, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
@@ -396,7 +332,7 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
     if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
     if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
     uint64_t number;
-    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoom(matR, matX, dY)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number) || !HasRoomFor(matR, AlignedBytes(matX) + AlignedBytes(dY))) return ACL_SPARSE_STATUS_INVALID_VALUE;
     const OnDevice device(handle);
     MmaArgs a = ArgsOf(matR, rowsOfX, buffer, number, dW, dW, ScalarsOf(handle, alpha, beta));
     char *room = BufferStart(buffer) + PlanLayoutFor(matR->nnz, matR->cols).total - 256;
@@ -419,6 +355,209 @@ aclsparseStatus_t b200spExpertsGrad(aclsparseHandle_t handle, b200spExpertRows_t
         });
     });
     return Finished(e, "b200spExpertsGrad");
+}
+
+// ---------------------------------------------------------------- rows in the order of the experts, and in 8 bits
+
+aclsparseStatus_t b200spExpertsOrderBufferSize(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, size_t *bufferSize)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    if (bufferSize == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const aclsparseStatus_t st = CheckRouted(matR);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    *bufferSize = NoteSize(matR, PlanLayoutFor(matR->nnz, matR->cols).total);
+    return ACL_SPARSE_STATUS_SUCCESS;
+}
+
+aclsparseStatus_t b200spExpertsDispatch(aclsparseHandle_t handle, const void *alpha, aclsparseConstSpMatDescr_t matR,
+                                        aclsparseConstDnMatDescr_t matX, const void *beta, aclsparseDnMatDescr_t matS,
+                                        aclsparseDnVecDescr_t offsets, const void *buffer)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    aclsparseStatus_t st = CheckRouted(matR);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(matX);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(matS);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckStarts(matR, offsets);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (matS->valueType != matX->valueType && matS->valueType != ACL_FLOAT) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (matX->rows != matR->rows || matS->rows != matR->nnz || matX->cols != matS->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const OnDevice device(handle);
+    RowsArgs a = RowsOf(matR, buffer, number);
+    a.width = (int)matX->cols;
+    a.perToken = matX->values;
+    a.ldToken = matX->ld;
+    a.out = matS->values;
+    a.ldOut = matS->ld;
+    a.starts = offsets == nullptr ? nullptr : static_cast<int *>(offsets->values);
+    a.sc = ScalarsOf(handle, alpha, beta);
+    const bool vectors = RowsAligned(matX) && RowsAligned(matS);
+    const cudaError_t e = WithTypes(matX->valueType, matS->valueType, [&](auto in, auto out) {
+        using In = decltype(in);
+        using Out = decltype(out);
+        if constexpr (std::is_same_v<In, Out> || sizeof(Out) == 4) {
+            const unsigned blocks = RowsBlocks(a.tokens * ((a.width + 32 * kStretch<In, Out> - 1) / (32 * kStretch<In, Out>)));
+            b200sp_note_launches(1);
+            return vectors ? b200sp::LaunchChained(ExpertsDispatchKernel<In, Out, true>, blocks, kRowsThreads, 0, handle->stream, a)
+                           : b200sp::LaunchChained(ExpertsDispatchKernel<In, Out, false>, blocks, kRowsThreads, 0, handle->stream, a);
+        } else {
+            return cudaErrorInvalidValue;  // refused above
+        }
+    });
+    return Finished(e, "b200spExpertsDispatch");
+}
+
+aclsparseStatus_t b200spExpertsCombine(aclsparseHandle_t handle, b200spExpertWeights_t weights, const void *alpha,
+                                       aclsparseConstSpMatDescr_t matR, aclsparseConstDnMatDescr_t matS, const void *beta,
+                                       aclsparseDnMatDescr_t matOut, const void *buffer)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    if (weights != B200SP_WEIGHTS_NONE && weights != B200SP_WEIGHTS_OF_R) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const bool weighted = weights == B200SP_WEIGHTS_OF_R;
+    aclsparseStatus_t st = CheckRouted(matR);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(matS);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(matOut);
+    if (st == ACL_SPARSE_STATUS_SUCCESS && weighted) st = CheckWeights(matR);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (UnlikeHalves(matS->valueType, matOut->valueType)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (matOut->rows != matR->rows || matS->rows != matR->nnz || matOut->cols != matS->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const OnDevice device(handle);
+    RowsArgs a = RowsOf(matR, buffer, number);
+    a.width = (int)matS->cols;
+    a.perEntry = matS->values;
+    a.ldEntry = matS->ld;
+    a.out = matOut->values;
+    a.ldOut = matOut->ld;
+    a.weights = weighted ? matR->values : nullptr;
+    a.weightType = matR->valueType;
+    a.sc = ScalarsOf(handle, alpha, beta);
+    const bool vectors = RowsAligned(matS) && RowsAligned(matOut);
+    const cudaError_t e = WithTypes(matS->valueType, matOut->valueType, [&](auto in, auto out) {
+        using In = decltype(in);
+        using Out = decltype(out);
+        const unsigned blocks = RowsBlocks(a.tokens * ((a.width + 32 * kStretch<In, Out> - 1) / (32 * kStretch<In, Out>)));
+        b200sp_note_launches(1);
+        return vectors ? b200sp::LaunchChained(ExpertsCombineKernel<In, Out, true>, blocks, kRowsThreads, 0, handle->stream, a)
+                       : b200sp::LaunchChained(ExpertsCombineKernel<In, Out, false>, blocks, kRowsThreads, 0, handle->stream, a);
+    });
+    return Finished(e, "b200spExpertsCombine");
+}
+
+aclsparseStatus_t b200spExpertsCombineGrad(aclsparseHandle_t handle, const void *alpha, aclsparseConstSpMatDescr_t matR,
+                                           aclsparseConstDnMatDescr_t dOut, aclsparseConstDnMatDescr_t matS, const void *beta,
+                                           aclsparseDnMatDescr_t dS, aclsparseDnVecDescr_t dValues, const void *buffer)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    aclsparseStatus_t st = CheckRouted(matR);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(dOut);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(dS);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckWeights(matR);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if ((matS == nullptr) != (dValues == nullptr)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (UnlikeHalves(dOut->valueType, dS->valueType)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+    if (dOut->rows != matR->rows || dS->rows != matR->nnz || dOut->cols != dS->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (matS != nullptr) {
+        st = CheckDense(matS);
+        if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+        if (matS->valueType != dS->valueType) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+        if (matS->rows != dS->rows || matS->cols != dS->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+        if (dValues->magic != b200sp::kDnVecMagic) return ACL_SPARSE_STATUS_INVALID_VALUE;
+        if (!IsFloatType(dValues->valueType)) return ACL_SPARSE_STATUS_NOT_SUPPORTED;
+        st = CheckNumbers(dValues, matR->nnz, dValues->valueType, BytesOf(dValues->valueType));
+        if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    }
+    if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const OnDevice device(handle);
+    RowsArgs a = RowsOf(matR, buffer, number);
+    a.width = (int)dOut->cols;
+    a.perToken = dOut->values;
+    a.ldToken = dOut->ld;
+    a.out = dS->values;
+    a.ldOut = dS->ld;
+    if (matS != nullptr) {
+        a.perEntry = matS->values;
+        a.ldEntry = matS->ld;
+        a.dValues = dValues->values;
+        a.dValuesType = dValues->valueType;
+    }
+    a.weights = matR->values;
+    a.weightType = matR->valueType;
+    a.sc = ScalarsOf(handle, alpha, beta);
+    const bool vectors = RowsAligned(dOut) && RowsAligned(dS) && (matS == nullptr || RowsAligned(matS));
+    const cudaError_t e = WithTypes(dS->valueType, dOut->valueType, [&](auto s, auto g) {
+        using T = decltype(s);
+        using G = decltype(g);
+        const bool cta = a.tokens < (long long)b200sp_sm_count() * kRowsWarps;
+        const unsigned blocks = RowsBlocks(cta ? a.tokens * kRowsWarps : a.tokens);
+        b200sp_note_launches(1);
+        if (cta)
+            return vectors ? b200sp::LaunchChained(ExpertsCombineGradKernel<T, G, true, kRowsWarps>, blocks, kRowsThreads, 0, handle->stream, a)
+                           : b200sp::LaunchChained(ExpertsCombineGradKernel<T, G, false, kRowsWarps>, blocks, kRowsThreads, 0, handle->stream, a);
+        return vectors ? b200sp::LaunchChained(ExpertsCombineGradKernel<T, G, true, 1>, blocks, kRowsThreads, 0, handle->stream, a)
+                       : b200sp::LaunchChained(ExpertsCombineGradKernel<T, G, false, 1>, blocks, kRowsThreads, 0, handle->stream, a);
+    });
+    return Finished(e, "b200spExpertsCombineGrad");
+}
+
+aclsparseStatus_t b200spQuantiseRows(aclsparseHandle_t handle, aclsparseConstDnMatDescr_t matX, aclsparseDnMatDescr_t matQ,
+                                     aclsparseDnVecDescr_t scales)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    aclsparseStatus_t st = CheckDense(matX);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckBytes(matQ);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckNumbers(scales, matQ->rows, ACL_FLOAT, 4);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (matX->rows != matQ->rows || matX->cols != matQ->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const OnDevice device(handle);
+    RowsArgs a{};
+    a.tokens = matX->rows;
+    a.width = (int)matX->cols;
+    a.perToken = matX->values;
+    a.ldToken = matX->ld;
+    a.out = matQ->values;
+    a.ldOut = matQ->ld;
+    a.scales = static_cast<float *>(scales->values);
+    const cudaError_t e = WithType(matX->valueType, [&](auto x) {
+        return LaunchQuantise<decltype(x), false>(a, QuantiseVectors(matX, matQ), handle->stream);
+    });
+    return Finished(e, "b200spQuantiseRows");
+}
+
+aclsparseStatus_t b200spExpertsQuantise(aclsparseHandle_t handle, aclsparseConstSpMatDescr_t matR, aclsparseConstDnMatDescr_t matX,
+                                        aclsparseDnMatDescr_t matQ, aclsparseDnVecDescr_t scales, aclsparseDnVecDescr_t offsets,
+                                        const void *buffer)
+{
+    if (handle == nullptr) return ACL_SPARSE_STATUS_HANDLE_IS_NULLPTR;
+    aclsparseStatus_t st = CheckRouted(matR);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckDense(matX);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckBytes(matQ);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckNumbers(scales, matQ->rows, ACL_FLOAT, 4);
+    if (st == ACL_SPARSE_STATUS_SUCCESS) st = CheckStarts(matR, offsets);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    if (matX->rows != matR->rows || matQ->rows != matR->nnz || matX->cols != matQ->cols) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    if (buffer == nullptr) return ACL_SPARSE_STATUS_INSUFFICIENT_RESOURCES;
+    uint64_t number;
+    if (!HoldsOrder(matR, buffer, handle->stream, &number)) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const OnDevice device(handle);
+    RowsArgs a = RowsOf(matR, buffer, number);
+    a.width = (int)matX->cols;
+    a.perToken = matX->values;
+    a.ldToken = matX->ld;
+    a.out = matQ->values;
+    a.ldOut = matQ->ld;
+    a.scales = static_cast<float *>(scales->values);
+    a.starts = offsets == nullptr ? nullptr : static_cast<int *>(offsets->values);
+    const cudaError_t e = WithType(matX->valueType, [&](auto x) {
+        return LaunchQuantise<decltype(x), true>(a, QuantiseVectors(matX, matQ), handle->stream);
+    });
+    return Finished(e, "b200spExpertsQuantise");
 }
 
 }  // extern "C"
