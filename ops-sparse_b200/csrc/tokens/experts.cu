@@ -398,7 +398,7 @@ aclsparseStatus_t b200spExpertsDispatch(aclsparseHandle_t handle, const void *al
         using In = decltype(in);
         using Out = decltype(out);
         if constexpr (std::is_same_v<In, Out> || sizeof(Out) == 4) {
-            const unsigned blocks = RowsBlocks(a.tokens * ((a.width + 32 * kStretch<In, Out> - 1) / (32 * kStretch<In, Out>)));
+            const unsigned blocks = RowsBlocks(a.tokens * ((a.width + kStretch - 1) / kStretch), kDispatchCtas);
             b200sp_note_launches(1);
             return vectors ? b200sp::LaunchChained(ExpertsDispatchKernel<In, Out, true>, blocks, kRowsThreads, 0, handle->stream, a)
                            : b200sp::LaunchChained(ExpertsDispatchKernel<In, Out, false>, blocks, kRowsThreads, 0, handle->stream, a);
@@ -440,7 +440,7 @@ aclsparseStatus_t b200spExpertsCombine(aclsparseHandle_t handle, b200spExpertWei
     const cudaError_t e = WithTypes(matS->valueType, matOut->valueType, [&](auto in, auto out) {
         using In = decltype(in);
         using Out = decltype(out);
-        const unsigned blocks = RowsBlocks(a.tokens * ((a.width + 32 * kStretch<In, Out> - 1) / (32 * kStretch<In, Out>)));
+        const unsigned blocks = RowsBlocks(a.tokens * ((a.width + kStretch - 1) / kStretch), kCombineCtas);
         b200sp_note_launches(1);
         return vectors ? b200sp::LaunchChained(ExpertsCombineKernel<In, Out, true>, blocks, kRowsThreads, 0, handle->stream, a)
                        : b200sp::LaunchChained(ExpertsCombineKernel<In, Out, false>, blocks, kRowsThreads, 0, handle->stream, a);
@@ -495,7 +495,7 @@ aclsparseStatus_t b200spExpertsCombineGrad(aclsparseHandle_t handle, const void 
         using T = decltype(s);
         using G = decltype(g);
         const bool cta = a.tokens < (long long)b200sp_sm_count() * kRowsWarps;
-        const unsigned blocks = RowsBlocks(cta ? a.tokens * kRowsWarps : a.tokens);
+        const unsigned blocks = RowsBlocks(cta ? a.tokens * kRowsWarps : a.tokens, kGradCtas);
         b200sp_note_launches(1);
         if (cta)
             return vectors ? b200sp::LaunchChained(ExpertsCombineGradKernel<T, G, true, kRowsWarps>, blocks, kRowsThreads, 0, handle->stream, a)

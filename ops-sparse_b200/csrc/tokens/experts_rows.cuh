@@ -26,16 +26,18 @@ struct RowsArgs {
 };
 
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
+constexpr int kDispatchCtas = 5, kCombineCtas = 4, kGradCtas = 2;  // resident on an SM: what their registers allow
+template <typename T> constexpr int kQuantiseCtas = sizeof(T) == 4 ? 4 : 6;
 
-// What every call of this file begins with: false without an order.
-__device__ __forceinline__ bool RowsBegin(const RowsArgs &a)
+// What every call of this file ends its beginning with: false without an order.  What has been read of the buffer by then (places may be any
+// numbers) leads to no access.
+__device__ __forceinline__ bool HasOrder(const RowsArgs &a)
 {
-    b200sp::WaitForPrevious();
     if (!StartsWith(a.header, a.mark, a.number)) {
         if (blockIdx.x == 0 && threadIdx.x == 0) atomicMax(&gExpertsError, kNoOrder);
         return false;
     }
-    if (a.starts != nullptr && blockIdx.x == 0)
+    if (a.starts != nullptr && blockIdx.x == gridDim.x - 1)
         for (int e = threadIdx.x; e <= a.experts; e += kRowsThreads) a.starts[e] = __ldg(a.offsets + e);
     return true;
 }
@@ -45,249 +47,288 @@ __device__ __forceinline__ int2 EntriesOf(const RowsArgs &a, long long token)
     return make_int2(max(0, __ldg(a.rowPtr + token)), min(a.nnz, __ldg(a.rowPtr + token + 1)));
 }
 
-template <typename In, typename Out> constexpr int kStretch = 16 / (sizeof(In) < sizeof(Out) ? (int)sizeof(In) : (int)sizeof(Out));
+// The entries of a token, and where the rows of the first 32 lie, a lane each; asked for ahead of the rows.
+struct TokenEntries {
+    int2 range;
+    int place;
+    float weight;
+    __device__ __forceinline__ void Rows(const RowsArgs &a, int e0, int lane)
+    {
+        place = 0;
+        weight = 1.0f;
+        if (e0 + lane < range.y) {
+            place = __ldg(a.places + e0 + lane);
+            if (a.weights != nullptr) weight = ValueAt(a.weights, a.weightType, e0 + lane);
+        }
+    }
+    __device__ __forceinline__ void Ask(const RowsArgs &a, long long token, int lane)
+    {
+        range = token < a.tokens ? EntriesOf(a, token) : make_int2(0, 0);
+        Rows(a, range.x, lane);
+    }
+};
 
-template <typename In, typename Out, bool kVector> __global__ void __launch_bounds__(kRowsThreads) ExpertsDispatchKernel(const RowsArgs a)
+template <typename In, typename Out, bool kVector>
+__global__ void __launch_bounds__(kRowsThreads, kDispatchCtas) ExpertsDispatchKernel(const RowsArgs a)
 {
-    constexpr int kN = kStretch<In, Out>;
-    if (!RowsBegin(a)) return;
+    b200sp::WaitForPrevious();
     const int lane = threadIdx.x & 31, end = __ldg(a.offsets + a.experts);
     const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-    Units u((long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5), (long long)gridDim.x * kRowsWarps, (a.width + 32 * kN - 1) / (32 * kN));
-    for (; u.row < a.tokens; u.Next()) {
-        const int2 entries = EntriesOf(a, u.row);
-        const int c0 = u.stretch * 32 * kN;
-        float v[kN];
-        LoadStretch<In, kN, kVector>(static_cast<const In *>(a.perToken) + u.row * a.ldToken, c0, lane, a.width, v);
+    Units u((long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5), (long long)gridDim.x * kRowsWarps, (a.width + kStretch - 1) / kStretch);
+    TokenEntries next;
+    next.Ask(a, u.row, lane);
+    if (!HasOrder(a)) return;
+    while (u.row < a.tokens) {
+        const int c0 = u.stretch * kStretch;
+        Raw<In> raw;
+        raw.template Load<kVector>(static_cast<const In *>(a.perToken) + u.row * a.ldToken, c0, lane, a.width);
+        TokenEntries now = next;
+        u.Next();
+        next.Ask(a, u.row, lane);
+        float v[8];
+        raw.Floats(v);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] *= alpha;
-        for (int e0 = entries.x; e0 < entries.y; e0 += 32) {
-            const int mine = e0 + lane < entries.y ? __ldg(a.places + e0 + lane) : 0, many = min(32, entries.y - e0);
+        for (int i = 0; i < 8; ++i) v[i] *= alpha;
+        Raw<Out> row, none;
+        row.Set(v);
+        none.Zero();
+        for (int e0 = now.range.x; e0 < now.range.y; e0 += 32) {
+            if (e0 > now.range.x) now.Rows(a, e0, lane);
+            const int many = min(32, now.range.y - e0);
             for (int j = 0; j < many; ++j) {
-                const int place = __shfl_sync(0xffffffffu, mine, j);
+                const int place = __shfl_sync(0xffffffffu, now.place, j);
                 Out *const to = static_cast<Out *>(a.out) + place * a.ldOut;
-                float w[kN];
-                if (beta != 0.0f) LoadStretch<Out, kN, kVector>(to, c0, lane, a.width, w);
+                if (beta == 0.0f) {
+                    if (place < end) row.template Store<kVector>(to, c0, lane, a.width);
+                    else none.template Store<kVector>(to, c0, lane, a.width);
+                } else {
+                    Raw<Out> old;
+                    old.template Load<kVector>(to, c0, lane, a.width);
+                    float w[8];
+                    old.Floats(w);
 #pragma unroll
-                for (int i = 0; i < kN; ++i) {
-                    const float x = place < end ? v[i] : 0.0f;
-                    w[i] = beta != 0.0f ? fmaf(beta, w[i], x) : x;
+                    for (int i = 0; i < 8; ++i) w[i] = fmaf(beta, w[i], place < end ? v[i] : 0.0f);
+                    old.Set(w);
+                    old.template Store<kVector>(to, c0, lane, a.width);
                 }
-                StoreStretch<Out, kN, kVector>(to, c0, lane, a.width, w);
             }
         }
     }
 }
 
-template <typename In, typename Out, bool kVector> __global__ void __launch_bounds__(kRowsThreads) ExpertsCombineKernel(const RowsArgs a)
+// Rows are asked for kRowsAhead at a time, and the places of the next unit's before this one's are summed.
+template <typename In, typename Out, bool kVector>
+__global__ void __launch_bounds__(kRowsThreads, kCombineCtas) ExpertsCombineKernel(const RowsArgs a)
 {
-    constexpr int kN = kStretch<In, Out>;
-    if (!RowsBegin(a)) return;
+    constexpr int kAhead = sizeof(In) == 4 ? 2 : 4;
+    b200sp::WaitForPrevious();
     const int lane = threadIdx.x & 31, end = __ldg(a.offsets + a.experts);
     const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-    Units u((long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5), (long long)gridDim.x * kRowsWarps, (a.width + 32 * kN - 1) / (32 * kN));
-    for (; u.row < a.tokens; u.Next()) {
-        const int2 entries = EntriesOf(a, u.row);
-        const int c0 = u.stretch * 32 * kN;
-        float sum[kN] = {};
-        for (int e0 = entries.x; e0 < entries.y; e0 += 32) {
-            int mine = end;
-            float weight = 1.0f;
-            if (e0 + lane < entries.y) {
-                mine = __ldg(a.places + e0 + lane);
-                if (a.weights != nullptr) weight = ValueAt(a.weights, a.weightType, e0 + lane);
-            }
-            const int many = min(32, entries.y - e0);
-            for (int j = 0; j < many; ++j) {
-                const int place = __shfl_sync(0xffffffffu, mine, j);
-                const float w = __shfl_sync(0xffffffffu, weight, j);
-                if (place >= end) continue;
-                float v[kN];
-                LoadStretch<In, kN, kVector>(static_cast<const In *>(a.perEntry) + place * a.ldEntry, c0, lane, a.width, v);
+    Units u((long long)blockIdx.x * kRowsWarps + (threadIdx.x >> 5), (long long)gridDim.x * kRowsWarps, (a.width + kStretch - 1) / kStretch);
+    TokenEntries next;
+    next.Ask(a, u.row, lane);
+    if (!HasOrder(a)) return;
+    while (u.row < a.tokens) {
+        const int c0 = u.stretch * kStretch;
+        const long long token = u.row;
+        TokenEntries now = next;
+        u.Next();
+        next.Ask(a, u.row, lane);
+        float sum[8] = {};
+        for (int e0 = now.range.x; e0 < now.range.y; e0 += 32) {
+            if (e0 > now.range.x) now.Rows(a, e0, lane);
+            const int many = min(32, now.range.y - e0);
+            for (int j0 = 0; j0 < many; j0 += kAhead) {
+                Raw<In> raw[kAhead];
+                bool in[kAhead];
 #pragma unroll
-                for (int i = 0; i < kN; ++i) sum[i] = fmaf(w, v[i], sum[i]);
+                for (int j = 0; j < kAhead; ++j) {
+                    const int place = __shfl_sync(0xffffffffu, now.place, (j0 + j) & 31);
+                    in[j] = j0 + j < many && place < end;
+                    if (in[j]) raw[j].template Load<kVector>(static_cast<const In *>(a.perEntry) + place * a.ldEntry, c0, lane, a.width);
+                }
+#pragma unroll
+                for (int j = 0; j < kAhead; ++j) {
+                    const float w = __shfl_sync(0xffffffffu, now.weight, (j0 + j) & 31);
+                    if (in[j]) {
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) sum[i] = fmaf(w, raw[j].At(i), sum[i]);
+                    }
+                }
             }
         }
-        Out *const to = static_cast<Out *>(a.out) + u.row * a.ldOut;
-        float old[kN];
-        if (beta != 0.0f) LoadStretch<Out, kN, kVector>(to, c0, lane, a.width, old);
+        Out *const to = static_cast<Out *>(a.out) + token * a.ldOut;
+        Raw<Out> out;
+        if (beta != 0.0f) {
+            out.template Load<kVector>(to, c0, lane, a.width);
 #pragma unroll
-        for (int i = 0; i < kN; ++i) sum[i] = beta != 0.0f ? fmaf(beta, old[i], alpha * sum[i]) : alpha * sum[i];
-        StoreStretch<Out, kN, kVector>(to, c0, lane, a.width, sum);
+            for (int i = 0; i < 8; ++i) sum[i] = fmaf(beta, out.At(i), alpha * sum[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sum[i] *= alpha;
+        }
+        out.Set(sum);
+        out.template Store<kVector>(to, c0, lane, a.width);
     }
 }
 
-// T: of S and dS; G: of dOut.  kWarps at a token, eight of its entries at a time.
+// T: of S and dS; G: of dOut.  kWarps at a token, kBatch of its entries at a time.
 template <typename T, typename G, bool kVector, int kWarps>
-__global__ void __launch_bounds__(kRowsThreads) ExpertsCombineGradKernel(const RowsArgs a)
+__global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKernel(const RowsArgs a)
 {
-    constexpr int kN = kStretch<T, G>, kBatch = 8;
-    __shared__ float sDot[kRowsWarps][kBatch];
-    if (!RowsBegin(a)) return;
+    constexpr int kBatch = 4;
+    __shared__ float sDot[2][kRowsWarps][kBatch];
+    b200sp::WaitForPrevious();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, end = __ldg(a.offsets + a.experts);
     const int within = warp % kWarps;
     const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
     constexpr int kTokens = kRowsWarps / kWarps;
-    for (long long t = (long long)blockIdx.x * kTokens + warp / kWarps; t < a.tokens; t += (long long)gridDim.x * kTokens) {
-        const int2 entries = EntriesOf(a, t);
+    const long long step = (long long)gridDim.x * kTokens;
+    long long t = (long long)blockIdx.x * kTokens + warp / kWarps;
+    int turn = 0;
+    TokenEntries next;
+    next.Ask(a, t, lane);
+    if (!HasOrder(a)) return;
+    for (; t < a.tokens; t += step) {
+        TokenEntries now = next;
+        next.Ask(a, t + step, lane);
         const G *const grad = static_cast<const G *>(a.perToken) + t * a.ldToken;
-        for (int e0 = entries.x; e0 < entries.y; e0 += kBatch) {
-            int mine = 0;
-            float weight = 0.0f;
-            const int many = min(kBatch, entries.y - e0);
-            if (lane < many) {
-                mine = __ldg(a.places + e0 + lane);
-                weight = alpha * ValueAt(a.weights, a.weightType, e0 + lane);
+        for (int e0 = now.range.x; e0 < now.range.y; e0 += kBatch) {
+            const int first = (e0 - now.range.x) & 31, many = min(kBatch, now.range.y - e0);
+            if (first == 0 && e0 > now.range.x) now.Rows(a, e0, lane);
+            int place[kBatch];
+            float weight[kBatch], dot[kBatch] = {};
+#pragma unroll
+            for (int j = 0; j < kBatch; ++j) {
+                place[j] = __shfl_sync(0xffffffffu, now.place, first + j);
+                weight[j] = alpha * __shfl_sync(0xffffffffu, now.weight, first + j);
             }
-            float dot[kBatch] = {};
-            for (int c0 = within * 32 * kN; c0 < a.width; c0 += kWarps * 32 * kN) {
-                float g[kN];
-                LoadStretch<G, kN, kVector>(grad, c0, lane, a.width, g);
+            for (int c0 = within * kStretch; c0 < a.width; c0 += kWarps * kStretch) {
+                Raw<G> raw;
+                raw.template Load<kVector>(grad, c0, lane, a.width);
+                Raw<T> rows[kBatch];
+                if (a.dValues != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        if (j < many && place[j] < end)
+                            rows[j].template Load<kVector>(static_cast<const T *>(a.perEntry) + place[j] * a.ldEntry, c0, lane, a.width);
+                        else rows[j].Zero();
+                    }
+                }
+                float g[8];
+                raw.Floats(g);
 #pragma unroll
                 for (int j = 0; j < kBatch; ++j) {
                     if (j >= many) break;
-                    const int place = __shfl_sync(0xffffffffu, mine, j);
-                    const float w = __shfl_sync(0xffffffffu, weight, j);
-                    float v[kN];
-                    if (a.dValues != nullptr && place < end) {
-                        LoadStretch<T, kN, kVector>(static_cast<const T *>(a.perEntry) + place * a.ldEntry, c0, lane, a.width, v);
+                    if (a.dValues != nullptr && place[j] < end) {
 #pragma unroll
-                        for (int i = 0; i < kN; ++i) dot[j] = fmaf(g[i], v[i], dot[j]);
+                        for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[i], rows[j].At(i), dot[j]);
                     }
-                    T *const to = static_cast<T *>(a.out) + place * a.ldOut;
-                    if (beta != 0.0f) LoadStretch<T, kN, kVector>(to, c0, lane, a.width, v);
+                    T *const to = static_cast<T *>(a.out) + place[j] * a.ldOut;
+                    float v[8];
 #pragma unroll
-                    for (int i = 0; i < kN; ++i) {
-                        const float x = place < end ? w * g[i] : 0.0f;
-                        v[i] = beta != 0.0f ? fmaf(beta, v[i], x) : x;
+                    for (int i = 0; i < 8; ++i) v[i] = place[j] < end ? weight[j] * g[i] : 0.0f;
+                    Raw<T> out;
+                    if (beta != 0.0f) {
+                        out.template Load<kVector>(to, c0, lane, a.width);
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) v[i] = fmaf(beta, out.At(i), v[i]);
                     }
-                    StoreStretch<T, kN, kVector>(to, c0, lane, a.width, v);
+                    out.Set(v);
+                    out.template Store<kVector>(to, c0, lane, a.width);
                 }
             }
             if (a.dValues == nullptr) continue;
-            float total = 0.0f;  // of entry `lane`
+            float total = 0.0f;  // of entry e0 + lane
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
                 if (lane == j) total = dot[j];
             }
-            if constexpr (kWarps > 1) {
-                if (lane < kBatch) sDot[warp][lane] = total;
+            if constexpr (kWarps > 1) {  // a CTA's warps are all at one token; two places in turn, as others may still read the one
+                if (lane < kBatch) sDot[turn][warp][lane] = total;
                 __syncthreads();
                 total = 0.0f;
                 if (lane < kBatch)
-                    for (int w = 0; w < kWarps; ++w) total += sDot[warp - within + w][lane];
-                __syncthreads();  // a CTA's warps are all at one token
+                    for (int w = 0; w < kWarps; ++w) total += sDot[turn][warp - within + w][lane];
+                turn ^= 1;
             }
             if (within == 0 && lane < many) {
-                const float old = beta != 0.0f ? beta * ValueAt(a.dValues, a.dValuesType, e0 + lane) : 0.0f;
-                SetValue(a.dValues, a.dValuesType, e0 + lane, beta != 0.0f ? fmaf(alpha, total, old) : alpha * total);
+                const float old = beta != 0.0f ? ValueAt(a.dValues, a.dValuesType, e0 + lane) : 0.0f;
+                SetValue(a.dValues, a.dValuesType, e0 + lane, beta != 0.0f ? fmaf(beta, old, alpha * total) : alpha * total);
             }
         }
     }
 }
 
-// Rows in 8 bits: of tokens (kOrdered false), or every token's into the rows of its entries.  kWarps at a row, which they keep in registers
-// up to kHeld elements a thread and read again beyond.
+// Rows in 8 bits: of tokens (kOrdered false), or every token's into the rows of its entries.  kWarps at a row, which they keep, every thread
+// what it has read, in shared memory up to 1024 elements a warp, and read again beyond.
 template <typename T, bool kVector, int kWarps, bool kOrdered>
-__global__ void __launch_bounds__(kRowsThreads) QuantiseKernel(const RowsArgs a)
+__global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel(const RowsArgs a)
 {
-    constexpr int kN = 8, kHeld = 32 * 4 / (kN * (int)sizeof(T));  // stretches: 32 registers
-    constexpr int kStep = kWarps * 32 * kN, kTokens = kRowsWarps / kWarps;
-    __shared__ uint32_t sTop[kRowsWarps];
-    if constexpr (kOrdered) {
-        if (!RowsBegin(a)) return;
-    } else {
-        b200sp::WaitForPrevious();
-    }
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, within = warp % kWarps;
+    constexpr int kHeld = 4;
+    constexpr int kStep = kWarps * kStretch, kTokens = kRowsWarps / kWarps;
+    __shared__ uint32_t sTop[2][kRowsWarps];
+    __shared__ Raw<T> sHeld[kHeld][kRowsThreads];
+    b200sp::WaitForPrevious();
+    if (kOrdered && !HasOrder(a)) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, within = warp % kWarps, c = within * kStretch;
     const int end = kOrdered ? __ldg(a.offsets + a.experts) : 0;
-    for (long long t = (long long)blockIdx.x * kTokens + warp / kWarps; t < a.tokens; t += (long long)gridDim.x * kTokens) {
+    int turn = 0;
+    for (long long t = (long long)blockIdx.x * kTokens + warp / kWarps; t < a.tokens; t += (long long)gridDim.x * kTokens, turn ^= 1) {
         const T *const row = static_cast<const T *>(a.perToken) + t * a.ldToken;
-        const int2 entries = kOrdered ? EntriesOf(a, t) : make_int2(0, 1);
-        const int c = within * 32 * kN;
-        T held[kHeld][kN];
+        int2 entries = make_int2(0, 1);
+        int mine = 0;  // where the row of entry `lane` goes
+        if constexpr (kOrdered) {
+            entries = EntriesOf(a, t);
+            if (entries.x + lane < entries.y) mine = __ldg(a.places + entries.x + lane);
+        }
+        Raw<T> held[kHeld];
+#pragma unroll
+        for (int h = 0; h < kHeld; ++h) held[h].template Load<kVector>(row, c + h * kStep, lane, a.width);
         uint32_t top = 0;
 #pragma unroll
         for (int h = 0; h < kHeld; ++h) {
-            if (c + h * kStep >= a.width) break;
-            float v[kN];
-            LoadStretch<T, kN, kVector>(row, c + h * kStep, lane, a.width, v);
-#pragma unroll
-            for (int i = 0; i < kN; ++i) {
-                held[h][i] = FromFloat<T>(v[i]);
-                top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
-            }
+            top = held[h].Top(top);
+            sHeld[h][threadIdx.x] = held[h];
         }
         for (long long c0 = c + (long long)kHeld * kStep; c0 < a.width; c0 += kStep) {
-            float v[kN];
-            LoadStretch<T, kN, kVector>(row, (int)c0, lane, a.width, v);
-#pragma unroll
-            for (int i = 0; i < kN; ++i) top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+            Raw<T> more;
+            more.template Load<kVector>(row, (int)c0, lane, a.width);
+            top = more.Top(top);
         }
-        top = __reduce_max_sync(0xffffffffu, top);
-        if constexpr (kWarps > 1) {
-            if (lane == 0) sTop[warp] = top;
-            __syncthreads();
-            top = __reduce_max_sync(0xffffffffu, lane < kWarps ? sTop[warp - within + lane] : 0u);
-            __syncthreads();  // a CTA's warps are all at one row
+        top = __reduce_max_sync(0xffffffffu, Raw<T>::TopOf(top));
+        if constexpr (kWarps > 1) {  // two places in turn: one is written while others may still read the other
+            if (lane == 0) sTop[turn][warp] = top;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / kWarps), "n"(32 * kWarps) : "memory");
+            top = __reduce_max_sync(0xffffffffu, lane < kWarps ? sTop[turn][warp - within + lane] : 0u);
         }
-        const EightBits eight(top);
-        auto store = [&](int8_t *to, int c0, const int (&q)[kN]) {
-            if constexpr (kVector) {
-                const int at = c0 + lane * kN;
-                if (at + kN <= a.width) {
-                    uint2 words;
-                    words.x = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | q[3] << 24;
-                    words.y = (q[4] & 255) | (q[5] & 255) << 8 | (q[6] & 255) << 16 | q[7] << 24;
-                    *reinterpret_cast<uint2 *>(to + at) = words;
-                } else {
-#pragma unroll
-                    for (int i = 0; i < kN; ++i)
-                        if (at + i < a.width) to[at + i] = (int8_t)q[i];
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < kN; ++i)
-                    if (c0 + 32 * i + lane < a.width) to[c0 + 32 * i + lane] = (int8_t)q[i];
-            }
-        };
+        const EightBits<T> eight(top);
         for (int e0 = entries.x; e0 < entries.y; e0 += 32) {
             const int many = min(32, entries.y - e0);
-            int mine = 0;
-            if (kOrdered && lane < many) mine = __ldg(a.places + e0 + lane);
-            auto write = [&](int c0, const float (&v)[kN]) {
-                int q[kN], zeros[kN] = {};
-#pragma unroll
-                for (int i = 0; i < kN; ++i) q[i] = eight.Of(v[i]);
+            if (kOrdered && e0 > entries.x) mine = lane < many ? __ldg(a.places + e0 + lane) : 0;
+            long long c0 = c;
+#pragma unroll 1
+            for (int h = 0; c0 < a.width; ++h, c0 += kStep) {
+                Raw<T> raw;
+                if (h < kHeld) raw = sHeld[h][threadIdx.x];
+                else raw.template Load<kVector>(row, (int)c0, lane, a.width);
+                float v[8];
+                raw.Floats(v);
+                const uint2 words = eight.Of(v);
                 if constexpr (kOrdered) {
                     for (int j = 0; j < many; ++j) {
                         const int place = __shfl_sync(0xffffffffu, mine, j);
-                        int8_t *const to = static_cast<int8_t *>(a.out) + place * a.ldOut;
-                        if (place < end) store(to, c0, q);
-                        else store(to, c0, zeros);
+                        StoreBytes<kVector>(static_cast<int8_t *>(a.out) + place * a.ldOut, (int)c0, lane, a.width, place < end ? words : make_uint2(0, 0));
                     }
                 } else {
-                    store(static_cast<int8_t *>(a.out) + t * a.ldOut, c0, q);
+                    StoreBytes<kVector>(static_cast<int8_t *>(a.out) + t * a.ldOut, (int)c0, lane, a.width, words);
                 }
-            };
-#pragma unroll
-            for (int h = 0; h < kHeld; ++h) {
-                if (c + h * kStep >= a.width) break;
-                float v[kN];
-#pragma unroll
-                for (int i = 0; i < kN; ++i) v[i] = ToFloat(held[h][i]);
-                write(c + h * kStep, v);
-            }
-            for (long long c0 = c + (long long)kHeld * kStep; c0 < a.width; c0 += kStep) {
-                float v[kN];
-                LoadStretch<T, kN, kVector>(row, (int)c0, lane, a.width, v);
-                write((int)c0, v);
             }
             if (within == 0) {
-                if (!kOrdered && lane == 0) a.scales[t] = eight.scale;
-                if (kOrdered && lane < many) a.scales[mine] = mine < end ? eight.scale : 0.0f;
+                if (!kOrdered && lane == 0) a.scales[t] = eight.Scale();
+                if (kOrdered && lane < many) a.scales[mine] = mine < end ? eight.Scale() : 0.0f;
             }
         }
     }
@@ -311,10 +352,10 @@ inline RowsArgs RowsOf(const aclsparseSpMatDescr *R, const void *buffer, uint64_
     a.experts = (int)R->cols;
     return a;
 }
-// CTAs for so many warps' work: as many as there are, or eight to an SM.
-inline unsigned RowsBlocks(long long warps)
+// CTAs for so many warps' work: as many as there are, or as many as the SMs hold.
+inline unsigned RowsBlocks(long long warps, int ctas)
 {
-    return (unsigned)std::min<long long>((warps + kRowsWarps - 1) / kRowsWarps, (long long)b200sp_sm_count() * 8);
+    return (unsigned)std::min<long long>((warps + kRowsWarps - 1) / kRowsWarps, (long long)b200sp_sm_count() * ctas);
 }
 // Calls f with types of elements; two unlike types of 16 bits are refused before.
 template <typename First, typename F> cudaError_t WithSecond(First x, aclDataType second, F &&f)
@@ -357,17 +398,20 @@ inline aclsparseStatus_t CheckBytes(const aclsparseDnMatDescr *m)
     return m->values == nullptr ? ACL_SPARSE_STATUS_INVALID_VALUE : ACL_SPARSE_STATUS_SUCCESS;
 }
 
+template <typename T, bool kOrdered, int kWarps> cudaError_t LaunchQuantise(const RowsArgs &a, bool vectors, cudaStream_t stream)
+{
+    b200sp_note_launches(1);
+    const unsigned blocks = RowsBlocks(a.tokens * kWarps, kQuantiseCtas<T>);
+    return vectors ? b200sp::LaunchChained(QuantiseKernel<T, true, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a)
+                   : b200sp::LaunchChained(QuantiseKernel<T, false, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a);
+}
+// As many warps as keep a row in registers; where there are few rows, a CTA's.
 template <typename T, bool kOrdered> cudaError_t LaunchQuantise(const RowsArgs &a, bool vectors, cudaStream_t stream)
 {
-    // A warp for a row, as long as it keeps the row in registers and there are rows for all SMs; else a CTA.
-    const bool cta = a.width > 32 * 128 / (int)sizeof(T) || a.tokens < (long long)b200sp_sm_count() * kRowsWarps;
-    const unsigned blocks = RowsBlocks(cta ? a.tokens * kRowsWarps : a.tokens);
-    b200sp_note_launches(1);
-    if (cta)
-        return vectors ? b200sp::LaunchChained(QuantiseKernel<T, true, kRowsWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a)
-                       : b200sp::LaunchChained(QuantiseKernel<T, false, kRowsWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a);
-    return vectors ? b200sp::LaunchChained(QuantiseKernel<T, true, 1, kOrdered>, blocks, kRowsThreads, 0, stream, a)
-                   : b200sp::LaunchChained(QuantiseKernel<T, false, 1, kOrdered>, blocks, kRowsThreads, 0, stream, a);
+    if (a.width > 4096 || a.tokens < (long long)b200sp_sm_count() * 4) return LaunchQuantise<T, kOrdered, 8>(a, vectors, stream);
+    if (a.width > 2048) return LaunchQuantise<T, kOrdered, 4>(a, vectors, stream);
+    if (a.width > 1024) return LaunchQuantise<T, kOrdered, 2>(a, vectors, stream);
+    return LaunchQuantise<T, kOrdered, 1>(a, vectors, stream);
 }
 inline bool QuantiseVectors(const aclsparseDnMatDescr *X, const aclsparseDnMatDescr *Q)
 {

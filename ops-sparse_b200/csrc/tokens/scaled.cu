@@ -140,11 +140,15 @@ aclsparseStatus_t Product(const char *call, const aclsparseContext *handle, Scal
     const Operand w = Aligned(W, &room, handle->stream, a, a.header != nullptr ? a.n : 0);
     if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, call);
     a.colsMost = TileColumns(a.rows, a.experts);
-    a.box = std::min(a.colsMost, 64);
+    const bool pair = a.colsMost >= 128 && a.n > kTileRows;
+    a.box = std::min(pair ? a.colsMost / 2 : a.colsMost, 64);
     CUtensorMap mapW, mapX;
     if (!MapOfBytes(&mapW, w.values, W->cols, W->rows, w.ld, kTileRows) || !MapOfBytes(&mapX, x.values, X->cols, X->rows, x.ld, a.box))
         return ACL_SPARSE_STATUS_INTERNAL_ERROR;
-    const cudaError_t e = WithType(Y->valueType, [&](auto out) { return LaunchScaled<decltype(out)>(a, mapW, mapX, handle->stream); });
+    const cudaError_t e = WithType(Y->valueType, [&](auto out) {
+        using Out = decltype(out);
+        return pair ? LaunchScaled<Out, true>(a, mapW, mapX, handle->stream) : LaunchScaled<Out, false>(a, mapW, mapX, handle->stream);
+    });
     return Finished(e, call);
 }
 

@@ -41,41 +41,57 @@ struct ScaledArgs {
 __device__ int gScaledError = 0;
 constexpr int kScaledWaitRanOut = 1, kScaledNoOrder = 2;
 
-__device__ __forceinline__ void CopyTile2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar)
+// bar: of this CTA, or with a pair of the first.
+template <bool kPair> __device__ __forceinline__ void CopyTile2(uint32_t dst, const CUtensorMap *map, int x, int y, uint32_t bar)
 {
-    asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
-                 "r"(x), "r"(y), "r"(bar)
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+                     "l"(map), "r"(x), "r"(y), "r"(bar)
+                     : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cta.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst), "l"(map),
+                     "r"(x), "r"(y), "r"(bar)
+                     : "memory");
 }
-__device__ __forceinline__ void MmaI8(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add)
+template <bool kPair> __device__ __forceinline__ void MmaI8(uint32_t d, uint64_t a, uint64_t b, uint32_t instr, bool add)
 {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
-                 : "memory");
+    if constexpr (kPair)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                     : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                     "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(instr), "r"((uint32_t)add)
+                     : "memory");
 }
 
 // A sum times its scales.  The product of the scales comes first, which is a normal number and leaves room for the sum if each of them lies
 // between 2^-63 and 2^48 (or is 0); `plain` says that all of a warp's do.  Else the whole is taken in f64.
 constexpr float kScaleLow = 0x1p-63f, kScaleHigh = 0x1p48f;
 __device__ __forceinline__ bool PlainScale(float s) { return s == 0.0f || (s >= kScaleLow && s <= kScaleHigh); }
-__device__ __noinline__ float ScaledFar(int sum, float x, float w, float alpha)
+// v: sums in, results out; x: the lane's, of which sum i wants lane i's.
+__device__ __forceinline__ void Scale32(float (&v)[32], float x, float w, float alpha, bool plain)
 {
-    return (float)((double)alpha * ((double)x * (double)w * (double)sum));
-}
-__device__ __forceinline__ float Scaled(int sum, float x, float w, float alpha, bool plain)
-{
-    return plain ? alpha * (x * w * (float)sum) : ScaledFar(sum, x, w, alpha);
+    if (plain) {
+#pragma unroll
+        for (int i = 0; i < 32; ++i) v[i] = alpha * (__shfl_sync(0xffffffffu, x, i) * w * (float)__float_as_int(v[i]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; ++i)
+            v[i] = (float)((double)alpha * ((double)__shfl_sync(0xffffffffu, x, i) * (double)w * (double)__float_as_int(v[i])));
+    }
 }
 
 // Channels [f0, f0 + 128) of the expert for rows [first, first + many) of X.
 struct ScaledTile {
     int expert, f0, first, many, wide, steps;  // wide: many, in whole units
 };
-struct ScaledTiles {
+template <bool kPair> struct ScaledTiles {
     const ScaledArgs &a;
     const int *sStart, *sOffset;  // as in Tiles
     int fTiles;
-    static constexpr int kUnit = 16;
+    static constexpr int kHigh = kPair ? 2 * kTileRows : kTileRows;
+    static constexpr int kUnit = kPair ? 32 : 16;  // that many rows of X at least, by the shapes of kind::i8
     __device__ __forceinline__ int Count(int lo, int hi) const { return fTiles * ((hi - lo + a.colsMost - 1) / a.colsMost); }
     __device__ __forceinline__ ScaledTile At(int t) const
     {
@@ -91,7 +107,7 @@ struct ScaledTiles {
         const int across = (count + a.colsMost - 1) / a.colsMost;
         const int per = ((count + across - 1) / across + kUnit - 1) / kUnit * kUnit;
         const int c = within % across * per;
-        m.f0 = within / across * kTileRows;
+        m.f0 = within / across * kHigh;
         m.first = from + c;
         m.many = min(per, count - c);
         m.wide = (m.many + kUnit - 1) / kUnit * kUnit;
@@ -100,7 +116,7 @@ struct ScaledTiles {
     }
 };
 
-template <typename Out>
+template <typename Out, bool kPair>
 __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const ScaledArgs a, const __grid_constant__ CUtensorMap mapW,
                                                                       const __grid_constant__ CUtensorMap mapX)
 {
@@ -109,10 +125,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     __shared__ uint32_t sTmem;
     __shared__ int sStart[kMaxExperts + 2], sOffset[kMaxExperts + 2];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int rank = kPair ? (int)(blockIdx.x & 1) : 0, first = kPair ? blockIdx.x >> 1 : blockIdx.x, step = kPair ? gridDim.x >> 1 : gridDim.x;
     const uint32_t base = (Shared(sRaw) + 1023u) & ~1023u;
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if constexpr (kPair) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(512) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     if (tid == 0) {
         for (int s = 0; s < a.stages; ++s) {
@@ -121,13 +143,13 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
         }
         for (int i = 0; i < 2; ++i) {
             BarInit(sDone + i, 1);
-            BarInit(sFree + i, kStoreWarps);
+            BarInit(sFree + i, kPair ? 2 * kStoreWarps : kStoreWarps);
         }
         BarInit(&sLast, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b200sp::WaitForPrevious();
-    const ScaledTiles tiles{a, sStart, sOffset, (a.n + kTileRows - 1) / kTileRows};
+    const ScaledTiles<kPair> tiles{a, sStart, sOffset, (a.n + ScaledTiles<kPair>::kHigh - 1) / ScaledTiles<kPair>::kHigh};
     const int groups = a.header != nullptr ? a.experts + 1 : 1;
     const bool ordered = a.header == nullptr || StartsWith(a.header, a.mark, a.number);
     for (int e = tid; e <= groups; e += kTileThreads) sOffset[e] = a.header == nullptr ? e * a.rows : ordered ? __ldg(a.offsets + e) : 0;
@@ -148,9 +170,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = sTmem;
-    const int all = ordered ? sStart[groups] : 0, first = blockIdx.x, step = gridDim.x;
+    const int all = ordered ? sStart[groups] : 0;
     if (!ordered && tid == 0 && blockIdx.x == 0) atomicMax(&gScaledError, kScaledNoOrder);
     bool failed = false;
 
@@ -158,27 +181,28 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
         Ring ring;
         for (int t = first; t < all && !failed; t += step) {
             const ScaledTile m = tiles.At(t);
-            const int row = m.expert * a.n + m.f0, copies = (m.wide + a.box - 1) / a.box;
+            const int share = kPair ? m.wide / 2 : m.wide, copies = (share + a.box - 1) / a.box;
+            const int rowW = m.expert * a.n + m.f0 + rank * kTileRows, rowX = m.first + rank * share;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
                 if (ring.round > 0 && !__all_sync(0xffffffffu, BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles))) {
                     failed = true;
                     break;
                 }
-                const uint32_t at = base + ring.stage * a.stageBytes, full = Shared(sFull + ring.stage);
+                const uint32_t at = base + ring.stage * a.stageBytes, full = kPair ? LeadersBar(sFull + ring.stage) : Shared(sFull + ring.stage);
                 if (Elected()) {
-                    BarExpect(sFull + ring.stage, kTileWBytes + copies * a.box * kTileDepth + a.extraTx);
-                    CopyTile2(at, &mapW, k * kTileDepth, row, full);
+                    if (rank == 0) BarExpect(sFull + ring.stage, (kPair ? 2 : 1) * (kTileWBytes + copies * a.box * kTileDepth) + a.extraTx);
+                    CopyTile2<kPair>(at, &mapW, k * kTileDepth, rowW, full);
                     for (int i = 0; i < copies; ++i)
-                        CopyTile2(at + kTileWBytes + i * a.box * kTileDepth, &mapX, k * kTileDepth, m.first + i * a.box, full);
+                        CopyTile2<kPair>(at + kTileWBytes + i * a.box * kTileDepth, &mapX, k * kTileDepth, rowX + i * a.box, full);
                 }
                 __syncwarp();
             }
         }
-        if (failed)  // copies on their way: a bounded chance to land
+        if (failed && rank == 0)  // copies on their way: a bounded chance to land
             for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
                 if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
-    } else if (warp == 1) {
-        constexpr uint32_t kInstr = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(kTileRows >> 4) << 24;  // signed operands, sums of 32 bits
+    } else if (warp == 1 && rank == 0) {
+        constexpr uint32_t kInstr = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(ScaledTiles<kPair>::kHigh >> 4) << 24;  // signed operands, sums of 32 bits
         const bool elected = Elected();
         const uint64_t firstW = OperandAt(base, false), firstX = OperandAt(base + kTileWBytes, false);
         Ring ring;
@@ -201,18 +225,18 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                 const uint32_t at = (uint32_t)(ring.stage * a.stageBytes) >> 4;
                 if (elected) {
 #pragma unroll
-                    for (int i = 0; i < kTileDepth / 32; ++i) MmaI8(to, firstW + (at + 2 * i), firstX + (at + 2 * i), shape, k > 0 || i > 0);
-                    MmaCommit<false>(sEmpty + ring.stage);
-                    if (k == m.steps - 1) MmaCommit<false>(sDone + acc);
+                    for (int i = 0; i < kTileDepth / 32; ++i) MmaI8<kPair>(to, firstW + (at + 2 * i), firstX + (at + 2 * i), shape, k > 0 || i > 0);
+                    MmaCommit<kPair>(sEmpty + ring.stage);
+                    if (k == m.steps - 1) MmaCommit<kPair>(sDone + acc);
                 }
                 __syncwarp();
             }
             ++tile;
         }
-        if (elected) MmaCommit<false>(&sLast);  // when every product started here is complete, also after a failure
+        if (elected) MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
         __syncwarp();
         (void)BarWait(&sLast, 0, a.waitCycles);
-    } else {
+    } else if (warp >= kFirstStore) {
         const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;  // the lanes of tensor memory that the warp may read; every other 32 columns
         const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
         Out *const sOut = reinterpret_cast<Out *>(sRaw + (base - Shared(sRaw)) + a.stages * a.stageBytes) + (warp - kFirstStore) * 1024;
@@ -220,9 +244,16 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
         int tile = 0;
         for (int t = first; t < all; t += step) {
             const ScaledTile m = tiles.At(t);
-            const int f0 = m.f0 + quarter * 32;  // the warp's 32 channels
+            const int f0 = m.f0 + rank * kTileRows + quarter * 32;  // the warp's 32 channels
             const bool in = f0 + lane < a.n;
+            // what the results are scaled by is asked for before they are waited for
             const float w = m.steps > 0 && in ? __ldg(a.scalesW + (long long)m.expert * a.n + f0 + lane) : 0.0f;
+            float scales[kTileColsMost / 64];
+#pragma unroll
+            for (int i = 0; i < kTileColsMost / 64; ++i) {
+                const int c = half * 32 + 64 * i + lane;
+                scales[i] = m.steps > 0 && c < m.many ? __ldg(a.scalesX + m.first + c) : 0.0f;
+            }
             const int acc = tile & 1, turn = tile >> 1;
             if (m.steps > 0) {
                 if (!BarWaitWarp(sDone + acc, (uint32_t)turn & 1u, a.waitCycles + m.steps * kTileStepCycles)) {
@@ -234,21 +265,22 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
             }
             const uint32_t from = tmem + ((uint32_t)quarter << 21) + acc * kTileColsMost;
             for (int c0 = half * 32; c0 < m.many; c0 += 64) {
-                float sums[32] = {};
-                if (m.steps > 0) LoadColumns32(from + c0, sums);
+                float v[32] = {};
+                const float x = scales[0];
+#pragma unroll
+                for (int i = 1; i < kTileColsMost / 64; ++i) scales[i - 1] = scales[i];
+                if (m.steps > 0) {
+                    LoadColumns32(from + c0, v);
+                    Scale32(v, x, w, alpha, __all_sync(0xffffffffu, PlainScale(w) && PlainScale(x)));
+                }
                 const int live = min(32, m.many - c0);
-                const float x = m.steps > 0 && lane < live ? __ldg(a.scalesX + m.first + c0 + lane) : 0.0f;
-                const bool plain = __all_sync(0xffffffffu, PlainScale(w) && PlainScale(x));
                 Out *const to = out + (long long)(m.first + c0) * a.ldy + f0;
                 if (sizeof(Out) == 2 && a.vectors && beta == 0.0f) {
                     if constexpr (sizeof(Out) == 2) {
                         // Through shared memory, so that 16 bytes of a row are stored at once and a row's 32 channels side by side.
                         constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const float xi = __shfl_sync(0xffffffffu, x, i);
-                            sOut[32 * i + lane] = FromFloat<Out>(m.steps > 0 ? Scaled(__float_as_int(sums[i]), xi, w, alpha, plain) : 0.0f);
-                        }
+                        for (int i = 0; i < 32; ++i) sOut[32 * i + lane] = FromFloat<Out>(v[i]);
                         __syncwarp();
 #pragma unroll
                         for (int i = 0; i < kPieces; ++i) {
@@ -270,9 +302,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                         for (int i = 0; i < 8; ++i) old[i] = beta != 0.0f && in && g + i < live ? ToFloat(to[(g + i) * a.ldy + lane]) : 0.0f;
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {
-                            const float xi = __shfl_sync(0xffffffffu, x, g + i);
-                            const float v = m.steps > 0 ? Scaled(__float_as_int(sums[g + i]), xi, w, alpha, plain) : 0.0f;
-                            if (in && g + i < live) to[(g + i) * a.ldy + lane] = FromFloat<Out>(beta != 0.0f ? fmaf(beta, old[i], v) : v);
+                            const float u = beta != 0.0f ? fmaf(beta, old[i], v[g + i]) : v[g + i];
+                            if (in && g + i < live) to[(g + i) * a.ldy + lane] = FromFloat<Out>(u);
                         }
                     }
                 }
@@ -280,7 +311,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
             if (m.steps > 0) {  // all that this warp reads of the accumulator
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
-                if (lane == 0) BarArriveAt(Shared(sFree + acc));
+                if (lane == 0) BarArriveAt(kPair ? LeadersBar(sFree + acc) : Shared(sFree + acc));
             }
         }
     }
@@ -288,7 +319,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     if (failed) atomicMax(&gScaledError, kScaledWaitRanOut);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.
+    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 0) {
+        if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+        else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+    }
 }
 
 // ---------------------------------------------------------------- host
@@ -307,15 +343,28 @@ inline bool MapOfBytes(CUtensorMap *map, const void *at, long long cols, long lo
 long long gScaledWaitCycles = kTileWaitCycles;
 unsigned gScaledExtraTx = 0;
 
-template <typename Out> cudaError_t LaunchScaled(ScaledArgs a, const CUtensorMap &mapW, const CUtensorMap &mapX, cudaStream_t stream)
+template <typename Out, bool kPair>
+cudaError_t LaunchScaled(ScaledArgs a, const CUtensorMap &mapW, const CUtensorMap &mapX, cudaStream_t stream)
 {
-    a.stageBytes = kTileWBytes + a.colsMost * kTileDepth;
+    a.stageBytes = kTileWBytes + a.colsMost * kTileDepth / (kPair ? 2 : 1);
     a.stages = std::min(kTileShared / a.stageBytes, kTileStagesMost);
     a.waitCycles = gScaledWaitCycles;
     a.extraTx = gScaledExtraTx;
-    const cudaError_t e = AllowShared<ScaledTensorKernel<Out>>(kTileShared + kTileStoreBytes<Out> + 1024);
+    const cudaError_t e = AllowShared<ScaledTensorKernel<Out, kPair>>(kTileShared + kTileStoreBytes<Out> + 1024);
     if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(b200sp_sm_count() / 2 * 2));
+    cfg.blockDim = dim3(kTileThreads);
+    cfg.dynamicSmemBytes = (size_t)(a.stages * a.stageBytes + kTileStoreBytes<Out> + 1024);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = 2;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = kPair ? 2 : 1;
     b200sp_note_launches(1);
-    return b200sp::LaunchChained(ScaledTensorKernel<Out>, (unsigned)b200sp_sm_count(), kTileThreads,
-                                 (size_t)(a.stages * a.stageBytes + kTileStoreBytes<Out> + 1024), stream, a, mapW, mapX);
+    return cudaLaunchKernelEx(&cfg, ScaledTensorKernel<Out, kPair>, a, mapW, mapX);
 }
