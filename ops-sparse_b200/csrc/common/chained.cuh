@@ -6,7 +6,7 @@
 // launch latency and the ramp-up are hidden.  A predecessor that is not a kernel (a copy, a memset) is waited for as
 // always.  Back-to-back products of a 4096-row matrix: 4.1 us apart with ordinary launches, 2.5 us (what the host takes to
 // issue one) with these; 2 entries in each of 805,575 rows: 16.4 and 10.4 us.
-// No kernel gives the next one leave to start earlier (griddepcontrol.launch_dependents): the waiting CTAs then hold the
+// No kernel of several waves gives the next one leave to start earlier (griddepcontrol.launch_dependents): the waiting CTAs then hold the
 // slots that the CTAs of a grid of several waves are about to take (14.0 us on the second example, and 16.3 instead of
 // 11.2 us on 27,197 rows of which 300 are long).
 #pragma once
@@ -17,6 +17,8 @@
 
 namespace b200sp {
 
+// For grids that leave most SMs idle: the next kernel is set up beside this one, and still waits for its end.
+__device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 template <typename... Params, typename... Args>

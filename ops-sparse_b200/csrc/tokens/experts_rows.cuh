@@ -25,6 +25,7 @@ struct RowsArgs {
     Scalars sc;
 };
 
+constexpr unsigned kFewCtas = 74;  // leave half of the SMs alone
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
 constexpr int kDispatchCtas = 5, kCombineCtas = 4, kGradCtas = 2;  // resident on an SM: what their registers allow
 template <typename T> constexpr int kQuantiseCtas = sizeof(T) == 4 ? 4 : 6;
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel
     constexpr int kStep = kWarps * kStretch, kTokens = kRowsWarps / kWarps;
     __shared__ uint32_t sTop[2][kRowsWarps];
     __shared__ Raw<T> sHeld[kHeld][kRowsThreads];
+    if (gridDim.x <= kFewCtas) b200sp::LetNextStart();
     b200sp::WaitForPrevious();
     if (kOrdered && !HasOrder(a)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, within = warp % kWarps, c = within * kStretch;

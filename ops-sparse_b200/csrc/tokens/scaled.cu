@@ -1,5 +1,6 @@
 // b200spScaledMM, b200spExpertsScaledMM: products in 8-bit integers with a scale for each row and channel.
 #include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 #include "b200sp_rows.h"
@@ -124,6 +125,48 @@ int TileColumns(long long rows, long long experts)
     return cols;
 }
 
+// How a product without experts is computed: by tiles, of a CTA, a pair of them, or a cluster that shares a tile's steps, or without tiles.  An estimate of the
+// time of every way, us, fitted to 620 products of 1 to 2048 rows by 512 x 4096 to 8192 x 4096 bytes; of the ways with tiles it takes one within 0.5 % of the
+// fastest on average and 5 % at worst.  (512 rows of 4096 by 4096: pairs 17, clusters of two 37; 16 rows: clusters of four 10, whole tiles 15; one row:
+// clusters 10, without tiles 6.6; four rows 10 and 12.6; 8 rows of 1024 by 1024: 6.4 and 3.7.)
+enum FormKind { kWhole, kPairs, kShared, kFew };
+struct Form {
+    FormKind kind;
+    int cols, split;
+};
+Form FormOf(long long rows, long long n, long long depth)
+{
+    const double steps = (double)((depth + kTileDepth - 1) / kTileDepth);
+    const int sms = b200sp_sm_count();
+    Form best{kWhole, 16, 1};
+    const double bytes = (double)n * (double)depth;
+    // W from DRAM, and the products of four bytes
+    double least = rows <= 16 ? 2.6 + bytes * (1.4e-7 + 1.2e-7 * (double)rows) : 1e300;
+    if (rows <= 16) best.kind = kFew;
+    const auto offer = [&](double us, FormKind kind, int cols, int split) {
+        us += 1e-7 * bytes;
+        if (us < least) least = us, best = {kind, cols, split};
+    };
+    for (int cols = 16; cols <= kTileColsMost; cols *= 2) {
+        const long long across = (rows + cols - 1) / cols, tiles = (n + kTileRows - 1) / kTileRows * across;
+        const auto wide = [&](int unit) { return (double)(((rows + across - 1) / across + unit - 1) / unit * unit); };
+        const auto whole = [&](double start, double step, double perRow, double store, double waves, double columns) {
+            return start + waves * std::max(steps * (step + perRow * columns), store + 0.0078 * columns) + 0.0078 * columns;
+        };
+        offer(whole(4.3, 0.309, 0.0004, 1.47, (double)((tiles + sms - 1) / sms), wide(16)), kWhole, cols, 1);
+        const long long pairs = (n + 2 * kTileRows - 1) / (2 * kTileRows) * across;
+        if (cols >= 64 && n > kTileRows)
+            offer(whole(4.7, 0.319, 0.0003, 1.35, (double)((pairs + sms / 2 - 1) / (sms / 2)), wide(32)), kPairs, cols, 1);
+        for (int split = 2; split <= kSplitMost && split <= steps; split *= 2) {
+            // one CTA an SM, and clusters that the SMs' groups hold side by side
+            if (tiles * split > (split == 2 ? sms : split == 4 ? 136 : 112)) break;
+            const double columns = (double)std::min<long long>(cols, (rows + 15) / 16 * 16);
+            offer(4.46 + std::ceil(steps / split) * (0.309 + 0.0004 * columns) + (0.0074 + 0.1685 / split) * columns, kShared, cols, split);
+        }
+    }
+    return best;
+}
+
 aclsparseStatus_t Product(const char *call, const aclsparseContext *handle, ScaledArgs a, const aclsparseDnMatDescr *X,
                           const aclsparseDnVecDescr *scalesX, const aclsparseDnMatDescr *W, const aclsparseDnVecDescr *scalesW,
                           const aclsparseDnMatDescr *Y, char *room)
@@ -139,15 +182,29 @@ aclsparseStatus_t Product(const char *call, const aclsparseContext *handle, Scal
     const Operand x = Aligned(X, &room, handle->stream, a, 0);
     const Operand w = Aligned(W, &room, handle->stream, a, a.header != nullptr ? a.n : 0);
     if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, call);
-    a.colsMost = TileColumns(a.rows, a.experts);
-    const bool pair = a.colsMost >= 128 && a.n > kTileRows;
-    a.box = std::min(pair ? a.colsMost / 2 : a.colsMost, 64);
+    Form form = a.header == nullptr ? FormOf(a.rows, a.n, X->cols) : Form{kWhole, TileColumns(a.rows, a.experts), 1};
+    if (a.header != nullptr) {
+        if (form.cols >= 128 && a.n > kTileRows) form.kind = kPairs;
+        // hardly an expert has more than one
+        if (4ll * a.rows <= a.experts) form.kind = kFew;
+    }
+    if (form.kind == kFew) {
+        const long long chunks = a.header == nullptr ? (a.rows + kFewRowsX - 1) / kFewRowsX : a.rows;
+        const cudaError_t e = WithType(Y->valueType, [&](auto out) {
+            return LaunchFew<decltype(out)>(a, x.values, x.ld, w.values, w.ld, (int)X->cols, chunks, handle->stream);
+        });
+        return Finished(e, call);
+    }
+    a.colsMost = form.cols;
+    a.split = form.split;
+    a.box = form.kind == kPairs ? a.colsMost / 2 : a.colsMost;
     CUtensorMap mapW, mapX;
     if (!MapOfBytes(&mapW, w.values, W->cols, W->rows, w.ld, kTileRows) || !MapOfBytes(&mapX, x.values, X->cols, X->rows, x.ld, a.box))
         return ACL_SPARSE_STATUS_INTERNAL_ERROR;
     const cudaError_t e = WithType(Y->valueType, [&](auto out) {
         using Out = decltype(out);
-        return pair ? LaunchScaled<Out, true>(a, mapW, mapX, handle->stream) : LaunchScaled<Out, false>(a, mapW, mapX, handle->stream);
+        if (form.kind == kShared) return LaunchSplit<Out>(a, mapW, mapX, handle->stream);
+        return form.kind == kPairs ? LaunchScaled<Out, true>(a, mapW, mapX, handle->stream) : LaunchScaled<Out, false>(a, mapW, mapX, handle->stream);
     });
     return Finished(e, call);
 }

@@ -33,6 +33,7 @@ struct ScaledArgs {
     long long ldy;
     int vectors;             // rows of Y start on 16 bytes
     int stages, stageBytes;
+    int split, tmemColumns;  // of ScaledSplitKernel
     Scalars sc;
     long long waitCycles;
     unsigned extraTx;        // 0 outside the wait test
@@ -82,6 +83,48 @@ __device__ __forceinline__ void Scale32(float (&v)[32], float x, float w, float 
     }
 }
 
+// The experts' first rows (and that of the group of no expert; without experts there is one group of all rows), and the first of the units of work,
+// `count` of a number of rows, of each.  By a whole CTA, synchronised when the first are there, of which warp 0 is the last.  False without an order.
+template <typename Count>
+__device__ __forceinline__ bool WorkTable(const ScaledArgs &a, int groups, int threads, int *sStart, int *sOffset, Count &&count)
+{
+    const int tid = threadIdx.x, lane = tid & 31;
+    const bool ordered = a.header == nullptr || StartsWith(a.header, a.mark, a.number);
+    for (int e = tid; e <= groups; e += threads) sOffset[e] = a.header == nullptr ? e * a.rows : ordered ? __ldg(a.offsets + e) : 0;
+    __syncthreads();
+    if (tid < 32) {
+        int run = 0;
+        for (int e0 = 0; e0 <= groups; e0 += 32) {
+            const int own = e0 + lane < groups ? count(sOffset[e0 + lane + 1] - sOffset[e0 + lane]) : 0;
+            int incl = own;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += up;
+            }
+            if (e0 + lane <= groups) sStart[e0 + lane] = run + incl - own;
+            run += __shfl_sync(0xffffffffu, incl, 31);
+        }
+    }
+    return ordered;
+}
+// The group that a unit of work is of.
+__device__ __forceinline__ int GroupOf(const int *sStart, int groups, int unit)
+{
+    int lo = 0, hi = groups;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (sStart[mid] <= unit) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float Scaled(int sum, float x, float w, float alpha)
+{
+    return PlainScale(w) && PlainScale(x) ? alpha * (x * w * (float)sum) : (float)((double)alpha * ((double)x * (double)w * (double)sum));
+}
+
 // Channels [f0, f0 + 128) of the expert for rows [first, first + many) of X.
 struct ScaledTile {
     int expert, f0, first, many, wide, steps;  // wide: many, in whole units
@@ -92,15 +135,10 @@ template <bool kPair> struct ScaledTiles {
     int fTiles;
     static constexpr int kHigh = kPair ? 2 * kTileRows : kTileRows;
     static constexpr int kUnit = kPair ? 32 : 16;  // that many rows of X at least, by the shapes of kind::i8
-    __device__ __forceinline__ int Count(int lo, int hi) const { return fTiles * ((hi - lo + a.colsMost - 1) / a.colsMost); }
+    __device__ __forceinline__ int Count(int rows) const { return fTiles * ((rows + a.colsMost - 1) / a.colsMost); }
     __device__ __forceinline__ ScaledTile At(int t) const
     {
-        int lo = 0, hi = a.header != nullptr ? a.experts + 1 : 1;
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (sStart[mid] <= t) lo = mid;
-            else hi = mid;
-        }
+        const int lo = GroupOf(sStart, a.header != nullptr ? a.experts + 1 : 1, t);
         ScaledTile m;
         m.expert = lo;
         const int within = t - sStart[lo], from = sOffset[lo], count = sOffset[lo + 1] - from;
@@ -151,23 +189,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     b200sp::WaitForPrevious();
     const ScaledTiles<kPair> tiles{a, sStart, sOffset, (a.n + ScaledTiles<kPair>::kHigh - 1) / ScaledTiles<kPair>::kHigh};
     const int groups = a.header != nullptr ? a.experts + 1 : 1;
-    const bool ordered = a.header == nullptr || StartsWith(a.header, a.mark, a.number);
-    for (int e = tid; e <= groups; e += kTileThreads) sOffset[e] = a.header == nullptr ? e * a.rows : ordered ? __ldg(a.offsets + e) : 0;
-    __syncthreads();
-    if (warp == 0) {
-        int run = 0;
-        for (int e0 = 0; e0 <= groups; e0 += 32) {
-            const int own = e0 + lane < groups ? tiles.Count(sOffset[e0 + lane], sOffset[e0 + lane + 1]) : 0;
-            int incl = own;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += up;
-            }
-            if (e0 + lane <= groups) sStart[e0 + lane] = run + incl - own;
-            run += __shfl_sync(0xffffffffu, incl, 31);
-        }
-    }
+    const bool ordered = WorkTable(a, groups, kTileThreads, sStart, sOffset, [&](int count) { return tiles.Count(count); });
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
@@ -327,6 +349,241 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     }
 }
 
+// Few tiles, as when some tokens are served: the CTAs of a cluster share the steps of one tile, and each adds up a part of its columns from
+// all their accumulators, through shared memory.  Sums of whole numbers may be regrouped.
+constexpr int kSplitThreads = 256, kSplitMost = 8;  // CTAs of a cluster: the portable most
+
+__device__ __forceinline__ int LoadRemote(uint32_t at, int rank)
+{
+    uint32_t there;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(there) : "r"(at), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(there) : "memory");
+    return v;
+}
+
+template <typename Out>
+__global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const ScaledArgs a, const __grid_constant__ CUtensorMap mapW,
+                                                                      const __grid_constant__ CUtensorMap mapX)
+{
+    extern __shared__ unsigned char sRaw[];
+    __shared__ uint64_t sFull[kTileStagesMost], sEmpty[kTileStagesMost], sDone;
+    __shared__ uint32_t sTmem;
+    __shared__ int sFailed;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int split = a.split, rank = (int)(blockIdx.x % split), tile = (int)(blockIdx.x / split);
+    const uint32_t base = (Shared(sRaw) + 1023u) & ~1023u;
+    if (warp == 0) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(Shared(&sTmem)), "r"(a.tmemColumns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    if (tid == 32) {
+        for (int s = 0; s < a.stages; ++s) {
+            BarInit(sFull + s, 1);
+            BarInit(sEmpty + s, 1);
+        }
+        BarInit(&sDone, 1);
+        sFailed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    b200sp::WaitForPrevious();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = sTmem;
+    // Tiles side by side along the rows of X first.
+    const int across = (a.rows + a.colsMost - 1) / a.colsMost, f0 = tile / across * kTileRows, first = tile % across * a.colsMost;
+    const int many = min(a.colsMost, a.rows - first), wide = (many + 15) / 16 * 16;
+    const int from = (int)((long long)a.steps * rank / split), to = (int)((long long)a.steps * (rank + 1) / split);
+    bool failed = false;
+    if (warp == 0) {
+        Ring ring;
+        const int copies = (wide + a.box - 1) / a.box;
+        for (int k = from; k < to; ++k, ring.Next(a.stages)) {
+            if (ring.round > 0 && !__all_sync(0xffffffffu, BarWait(sEmpty + ring.stage, ring.Emptied(), a.waitCycles))) {
+                failed = true;
+                break;
+            }
+            const uint32_t at = base + ring.stage * a.stageBytes, full = Shared(sFull + ring.stage);
+            if (Elected()) {
+                BarExpect(sFull + ring.stage, kTileWBytes + copies * a.box * kTileDepth + a.extraTx);
+                CopyTile2<false>(at, &mapW, k * kTileDepth, f0, full);
+                for (int i = 0; i < copies; ++i)
+                    CopyTile2<false>(at + kTileWBytes + i * a.box * kTileDepth, &mapX, k * kTileDepth, first + i * a.box, full);
+            }
+            __syncwarp();
+        }
+        if (failed)  // copies on their way: a bounded chance to land
+            for (int i = 0; i < a.stages; ++i, ring.Next(a.stages))
+                if (ring.round > 0) (void)BarWait(sFull + ring.stage, ring.Emptied(), a.waitCycles);
+    } else if (warp == 1) {
+        const uint32_t shape = 2u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(wide >> 3) << 17 | (uint32_t)(kTileRows >> 4) << 24;
+        const bool elected = Elected();
+        const uint64_t firstW = OperandAt(base, false), firstX = OperandAt(base + kTileWBytes, false);
+        Ring ring;
+        for (int k = from; k < to; ++k, ring.Next(a.stages)) {
+            if (!__all_sync(0xffffffffu, BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles))) {
+                failed = true;
+                break;
+            }
+            const uint32_t at = (uint32_t)(ring.stage * a.stageBytes) >> 4;
+            if (elected) {
+#pragma unroll
+                for (int i = 0; i < kTileDepth / 32; ++i) MmaI8<false>(tmem, firstW + (at + 2 * i), firstX + (at + 2 * i), shape, k > from || i > 0);
+                MmaCommit<false>(sEmpty + ring.stage);
+            }
+            __syncwarp();
+        }
+        if (elected) MmaCommit<false>(&sDone);  // when every product started here is complete, also after a failure
+    }
+    __syncwarp();
+    if (!BarWaitWarp(&sDone, 0, 2 * a.waitCycles + (to - from) * kTileStepCycles)) failed = true;  // longer than the waits above
+    if (failed) sFailed = 1;
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    __syncthreads();
+    // The sums, a column of 128 channels after the other, where the stages were.
+    const int quarter = warp & 3;
+    if (sFailed == 0) {
+        for (int c0 = (warp >> 2) * 32; c0 < wide; c0 += 64) {
+            float v[32];
+            LoadColumns32(tmem + ((uint32_t)quarter << 21) + c0, v);
+            int *const sums = reinterpret_cast<int *>(sRaw + (base - Shared(sRaw))) + c0 * kTileRows + quarter * 32 + lane;
+#pragma unroll
+            for (int i = 0; i < 32; ++i)
+                if (c0 + i < wide) sums[i * kTileRows] = __float_as_int(v[i]);
+        }
+    }
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    int bad = 0;
+    for (int r = 0; r < split; ++r) bad |= LoadRemote(Shared(&sFailed), r);
+    if (bad == 0) {
+        const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
+        const int f = tid & (kTileRows - 1), channel = f0 + f;
+        const bool in = channel < a.n;
+        const float w = in ? __ldg(a.scalesW + channel) : 0.0f;
+        constexpr int kTogether = 4;  // columns whose sums are asked for at once
+        for (int c0 = rank * 2 + (tid >> 7); c0 < many; c0 += 2 * split * kTogether) {
+            int sum[kTogether] = {};
+            float x[kTogether], old[kTogether];
+#pragma unroll
+            for (int u = 0; u < kTogether; ++u) {
+                const int c = min(c0 + 2 * split * u, many - 1);
+                const uint32_t at = base + (c * kTileRows + f) * 4;
+                for (int r = 0; r < split; ++r) sum[u] += LoadRemote(at, r);
+                x[u] = __ldg(a.scalesX + first + c);
+                old[u] = beta != 0.0f && in ? ToFloat(static_cast<const Out *>(a.y)[(long long)(first + c) * a.ldy + channel]) : 0.0f;
+            }
+#pragma unroll
+            for (int u = 0; u < kTogether; ++u) {
+                const int c = c0 + 2 * split * u;
+                const float v = Scaled(sum[u], x[u], w, alpha);
+                if (in && c < many)
+                    static_cast<Out *>(a.y)[(long long)(first + c) * a.ldy + channel] = FromFloat<Out>(beta != 0.0f ? fmaf(beta, old[u], v) : v);
+            }
+        }
+    } else if (rank == 0 && tid == 0) {
+        atomicMax(&gScaledError, kScaledWaitRanOut);
+    }
+    // The others may still read this CTA's sums.
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmemColumns) : "memory");
+}
+
+// Few rows at a matrix: no tile, but warps at two rows of W and of X.  What moves is W, in pieces of 512 bytes of a row, of which a warp asks for eight at
+// once; rows of X come from L1.  Products of four bytes at a time (dp4a).  With `parts` > 1 so many warps share an item's columns.
+// One row of 4096 by 4096: 6.6 us, of which 2.5 are a launch and its ends; 2.6 is the matrix at the copy rate.  Other shapes, rows of X x of W, pieces: 1 x 2, 8
+// 9.3 us, 1 x 4, 4 8.4, 2 x 4, 2 8.6.  Eight rows of X are bound by the rate of dp4a, some 10 lanes a clock and SM: 19 us; by the int8 products of a
+// warp (mma.sync) 10.3, but one row 8.6, and small matrices half as long again.
+constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewPiece = 512, kFewRowsX = 2;
+
+template <typename Out>
+__global__ void __launch_bounds__(kFewThreads) ScaledFewKernel(const ScaledArgs a, const int8_t *__restrict__ matX, long long ldx,
+                                                               const int8_t *__restrict__ matW, long long ldw, int depth, int parts)
+{
+    constexpr int kM = kFewRowsX, kR = 2, kAhead = 4;
+    __shared__ int sStart[kMaxExperts + 2], sOffset[kMaxExperts + 2];
+    __shared__ int sPart[2][kFewWarps][kM * kR];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    b200sp::WaitForPrevious();
+    const int groups = a.header != nullptr ? a.experts + 1 : 1, perRow = (a.n + kR - 1) / kR;
+    const bool ordered = WorkTable(a, groups, kFewThreads, sStart, sOffset, [&](int rows) { return (rows + kM - 1) / kM * perRow; });
+    __syncthreads();
+    if (!ordered) {
+        if (tid == 0 && blockIdx.x == 0) atomicMax(&gScaledError, kScaledNoOrder);
+        return;
+    }
+    const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
+    const int all = sStart[groups], side = kFewWarps / parts, part = warp % parts;
+    const int pieces = depth / 16, rest = depth % 16;  // of 16 bytes
+    int turn = 0;
+    for (long long item = (long long)blockIdx.x * side + warp / parts; item < all; item += (long long)gridDim.x * side, turn ^= 1) {
+        const int expert = GroupOf(sStart, groups, (int)item), within = (int)item - sStart[expert];
+        const int chunk = within / perRow, f0 = (within - chunk * perRow) * kR;
+        const int first = sOffset[expert] + chunk * kM, many = min(kM, sOffset[expert + 1] - first);
+        const bool live = expert < a.experts;
+        int sum[kR][kM] = {};
+        if (live) {
+            const int8_t *w[kR];
+#pragma unroll
+            for (int r = 0; r < kR; ++r) w[r] = matW + ((long long)expert * a.n + min(f0 + r, a.n - 1)) * ldw;
+            const int8_t *const x = matX + first * ldx;
+            for (int p0 = part * 32 + lane; p0 < pieces; p0 += parts * 32 * kAhead) {
+                int4 v[kAhead][kR];
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int p = p0 + u * parts * 32;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r)
+                        v[u][r] = p < pieces ? __ldg(reinterpret_cast<const int4 *>(w[r]) + p) : make_int4(0, 0, 0, 0);
+                }
+#pragma unroll
+                for (int u = 0; u < kAhead; ++u) {
+                    const int p = min(p0 + u * parts * 32, pieces - 1);
+#pragma unroll
+                    for (int m = 0; m < kM; ++m) {
+                        if (m >= many) break;
+                        const int4 y = __ldg(reinterpret_cast<const int4 *>(x + m * ldx) + p);
+#pragma unroll
+                        for (int r = 0; r < kR; ++r)
+                            sum[r][m] = __dp4a(v[u][r].w, y.w, __dp4a(v[u][r].z, y.z, __dp4a(v[u][r].y, y.y, __dp4a(v[u][r].x, y.x, sum[r][m]))));
+                    }
+                }
+            }
+            if (part == 0 && lane < rest) {  // the last columns, which are no whole piece
+                const int c = pieces * 16 + lane;
+#pragma unroll
+                for (int m = 0; m < kM; ++m) {
+                    if (m >= many) break;
+#pragma unroll
+                    for (int r = 0; r < kR; ++r) sum[r][m] += (int)w[r][c] * (int)x[m * ldx + c];
+                }
+            }
+        }
+        int mine = 0;  // of lane m * kR + r: the sum of row m and channel r
+#pragma unroll
+        for (int m = 0; m < kM; ++m)
+#pragma unroll
+            for (int r = 0; r < kR; ++r) {
+                const int total = __reduce_add_sync(0xffffffffu, sum[r][m]);
+                if (lane == m * kR + r) mine = total;
+            }
+        if (parts > 1) {  // two places in turn: one is written while others may still read the other
+            if (lane < kM * kR) sPart[turn][warp][lane] = mine;
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / parts), "r"(32 * parts) : "memory");
+            if (part != 0) continue;
+            mine = 0;
+            if (lane < kM * kR)
+                for (int i = 0; i < parts; ++i) mine += sPart[turn][warp + i][lane];
+        }
+        const int m = lane / kR, f = f0 + lane % kR;
+        if (m >= many || f >= a.n) continue;
+        float v = 0.0f;
+        if (live) v = Scaled(mine, __ldg(a.scalesX + first + m), __ldg(a.scalesW + (long long)expert * a.n + f), alpha);
+        Out *const to = static_cast<Out *>(a.y) + (first + m) * a.ldy + f;
+        *to = FromFloat<Out>(beta != 0.0f ? fmaf(beta, ToFloat(*to), v) : v);
+    }
+}
+
 // ---------------------------------------------------------------- host
 
 // Rows of bytes, `high` of them by 128, swizzled; what is past the last column or row arrives as zeros.
@@ -367,4 +624,45 @@ cudaError_t LaunchScaled(ScaledArgs a, const CUtensorMap &mapW, const CUtensorMa
     cfg.numAttrs = kPair ? 2 : 1;
     b200sp_note_launches(1);
     return cudaLaunchKernelEx(&cfg, ScaledTensorKernel<Out, kPair>, a, mapW, mapX);
+}
+
+template <typename Out> cudaError_t LaunchSplit(ScaledArgs a, const CUtensorMap &mapW, const CUtensorMap &mapX, cudaStream_t stream)
+{
+    a.stageBytes = kTileWBytes + a.colsMost * kTileDepth;
+    a.stages = std::min({kTileShared / a.stageBytes, kTileStagesMost, (a.steps + a.split - 1) / a.split});
+    a.tmemColumns = std::max(32, a.colsMost);
+    a.waitCycles = gScaledWaitCycles;
+    a.extraTx = gScaledExtraTx;
+    const cudaError_t e = AllowShared<ScaledSplitKernel<Out>>(kTileShared + 1024);
+    if (e != cudaSuccess) return e;
+    const long long tiles = (long long)((a.n + kTileRows - 1) / kTileRows) * ((a.rows + a.colsMost - 1) / a.colsMost);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)(tiles * a.split));
+    cfg.blockDim = dim3(kSplitThreads);
+    cfg.dynamicSmemBytes = (size_t)(std::max(a.stages * a.stageBytes, a.colsMost * kTileRows * 4) + 1024);
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[2] = {};
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)a.split;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    b200sp_note_launches(1);
+    return cudaLaunchKernelEx(&cfg, ScaledSplitKernel<Out>, a, mapW, mapX);
+}
+
+// chunks: of two rows of X, at most.
+template <typename Out>
+cudaError_t LaunchFew(const ScaledArgs &a, const void *x, long long ldx, const void *w, long long ldw, int depth, long long chunks, cudaStream_t stream)
+{
+    // Warps for all SMs: items that are fewer are shared, as long as a warp has columns of its own.
+    const long long items = (a.n + 1) / 2 * chunks, warps = (long long)b200sp_sm_count() * 24;
+    int parts = 1;
+    while (parts < kFewWarps && items * parts < warps && depth > parts * kFewPiece) parts *= 2;
+    const long long ctas = (items * parts + kFewWarps - 1) / kFewWarps;
+    b200sp_note_launches(1);
+    return b200sp::LaunchChained(ScaledFewKernel<Out>, (unsigned)std::min(ctas, (long long)b200sp_sm_count() * 4), kFewThreads, 0, stream, a,
+                                 static_cast<const int8_t *>(x), ldx, static_cast<const int8_t *>(w), ldw, depth, parts);
 }
