@@ -141,8 +141,9 @@ Form FormOf(long long rows, long long n, long long depth)
     Form best{kWhole, 16, 1};
     const double bytes = (double)n * (double)depth;
     // W from DRAM, and the products of four bytes
-    double least = rows <= 16 ? 2.6 + bytes * (1.4e-7 + 1.2e-7 * (double)rows) : 1e300;
-    if (rows <= 16) best.kind = kFew;
+    const bool few = rows <= 16 && n < 1 << 26;  // its items are counted in 31 bits
+    double least = few ? 2.6 + bytes * (1.4e-7 + 1.2e-7 * (double)rows) : 1e300;
+    if (few) best.kind = kFew;
     const auto offer = [&](double us, FormKind kind, int cols, int split) {
         us += 1e-7 * bytes;
         if (us < least) least = us, best = {kind, cols, split};

@@ -16,8 +16,8 @@ constexpr int kTileShared = 192 << 10;              // for stages
 constexpr int kTileStagesMost = 12;
 constexpr int kStoreWarps = 8, kFirstStore = 2;     // warp 0 requests, 1 multiplies, 2 ... 9 store
 constexpr int kTileThreads = 32 * (kFirstStore + kStoreWarps);
-// 32 x 32 results of each storing warp, of 16 bits; 32 of f32 are 128 bytes side by side as the lanes have them.
-template <typename Out> constexpr int kTileStoreBytes = sizeof(Out) == 2 ? kStoreWarps * 32 * 32 * 2 : 0;
+// 32 rows of Y by 128 channels, of 16 bits, of each half of the storing warps; 32 of f32 are 128 bytes side by side as the lanes have them.
+template <typename Out> constexpr int kTileStoreBytes = sizeof(Out) == 2 ? 2 * 32 * kTileRows * 2 : 0;
 constexpr long long kTileWaitCycles = 4'000'000'000;  // two seconds
 constexpr long long kTileStepCycles = 4096;           // and so many for each step of a tile, for its results
 
@@ -70,6 +70,19 @@ template <bool kPair> __device__ __forceinline__ void MmaI8(uint32_t d, uint64_t
 // between 2^-63 and 2^48 (or is 0); `plain` says that all of a warp's do.  Else the whole is taken in f64.
 constexpr float kScaleLow = 0x1p-63f, kScaleHigh = 0x1p48f;
 __device__ __forceinline__ bool PlainScale(float s) { return s == 0.0f || (s >= kScaleLow && s <= kScaleHigh); }
+// The four warps of a half of a tile's columns.
+__device__ __forceinline__ void StoreBarrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+// Whether a wait ran out for none of them: they go on together, or not at all.
+__device__ __forceinline__ bool StoreAgree(int half, bool ok)
+{
+    uint32_t all;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(all)
+                 : "r"((uint32_t)ok), "r"(1 + half)
+                 : "memory");
+    return all != 0;
+}
+
 // v: sums in, results out; x: the lane's, of which sum i wants lane i's.
 __device__ __forceinline__ void Scale32(float (&v)[32], float x, float w, float alpha, bool plain)
 {
@@ -261,7 +274,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     } else if (warp >= kFirstStore) {
         const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;  // the lanes of tensor memory that the warp may read; every other 32 columns
         const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
-        Out *const sOut = reinterpret_cast<Out *>(sRaw + (base - Shared(sRaw)) + a.stages * a.stageBytes) + (warp - kFirstStore) * 1024;
+        Out *const sOut = reinterpret_cast<Out *>(sRaw + (base - Shared(sRaw)) + a.stages * a.stageBytes) + half * (32 * kTileRows);
         Out *const out = static_cast<Out *>(a.y);
         int tile = 0;
         for (int t = first; t < all; t += step) {
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
             }
             const int acc = tile & 1, turn = tile >> 1;
             if (m.steps > 0) {
-                if (!BarWaitWarp(sDone + acc, (uint32_t)turn & 1u, a.waitCycles + m.steps * kTileStepCycles)) {
+                if (!StoreAgree(half, BarWaitWarp(sDone + acc, (uint32_t)turn & 1u, a.waitCycles + m.steps * kTileStepCycles))) {
                     failed = true;
                     break;
                 }
@@ -299,21 +312,20 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                 Out *const to = out + (long long)(m.first + c0) * a.ldy + f0;
                 if (sizeof(Out) == 2 && a.vectors && beta == 0.0f) {
                     if constexpr (sizeof(Out) == 2) {
-                        // Through shared memory, so that 16 bytes of a row are stored at once and a row's 32 channels side by side.
-                        constexpr int kN = 16 / (int)sizeof(Out), kPieces = 32 / kN;
+                        // Through shared memory, where the four warps of these columns meet, so that 256 bytes of a row are stored side by side.
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) sOut[32 * i + lane] = FromFloat<Out>(v[i]);
-                        __syncwarp();
+                        for (int i = 0; i < 32; ++i) sOut[kTileRows * i + quarter * 32 + lane] = FromFloat<Out>(v[i]);
+                        StoreBarrier(half);
 #pragma unroll
-                        for (int i = 0; i < kPieces; ++i) {
-                            const int c = (32 * i + lane) / kPieces, at = lane % kPieces * kN;
-                            const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + 32 * c + at);
-                            Out *const row = to + c * a.ldy + at;
-                            if (c < live && f0 + at + kN <= a.n) *reinterpret_cast<uint4 *>(row) = piece;
+                        for (int i = 0; i < 4; ++i) {
+                            const int c = quarter * 8 + 2 * i + (lane >> 4), at = (lane & 15) * 8, channel = f0 - quarter * 32 + at;
+                            const uint4 piece = *reinterpret_cast<const uint4 *>(sOut + kTileRows * c + at);
+                            Out *const row = to + c * a.ldy - quarter * 32 + at;
+                            if (c < live && channel + 8 <= a.n) *reinterpret_cast<uint4 *>(row) = piece;
                             else if (c < live)  // the last channels
-                                for (int j = 0; f0 + at + j < a.n; ++j) row[j] = sOut[32 * c + at + j];
+                                for (int j = 0; channel + j < a.n; ++j) row[j] = sOut[kTileRows * c + at + j];
                         }
-                        __syncwarp();
+                        StoreBarrier(half);
                     }
                 } else {
                     // A channel a lane.  What is read is asked for before anything is stored.

@@ -285,27 +285,29 @@ def test_scaled_product(pkg, handle, many, depth, channels, out, alpha, beta, pa
     assert torch.equal(outside(y, whole), kept)
 
 
-def test_scaled_extreme_scales(pkg, handle):
-    """Scales whose product f32 cannot hold, of sums that bring the result back, and some that are not finite."""
+@pytest.mark.parametrize("many,depth,channels", [(2, 512, 200), (40, 512, 200), (40, 128, 30000), (320, 512, 200)],
+                         ids=["rows", "clusters", "whole", "pairs"])
+def test_scaled_extreme_scales(pkg, handle, many, depth, channels):
+    """Scales whose product f32 cannot hold, of sums that bring the result back, and some that are not finite, in every way of the product."""
     from ops_sparse_b200 import api
     g = gen(77)
-    x, w = eights(g, 40, 512), eights(g, 200, 512)
+    x, w = eights(g, many, depth), eights(g, channels, depth)
     x[:, 0] = 127
-    sx = torch.tensor([1e-30, 1e-25, 1e25, 1e38, 1.0, 0.0, 1e-38, 1e-45], device="cuda").repeat(5)
-    sw = torch.tensor([1e-20, 1e-10, 1.0, 1e10, 1e-25, 1e-38, 3e38, 0.0], device="cuda").repeat(25)
+    sx = torch.tensor([1e-30, 1e25, 1e-25, 1e38, 1.0, 0.0, 1e-38, 1e-45], device="cuda").repeat(many // 8 + 1)[:many].contiguous()
+    sw = torch.tensor([1e-20, 1e-10, 1.0, 1e10, 1e-25, 1e-38, 3e38, 0.0], device="cuda").repeat(channels // 8)
     for alpha in (1.0, 1e15, 1e-15):
-        y = torch.empty(40, 200, device="cuda")
+        y = torch.empty(many, channels, device="cuda")
         api.scaled_mm(handle, mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), mat(api, y), alpha=alpha)
         torch.cuda.synchronize()
         want, _ = rows.scaled(x, sx, w, sw, float(torch.tensor(alpha)), 0.0, y)
         held = want.float().double()  # infinite where f32 is
         ref.close(y, torch.where(want.abs() > 3.4028235e38, held, want), ref.rounding(y.dtype, want) + 5 * F32 * want.abs())
-    sx = torch.ones(40, device="cuda")
-    sx[3], sx[4] = math.nan, math.inf
-    y = torch.empty(40, 200, dtype=torch.float16, device="cuda")
-    api.scaled_mm(handle, mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(torch.ones(200, device="cuda")), mat(api, y))
-    torch.cuda.synchronize()
-    assert bool(y[3].isnan().all()) and bool((~y[4].isfinite()).all()) and not bool(y[[0, 1, 2, 5, 39]].isnan().any())
+    sx = torch.ones(many, device="cuda")
+    sx[0], sx[1] = math.nan, math.inf
+    y = torch.empty(many, channels, dtype=torch.float16, device="cuda")
+    api.scaled_mm(handle, mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(torch.full((channels,), 1e-3, device="cuda")), mat(api, y))
+    no_error(pkg)
+    assert bool(y[0].isnan().all()) and bool((~y[1].isfinite()).all()) and not bool(y[2:].isnan().any())
 
 
 EXPERTS = [  # tokens, experts, k, depth, channels, out, alpha, beta, pad, wild, ragged
@@ -318,6 +320,9 @@ EXPERTS = [  # tokens, experts, k, depth, channels, out, alpha, beta, pad, wild,
     (700, 1024, 2, 48, 9, "f32", 1.0, -1.0, 0, 0.05, True),
     (50, 3, 1, 64, 70, "f32", 1.0, 0.0, 0, 1.0, False),  # no entry has an expert
     (1500, 2, 1, 640, 264, "f32", 1.0, 0.0, 0, 0.0, False),
+    (1, 64, 8, 2048, 130, "bf16", 1.0, 0.0, 0, 0.0, False),  # hardly an expert with more than one entry: no tiles
+    (1, 100, 9, 777, 33, "f32", 2.0, 0.5, 7, 0.3, False),
+    (8, 1024, 24, 520, 31, "f16", 1e-3, 0.0, 0, 0.1, True),
 ]
 
 
@@ -344,3 +349,327 @@ def test_experts_scaled_product(pkg, handle, tokens, experts, k, depth, channels
     api.experts_scaled_mm(handle, R, X, api.DnVec(sx), W, api.DnVec(sw), Y, alpha, beta, buffer=buffer)
     no_error(pkg)
     ref.close(y, want, ref.rounding(y.dtype, want) + 5 * F32 * size)
+
+
+# ---------------------------------------------------------------- used together, on streams and in graphs
+
+def test_layer_in_eight_bits(pkg, handle):
+    """Routing, rows to 8 bits in the order of the experts, two products with the experts' matrices, the weighted sum: one run."""
+    from ops_sparse_b200 import api
+    g = gen(11)
+    tokens, experts, k, d, n = 70, 12, 3, 144, 200
+    logits, x = torch.randn(tokens, experts, generator=g, device="cuda"), matrix(g, tokens, d, "bf16")[0]
+    R = api.CsrMatrix(torch.empty(tokens + 1, dtype=torch.int32, device="cuda"), torch.empty(tokens * k, dtype=torch.int32, device="cuda"),
+                      torch.empty(tokens * k, device="cuda"), tokens, experts)
+    weights = [torch.randn(experts * rows_, cols, generator=g, device="cuda") for rows_, cols in ((n, d), (d, n))]
+    held, scales = [], []
+    for w in weights:
+        held.append(torch.empty(w.shape, dtype=torch.int8, device="cuda"))
+        scales.append(torch.empty(len(w), device="cuda"))
+        api.quantise_rows(handle, mat(api, w), mat(api, held[-1]), api.DnVec(scales[-1]))
+    q, p = (torch.empty(tokens * k, c, dtype=torch.int8, device="cuda") for c in (d, n))
+    sq, sp = torch.empty(tokens * k, device="cuda"), torch.empty(tokens * k, device="cuda")
+    y, z, out = torch.empty(tokens * k, n, device="cuda"), torch.empty(tokens * k, d, device="cuda"), torch.empty_like(x)
+    Q, P, Y, Z = mat(api, q), mat(api, p), mat(api, y), mat(api, z)
+    W = [mat(api, w) for w in held]
+    size = max(api.experts_scaled_mm_buffer_size(handle, R, Q, W[0], Y), api.experts_scaled_mm_buffer_size(handle, R, P, W[1], Z))
+    buffer = torch.empty(size, dtype=torch.uint8, device="cuda")
+    api.route(handle, api.RouteRule(), mat(api, logits), None, R)
+    api.experts_preprocess(handle, R, buffer)
+    api.experts_quantise(handle, R, mat(api, x), Q, api.DnVec(sq), buffer=buffer)
+    api.experts_scaled_mm(handle, R, Q, api.DnVec(sq), W[0], api.DnVec(scales[0]), Y, buffer=buffer)
+    torch.nn.functional.silu(y, inplace=True)
+    api.quantise_rows(handle, Y, P, api.DnVec(sp))
+    api.experts_scaled_mm(handle, R, P, api.DnVec(sp), W[1], api.DnVec(scales[1]), Z, buffer=buffer)
+    api.experts_combine(handle, R, Z, mat(api, out), buffer=buffer)
+    no_error(pkg)
+    # step by step in 64 bits, every step from what the one before left
+    order, places, starts = rows.order_of(R.col_ind, experts)
+    token = ref.rows_of(R.row_ptr, tokens * k)[order]
+    want_q, want_s = rows.quantise(x)
+    assert torch.equal(q.cpu(), want_q[token]) and torch.equal(sq.double().cpu(), want_s[token])
+    want_p, want_sp = rows.quantise(y)
+    assert torch.equal(p.cpu(), want_p) and torch.equal(sp.double().cpu(), want_sp)
+    for e in range(experts):
+        a, b = int(starts[e]), int(starts[e + 1])
+        want, many = rows.scaled(p[a:b], sp[a:b], held[1][e * d:(e + 1) * d], scales[1][e * d:(e + 1) * d], 1.0, 0.0, z[a:b])
+        ref.close(z[a:b], want, 5 * F32 * many)
+    want, many, _ = rows.combine(R.row_ptr, R.col_ind, R.values, z, experts, 1.0, 0.0, out)
+    ref.close(out, want, ref.rounding(out.dtype, want) + 5 * F32 * many)
+
+
+def test_dispatch_combine_gradients_of_a_layer(pkg, handle):
+    """Dispatch, a product of every expert, combine, and back: against 64 bits' automatic differentiation."""
+    from ops_sparse_b200 import api
+    g = gen(12)
+    tokens, experts, k, d = 45, 7, 2, 40
+    R = routed(api, g, tokens, experts, k)
+    x, w, d_out = torch.randn(tokens, d, generator=g, device="cuda"), torch.randn(experts, d, d, generator=g, device="cuda"), torch.randn(tokens, d, generator=g, device="cuda")
+    buffer, starts = ordered(api, handle, R), torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    new = lambda rows_: torch.empty(rows_, d, device="cuda")  # noqa: E731
+    s, z, out, d_z, d_x, d_values = new(R.nnz), new(R.nnz), new(tokens), new(R.nnz), new(tokens), torch.empty(R.nnz, device="cuda")
+    api.experts_dispatch(handle, R, mat(api, x), mat(api, s), offsets=api.DnVec(starts), buffer=buffer)
+    at = starts.tolist()
+    for e in range(experts):
+        z[at[e]:at[e + 1]] = (s[at[e]:at[e + 1]].double() @ w[e].double()).float()
+    api.experts_combine(handle, R, mat(api, z), mat(api, out), buffer=buffer)
+    api.experts_combine_grad(handle, R, mat(api, d_out), mat(api, z), mat(api, d_z), api.DnVec(d_values), buffer=buffer)
+    d_s = torch.cat([(d_z[at[e]:at[e + 1]].double() @ w[e].double().T).float() for e in range(experts)])
+    api.experts_combine(handle, R, mat(api, d_s), mat(api, d_x), weighted=False, buffer=buffer)
+    no_error(pkg)
+    leaf, values = x.double().requires_grad_(), R.values.double().requires_grad_()
+    token = torch.arange(tokens, device="cuda").repeat_interleave(k)
+    terms = values[:, None] * torch.einsum("ih,ihf->if", leaf[token], w.double()[R.col_ind.long()])
+    total = torch.zeros(tokens, d, dtype=torch.float64, device="cuda").index_add(0, token, terms)
+    gx, gv = torch.autograd.grad((total * d_out.double()).sum(), (leaf, values))
+    # sums of d products, whose terms are f32 roundings of sums of k (or d) terms: all of them within 6 d of 2^-24 of the largest sizes
+    total, gx, gv = total.detach(), gx.detach(), gv.detach()
+    size = float(d_out.abs().max()) * float(w.abs().max()) * d * max(1.0, float(R.values.abs().max()))
+    assert float((out.double() - total).abs().max()) <= 6 * F32 * k * size * float(x.abs().max())
+    assert float((d_x.double() - gx).abs().max()) <= 6 * F32 * d * size
+    assert float((d_values.double() - gv).abs().max()) <= 6 * F32 * d * d * size * float(x.abs().max())
+
+
+def small(api, handle, g, tokens=40, experts=6, k=2, n=48, d=64, h=None):
+    """A routing with everything that the calls take, and all of them as functions of a handle."""
+    R = routed(api, g, tokens, experts, k)
+    x, s = matrix(g, tokens, d, "f32")[0], matrix(g, R.nnz, d, "f32")[0]
+    w, sw = eights(g, experts * n, d), torch.rand(experts * n, generator=g, device="cuda")
+    made = {"S": torch.zeros(R.nnz, d, device="cuda"), "out": torch.zeros(tokens, d, device="cuda"), "dS": torch.zeros(R.nnz, d, device="cuda"),
+            "dv": torch.zeros(R.nnz, device="cuda"), "q": torch.zeros(R.nnz, d, dtype=torch.int8, device="cuda"),
+            "sq": torch.zeros(R.nnz, device="cuda"), "y": torch.zeros(R.nnz, n, device="cuda"),
+            "starts": torch.zeros(experts + 1, dtype=torch.int32, device="cuda")}
+    q, W = mat(api, made["q"]), mat(api, w)
+    vec = {name: api.DnVec(made[name]) for name in ("dv", "sq", "starts")}
+    m = {name: mat(api, made[name]) for name in ("S", "out", "dS", "y")}
+    X, S, SW = mat(api, x), mat(api, s), api.DnVec(sw)
+    buffer = torch.zeros(api.experts_scaled_mm_buffer_size(handle, R, q, W, m["y"]), dtype=torch.uint8, device="cuda")
+
+    def run(h):
+        api.experts_dispatch(h, R, X, m["S"], offsets=vec["starts"], buffer=buffer)
+        api.experts_combine(h, R, S, m["out"], buffer=buffer)
+        api.experts_combine_grad(h, R, X, S, m["dS"], vec["dv"], buffer=buffer)
+        api.experts_quantise(h, R, X, q, vec["sq"], buffer=buffer)
+        api.experts_scaled_mm(h, R, q, vec["sq"], W, SW, m["y"], buffer=buffer)
+
+    def check():
+        order, places, starts = rows.order_of(R.col_ind, experts)
+        token = ref.rows_of(R.row_ptr, R.nnz)
+        assert torch.equal(made["starts"].cpu(), starts) and torch.equal(made["S"].cpu(), x.cpu()[token[order]])
+        want, size, many = rows.combine(R.row_ptr, R.col_ind, R.values, s, experts, 1.0, 0.0, made["out"])
+        ref.close(made["out"], want, (many + 2) * F32 * size)
+        want, want_v, size_v = rows.combine_grad(R.row_ptr, R.col_ind, R.values, x, s, experts, 1.0, 0.0, made["dS"], made["dv"])
+        ref.close(made["dS"], want, 3 * F32 * want.abs())
+        ref.close(made["dv"], want_v, (d + 2) * F32 * size_v)
+        want_q, want_s = rows.quantise(x)
+        assert torch.equal(made["q"].cpu(), want_q[token[order]])
+        for e in range(experts):
+            a, b, c = int(starts[e]), int(starts[e + 1]), slice(e * n, (e + 1) * n)
+            want, size = rows.scaled(made["q"][a:b], want_s[token[order]][a:b], w[c], sw[c], 1.0, 0.0, made["y"][a:b])
+            ref.close(made["y"][a:b], want, 5 * F32 * size)
+
+    return R, buffer, made, run, check, (X, S, W, SW, q)
+
+
+def test_captured_and_replayed_on_other_routings(pkg, handle):
+    """A graph of the order and all that follows it, replayed on new columns, on a stream of its own."""
+    from ops_sparse_b200 import api
+    g = gen(21)
+    stream = torch.cuda.Stream()
+    h = api.Handle(stream)
+    R, buffer, made, run, check, keep = small(api, h, g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        api.experts_preprocess(h, R, buffer)
+        run(h)
+    for seed in (1, 2):
+        fresh = gen(seed)
+        other = torch.randn((40, 6), generator=fresh, device="cuda").topk(2, dim=1).indices.sort(dim=1).values
+        R.col_ind.copy_(other.to(torch.int32).flatten())
+        R.values.copy_(torch.randn(80, generator=fresh, device="cuda"))
+        torch.cuda.synchronize()
+        graph.replay()
+        no_error(pkg)
+        check()
+    h.close()
+    assert keep
+
+
+def test_order_that_has_not_been_made(pkg, handle):
+    """A captured Preprocess that has not been replayed has left no order: calls after it touch nothing and say so; replayed, they run."""
+    from ops_sparse_b200 import api
+    L = pkg.lib()
+    stream = torch.cuda.Stream()
+    h = api.Handle(stream)
+    R, buffer, made, run, check, keep = small(api, h, gen(22))
+    X, S, W, SW, q = keep
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        api.experts_preprocess(h, R, buffer)
+    L.b200sp_experts_error_clear()
+    L.b200sp_scaled_error_clear()
+    m = {name: mat(api, made[name]) for name in ("S", "out", "dS", "y")}
+    dv, sq = api.DnVec(made["dv"]), api.DnVec(made["sq"])
+    calls = [lambda: api.experts_dispatch(h, R, X, m["S"], buffer=buffer), lambda: api.experts_combine(h, R, S, m["out"], buffer=buffer),
+             lambda: api.experts_combine_grad(h, R, X, S, m["dS"], dv, buffer=buffer),
+             lambda: api.experts_quantise(h, R, X, q, sq, buffer=buffer)]
+    for call in calls:
+        call()
+        assert L.b200sp_experts_error() == 2
+        L.b200sp_experts_error_clear()
+    api.experts_scaled_mm(h, R, q, sq, W, SW, m["y"], buffer=buffer)
+    assert L.b200sp_scaled_error() == 2 and L.b200sp_experts_error() == 0
+    L.b200sp_scaled_error_clear()
+    assert all(not bool(t.any()) for t in made.values())
+    graph.replay()
+    torch.cuda.synchronize()
+    run(h)
+    no_error(pkg)
+    check()
+    h.close()
+
+
+def test_stale_order_is_refused(pkg, handle):
+    from ops_sparse_b200 import api
+    g = gen(23)
+    R, buffer, made, run, check, keep = small(api, handle, g)
+    bad = pkg.ACL_SPARSE_STATUS_INVALID_VALUE
+
+    def refused(call):
+        with pytest.raises(pkg.AclSparseError) as e:
+            call()
+        assert e.value.status == bad
+
+    refused(lambda: run(handle))  # never ordered
+    api.experts_preprocess(handle, R, buffer)
+    run(handle)
+    check()
+    api.route(handle, api.RouteRule(), api.DnMat.row_major(torch.randn(40, 6, generator=g, device="cuda")), None, R)
+    refused(lambda: run(handle))  # the routing has changed
+    api.experts_preprocess(handle, R, buffer)
+    run(handle)
+    no_error(pkg)
+    check()
+    # a copy for a product without experts is written into the buffer: the order is gone
+    x, w = eights(g, 20, 40, 1), eights(g, 30, 40)
+    y = torch.empty(20, 30, device="cuda")
+    one = torch.ones(30, device="cuda")
+    api.scaled_mm(handle, mat(api, x), api.DnVec(one[:20]), mat(api, w), api.DnVec(one), mat(api, y), buffer=buffer)
+    refused(lambda: run(handle))
+    want, size = rows.scaled(x, one[:20], w, one, 1.0, 0.0, y)
+    ref.close(y, want, 5 * F32 * size)
+
+
+def test_scalars_on_the_device(pkg, handle):
+    from ops_sparse_b200 import api
+    g = gen(24)
+    R, buffer, made, run, check, (X, S, W, SW, q) = small(api, handle, g)
+    api.experts_preprocess(handle, R, buffer)
+    run(handle)
+    alpha, beta = torch.tensor([0.5], device="cuda"), torch.tensor([-2.0], device="cuda")
+    before = {name: t.clone() for name, t in made.items()}
+    m = {name: mat(api, made[name]) for name in ("S", "out", "dS", "y")}
+    dv, sq = api.DnVec(made["dv"]), api.DnVec(made["sq"])
+    h = api.Handle()
+    h.set_pointer_mode_device(True)
+    api.experts_dispatch(h, R, X, m["S"], alpha, beta, buffer=buffer)
+    api.experts_combine(h, R, S, m["out"], alpha, beta, buffer=buffer)
+    api.experts_combine_grad(h, R, X, S, m["dS"], dv, alpha, beta, buffer=buffer)
+    api.experts_scaled_mm(h, R, q, sq, W, SW, m["y"], alpha, beta, buffer=buffer)
+    few = torch.ones(2, 48, device="cuda")
+    api.scaled_mm(h, api.DnMat(q.values[:2], 2, 64, 64), api.DnVec(made["sq"][:2]), api.DnMat(W.values[:48], 48, 64, 64), api.DnVec(SW.values[:48]),
+                  mat(api, few), alpha, beta)
+    no_error(pkg)
+    for name in ("S", "out", "dS", "dv", "y"):  # 0.5 t - 2 t, from sums that are the same bits
+        want = -1.5 * before[name].double()
+        ref.close(made[name], want, 3 * F32 * 2.5 * want.abs())
+    want, size = rows.scaled(q.values[:2], made["sq"][:2], W.values[:48], SW.values[:48], 0.5, -2.0, torch.ones(2, 48))
+    ref.close(few, want, 5 * F32 * size)
+    h.close()
+
+
+def test_same_bits_in_every_run(pkg, handle):
+    from ops_sparse_b200 import api
+    g = gen(25)
+    R, buffer, made, run, check, keep = small(api, handle, g, tokens=1500, experts=9, k=3, n=130, d=264)
+    api.experts_preprocess(handle, R, buffer)
+    run(handle)
+    torch.cuda.synchronize()
+    first = {name: t.clone() for name, t in made.items()}
+    for _ in range(3):
+        run(handle)
+        torch.cuda.synchronize()
+        assert all(torch.equal(first[name], t) for name, t in made.items())
+    assert keep
+
+
+@pytest.mark.parametrize("many,depth,channels", [(300, 2048, 600), (40, 2048, 300), (40, 512, 20000)], ids=["pairs", "clusters", "whole"])
+def test_scaled_wait_that_runs_out(pkg, handle, many, depth, channels):
+    """Every wait for a copy runs out (bytes are expected that nobody sends): the flag says so, Y is as it was, and the next product is right."""
+    from ops_sparse_b200 import api
+    L, g = pkg.lib(), gen(26)
+    x, w = eights(g, many, depth), eights(g, channels, depth)
+    sx, sw = torch.rand(many, generator=g, device="cuda"), torch.rand(channels, generator=g, device="cuda")
+    y = torch.full((many, channels), 3.0, dtype=torch.bfloat16, device="cuda")
+    args = (mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), mat(api, y))
+    L.b200sp_scaled_wait_test(200_000, 16)
+    try:
+        api.scaled_mm(handle, *args)
+        asked = L.b200sp_scaled_error()
+        left = bool((y == 3.0).all())
+    finally:
+        L.b200sp_scaled_wait_test(0, 0)
+        L.b200sp_scaled_error_clear()
+    assert asked == 1 and left
+    api.scaled_mm(handle, *args)
+    no_error(pkg)
+    want, size = rows.scaled(x, sx, w, sw, 1.0, 0.0, y)
+    ref.close(y, want, ref.rounding(y.dtype, want) + 5 * F32 * size)
+
+
+def test_rows_beyond_32_bits(pkg, handle):
+    """Rows that lie more than 2^32 bytes (and 2^31 elements) apart."""
+    from ops_sparse_b200 import api
+    g = gen(27)
+    far, width = 2 ** 30 + 16, 40
+    R = api.CsrMatrix(torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 1, 2], dtype=torch.int32, device="cuda"),
+                      torch.tensor([1.0, -2.0, 0.5, 3.0], device="cuda"), 2, 3)
+    buffer = ordered(api, handle, R)
+    s = torch.zeros(3 * far + width, dtype=torch.bfloat16, device="cuda")
+    view = s.as_strided((4, width), (far, 1))
+    x = torch.randn(2, width, generator=g, device="cuda").bfloat16()
+    S = api.DnMat(s, 4, width, far)
+    api.experts_dispatch(handle, R, mat(api, x), S, buffer=buffer)
+    torch.cuda.synchronize()
+    assert torch.equal(view.cpu(), x.cpu()[[0, 1, 0, 1]])
+    out = torch.empty(2, width, device="cuda")
+    api.experts_combine(handle, R, S, mat(api, out), buffer=buffer)
+    torch.cuda.synchronize()
+    ref.close(out, torch.stack([-1.0 * x[0].double(), 3.5 * x[1].double()]), 4 * F32 * 4 * x.double().abs())
+    d_values = torch.empty(4, device="cuda")
+    api.experts_combine_grad(handle, R, mat(api, x), S, S, api.DnVec(d_values), buffer=buffer)
+    torch.cuda.synchronize()
+    ref.close(view, torch.stack([x[0], 0.5 * x[1], -2.0 * x[0], 3.0 * x[1]]).double(), 0.01 * torch.ones(4, width))
+    del view, S, s
+    far = 2 ** 31 - 16
+    q = torch.zeros(3 * far + width, dtype=torch.int8, device="cuda")
+    view = q.as_strided((4, width), (far, 1))
+    scales = torch.empty(4, device="cuda")
+    Q = api.DnMat(q, 4, width, far)
+    api.experts_quantise(handle, R, mat(api, x), Q, api.DnVec(scales), buffer=buffer)
+    torch.cuda.synchronize()
+    want, _ = rows.quantise(x)
+    assert torch.equal(view.cpu(), want[[0, 1, 0, 1]])
+    y = torch.empty(4, 4, device="cuda")
+    api.scaled_mm(handle, Q, api.DnVec(scales), Q, api.DnVec(scales), mat(api, y))  # without tiles
+    torch.cuda.synchronize()
+    want, size = rows.scaled(view, scales, view, scales, 1.0, 0.0, y)
+    ref.close(y, want, 5 * F32 * size)
+    one = api.CsrMatrix(R.row_ptr, torch.zeros(4, dtype=torch.int32, device="cuda"), R.values, 2, 1)
+    tiles = torch.empty(4, 4, device="cuda")
+    more = ordered(api, handle, one, api.experts_scaled_mm_buffer_size(handle, one, Q, Q, mat(api, tiles)))
+    api.experts_scaled_mm(handle, one, Q, api.DnVec(scales), Q, api.DnVec(scales), mat(api, tiles), buffer=more)
+    no_error(pkg)
+    ref.close(tiles, want, 5 * F32 * size)
