@@ -2,7 +2,10 @@
 //
 // dispatch: S[place(i)] = alpha X[token(i)]; combine: out[t] = alpha sum of w_i S[place(i)]; its gradient: dS[place(i)] = alpha w_i dOut[t],
 // dw_i = alpha <dOut[t], S[place(i)]>.  All go by tokens, whose entries lie side by side in R: a token's row is read (or written) once and stays in
-// registers while the rows of its entries, which lie anywhere, are written (or read).  What bounds them is DRAM.
+// registers while the rows of its entries, which lie anywhere, are written (or read).  What bounds them is DRAM; neighbouring warps take neighbouring
+// stretches of a row, so that a row is read or written as a whole at about one time.
+// One B200, bf16, us (the bytes at the copy rate of 6550 GB/s in brackets): rows of 8192 tokens of 4096 to four of 32 experts 57 (51); the weighted sum of eight
+// of 64 experts' rows of 2048 for 8192 tokens 57 (46); its gradient, four of 32, 64 (46); one token's eight rows 4, which is a launch and the host's call.
 #pragma once
 
 struct RowsArgs {
@@ -117,7 +120,8 @@ __global__ void __launch_bounds__(kRowsThreads, kDispatchCtas) ExpertsDispatchKe
     }
 }
 
-// Rows are asked for kRowsAhead at a time, and the places of the next unit's before this one's are summed.
+// Rows are asked for kAhead at a time, and the places of the next unit's before this one's are summed: one row after the other, by a grid of more CTAs than the
+// SMs hold, took 87 us where this takes 57.  (The next unit's rows brought to L2 ahead: 61.)
 template <typename In, typename Out, bool kVector>
 __global__ void __launch_bounds__(kRowsThreads, kCombineCtas) ExpertsCombineKernel(const RowsArgs a)
 {
@@ -173,7 +177,9 @@ __global__ void __launch_bounds__(kRowsThreads, kCombineCtas) ExpertsCombineKern
     }
 }
 
-// T: of S and dS; G: of dOut.  kWarps at a token, kBatch of its entries at a time.
+// T: of S and dS; G: of dOut.  kWarps at a token, kBatch of its entries at a time, whose rows are asked for before any is stored to: 64 us where one after the
+// other takes 77.  Others: the next stretch asked for ahead 71, rows brought to L2 ahead 73, a CTA at a token of 2048 columns 85, 24 warps an SM instead of
+// 16 the same.
 template <typename T, typename G, bool kVector, int kWarps>
 __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKernel(const RowsArgs a)
 {
@@ -264,7 +270,8 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
 }
 
 // Rows in 8 bits: of tokens (kOrdered false), or every token's into the rows of its entries.  kWarps at a row, which they keep, every thread
-// what it has read, in shared memory up to 1024 elements a warp, and read again beyond.
+// what it has read, in shared memory up to 1024 elements a warp, and read again beyond.  (Kept in registers, the loop unrolled around them, it took 128 of them
+// and twice as long.)  What bounds it are instructions, 2.7 a clock: 8192 rows of 4096 bf16 27 us (15 at the copy rate), of 1024 f32 10.6 (6.4).
 template <typename T, bool kVector, int kWarps, bool kOrdered>
 __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel(const RowsArgs a)
 {

@@ -4,6 +4,12 @@
 // when single tokens are served, N shrinks and what moves is W.  With experts, whose rows lie side by side, a tile is one expert's.
 // One warp requests both operands by TMA, in rows of 128 bytes, swizzled; one starts the products; eight empty the accumulators, of which there are
 // two: the next tile is summed meanwhile.  Sums are whole numbers of 32 bits; they are scaled in f32 and rounded once.
+// Many rows go to pairs of CTAs on tiles of 256 channels, which read half as much of X; few tiles to clusters that share their steps (ScaledSplitKernel); few rows
+// to warps without tiles (ScaledFewKernel).  FormOf decides.
+// What bounds it: with many rows the tensor cores (67 % of the cycles) and what a step asks of shared memory and L2 (32 KB a CTA in some 650 clocks, of which its
+// products take 512), in long runs the power cap; with short sums the storing of the results (8000 clocks a tile).  One B200: 8192 x 4096 by 4096 bf16 out 97 us (2.8 POPS),
+// 8192 x 4096 by 8192 183 alone and 220 in runs of seconds, 32,768 x 2048 by 2048 115; the rows of 8192 tokens, four of 32 experts, 2048 x 2048 126.
+// By single CTAs on tiles of 128 channels: 5 to 10 % longer.  Results stored 64 bytes of a row at a time by two bytes a lane: twice as long as 16 a lane.
 //
 // Every wait is bounded.  One that ran out ends its warp's work, raises the flag of b200sp_scaled_error and leaves rows of the output unwritten.
 #pragma once
@@ -362,8 +368,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
 }
 
 // Few tiles, as when some tokens are served: the CTAs of a cluster share the steps of one tile, and each adds up a part of its columns from
-// all their accumulators, through shared memory.  Sums of whole numbers may be regrouped.
+// all their accumulators, through shared memory.  Sums of whole numbers may be regrouped.  61 rows of 4096 by 4096: 11.2 us, 14.4 by whole tiles; 61 of 2040 by
+// 1111 7.3 and 9.5.  What bounds it is latency: a launch, its ends and two meetings of the cluster are 5 us.
 constexpr int kSplitThreads = 256, kSplitMost = 8;  // CTAs of a cluster: the portable most
+// At least so much shared memory: not beside a CTA of the other kernels that take tensor memory, nor more of them on an SM than it has columns for.
+// Clusters (and pairs) of two streams that each wait for the tensor memory of the other would wait for ever.
+constexpr int kSplitShared = 48 << 10;
 
 __device__ __forceinline__ int LoadRemote(uint32_t at, int rank)
 {
@@ -651,7 +661,7 @@ template <typename Out> cudaError_t LaunchSplit(ScaledArgs a, const CUtensorMap 
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3((unsigned)(tiles * a.split));
     cfg.blockDim = dim3(kSplitThreads);
-    cfg.dynamicSmemBytes = (size_t)(std::max(a.stages * a.stageBytes, a.colsMost * kTileRows * 4) + 1024);
+    cfg.dynamicSmemBytes = (size_t)(std::max({a.stages * a.stageBytes, a.colsMost * kTileRows * 4, kSplitShared}) + 1024);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2] = {};
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
