@@ -51,6 +51,9 @@ __device__ __forceinline__ int2 EntriesOf(const RowsArgs &a, long long token)
     return make_int2(max(0, __ldg(a.rowPtr + token)), min(a.nnz, __ldg(a.rowPtr + token + 1)));
 }
 
+// (A row's pitch has 31 bits, so that this is one multiplication.)
+template <typename T> __device__ __forceinline__ T *RowAt(T *rows, int row, long long pitch) { return rows + (long long)row * (int)pitch; }
+
 // The entries of a token, and where the rows of the first 32 lie, a lane each; asked for ahead of the rows.
 struct TokenEntries {
     int2 range;
@@ -101,7 +104,7 @@ __global__ void __launch_bounds__(kRowsThreads, kDispatchCtas) ExpertsDispatchKe
             const int many = min(32, now.range.y - e0);
             for (int j = 0; j < many; ++j) {
                 const int place = __shfl_sync(0xffffffffu, now.place, j);
-                Out *const to = static_cast<Out *>(a.out) + place * a.ldOut;
+                Out *const to = RowAt(static_cast<Out *>(a.out), place, a.ldOut);
                 if (beta == 0.0f) {
                     if (place < end) row.template Store<kVector>(to, c0, lane, a.width);
                     else none.template Store<kVector>(to, c0, lane, a.width);
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kRowsThreads, kCombineCtas) ExpertsCombineKern
                 for (int j = 0; j < kAhead; ++j) {
                     const int place = __shfl_sync(0xffffffffu, now.place, (j0 + j) & 31);
                     in[j] = j0 + j < many && place < end;
-                    if (in[j]) raw[j].template Load<kVector>(static_cast<const In *>(a.perEntry) + place * a.ldEntry, c0, lane, a.width);
+                    if (in[j]) raw[j].template Load<kVector>(RowAt(static_cast<const In *>(a.perEntry), place, a.ldEntry), c0, lane, a.width);
                 }
 #pragma unroll
                 for (int j = 0; j < kAhead; ++j) {
@@ -218,7 +221,7 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
 #pragma unroll
                     for (int j = 0; j < kBatch; ++j) {
                         if (j < many && place[j] < end)
-                            rows[j].template Load<kVector>(static_cast<const T *>(a.perEntry) + place[j] * a.ldEntry, c0, lane, a.width);
+                            rows[j].template Load<kVector>(RowAt(static_cast<const T *>(a.perEntry), place[j], a.ldEntry), c0, lane, a.width);
                         else rows[j].Zero();
                     }
                 }
@@ -231,7 +234,7 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
 #pragma unroll
                         for (int i = 0; i < 8; ++i) dot[j] = fmaf(g[i], rows[j].At(i), dot[j]);
                     }
-                    T *const to = static_cast<T *>(a.out) + place[j] * a.ldOut;
+                    T *const to = RowAt(static_cast<T *>(a.out), place[j], a.ldOut);
                     float v[8];
 #pragma unroll
                     for (int i = 0; i < 8; ++i) v[i] = place[j] < end ? weight[j] * g[i] : 0.0f;
@@ -271,7 +274,7 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
 
 // Rows in 8 bits: of tokens (kOrdered false), or every token's into the rows of its entries.  kWarps at a row, which they keep, every thread
 // what it has read, in shared memory up to 1024 elements a warp, and read again beyond.  (Kept in registers, the loop unrolled around them, it took 128 of them
-// and twice as long.)  What bounds it are instructions, 2.7 a clock: 8192 rows of 4096 bf16 27 us (15 at the copy rate), of 1024 f32 10.6 (6.4).
+// and twice as long.)  What bounds it are the steps of a row, one after the other, and 130 instructions for 256 elements: 8192 rows of 4096 bf16 24 us (15 at the copy rate), of 1024 f32 11 (6.4).
 template <typename T, bool kVector, int kWarps, bool kOrdered>
 __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel(const RowsArgs a)
 {
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel
                 if constexpr (kOrdered) {
                     for (int j = 0; j < many; ++j) {
                         const int place = __shfl_sync(0xffffffffu, mine, j);
-                        StoreBytes<kVector>(static_cast<int8_t *>(a.out) + place * a.ldOut, (int)c0, lane, a.width, place < end ? words : make_uint2(0, 0));
+                        StoreBytes<kVector>(RowAt(static_cast<int8_t *>(a.out), place, a.ldOut), (int)c0, lane, a.width, place < end ? words : make_uint2(0, 0));
                     }
                 } else {
                     StoreBytes<kVector>(static_cast<int8_t *>(a.out) + t * a.ldOut, (int)c0, lane, a.width, words);
@@ -361,7 +364,8 @@ inline RowsArgs RowsOf(const aclsparseSpMatDescr *R, const void *buffer, uint64_
     a.experts = (int)R->cols;
     return a;
 }
-// CTAs for so many warps' work: as many as there are, or as many as the SMs hold.
+// CTAs for so many warps' work: as many as there are, or as many as the SMs hold.  (Twice to eight times as many: combine 57 -> 57 to 63 us, dispatch without
+// its order 58 -> 58 to 62.  Rounding to 8 bits, which waits for a row before it begins with the next, gains by four times as many: 27 -> 24.)
 inline unsigned RowsBlocks(long long warps, int ctas)
 {
     return (unsigned)std::min<long long>((warps + kRowsWarps - 1) / kRowsWarps, (long long)b200sp_sm_count() * ctas);
@@ -410,7 +414,7 @@ inline aclsparseStatus_t CheckBytes(const aclsparseDnMatDescr *m)
 template <typename T, bool kOrdered, int kWarps> cudaError_t LaunchQuantise(const RowsArgs &a, bool vectors, cudaStream_t stream)
 {
     b200sp_note_launches(1);
-    const unsigned blocks = RowsBlocks(a.tokens * kWarps, kQuantiseCtas<T>);
+    const unsigned blocks = RowsBlocks(a.tokens * kWarps, kQuantiseCtas<T> * 4);
     return vectors ? b200sp::LaunchChained(QuantiseKernel<T, true, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a)
                    : b200sp::LaunchChained(QuantiseKernel<T, false, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a);
 }

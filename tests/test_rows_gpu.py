@@ -673,3 +673,82 @@ def test_rows_beyond_32_bits(pkg, handle):
     api.experts_scaled_mm(handle, one, Q, api.DnVec(scales), Q, api.DnVec(scales), mat(api, tiles), buffer=more)
     no_error(pkg)
     ref.close(tiles, want, 5 * F32 * size)
+
+
+@pytest.mark.parametrize("half", ["f16", "bf16"])
+def test_rows_of_32_bits_summed_into_16(pkg, handle, half):
+    """Products' results in f32, their sum and its gradient in 16 bits; numbers that f16 cannot hold become infinite."""
+    from ops_sparse_b200 import api
+    g = gen(31)
+    R = routed(api, g, 90, 11, 3, wild=0.1, kind=half)
+    s, _ = matrix(g, R.nnz, 130, "f32", 2)
+    s[5] = 1e6
+    out, whole = matrix(g, 90, 130, half, 6)
+    buffer = ordered(api, handle, R)
+    for beta in (0.0, 1.5):
+        want, size, many = rows.combine(R.row_ptr, R.col_ind, R.values, s, 11, 2.0, beta, out)
+        held = want.to(DTYPE[half]).double()  # infinite where the type is
+        kept = outside(out, whole).clone()
+        api.experts_combine(handle, R, mat(api, s), mat(api, out), 2.0, beta, buffer=buffer)
+        no_error(pkg)
+        ref.close(out, torch.where(held.isinf(), held, want), ref.rounding(out.dtype, want) + (many + 2) * F32 * size)
+        assert torch.equal(outside(out, whole), kept)
+        out.copy_(torch.randn(90, 130, generator=g, device="cuda"))
+    d_s, d_values = torch.empty(R.nnz, 130, device="cuda"), torch.empty(R.nnz, device="cuda").to(DTYPE[half])
+    s[5] = 1.0
+    want, want_v, size_v = rows.combine_grad(R.row_ptr, R.col_ind, R.values, out, s, 11, 1.0, 0.0, d_s, d_values)
+    api.experts_combine_grad(handle, R, mat(api, out), mat(api, s), mat(api, d_s), api.DnVec(d_values), buffer=buffer)
+    no_error(pkg)
+    ref.close(d_s, want, 3 * F32 * want.abs())
+    ref.close(d_values, want_v, ref.rounding(d_values.dtype, want_v) + 132 * F32 * size_v)
+
+
+def test_room_for_copies_has_to_be_asked_for(pkg, handle):
+    """Operands off 16 bytes are copied behind the order: refused where no BufferSize call through this routing has counted them."""
+    from ops_sparse_b200 import api
+    g = gen(32)
+    R = routed(api, g, 30, 5, 2)
+    x, w = eights(g, R.nnz, 33, 3), eights(g, 5 * 20, 33, 0)
+    sx, sw, y = torch.rand(R.nnz, generator=g, device="cuda"), torch.rand(100, generator=g, device="cuda"), torch.empty(R.nnz, 20, device="cuda")
+    buffer = ordered(api, handle, R, 1 << 20)
+    args = (mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), mat(api, y))
+    with pytest.raises(pkg.AclSparseError) as e:
+        api.experts_scaled_mm(handle, R, *args, buffer=buffer)
+    assert e.value.status == pkg.ACL_SPARSE_STATUS_INVALID_VALUE
+    assert api.experts_scaled_mm_buffer_size(handle, R, args[0], args[2], args[4]) <= buffer.numel()
+    api.experts_scaled_mm(handle, R, *args, buffer=buffer)
+    no_error(pkg)
+    _, _, starts = rows.order_of(R.col_ind, 5)
+    for e in range(5):
+        a, b, c = int(starts[e]), int(starts[e + 1]), slice(20 * e, 20 * e + 20)
+        want, size = rows.scaled(x[a:b], sx[a:b], w[c], sw[c], 1.0, 0.0, y[a:b])
+        ref.close(y[a:b], want, 5 * F32 * size)
+
+
+def test_two_streams_at_once(pkg, handle):
+    """Products of all forms on two streams side by side, again and again: the same bits as one after the other."""
+    from ops_sparse_b200 import api
+    g = gen(33)
+    jobs = []
+    for many, depth, channels, out in ((300, 2048, 600, "f32"), (40, 2048, 300, "f32"), (2, 512, 900, "bf16"), (40, 128, 20000, "bf16"), (20, 96, 200, "f16")):
+        x, w = eights(g, many, depth), eights(g, channels, depth)
+        sx, sw = torch.rand(many, generator=g, device="cuda") * 1e-3, torch.rand(channels, generator=g, device="cuda") * 1e-3
+        y = torch.empty(many, channels, dtype=DTYPE[out], device="cuda")
+        jobs.append((mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), y))
+        api.scaled_mm(handle, *jobs[-1][:4], mat(api, y))
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    handles = [api.Handle(s) for s in streams]
+    copies = [[(j, torch.empty_like(j[4])) for j in jobs] for _ in streams]
+    made = [[(j, y, mat(api, y)) for j, y in c] for c in copies]
+    torch.cuda.synchronize()
+    for turn in range(20):
+        for i in range(len(jobs)):
+            for k, h in enumerate(handles):
+                j, _, Y = made[k][(i + 2 * k + turn) % len(jobs)]
+                api.scaled_mm(h, *j[:4], Y)
+    no_error(pkg)
+    for c in made:
+        assert all(torch.equal(j[4], y) for j, y, _ in c)
+    for h in handles:
+        h.close()
