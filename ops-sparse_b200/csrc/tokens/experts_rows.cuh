@@ -313,6 +313,7 @@ __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel
         top = __reduce_max_sync(0xffffffffu, Raw<T>::TopOf(top));
         if constexpr (kWarps > 1) {  // two places in turn: one is written while others may still read the other
             if (lane == 0) sTop[turn][warp] = top;
+            __syncwarp();
             asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / kWarps), "n"(32 * kWarps) : "memory");
             top = __reduce_max_sync(0xffffffffu, lane < kWarps ? sTop[turn][warp - within + lane] : 0u);
         }

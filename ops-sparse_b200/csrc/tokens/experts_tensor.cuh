@@ -172,10 +172,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
             run += __shfl_sync(0xffffffffu, incl, 31);
         }
     }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    TensorBefore();
     __syncthreads();
-    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if constexpr (kPair) ClusterMeet();
+    TensorAfter();
     const uint32_t tmem = sTmem;
     const int all = ordered ? sStart[groups] : 0;
     if (!ordered && tid == 0 && blockIdx.x == 0) atomicMax(&gExpertsError, kNoOrder);
@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 failed = true;
                 break;
             }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            TensorAfter();
             const uint32_t shape = kInstr | (uint32_t)(m.wide >> 3) << 17, to = tmem + acc * kMmaColsMost;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
                 if (!__all_sync(0xffffffffu, BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles))) {
@@ -381,7 +381,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                     failed = true;
                     break;
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                TensorAfter();
                 ++tile;
             }
             const int f0 = m.f0 + rank * kMmaRows + quarter * 32;  // the warp's 32 rows of the tile
@@ -392,7 +392,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
                 float v[32] = {};
                 if (m.steps > 0) LoadColumns32(from + c0, v);
                 if (m.steps > 0 && c0 + 32 >= m.many) {  // all that this warp reads of the accumulator
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    TensorBefore();
                     __syncwarp();
                     if (lane == 0) BarArriveAt(LeadersBar(sFree + acc));
                 }
@@ -491,10 +491,11 @@ __global__ void __launch_bounds__(kMmaThreads, 1) ExpertsTensorKernel(const MmaA
     }
     __syncwarp();
     if (failed) atomicMax(&gExpertsError, kWaitRanOut);
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    TensorBefore();
     __syncthreads();
     // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.
-    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (kPair) ClusterMeet();
+    TensorAfter();
     if (warp == 0) {
         if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");

@@ -77,11 +77,16 @@ template <bool kPair> __device__ __forceinline__ void MmaI8(uint32_t d, uint64_t
 constexpr float kScaleLow = 0x1p-63f, kScaleHigh = 0x1p48f;
 __device__ __forceinline__ bool PlainScale(float s) { return s == 0.0f || (s >= kScaleLow && s <= kScaleHigh); }
 // The four warps of a half of a tile's columns.
-__device__ __forceinline__ void StoreBarrier(int half) { asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory"); }
+__device__ __forceinline__ void StoreBarrier(int half)
+{
+    __syncwarp();
+    asm volatile("bar.sync %0, 128;" ::"r"(1 + half) : "memory");
+}
 // Whether a wait ran out for none of them: they go on together, or not at all.
 __device__ __forceinline__ bool StoreAgree(int half, bool ok)
 {
     uint32_t all;
+    __syncwarp();
     asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.and.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(all)
                  : "r"((uint32_t)ok), "r"(1 + half)
@@ -209,10 +214,10 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     const ScaledTiles<kPair> tiles{a, sStart, sOffset, (a.n + ScaledTiles<kPair>::kHigh - 1) / ScaledTiles<kPair>::kHigh};
     const int groups = a.header != nullptr ? a.experts + 1 : 1;
     const bool ordered = WorkTable(a, groups, kTileThreads, sStart, sOffset, [&](int count) { return tiles.Count(count); });
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    TensorBefore();
     __syncthreads();
-    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if constexpr (kPair) ClusterMeet();
+    TensorAfter();
     const uint32_t tmem = sTmem;
     const int all = ordered ? sStart[groups] : 0;
     if (!ordered && tid == 0 && blockIdx.x == 0) atomicMax(&gScaledError, kScaledNoOrder);
@@ -256,7 +261,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                 failed = true;
                 break;
             }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            TensorAfter();
             const uint32_t shape = kInstr | (uint32_t)(m.wide >> 3) << 17, to = tmem + acc * kTileColsMost;
             for (int k = 0; k < m.steps; ++k, ring.Next(a.stages)) {
                 if (!__all_sync(0xffffffffu, BarWait(sFull + ring.stage, ring.Filled(), a.waitCycles))) {
@@ -301,7 +306,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                     failed = true;
                     break;
                 }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                TensorAfter();
                 ++tile;
             }
             const uint32_t from = tmem + ((uint32_t)quarter << 21) + acc * kTileColsMost;
@@ -349,7 +354,7 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
                 }
             }
             if (m.steps > 0) {  // all that this warp reads of the accumulator
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                TensorBefore();
                 __syncwarp();
                 if (lane == 0) BarArriveAt(kPair ? LeadersBar(sFree + acc) : Shared(sFree + acc));
             }
@@ -357,10 +362,11 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     }
     __syncwarp();
     if (failed) atomicMax(&gScaledError, kScaledWaitRanOut);
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    TensorBefore();
     __syncthreads();
     // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.
-    if constexpr (kPair) asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    if constexpr (kPair) ClusterMeet();
+    TensorAfter();
     if (warp == 0) {
         if constexpr (kPair) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
         else asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
@@ -409,9 +415,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const Scal
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     b200sp::WaitForPrevious();
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    TensorBefore();
     __syncthreads();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    TensorAfter();
     const uint32_t tmem = sTmem;
     // Tiles side by side along the rows of X first.
     const int across = (a.rows + a.colsMost - 1) / a.colsMost, f0 = tile / across * kTileRows, first = tile % across * a.colsMost;
@@ -461,7 +467,7 @@ __global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const Scal
     __syncwarp();
     if (!BarWaitWarp(&sDone, 0, 2 * a.waitCycles + (to - from) * kTileStepCycles)) failed = true;  // longer than the waits above
     if (failed) sFailed = 1;
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    TensorAfter();
     __syncthreads();
     // The sums, a column of 128 channels after the other, where the stages were.
     const int quarter = warp & 3;
@@ -475,7 +481,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const Scal
                 if (c0 + i < wide) sums[i * kTileRows] = __float_as_int(v[i]);
         }
     }
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    TensorBefore();  // all that is read of tensor memory
+    ClusterMeet();
     int bad = 0;
     for (int r = 0; r < split; ++r) bad |= LoadRemote(Shared(&sFailed), r);
     if (bad == 0) {
@@ -507,7 +514,8 @@ __global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const Scal
         atomicMax(&gScaledError, kScaledWaitRanOut);
     }
     // The others may still read this CTA's sums.
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+    ClusterMeet();
+    TensorAfter();
     if (warp == 0) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(a.tmemColumns) : "memory");
 }
 
@@ -591,6 +599,7 @@ __global__ void __launch_bounds__(kFewThreads) ScaledFewKernel(const ScaledArgs 
             }
         if (parts > 1) {  // two places in turn: one is written while others may still read the other
             if (lane < kM * kR) sPart[turn][warp][lane] = mine;
+            __syncwarp();
             asm volatile("bar.sync %0, %1;" ::"r"(1 + warp / parts), "r"(32 * parts) : "memory");
             if (part != 0) continue;
             mine = 0;

@@ -64,6 +64,15 @@ __device__ __forceinline__ bool BarWaitWarp(uint64_t *bar, uint32_t parity, long
     if ((threadIdx.x & 31) == 0) ok = BarWait(bar, parity, limit);
     return __all_sync(0xffffffffu, ok);
 }
+// All CTAs of a cluster meet.  Like all `.aligned` instructions it is for whole warps: lanes that have gone different ways come together before it.
+__device__ __forceinline__ void ClusterMeet()
+{
+    __syncwarp();
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Tensor memory that some threads have used and others go on with (or free): the ones order what they did before a barrier, the others what they do after it.
+__device__ __forceinline__ void TensorBefore() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void TensorAfter() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 // bar: of this CTA, or with a pair of the first.
 template <bool kPair> __device__ __forceinline__ void CopyTile3(uint32_t dst, const CUtensorMap *map, int x, int y, int z, uint32_t bar)
 {
@@ -102,6 +111,7 @@ template <bool kPair> __device__ __forceinline__ void MmaCommit(uint64_t *bar)
 __device__ __forceinline__ void LoadColumns32(uint32_t at, float (&v)[32])
 {
     uint32_t r[32];
+    __syncwarp();
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, %17, %18, %19, "
         "%20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"

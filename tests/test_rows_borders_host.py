@@ -1,0 +1,47 @@
+"""CPU: operators of include/b200sp_rows.h at their borders -- what no result shows (the order of a kernel's ends, which kernel a product
+goes to) and calls that have to be refused before anything is launched."""
+from __future__ import annotations
+
+import re
+from pathlib import Path
+
+import pytest
+
+SOURCES = Path(__file__).resolve().parents[1] / "ops-sparse_b200" / "csrc" / "tokens"
+
+
+def _code(name):
+    return re.sub(r"//[^\n]*", "", (SOURCES / name).read_text())
+
+
+def _kernels(name):
+    """Every kernel's body, by name."""
+    code, found = _code(name), {}
+    for m in re.finditer(r"__global__ void[^;{]*?\b(\w+Kernel)\(", code):
+        start = code.index("{", m.end())
+        found[m.group(1)] = code[start:code.index("\n}\n", start)]
+    return found
+
+
+@pytest.mark.parametrize("name", ["tensor.cuh", "experts_tensor.cuh", "scaled_tensor.cuh", "experts_rows.cuh"])
+def test_barriers_and_loads_for_whole_warps(name):
+    """Instructions that a warp's lanes have to reach together come right behind a __syncwarp()."""
+    code, seen = _code(name), 0
+    for m in re.finditer(r'asm volatile\(\s*"[^;]*(barrier\.cluster\.arrive|tcgen05\.ld|bar\.sync|bar\.red)', code):
+        assert re.search(r"__syncwarp\(\);\s*$", code[:m.start()]), code[m.start() - 80:m.end()]
+        seen += 1
+    assert seen >= 1 or name == "experts_tensor.cuh"
+
+
+@pytest.mark.parametrize("name,kernel", [("experts_tensor.cuh", "ExpertsTensorKernel"), ("scaled_tensor.cuh", "ScaledTensorKernel"),
+                                         ("scaled_tensor.cuh", "ScaledSplitKernel")])
+def test_tensor_memory_is_freed_behind_its_readers(name, kernel):
+    """The last reads of tensor memory, a fence, a barrier, a fence, then it is freed."""
+    body = _kernels(name)[kernel]
+    end = body[body.rindex("LoadColumns32"):]
+    before = re.search(r"TensorBefore\(\)|fence::before_thread_sync", end)
+    assert before
+    meets = re.search(r"__syncthreads\(\)|ClusterMeet\(\)|barrier\.cluster", end[before.end():])
+    assert meets
+    rest = end[before.end() + meets.end():]
+    assert re.search(r"TensorAfter\(\)|fence::after_thread_sync", rest[:rest.index("dealloc")])
