@@ -281,7 +281,6 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
         }
         if (elected) MmaCommit<kPair>(&sLast);  // when every product started here is complete, also after a failure
         __syncwarp();
-        (void)BarWait(&sLast, 0, a.waitCycles);
     } else if (warp >= kFirstStore) {
         const int quarter = warp & 3, half = (warp - kFirstStore) >> 2;  // the lanes of tensor memory that the warp may read; every other 32 columns
         const float alpha = a.sc.Alpha(), beta = a.sc.Beta();
@@ -364,6 +363,8 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
     if (failed) atomicMax(&gScaledError, kScaledWaitRanOut);
     TensorBefore();
     __syncthreads();
+    // Every product has ended, and in a pair the last signal of the first CTA's commits has come in at the other one, too, before either of them ends.
+    if (warp == 0) (void)BarWaitWarp(&sLast, 0, a.waitCycles);
     // The other CTA may still signal barriers here, and the pair's tensor memory is freed by both.
     if constexpr (kPair) ClusterMeet();
     TensorAfter();

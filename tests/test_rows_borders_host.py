@@ -45,3 +45,12 @@ def test_tensor_memory_is_freed_behind_its_readers(name, kernel):
     assert meets
     rest = end[before.end() + meets.end():]
     assert re.search(r"TensorAfter\(\)|fence::after_thread_sync", rest[:rest.index("dealloc")])
+
+
+@pytest.mark.parametrize("name,kernel", [("experts_tensor.cuh", "ExpertsTensorKernel"), ("scaled_tensor.cuh", "ScaledTensorKernel")])
+def test_both_ctas_of_a_pair_see_the_last_signal(name, kernel):
+    """Commits of the first CTA of a pair signal barriers in both: neither ends before the last one has come in where it is."""
+    body = _kernels(name)[kernel]
+    end = body[body.rindex("__syncthreads()"):]
+    wait = re.search(r"\n    if \(warp == 0\) [^;\n]*BarWaitWarp\(&sLast", end)  # of every CTA, outside the branches of the first
+    assert wait and wait.start() < end.index("dealloc") and body.count("MmaCommit<kPair>(&sLast)") == 1
