@@ -26,7 +26,6 @@ __global__ void __launch_bounds__(kSortThreads, 1) ExpertsOrderKernel(const Sort
                                                                      const uint64_t number)
 {
     extern __shared__ unsigned char sSort[];
-    b200sp::LetNextStart();
     b200sp::WaitForPrevious();
     if (blockIdx.x == 0 && threadIdx.x == 0) {
         header[0] = mark;

@@ -28,7 +28,12 @@ struct RowsArgs {
     Scalars sc;
 };
 
-constexpr unsigned kFewCtas = 74;  // leave half of the SMs alone
+// Rounding to 8 bits lets the next kernel in early (a product takes every SM, and keeps other streams from them while it waits) only where it is a matter of some us:
+// by half of the SMs, rows that are held, and so many stretches of rows to be written, eight of a row at least, all by one CTA at worst, 18 us (f32 23).  16 tokens to eight of 64 experts, order,
+// rounding and product 32.1 us, without 32.6; one row of 4096 and its product 6.57 and 6.7.  (The order of the entries, by eight SMs, does not: one of
+// 1,048,576 entries takes 285 us, in which another stream's product ends in 17, and not in 440; behind orders of 8 to 32,768 entries nothing is gained.)
+constexpr unsigned kFewCtas = 74;
+constexpr long long kFewPieces = 2048;
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;
 constexpr int kDispatchCtas = 5, kCombineCtas = 4, kGradCtas = 2;  // resident on an SM: what their registers allow
 template <typename T> constexpr int kQuantiseCtas = sizeof(T) == 4 ? 4 : 6;
@@ -282,7 +287,8 @@ __global__ void __launch_bounds__(kRowsThreads, kQuantiseCtas<T>) QuantiseKernel
     constexpr int kStep = kWarps * kStretch, kTokens = kRowsWarps / kWarps;
     __shared__ uint32_t sTop[2][kRowsWarps];
     __shared__ Raw<T> sHeld[kHeld][kRowsThreads];
-    if (gridDim.x <= kFewCtas) b200sp::LetNextStart();
+    if (gridDim.x <= kFewCtas && a.width <= kHeld * kStep && (!kOrdered || (long long)a.nnz * max((a.width + kStretch - 1) / kStretch, kRowsWarps) <= kFewPieces))
+        b200sp::LetNextStart();
     b200sp::WaitForPrevious();
     if (kOrdered && !HasOrder(a)) return;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, within = warp % kWarps, c = within * kStretch;
