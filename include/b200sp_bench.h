@@ -27,11 +27,17 @@ aclsparseStatus_t b200spRepeatSpMM(aclsparseHandle_t handle, aclsparseOperation_
                                    aclsparseConstDnMatDescr_t matB, const void *beta, aclsparseDnMatDescr_t matC,
                                    aclDataType computeType, aclsparseSpMMAlg_t alg, void *buffer, int reps);
 
-/* What aclsparseSpMMPreprocess recorded for matA: info = {long-row segments, units of the column-block path
+/* For benchmarks and tests that have to say which kernels a product runs.
+ * What aclsparseSpMMPreprocess recorded for matA: info = {long-row segments, units of the column-block path
  * (0 = the long rows are summed by segments), long rows, 1 if a plan is recorded}. */
 aclsparseStatus_t b200spSpMMPlanInfo(aclsparseConstSpMatDescr_t matA, int32_t info[4]);
 /* *on = 1 if a product with this plan, with B and C in 16-byte aligned rows, gives its rows to the row-stream kernel. */
 aclsparseStatus_t b200spSpMMToRowStream(aclsparseConstSpMatDescr_t matA, int32_t *on);
+
+/* How b200spScaledMM (matR NULL) or b200spExpertsScaledMM computes this product on the current device: info = {0: tiles of a CTA, 1: of a pair of
+ * CTAs, 2: tiles whose steps a cluster shares, 3: without tiles; rows of X of a tile at most; CTAs of such a cluster, else 1}. */
+aclsparseStatus_t b200spScaledMMInfo(aclsparseConstSpMatDescr_t matR, aclsparseConstDnMatDescr_t matX, aclsparseConstDnMatDescr_t matW,
+                                     aclsparseConstDnMatDescr_t matY, int32_t info[3]);
 
 /* Row-sharded operator on several GPUs: `reps` steps, step i = b200spMgPush of this rank's slice (`slice`,
  * `offset`, `bytes` as for b200spMgPush) with sequence number firstSeq + i into replica (firstSeq + i) % replicas,

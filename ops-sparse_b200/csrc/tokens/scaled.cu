@@ -3,6 +3,7 @@
 #include <cmath>
 #include <type_traits>
 
+#include "b200sp_bench.h"
 #include "b200sp_rows.h"
 #include "tokens/common.cuh"
 #include "tokens/experts_plan.cuh"
@@ -168,6 +169,16 @@ Form FormOf(long long rows, long long n, long long depth)
     return best;
 }
 
+// With experts, of whose rows the host knows the average only.
+Form FormOfExperts(long long rows, long long n, long long experts)
+{
+    Form form{kWhole, TileColumns(rows, experts), 1};
+    if (form.cols >= 128 && n > kTileRows) form.kind = kPairs;
+    // hardly an expert has more than one
+    if (4 * rows <= experts) form.kind = kFew;
+    return form;
+}
+
 aclsparseStatus_t Product(const char *call, const aclsparseContext *handle, ScaledArgs a, const aclsparseDnMatDescr *X,
                           const aclsparseDnVecDescr *scalesX, const aclsparseDnMatDescr *W, const aclsparseDnVecDescr *scalesW,
                           const aclsparseDnMatDescr *Y, char *room)
@@ -183,12 +194,7 @@ aclsparseStatus_t Product(const char *call, const aclsparseContext *handle, Scal
     const Operand x = Aligned(X, &room, handle->stream, a, 0);
     const Operand w = Aligned(W, &room, handle->stream, a, a.header != nullptr ? a.n : 0);
     if (x.error != cudaSuccess || w.error != cudaSuccess) return Finished(x.error != cudaSuccess ? x.error : w.error, call);
-    Form form = a.header == nullptr ? FormOf(a.rows, a.n, X->cols) : Form{kWhole, TileColumns(a.rows, a.experts), 1};
-    if (a.header != nullptr) {
-        if (form.cols >= 128 && a.n > kTileRows) form.kind = kPairs;
-        // hardly an expert has more than one
-        if (4ll * a.rows <= a.experts) form.kind = kFew;
-    }
+    const Form form = a.header == nullptr ? FormOf(a.rows, a.n, X->cols) : FormOfExperts(a.rows, a.n, a.experts);
     if (form.kind == kFew) {
         const long long chunks = a.header == nullptr ? (a.rows + kFewRowsX - 1) / kFewRowsX : a.rows;
         const cudaError_t e = WithType(Y->valueType, [&](auto out) {
@@ -316,6 +322,19 @@ aclsparseStatus_t b200spExpertsScaledMM(aclsparseHandle_t handle, const void *al
     a.experts = (int)matR->cols;
     a.sc = ScalarsOf(handle, alpha, beta);
     return Product("b200spExpertsScaledMM", handle, a, matX, scalesX, matW, scalesW, matY, p + L.total - 256);
+}
+
+aclsparseStatus_t b200spScaledMMInfo(aclsparseConstSpMatDescr_t matR, aclsparseConstDnMatDescr_t matX, aclsparseConstDnMatDescr_t matW,
+                                     aclsparseConstDnMatDescr_t matY, int32_t info[3])
+{
+    if (info == nullptr) return ACL_SPARSE_STATUS_INVALID_VALUE;
+    const aclsparseStatus_t st = matR == nullptr ? CheckOperands(matX, matW, matY, 1) : CheckExperts(matR, matX, matW, matY);
+    if (st != ACL_SPARSE_STATUS_SUCCESS) return st;
+    const Form form = matR == nullptr ? FormOf(matX->rows, matY->cols, matX->cols) : FormOfExperts(matX->rows, matY->cols, matR->cols);
+    info[0] = form.kind;
+    info[1] = form.kind == kFew ? 0 : form.cols;
+    info[2] = form.kind == kShared ? form.split : 1;
+    return ACL_SPARSE_STATUS_SUCCESS;
 }
 
 }  // extern "C"

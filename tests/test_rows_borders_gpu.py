@@ -1,13 +1,16 @@
 """GPU: operators of include/b200sp_rows.h at their borders -- beside other streams, in each form of a product, at far addresses."""
 from __future__ import annotations
 
+import math
+from ctypes import c_int32
+
 import pytest
 import torch
 
 import rows_reference as rows
 import token_reference as ref
 from test_rows_gpu import eights, no_error, ordered, routed
-from test_tokens_gpu import gen, mat
+from test_tokens_gpu import gen, mat, matrix, outside
 from token_reference import DTYPE, F32
 
 pytestmark = pytest.mark.gpu
@@ -48,3 +51,174 @@ def test_long_order_leaves_the_sms_to_other_streams(pkg, handle):
     ref.close(out, want, 5 * F32 * size)
     first.close()
     other.close()
+
+
+# ---------------------------------------------------------------- products in 8 bits, each in the form that it says
+
+WHOLE, PAIRS, SHARED, FEW = range(4)
+
+
+def form_of(pkg, X, W, Y, R=None):
+    info = (c_int32 * 3)()
+    assert pkg.lib().b200spScaledMMInfo(None if R is None else R.raw, X.raw, W.raw, Y.raw, info) == 0
+    return tuple(info)
+
+
+def exact_sums(x, w):
+    """Sums of products of 8 bits, in 64, on the GPU."""
+    return x.double() @ w.double().T
+
+
+FORMS = [  # rows, depth, channels, out, alpha, beta, pad and shift of Y, form
+    (1836, 38, 2524, "bf16", 1.0, 0.0, 4, 0, (PAIRS, 64, 1)),  # rows of Y on 16 bytes that end within a piece
+    (900, 128, 4744, "f16", 0.5, 0.0, 0, 0, (PAIRS, 64, 1)),
+    (900, 128, 4744, "bf16", 1.0, 0.5, 1, 1, (PAIRS, 64, 1)),
+    (638, 32, 13146, "f32", 1.0, 0.0, 0, 0, (PAIRS, 128, 1)),
+    (842, 32, 14333, "bf16", 2.0, 0.0, 3, 0, (PAIRS, 256, 1)),
+    (2048, 4096, 4096, "bf16", 1.0, 0.0, 0, 0, (PAIRS, 256, 1)),
+    (2048, 4096, 4096, "f32", -1.0, 2.0, 0, 0, (PAIRS, 256, 1)),
+    (4096, 2048, 2048, "f16", 1.0, 0.0, 0, 0, (PAIRS, 256, 1)),
+    (17, 2048, 4360, "bf16", 1.0, 0.0, 0, 0, (SHARED, 16, 2)),
+    (1128, 2950, 138, "f32", 1.0, 1.0, 0, 0, (SHARED, 32, 2)),
+    (39, 4008, 5224, "f16", 1.0, 0.0, 0, 0, (SHARED, 64, 2)),
+    (66, 2788, 2212, "bf16", 1.0, -0.5, 5, 3, (SHARED, 128, 4)),
+    (142, 3856, 4062, "f32", 1.0, 0.0, 0, 0, (SHARED, 256, 4)),
+    (132, 1941, 1724, "bf16", 1.0, 0.0, 4, 0, (SHARED, 256, 8)),
+    (320, 512, 200, "bf16", 1.0, 0.0, 0, 0, (WHOLE, 16, 1)),
+    (700, 512, 4100, "bf16", 1.0, 0.0, 4, 0, (WHOLE, 256, 1)),
+    (16, 2048, 640, "f32", 1.0, 1.0, 0, 0, (FEW, 0, 1)),
+]
+
+
+@pytest.mark.parametrize("many,depth,channels,out,alpha,beta,pad,shift,form", FORMS)
+def test_scaled_product_of_a_form(pkg, handle, many, depth, channels, out, alpha, beta, pad, shift, form):
+    from ops_sparse_b200 import api
+    g = gen(many + depth + channels)
+    x, w = eights(g, many, depth, -depth % 16), eights(g, channels, depth, -depth % 16)
+    sx, sw = torch.rand(many, generator=g, device="cuda") * 1e-2, torch.rand(channels, generator=g, device="cuda") * 1e-3
+    y, whole = matrix(g, many, channels, out, pad, shift)
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    assert form_of(pkg, X, W, Y) == form and api.scaled_mm_buffer_size(handle, X, W, Y) == 0
+    want = alpha * exact_sums(x, w) * sx.double()[:, None] * sw.double()
+    old = beta * y.double() if beta else torch.zeros_like(want)
+    if beta == 0:
+        y.fill_(math.nan)  # must not be read
+    kept = outside(y, whole).clone()
+    api.scaled_mm(handle, X, api.DnVec(sx), W, api.DnVec(sw), Y, alpha, beta)
+    no_error(pkg)
+    # the sum is exact; its f32, the scales' product, theirs, alpha's and beta's are rounded, then the result
+    ref.close(y, want + old, ref.rounding(y.dtype, want + old) + 5 * F32 * (want.abs() + old.abs()))
+    assert torch.equal(outside(y, whole), kept)
+
+
+@pytest.mark.parametrize("many,depth,channels,form", [(900, 128, 4744, (PAIRS, 64, 1)), (17, 2048, 4360, (SHARED, 16, 2))])
+def test_scaled_extreme_scales_of_a_form(pkg, handle, many, depth, channels, form):
+    """Scales whose product f32 cannot hold, of sums that bring the result back, and some that are not finite."""
+    from ops_sparse_b200 import api
+    g = gen(79)
+    x, w = eights(g, many, depth), eights(g, channels, depth)
+    x[:, 0] = 127
+    sx = torch.tensor([1e-30, 1e25, 1e-25, 1e38, 1.0, 0.0, 1e-38, 1e-45], device="cuda").repeat(many // 8 + 1)[:many].contiguous()
+    sw = torch.tensor([1e-20, 1e-10, 1.0, 1e10, 1e-25, 1e-38, 3e38, 0.0], device="cuda").repeat(channels // 8)
+    y = torch.empty(many, channels, device="cuda")
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    assert form_of(pkg, X, W, Y) == form
+    sums = exact_sums(x, w)
+    for alpha in (1.0, 2.0 ** 50, 2.0 ** -50):
+        api.scaled_mm(handle, X, api.DnVec(sx), W, api.DnVec(sw), Y, alpha=alpha)
+        torch.cuda.synchronize()
+        want = alpha * (sums * sx.double()[:, None] * sw.double())
+        held = want.float().double()  # infinite where f32 is
+        ref.close(y, torch.where(want.abs() > 3.4028235e38, held, want), ref.rounding(y.dtype, want) + 5 * F32 * want.abs())
+    sx = torch.ones(many, device="cuda")
+    sx[0], sx[1] = math.nan, math.inf
+    half = torch.empty(many, channels, dtype=torch.float16, device="cuda")
+    api.scaled_mm(handle, X, api.DnVec(sx), W, api.DnVec(torch.full((channels,), 1e-3, device="cuda")), mat(api, half))
+    no_error(pkg)
+    assert bool(half[0].isnan().all()) and bool((~half[1].isfinite()).all()) and not bool(half[2:].isnan().any())
+
+
+@pytest.mark.parametrize("tokens,experts,k,depth,channels,out,pad,form", [
+    (900, 4, 2, 384, 520, "bf16", 0, (PAIRS, 256, 1)), (901, 4, 2, 272, 393, "f16", 7, (PAIRS, 256, 1)),
+    (333, 9, 2, 640, 260, "bf16", 4, (PAIRS, 128, 1)), (333, 9, 2, 640, 128, "bf16", 0, (WHOLE, 128, 1)),
+    (1, 8, 2, 512, 300, "bf16", 4, (FEW, 0, 1)), (2, 8, 2, 512, 300, "bf16", 4, (WHOLE, 16, 1)),
+])
+def test_experts_scaled_product_of_a_form(pkg, handle, tokens, experts, k, depth, channels, out, pad, form):
+    """Results of 16 bits in rows that start on 16 bytes: stored by way of shared memory, with ends within a piece and a tile."""
+    from ops_sparse_b200 import api
+    g = gen(tokens + depth + channels)
+    R = routed(api, g, tokens, experts, k, 1.0, 0.05 if tokens > 9 else 0.0)
+    x, w = eights(g, R.nnz, depth), eights(g, experts * channels, depth)
+    sx, sw = torch.rand(R.nnz, generator=g, device="cuda") * 1e-2, torch.rand(experts * channels, generator=g, device="cuda") * 1e-3
+    y, whole = matrix(g, R.nnz, channels, out, pad)
+    X, W, Y = mat(api, x), mat(api, w), mat(api, y)
+    assert form_of(pkg, X, W, Y, R) == form
+    _, _, starts = rows.order_of(R.col_ind, experts)
+    sx[int(starts[-1]):] = math.nan  # rows of no expert are not looked at
+    want = torch.zeros(y.shape, dtype=torch.float64, device="cuda")
+    for e in range(experts):
+        a, b, c = int(starts[e]), int(starts[e + 1]), slice(e * channels, (e + 1) * channels)
+        want[a:b] = exact_sums(x[a:b], w[c]) * sx[a:b].double()[:, None] * sw[c].double()
+    y.fill_(math.nan)
+    kept = outside(y, whole).clone()
+    buffer = ordered(api, handle, R, api.experts_scaled_mm_buffer_size(handle, R, X, W, Y))
+    api.experts_scaled_mm(handle, R, X, api.DnVec(sx), W, api.DnVec(sw), Y, buffer=buffer)
+    no_error(pkg)
+    ref.close(y, want, ref.rounding(y.dtype, want) + 5 * F32 * want.abs())
+    assert torch.equal(outside(y, whole), kept)
+
+
+@pytest.mark.parametrize("many,depth,channels,form", [(2048, 4096, 4096, (PAIRS, 256, 1)), (900, 128, 4744, (PAIRS, 64, 1)),
+                                                      (17, 2048, 4360, (SHARED, 16, 2))])
+def test_scaled_wait_that_runs_out_in_a_form(pkg, handle, many, depth, channels, form):
+    """Every wait for a copy runs out (bytes are expected that nobody sends): the flag says so, Y is as it was, and the next product is right."""
+    from ops_sparse_b200 import api
+    L, g = pkg.lib(), gen(26)
+    x, w = eights(g, many, depth), eights(g, channels, depth)
+    sx, sw = torch.rand(many, generator=g, device="cuda"), torch.rand(channels, generator=g, device="cuda")
+    y = torch.full((many, channels), 3.0, dtype=torch.bfloat16, device="cuda")
+    args = (mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), mat(api, y))
+    assert form_of(pkg, args[0], args[2], args[4]) == form
+    L.b200sp_scaled_wait_test(200_000, 16)
+    try:
+        api.scaled_mm(handle, *args)
+        asked = L.b200sp_scaled_error()
+        left = bool((y == 3.0).all())
+    finally:
+        L.b200sp_scaled_wait_test(0, 0)
+        L.b200sp_scaled_error_clear()
+    assert asked == 1 and left
+    api.scaled_mm(handle, *args)
+    no_error(pkg)
+    want = exact_sums(x, w) * sx.double()[:, None] * sw.double()
+    ref.close(y, want, ref.rounding(y.dtype, want) + 5 * F32 * want.abs())
+
+
+def test_all_forms_on_two_streams_at_once(pkg, handle):
+    """Products of all forms on two streams side by side, again and again: the same bits as one after the other."""
+    from ops_sparse_b200 import api
+    g, jobs, forms = gen(34), [], set()
+    for many, depth, channels, out in ((2048, 4096, 4096, "bf16"), (900, 128, 4744, "bf16"), (638, 32, 13146, "f32"), (17, 2048, 4360, "f16"),
+                                       (142, 3856, 4062, "f32"), (700, 512, 4100, "bf16"), (2, 512, 900, "bf16")):
+        x, w = eights(g, many, depth), eights(g, channels, depth)
+        sx, sw = torch.rand(many, generator=g, device="cuda") * 1e-3, torch.rand(channels, generator=g, device="cuda") * 1e-3
+        y = torch.empty(many, channels, dtype=DTYPE[out], device="cuda")
+        jobs.append((mat(api, x), api.DnVec(sx), mat(api, w), api.DnVec(sw), y))
+        forms.add(form_of(pkg, jobs[-1][0], jobs[-1][2], mat(api, y))[0])
+        api.scaled_mm(handle, *jobs[-1][:4], mat(api, y))
+    assert forms == {WHOLE, PAIRS, SHARED, FEW}
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    handles = [api.Handle(s) for s in streams]
+    made = [[(j, y, mat(api, y)) for j, y in [(j, torch.empty_like(j[4])) for j in jobs]] for _ in streams]
+    torch.cuda.synchronize()
+    for turn in range(20):
+        for i in range(len(jobs)):
+            for k, h in enumerate(handles):
+                j, _, Y = made[k][(i + 3 * k + turn) % len(jobs)]
+                api.scaled_mm(h, *j[:4], Y)
+    no_error(pkg)
+    for c in made:
+        assert all(torch.equal(j[4], y) for j, y, _ in c)
+    for h in handles:
+        h.close()

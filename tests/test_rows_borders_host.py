@@ -3,9 +3,12 @@ goes to) and calls that have to be refused before anything is launched."""
 from __future__ import annotations
 
 import re
+from ctypes import c_int32
 from pathlib import Path
 
 import pytest
+
+from test_tokens_host import _csr, _mat
 
 SOURCES = Path(__file__).resolve().parents[1] / "ops-sparse_b200" / "csrc" / "tokens"
 
@@ -54,3 +57,22 @@ def test_both_ctas_of_a_pair_see_the_last_signal(name, kernel):
     end = body[body.rindex("__syncthreads()"):]
     wait = re.search(r"\n    if \(warp == 0\) [^;\n]*BarWaitWarp\(&sLast", end)  # of every CTA, outside the branches of the first
     assert wait and wait.start() < end.index("dealloc") and body.count("MmaCommit<kPair>(&sLast)") == 1
+
+
+def test_the_form_of_a_product(pkg):
+    """Which kernel a product goes to can be asked for, under the product's own checks."""
+    f, I8, info = pkg.lib().b200spScaledMMInfo, pkg.ACL_INT8, (c_int32 * 3)()
+    bad = pkg.ACL_SPARSE_STATUS_INVALID_VALUE
+
+    def form(many, depth, channels, R=None, experts=1):
+        info[:] = [-1] * 3
+        assert f(R, _mat(pkg, many, depth, I8), _mat(pkg, experts * channels, depth, I8), _mat(pkg, many, channels), info) == 0
+        return tuple(info)
+
+    assert form(1, 4096, 4096) == (3, 0, 1) and form(8192, 4096, 4096)[0] == 1 and form(61, 4096, 4096)[0] == 2
+    assert form(320, 512, 200)[0] == 0 and form(8192, 4096, 128)[0] != 1  # a pair has channels for both of its CTAs
+    assert form(20, 64, 300, _csr(pkg, 10, 4, 20), 4) == (0, 16, 1) and form(2, 64, 300, _csr(pkg, 1, 8, 2), 8) == (3, 0, 1)
+    X, W, Y = _mat(pkg, 20, 64, I8), _mat(pkg, 48, 64, I8), _mat(pkg, 20, 48)
+    assert f(None, X, W, Y, None) == f(None, None, W, Y, info) == f(None, X, W, _mat(pkg, 20, 47), info) == bad
+    assert f(_csr(pkg, 10, 4, 21), X, W, _mat(pkg, 20, 12), info) == bad and f(_csr(pkg, 10, 4, 20), X, W, _mat(pkg, 20, 12), info) == 0
+    assert f(None, X, W, _mat(pkg, 20, 48, I8), info) == pkg.ACL_SPARSE_STATUS_NOT_SUPPORTED
