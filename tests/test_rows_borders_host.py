@@ -3,10 +3,12 @@ goes to) and calls that have to be refused before anything is launched."""
 from __future__ import annotations
 
 import re
+import types
 from ctypes import c_int32
 from pathlib import Path
 
 import pytest
+import torch
 
 from test_tokens_host import _csr, _mat
 
@@ -76,3 +78,27 @@ def test_the_form_of_a_product(pkg):
     assert f(None, X, W, Y, None) == f(None, None, W, Y, info) == f(None, X, W, _mat(pkg, 20, 47), info) == bad
     assert f(_csr(pkg, 10, 4, 21), X, W, _mat(pkg, 20, 12), info) == bad and f(_csr(pkg, 10, 4, 20), X, W, _mat(pkg, 20, 12), info) == 0
     assert f(None, X, W, _mat(pkg, 20, 48, I8), info) == pkg.ACL_SPARSE_STATUS_NOT_SUPPORTED
+
+
+def test_closed_optional_descriptors_are_refused(pkg):
+    """A closed optional argument is no absent one: its NULL would say so."""
+    from ops_sparse_b200 import api
+    nobody = types.SimpleNamespace(_h=None, device_scalars=False)  # a call that gets as far is refused for it
+    R = api.CsrMatrix(torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), torch.zeros(4), 2, 4)
+    X, S, Q = api.DnMat.row_major(torch.zeros(2, 8)), api.DnMat.row_major(torch.zeros(4, 8)), api.DnMat.row_major(torch.zeros(4, 8, dtype=torch.int8))
+    values, starts, scales = api.DnVec(torch.zeros(4)), api.DnVec(torch.zeros(5, dtype=torch.int32)), api.DnVec(torch.zeros(4))
+    gone, gone_S = api.DnVec(torch.zeros(5, dtype=torch.int32)), api.DnMat.row_major(torch.zeros(4, 8))
+    gone.close()
+    gone_S.close()
+    calls = {  # with what is closed, and with what is not
+        "offsets": [(lambda v: api.experts_dispatch(nobody, R, X, S, offsets=v), gone, starts),
+                    (lambda v: api.experts_quantise(nobody, R, X, Q, scales, offsets=v), gone, starts)],
+        "S": [(lambda v: api.experts_combine_grad(nobody, R, X, v, S, values), gone_S, S)],
+        "d_values": [(lambda v: api.experts_combine_grad(nobody, R, X, S, S, v), gone, values)]}
+    for name, some in calls.items():
+        for call, closed, held in some:
+            with pytest.raises(ValueError, match=f"{name} has been closed"):
+                call(closed)
+            for other in (held, None):
+                with pytest.raises(pkg.AclSparseError, match="HANDLE_IS_NULLPTR"):
+                    call(other)
