@@ -222,3 +222,90 @@ def test_all_forms_on_two_streams_at_once(pkg, handle):
         assert all(torch.equal(j[4], y) for j, y, _ in c)
     for h in handles:
         h.close()
+
+
+# ---------------------------------------------------------------- gradients, and rows far apart
+
+def test_gradients_of_a_layer_term_by_term(pkg, handle):
+    """Dispatch, a product of every expert, combine, and back, against 64 bits' automatic differentiation, within what the terms of each sum allow."""
+    from ops_sparse_b200 import api
+    g = gen(12)
+    tokens, experts, k, d = 45, 7, 2, 40
+    R = routed(api, g, tokens, experts, k)
+    x, w, d_out = (torch.randn(s, generator=g, device="cuda") for s in ((tokens, d), (experts, d, d), (tokens, d)))
+    buffer, starts = ordered(api, handle, R), torch.empty(experts + 1, dtype=torch.int32, device="cuda")
+    new = lambda many: torch.full((many, d), math.nan, device="cuda")  # noqa: E731
+    s, z, out, d_z, d_x, d_values = new(R.nnz), new(R.nnz), new(tokens), new(R.nnz), new(tokens), torch.empty(R.nnz, device="cuda")
+    api.experts_dispatch(handle, R, mat(api, x), mat(api, s), offsets=api.DnVec(starts), buffer=buffer)
+    at = starts.tolist()
+    for e in range(experts):
+        z[at[e]:at[e + 1]] = (s[at[e]:at[e + 1]].double() @ w[e].double()).float()
+    api.experts_combine(handle, R, mat(api, z), mat(api, out), buffer=buffer)
+    api.experts_combine_grad(handle, R, mat(api, d_out), mat(api, z), mat(api, d_z), api.DnVec(d_values), buffer=buffer)
+    d_s = torch.cat([(d_z[at[e]:at[e + 1]].double() @ w[e].double().T).float() for e in range(experts)])
+    api.experts_combine(handle, R, mat(api, d_s), mat(api, d_x), weighted=False, buffer=buffer)
+    no_error(pkg)
+    leaf, values = x.double().requires_grad_(), R.values.double().requires_grad_()
+    token, G, W = torch.arange(tokens, device="cuda").repeat_interleave(k), d_out.double(), w.double()[R.col_ind.long()]
+    rows_ = torch.einsum("ih,ihf->if", leaf[token], W)
+    total = torch.zeros(tokens, d, dtype=torch.float64, device="cuda").index_add(0, token, values[:, None] * rows_)
+    gx, gv = torch.autograd.grad((total * G).sum(), (leaf, values))
+    rows_, values, total = rows_.detach(), values.detach(), total.detach()
+    of_token = lambda terms: torch.zeros(tokens, d, dtype=torch.float64, device="cuda").index_add(0, token, terms)  # noqa: E731
+    # rows of f32, a product and a sum for each of a token's k entries, alpha
+    ref.close(out, total, (k + 2) * F32 * of_token((values[:, None] * rows_).abs()), "sums")
+    # rows of f32, d products each added with one rounding, the sums of a warp's lanes among them, alpha
+    ref.close(d_values, gv, (d + 2) * F32 * (G[token] * rows_).abs().sum(1), "weights' gradient")
+    # alpha w and its product with dOut, rows of f32, a sum for each of the k entries, alpha
+    ref.close(d_x, gx, (k + 4) * F32 * of_token(torch.einsum("if,ihf->ih", (values[:, None] * G[token]).abs(), W.abs())), "tokens' gradient")
+
+
+def test_gradients_of_rows_beyond_32_bits(pkg, handle):
+    """The weights' gradient of rows that lie 2^31 bytes apart, and theirs, beside them and in their place."""
+    from ops_sparse_b200 import api
+    g = gen(28)
+    far, width = 2 ** 30 + 16, 40
+    R = api.CsrMatrix(torch.tensor([0, 2, 4], dtype=torch.int32, device="cuda"), torch.tensor([0, 2, 1, 2], dtype=torch.int32, device="cuda"),
+                      torch.tensor([1.0, -2.0, 0.5, 3.0], device="cuda"), 2, 3)
+    buffer = ordered(api, handle, R)
+    s = torch.zeros(3 * far + width, dtype=torch.bfloat16, device="cuda")
+    view = s.as_strided((4, width), (far, 1))
+    view.copy_(torch.randn(4, width, generator=g, device="cuda"))
+    x = torch.randn(2, width, generator=g, device="cuda").bfloat16()
+    S, held = api.DnMat(s, 4, width, far), view.clone()
+    d_rows, d_values = torch.empty(4, width, device="cuda").bfloat16(), torch.empty(4, device="cuda")
+    want, want_v, size_v = rows.combine_grad(R.row_ptr, R.col_ind, R.values, x, held, 3, 1.0, 0.0, d_rows, d_values)
+    for to, seen in ((mat(api, d_rows), d_rows), (S, view)):
+        d_values.fill_(math.nan)
+        api.experts_combine_grad(handle, R, mat(api, x), S, to, api.DnVec(d_values), buffer=buffer)
+        no_error(pkg)
+        ref.close(d_values, want_v, (width + 2) * F32 * size_v)
+        ref.close(seen, want, ref.rounding(torch.bfloat16, want) + 2 * F32 * want.abs())
+
+
+@pytest.mark.parametrize("out,beta", [("bf16", 0.0), ("f16", 0.5), ("f32", 0.0)])
+@pytest.mark.parametrize("many,depth,channels,kind", [(2, 96, 72, FEW), (4, 4096, 4096, SHARED), (4, 96, 72, None)], ids=["rows", "clusters", "tiles"])
+def test_results_beyond_32_bits(pkg, handle, many, depth, channels, kind, out, beta):
+    """Rows of Y that lie more than 2^31 elements from the first; `None`: those of an expert, by tiles."""
+    from ops_sparse_b200 import api
+    g = gen(many + depth)
+    far = (2 ** 31 if many == 2 else 2 ** 30) - 16 if out == "f32" else 2 ** 31 - 16
+    x, w = eights(g, many, depth), eights(g, channels, depth)
+    sx, sw = torch.rand(many, generator=g, device="cuda") * 1e-2, torch.rand(channels, generator=g, device="cuda") * 1e-3
+    y = torch.zeros((many - 1) * far + channels, dtype=DTYPE[out], device="cuda")
+    view = y.as_strided((many, channels), (far, 1))
+    view.copy_(torch.randn(many, channels, generator=g, device="cuda"))
+    X, W, Y = mat(api, x), mat(api, w), api.DnMat(y, many, channels, far)
+    want = exact_sums(x, w) * sx.double()[:, None] * sw.double()
+    old = beta * view.double()
+    if kind is None:
+        R = api.CsrMatrix(torch.tensor([0, many], dtype=torch.int32, device="cuda"), torch.zeros(many, dtype=torch.int32, device="cuda"),
+                          torch.ones(many, device="cuda"), 1, 1)
+        assert form_of(pkg, X, W, Y, R)[0] == WHOLE
+        buffer = ordered(api, handle, R, api.experts_scaled_mm_buffer_size(handle, R, X, W, Y))
+        api.experts_scaled_mm(handle, R, X, api.DnVec(sx), W, api.DnVec(sw), Y, 1.0, beta, buffer=buffer)
+    else:
+        assert form_of(pkg, X, W, Y)[0] == kind
+        api.scaled_mm(handle, X, api.DnVec(sx), W, api.DnVec(sw), Y, 1.0, beta)
+    no_error(pkg)
+    ref.close(view, want + old, ref.rounding(y.dtype, want + old) + 5 * F32 * (want.abs() + old.abs()))
