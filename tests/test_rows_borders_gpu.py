@@ -309,3 +309,79 @@ def test_results_beyond_32_bits(pkg, handle, many, depth, channels, kind, out, b
         api.scaled_mm(handle, X, api.DnVec(sx), W, api.DnVec(sw), Y, 1.0, beta)
     no_error(pkg)
     ref.close(view, want + old, ref.rounding(y.dtype, want + old) + 5 * F32 * (want.abs() + old.abs()))
+
+
+# ---------------------------------------------------------------- rounding to 8 bits
+
+@pytest.mark.parametrize("kind,bits,far", [("bf16", 8, 0), ("bf16", 8, -110), ("bf16", 8, 110), ("f16", 11, 0)])
+def test_every_quotient_of_16_bits(pkg, handle, kind, bits, far):
+    """Each mantissa as a row's largest value, beside every value of ten powers of two below it: all quotients there are, halves among them."""
+    from ops_sparse_b200 import api
+    mantissas = torch.arange(2 ** (bits - 1), 2 ** bits, dtype=torch.float64, device="cuda")
+    values = torch.cat([mantissas * 2.0 ** -e for e in range(10)])
+    x = torch.where(values[None] <= mantissas[:, None], values[None], 0.0)
+    x[:, 1::2] *= -1
+    x[:, -1] = mantissas
+    x = (x * 2.0 ** (far - 4)).to(DTYPE[kind])
+    size, top = x.double().abs(), x.double().abs().amax(1, keepdim=True)
+    want = torch.floor(127 * size / top)
+    over = 254 * size - (2 * want + 1) * top  # exact: few bits each
+    want = torch.sign(x.double()) * (want + ((over > 0) | ((over == 0) & (want % 2 == 1))))
+    assert int((over == 0).sum()) > 0 and torch.equal(top[:, 0], mantissas * 2.0 ** (far - 4))
+    q, scales = torch.empty(x.shape, dtype=torch.int8, device="cuda"), torch.empty(len(x), device="cuda")
+    api.quantise_rows(handle, mat(api, x), mat(api, q), api.DnVec(scales))
+    torch.cuda.synchronize()
+    assert torch.equal(q.double(), want) and torch.equal(scales.cpu(), top[:, 0].float().cpu() / 127)
+
+
+@pytest.mark.parametrize("many,width,kind", [(9000, 2300, "bf16"), (14000, 1100, "f32"), (4100, 4200, "f16"), (40000, 40, "f32"), (5000, 8300, "bf16")])
+def test_more_rows_to_8_bits_than_ctas(pkg, handle, many, width, kind):
+    """CTAs that go on to further rows, with one to eight warps at each."""
+    from ops_sparse_b200 import api
+    x, _ = matrix(gen(many), many, width, kind, -width % 8)
+    x[::3] *= 2.0 ** -10
+    size, top = x.double().abs(), x.double().abs().amax(1, keepdim=True)
+    want = torch.floor(127 * size / top)
+    over = 254 * size - (2 * want + 1) * top
+    want = torch.sign(x.double()) * (want + ((over > 0) | ((over == 0) & (want % 2 == 1))))
+    q, scales = torch.empty(x.shape, dtype=torch.int8, device="cuda"), torch.empty(many, device="cuda")
+    api.quantise_rows(handle, mat(api, x), mat(api, q), api.DnVec(scales))
+    torch.cuda.synchronize()
+    assert torch.equal(q.double(), want) and torch.equal(scales.cpu(), top[:, 0].float().cpu() / 127)
+
+
+def test_copies_of_operands_in_a_graph(pkg, handle):
+    """Operands off 16 bytes, captured with the order of a routing and without, replayed on other values; the order is made anew in between."""
+    from ops_sparse_b200 import api
+    g, stream = gen(61), torch.cuda.Stream()
+    h = api.Handle(stream)
+    R = routed(api, g, 30, 5, 2)
+    x, w, w1 = eights(g, R.nnz, 33, 3), eights(g, 5 * 20, 33), eights(g, 50, 33)
+    sx, sw, one = torch.rand(R.nnz, generator=g, device="cuda"), torch.rand(100, generator=g, device="cuda"), torch.rand(50, generator=g, device="cuda")
+    y, y1 = torch.empty(R.nnz, 20, device="cuda"), torch.empty(R.nnz, 50, device="cuda")
+    X, W, W1, Y, Y1 = mat(api, x), mat(api, w), mat(api, w1), mat(api, y), mat(api, y1)
+    SX, SW, ONE = api.DnVec(sx), api.DnVec(sw), api.DnVec(one)
+    size = api.experts_scaled_mm_buffer_size(h, R, X, W, Y)
+    buffer = torch.full((size + 3,), 255, dtype=torch.uint8, device="cuda")[3:]
+    own = torch.full((api.scaled_mm_buffer_size(h, X, W1, Y1) + 5,), 255, dtype=torch.uint8, device="cuda")[5:]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        api.experts_preprocess(h, R, buffer)
+        api.experts_scaled_mm(h, R, X, SX, W, SW, Y, buffer=buffer)
+        api.scaled_mm(h, X, SX, W1, ONE, Y1, buffer=own)
+    for turn in range(3):
+        x.copy_(eights(g, R.nnz, 33))
+        w.copy_(eights(g, 100, 33))
+        R.col_ind.copy_(torch.randint(0, 5, (R.nnz,), generator=g, device="cuda").int())
+        torch.cuda.synchronize()
+        graph.replay()
+        no_error(pkg)
+        _, _, starts = rows.order_of(R.col_ind, 5)
+        for e in range(5):
+            a, b, c = int(starts[e]), int(starts[e + 1]), slice(20 * e, 20 * e + 20)
+            want, much = rows.scaled(x[a:b], sx[a:b], w[c], sw[c], 1.0, 0.0, y[a:b])
+            ref.close(y[a:b], want, 5 * F32 * much)
+        want, much = rows.scaled(x, sx, w1, one, 1.0, 0.0, y1)
+        ref.close(y1, want, 5 * F32 * much)
+    h.close()
