@@ -1,4 +1,6 @@
-// b200spExpertsMM, b200spExpertsGrad: products of the rows of tokens with the matrices of the experts that they are routed to.
+// The calls around a routing to experts but those in 8-bit products: the order of its entries (b200spExpertsPreprocess), products of the rows of tokens with the
+// experts' matrices and their gradients (b200spExpertsMM, b200spExpertsGrad; experts_tensor.cuh), rows in the order of the experts, back, and in 8 bits
+// (b200spExpertsDispatch, b200spExpertsCombine, b200spExpertsCombineGrad, b200spExpertsQuantise, b200spQuantiseRows; experts_rows.cuh).
 //
 // The entries of R, in CSR order, are sorted by expert once (b200spExpertsPreprocess); a product then takes the entries of one
 // expert after the other.  Its rows are gathered from X as they lie and its results stored in the rows of their

@@ -2,7 +2,7 @@
 //
 // dispatch: S[place(i)] = alpha X[token(i)]; combine: out[t] = alpha sum of w_i S[place(i)]; its gradient: dS[place(i)] = alpha w_i dOut[t],
 // dw_i = alpha <dOut[t], S[place(i)]>.  All go by tokens, whose entries lie side by side in R: a token's row is read (or written) once and stays in
-// registers while the rows of its entries, which lie anywhere, are written (or read).  What bounds them is DRAM; neighbouring warps take neighbouring
+// registers while the rows of its entries, which lie anywhere, are written (or read).  What bounds dispatch and combine is DRAM; neighbouring warps take neighbouring
 // stretches of a row, so that a row is read or written as a whole at about one time.
 // One B200, bf16, us (the bytes at the copy rate of 6550 GB/s in brackets): rows of 8192 tokens of 4096 to four of 32 experts 57 (51); the weighted sum of eight
 // of 64 experts' rows of 2048 for 8192 tokens 57 (46); its gradient, four of 32, 64 (46); one token's eight rows 4, which is a launch and the host's call.
@@ -187,7 +187,8 @@ __global__ void __launch_bounds__(kRowsThreads, kCombineCtas) ExpertsCombineKern
 
 // T: of S and dS; G: of dOut.  kWarps at a token, kBatch of its entries at a time, whose rows are asked for before any is stored to: 64 us where one after the
 // other takes 77.  Others: the next stretch asked for ahead 71, rows brought to L2 ahead 73, a CTA at a token of 2048 columns 85, 24 warps an SM instead of
-// 16 the same.
+// 16 the same.  What bounds it is the latency of rows: DRAM is busy half of the time (4.1 TB/s), and half of what a warp's instruction takes is waiting for
+// loads, with 14 warps an SM (95 registers allow two CTAs) that store between them.
 template <typename T, typename G, bool kVector, int kWarps>
 __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKernel(const RowsArgs a)
 {
@@ -425,7 +426,7 @@ template <typename T, bool kOrdered, int kWarps> cudaError_t LaunchQuantise(cons
     return vectors ? b200sp::LaunchChained(QuantiseKernel<T, true, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a)
                    : b200sp::LaunchChained(QuantiseKernel<T, false, kWarps, kOrdered>, blocks, kRowsThreads, 0, stream, a);
 }
-// As many warps as keep a row in registers; where there are few rows, a CTA's.
+// As many warps as keep a row in shared memory, 1024 elements each; where there are few rows, a CTA's.
 template <typename T, bool kOrdered> cudaError_t LaunchQuantise(const RowsArgs &a, bool vectors, cudaStream_t stream)
 {
     if (a.width > 4096 || a.tokens < (long long)b200sp_sm_count() * 4) return LaunchQuantise<T, kOrdered, 8>(a, vectors, stream);

@@ -127,8 +127,9 @@ int TileColumns(long long rows, long long experts)
 }
 
 // How a product without experts is computed: by tiles, of a CTA, a pair of them, or a cluster that shares a tile's steps, or without tiles.  An estimate of the
-// time of every way, us, fitted to 620 products of 1 to 2048 rows by 512 x 4096 to 8192 x 4096 bytes; of the ways with tiles it takes one within 0.5 % of the
-// fastest on average and 5 % at worst.  (512 rows of 4096 by 4096: pairs 17, clusters of two 37; 16 rows: clusters of four 10, whole tiles 15; one row:
+// time of every way, us, fitted to 620 timings of 48 products, 1 to 2048 rows by six matrices of 128 KB to 17 MB, in the ways and widths of tiles that each allows.  On
+// 70 other products (1 to 2048 rows, 128 to 8192 channels, 256 to 8192 columns) it takes one 1.7 % slower than the fastest on average; eight lose 5 % or more,
+// one 21 %: 16 rows of 672 by 2392, without tiles 7.4, by tiles of 32 6.1.  (512 rows of 4096 by 4096: pairs 17, clusters of two 37; 16 rows: clusters of four 10, whole tiles 15; one row:
 // clusters 10, without tiles 6.6; four rows 10 and 12.6; 8 rows of 1024 by 1024: 6.4 and 3.7.)
 enum FormKind { kWhole, kPairs, kShared, kFew };
 struct Form {
@@ -169,7 +170,11 @@ Form FormOf(long long rows, long long n, long long depth)
     return best;
 }
 
-// With experts, of whose rows the host knows the average only.
+// With experts, of whose rows the host knows the average only.  us for 32 experts of 2048 x 2048, four a token, by CTAs on 32 and 64 rows, by pairs on 128 and 256: 64
+// tokens 29, 29, 30, 31; 256 tokens 37, 30, 31, 32; 1024 tokens 96, 58, 43, 35; 4096 tokens 332, 180, 105, 73.  Single CTAs on as many rows as the pairs: 1024 tokens
+// 44 and 37, 4096 107 and 77.  Without tiles, and by tiles of 16: 64 experts of 2048 x 2048, eight a token, one token 8.4 and 10.5, two 15.7 and 16.8, four 27.3
+// and 23.9.  (The border is right for such; it goes by entries alone: of few experts more would be faster without tiles -- two tokens to two of eight of 4096 x 4096
+// 8.6, and 14.7 as it is -- and of many fewer: eight tokens to eight of 256 of 2048 x 2048 42 by tiles, and 55 as it is.)
 Form FormOfExperts(long long rows, long long n, long long experts)
 {
     Form form{kWhole, TileColumns(rows, experts), 1};
