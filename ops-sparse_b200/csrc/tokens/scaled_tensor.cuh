@@ -377,11 +377,12 @@ __global__ void __launch_bounds__(kTileThreads, 1) ScaledTensorKernel(const Scal
 
 // Few tiles, as when some tokens are served: the CTAs of a cluster share the steps of one tile, and each adds up a part of its columns from
 // all their accumulators, through shared memory.  Sums of whole numbers may be regrouped.  61 rows of 4096 by 4096: 11.2 us, 14.4 by whole tiles; 61 of 2040 by
-// 1111 7.3 and 9.5.  What bounds it is latency: a launch, its ends and two meetings of the cluster are 5 us.
+// 1111 7.1 and 9.5.  What bounds it is latency: a launch, its ends and two meetings of the cluster are 5 us.
 constexpr int kSplitThreads = 256, kSplitMost = 8;  // CTAs of a cluster: the portable most
-// At least so much shared memory: not beside a CTA of the other kernels that take tensor memory, nor more of them on an SM than it has columns for.
-// Clusters (and pairs) of two streams that each wait for the tensor memory of the other would wait for ever.
-constexpr int kSplitShared = 48 << 10;
+// At least so much shared memory, which leaves no room for another CTA that takes tensor memory, of this library or any other, and fills shared memory with tiles for
+// it.  Clusters (and pairs) of two streams that each wait for the tensor memory of the other would wait for ever.  (It costs nothing: FormOf takes no more clusters
+// than have SMs of their own.)
+constexpr int kSplitShared = kTileShared;
 
 __device__ __forceinline__ int LoadRemote(uint32_t at, int rank)
 {

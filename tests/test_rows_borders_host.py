@@ -102,3 +102,17 @@ def test_closed_optional_descriptors_are_refused(pkg):
             for other in (held, None):
                 with pytest.raises(pkg.AclSparseError, match="HANDLE_IS_NULLPTR"):
                     call(other)
+
+
+@pytest.mark.parametrize("name,unit,most", [("scaled_tensor.cuh", "kTile", "kTileColsMost"), ("experts_tensor.cuh", "kMma", "kMmaColsMost")])
+def test_clusters_on_tensor_memory_have_their_sms_to_themselves(name, unit, most):
+    """CTAs that wait for each other must not wait for tensor memory, too: whatever the width of tiles, no other CTA with tiles in shared memory fits beside."""
+    code = _code(name)
+    number = lambda n: eval(re.search(rf"constexpr int {n} = ([^;]+);", code).group(1), {"kTileShared": 192 << 10, "kTileRows": 128, "kTileDepth": 128,  # noqa: E731
+                                                                                       "kMmaRows": 128, "kMmaDepth": 64})
+    shared, stages, first = number(f"{unit}Shared"), number(f"{unit}StagesMost"), number("kTileWBytes" if unit == "kTile" else "kMmaABytes")
+    for cols in (16, 32, 64, 128, 256):
+        for stage in (first + cols * 128, first + cols * 64):
+            assert min(shared // stage, stages) * stage >= 160 << 10  # of 228
+    if unit == "kTile":
+        assert number("kSplitShared") >= 160 << 10 and "kSplitShared}" in code
