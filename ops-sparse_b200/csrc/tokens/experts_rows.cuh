@@ -256,11 +256,12 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
             }
             if (a.dValues == nullptr) continue;
             float total = 0.0f;  // of entry e0 + lane
+            bool in = false;     // it has an expert
 #pragma unroll
             for (int j = 0; j < kBatch; ++j) {
 #pragma unroll
                 for (int d = 16; d > 0; d >>= 1) dot[j] += __shfl_xor_sync(0xffffffffu, dot[j], d);
-                if (lane == j) total = dot[j];
+                if (lane == j) total = dot[j], in = place[j] < end;
             }
             if constexpr (kWarps > 1) {  // a CTA's warps are all at one token; two places in turn, as others may still read the one
                 if (lane < kBatch) sDot[turn][warp][lane] = total;
@@ -272,7 +273,8 @@ __global__ void __launch_bounds__(kRowsThreads, kGradCtas) ExpertsCombineGradKer
             }
             if (within == 0 && lane < many) {
                 const float old = beta != 0.0f ? ValueAt(a.dValues, a.dValuesType, e0 + lane) : 0.0f;
-                SetValue(a.dValues, a.dValuesType, e0 + lane, beta != 0.0f ? fmaf(beta, old, alpha * total) : alpha * total);
+                const float term = in ? alpha * total : 0.0f;  // whatever alpha is
+                SetValue(a.dValues, a.dValuesType, e0 + lane, beta != 0.0f ? fmaf(beta, old, term) : term);
             }
         }
     }

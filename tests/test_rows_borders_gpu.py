@@ -283,6 +283,28 @@ def test_gradients_of_rows_beyond_32_bits(pkg, handle):
         ref.close(seen, want, ref.rounding(torch.bfloat16, want) + 2 * F32 * want.abs())
 
 
+@pytest.mark.parametrize("tokens", [3, 2000])
+@pytest.mark.parametrize("beta", [0.0, 2.0])
+def test_entries_of_no_expert_whatever_alpha_is(pkg, handle, tokens, beta):
+    """Their first terms are 0 in every call, with an alpha that is not finite, too."""
+    from ops_sparse_b200 import api
+    g = gen(71)
+    R = routed(api, g, tokens, 6, 2, wild=0.5)
+    buffer = ordered(api, handle, R)
+    _, places, starts = rows.order_of(R.col_ind, 6)
+    end, none = int(starts[-1]), places >= int(starts[-1])
+    assert 0 < end < R.nnz
+    x, s = matrix(g, tokens, 24, "f32")[0], matrix(g, R.nnz, 24, "f32")[0]
+    d_rows, d_values, out = matrix(g, R.nnz, 24, "f32")[0], torch.randn(R.nnz, generator=g, device="cuda"), matrix(g, R.nnz, 24, "f32")[0]
+    want = [beta * t.cpu() for t in (d_rows[end:], d_values.cpu()[none], out[end:])]
+    api.experts_combine_grad(handle, R, mat(api, x), mat(api, s), mat(api, d_rows), api.DnVec(d_values), math.inf, beta, buffer=buffer)
+    api.experts_dispatch(handle, R, mat(api, x), mat(api, out), math.inf, beta, buffer=buffer)
+    no_error(pkg)
+    for t, w in zip((d_rows[end:], d_values.cpu()[none], out[end:]), want):
+        assert torch.equal(t.cpu(), w)
+    assert not bool(d_rows[:end].isfinite().any()) and not bool(out[:end].isfinite().any())
+
+
 @pytest.mark.parametrize("out,beta", [("bf16", 0.0), ("f16", 0.5), ("f32", 0.0)])
 @pytest.mark.parametrize("many,depth,channels,kind", [(2, 96, 72, FEW), (4, 4096, 4096, SHARED), (4, 96, 72, None)], ids=["rows", "clusters", "tiles"])
 def test_results_beyond_32_bits(pkg, handle, many, depth, channels, kind, out, beta):
