@@ -73,8 +73,8 @@ aclsparseStatus_t b200spExpertsQuantise(aclsparseHandle_t handle, aclsparseConst
 /* ---- Products in 8 bits ----
  * Y[i][j] = alpha * scalesX[i] * scalesW[j] * (sum of X[i][c] * W[j][c]) + beta * Y[i][j].  X, W: ACL_INT8, of the same columns, 131,071 at
  * most: the sums are exact.  scalesX, scalesW: ACL_FLOAT, one for every row.  Y: f32, f16 or bf16.  Fastest where the rows of X and W
- * start on 16 bytes; others are copied into the buffer in every call, weights, too (one row of 4096 by 4096 13 us, where 6.6).  buffer: of the size that this says (0: it may be NULL) for one call
- * at a time. */
+ * start on 16 bytes; others are copied into the buffer in every call, weights, too (one row of 4096 by 4096 13 us, where 6.6).  buffer: of the size
+ * that this says (0: it may be NULL) for one call at a time. */
 aclsparseStatus_t b200spScaledMMBufferSize(aclsparseHandle_t handle, aclsparseConstDnMatDescr_t matX,
                                            aclsparseConstDnMatDescr_t matW, aclsparseConstDnMatDescr_t matY, size_t *bufferSize);
 aclsparseStatus_t b200spScaledMM(aclsparseHandle_t handle, const void *alpha, aclsparseConstDnMatDescr_t matX,

@@ -17,8 +17,9 @@
 
 namespace b200sp {
 
-// For grids that leave most SMs idle and end within some us: the next kernel is set up beside this one, and still waits for its end, on the SMs that it will need, which
-// no other stream has meanwhile.  One row of 4096 to 8 bits, again and again: 3.3 us apart instead of 4.9.
+// For grids that leave most SMs idle and end within some us: the next kernel is set up beside this one, and still waits for
+// its end, on the SMs that it will need, which no other stream has meanwhile.  One row of 4096 to 8 bits, again and again:
+// 3.3 us apart instead of 4.9.
 __device__ __forceinline__ void LetNextStart() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void WaitForPrevious() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 

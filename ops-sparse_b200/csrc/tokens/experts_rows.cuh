@@ -29,9 +29,10 @@ struct RowsArgs {
 };
 
 // Rounding to 8 bits lets the next kernel in early (a product takes every SM, and keeps other streams from them while it waits) only where it is a matter of some us:
-// by half of the SMs, rows that are held, and so many stretches of rows to be written, eight of a row at least, all by one CTA at worst, 18 us (f32 23).  16 tokens to eight of 64 experts, order,
-// rounding and product 32.1 us, without 32.6; one row of 4096 and its product 6.57 and 6.7.  (The order of the entries, by eight SMs, does not: one of
-// 1,048,576 entries takes 285 us, in which another stream's product ends in 17, and not in 440; behind orders of 8 to 32,768 entries nothing is gained.)
+// by half of the SMs, rows that are held, and so many stretches of rows to be written, eight of a row at least, all by one CTA at worst, 18 us (f32 23).  16 tokens
+// to eight of 64 experts, order, rounding and product 32.1 us, without 32.6; one row of 4096 and its product 6.57 and 6.7.  (The order of the entries, by eight SMs,
+// does not: one of 1,048,576 entries takes 285 us, in which another stream's product ends in 17, and not in 440; behind orders of 8 to 32,768 entries nothing is
+// gained.)
 constexpr unsigned kFewCtas = 74;
 constexpr long long kFewPieces = 2048;
 constexpr int kRowsThreads = 256, kRowsWarps = kRowsThreads / 32;

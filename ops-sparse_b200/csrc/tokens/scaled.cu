@@ -128,9 +128,9 @@ int TileColumns(long long rows, long long experts)
 
 // How a product without experts is computed: by tiles, of a CTA, a pair of them, or a cluster that shares a tile's steps, or without tiles.  An estimate of the
 // time of every way, us, fitted to 620 timings of 48 products, 1 to 2048 rows by six matrices of 128 KB to 17 MB, in the ways and widths of tiles that each allows.  On
-// 70 other products (1 to 2048 rows, 128 to 8192 channels, 256 to 8192 columns) it takes one 1.7 % slower than the fastest on average; eight lose 5 % or more,
-// one 21 %: 16 rows of 672 by 2392, without tiles 7.4, by tiles of 32 6.1.  (512 rows of 4096 by 4096: pairs 17, clusters of two 37; 16 rows: clusters of four 10, whole tiles 15; one row:
-// clusters 10, without tiles 6.6; four rows 10 and 12.6; 8 rows of 1024 by 1024: 6.4 and 3.7.)
+// 70 other products (1 to 2048 rows, 128 to 8192 channels, 256 to 8192 columns) it takes one 1.7 % slower than the fastest on average; eight lose 5 % or more, one
+// 21 %: 16 rows of 672 by 2392, without tiles 7.4, by tiles of 32 6.1.  (512 rows of 4096 by 4096: pairs 17, clusters of two 37; 16 rows: clusters of four 10, whole
+// tiles 15; one row: clusters 10, without tiles 6.6; four rows 10 and 12.6; 8 rows of 1024 by 1024: 6.4 and 3.7.)
 enum FormKind { kWhole, kPairs, kShared, kFew };
 struct Form {
     FormKind kind;

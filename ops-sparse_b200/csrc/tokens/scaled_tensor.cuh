@@ -7,10 +7,10 @@
 // Many rows go to pairs of CTAs on tiles of 256 channels, which read half as much of X; few tiles to clusters that share their steps (ScaledSplitKernel); few rows
 // to warps without tiles (ScaledFewKernel).  FormOf decides.
 // What bounds it: with many rows the tensor cores (67 % of the cycles) and what a step asks of shared memory and L2 (32 KB a CTA in some 650 clocks, of which its
-// products take 512), in long runs the power cap; with short sums the storing of the results (8000 clocks a tile; one of 16 steps takes
-// 16,500 in all, as much as its products and that together).  One B200: 8192 x 4096 by 4096 bf16 out 97 us (2.8 POPS),
-// 8192 x 4096 by 8192 183 alone and 220 in runs of seconds, 32,768 x 2048 by 2048 115; the rows of 8192 tokens, four of 32 experts, 2048 x 2048 126.
-// By single CTAs on tiles of 128 channels: 5 to 10 % longer.  Results stored 64 bytes of a row at a time by two bytes a lane: twice as long as 16 a lane.
+// products take 512), in long runs the power cap; with short sums the storing of the results (8000 clocks a tile; one of 16 steps takes 16,500 in all, as much as
+// its products and that together).  One B200: 8192 x 4096 by 4096 bf16 out 97 us (2.8 POPS), 8192 x 4096 by 8192 183 alone and 220 in runs of seconds, 32,768 x 2048
+// by 2048 115; the rows of 8192 tokens, four of 32 experts, 2048 x 2048 126. By single CTAs on tiles of 128 channels: 5 to 10 % longer.  Results stored 64 bytes of
+// a row at a time by two bytes a lane: twice as long as 16 a lane.
 //
 // Every wait is bounded.  One that ran out ends its warp's work, raises the flag of b200sp_scaled_error and leaves rows of the output unwritten.
 #pragma once
@@ -524,9 +524,9 @@ __global__ void __launch_bounds__(kSplitThreads, 1) ScaledSplitKernel(const Scal
 
 // Few rows at a matrix: no tile, but warps at two rows of W and of X.  What moves is W, in pieces of 512 bytes of a row, of which a warp asks for eight at
 // once; rows of X come from L1.  Products of four bytes at a time (dp4a).  With `parts` > 1 so many warps share an item's columns.
-// One row of 4096 by 4096: 6.6 us with the matrix from DRAM, 4.7 from L2; 2.5 are a launch and its ends, 2.6 the matrix at the copy rate.  Other shapes, rows of X x of W, pieces: 1 x 2, 8
-// 9.3 us, 1 x 4, 4 8.4, 2 x 4, 2 8.6.  Eight rows of X are bound by the rate of dp4a, some 10 lanes a clock and SM: 19 us; by the int8 products of a
-// warp (mma.sync) 10.3, but one row 8.6, and small matrices half as long again.
+// One row of 4096 by 4096: 6.6 us with the matrix from DRAM, 4.7 from L2; 2.5 are a launch and its ends, 2.6 the matrix at the copy rate.  Other shapes, rows of X x
+// of W, pieces: 1 x 2, 8 9.3 us, 1 x 4, 4 8.4, 2 x 4, 2 8.6.  Eight rows of X are bound by the rate of dp4a, some 10 lanes a clock and SM: 19 us; by the int8
+// products of a warp (mma.sync) 10.3, but one row 8.6, and small matrices half as long again.
 constexpr int kFewThreads = 256, kFewWarps = kFewThreads / 32, kFewPiece = 512, kFewRowsX = 2;
 
 template <typename Out>
